@@ -10,7 +10,8 @@ import os
 HERE = os.path.dirname(os.path.abspath(__file__))
 LIB_PATH = os.path.join(HERE, "libcome_b200.so")
 
-COME_F32, COME_F16, COME_BF16 = 0, 1, 2
+COME_F32, COME_F16, COME_BF16, COME_E4M3 = 0, 1, 2, 3
+COME_ACT_SILU, COME_ACT_GELU = 0, 1
 COME_OK, COME_ERR_ARG, COME_ERR_CUDA, COME_ERR_UNSUPPORTED, COME_ERR_DEVICE = 0, -1, -2, -3, -4
 COME_SELECT_RANK, COME_SELECT_ABS, COME_SELECT_ZSCORE = 0, 1, 2
 COME_SCOPE_BATCH, COME_SCOPE_FRAME = 0, 1
@@ -20,6 +21,8 @@ EXPORTS = (
     "come_merge_plan_workspace_bytes", "come_merge_plan", "come_merge_plan_static", "come_merge", "come_merge_layernorm", "come_unmerge",
     "come_unmerge_strided", "come_unmerge_residual", "come_residual_layernorm", "come_suffix_add", "come_suffix_split",
     "come_attn_varlen_fwd", "come_attn_varlen_fwd_rows", "come_attn_cross_fwd", "come_attn_cross_fwd_parts", "come_attn_combine", "come_attn_combine_parts", "come_attn_set_cta_limit", "come_qkv_prepare", "come_packed_positions",
+    "come_residual_rmsnorm", "come_quantize_rows", "come_quantize_weight", "come_matmul_e4m3", "come_gated_matmul_e4m3", "come_gated_matmul",
+    "come_gated_matmul_grad", "come_gated_grad_input", "come_gated_grad_weight", "come_gated_grad_bias",
     "come_device_status", "come_selftest_bounded_wait", "come_selftest_attn_stall", "come_attn_work_list",
     "come_peer_alloc", "come_peer_open", "come_peer_close", "come_peer_free", "come_peer_copy", "come_peer_signal", "come_peer_wait",
 )
@@ -82,6 +85,17 @@ def lib() -> C.CDLL:
     l.come_attn_set_cta_limit.argtypes = [i32]
     l.come_qkv_prepare.argtypes = [vp, i32, i64, i32, i32, vp, vp, vp, vp, f32, vp, vp, vp, i64, vp, vp, vp]
     l.come_packed_positions.argtypes = [vp, vp, i64, C.POINTER(Layout), vp, vp]
+    l.come_residual_rmsnorm.argtypes = [vp, vp, vp, i64, i64, i32, vp, f32, vp, vp, vp, i64, vp, i64, i64, vp]
+    l.come_quantize_rows.argtypes = [vp, i32, i64, i64, i64, vp, i64, vp, i64, i64, vp]
+    l.come_quantize_weight.argtypes = [vp, i32, i64, i64, i64, vp, i64, vp, i64, vp]
+    l.come_matmul_e4m3.argtypes = [vp, i64, vp, i64, i64, vp, i64, vp, i64, vp, i64, i64, i64, vp, i64, i32, vp]
+    l.come_gated_matmul_e4m3.argtypes = [vp, i64, vp, i64, i64, vp, i64, vp, i64, vp, i64, vp, i64, vp, vp, i32, i64, i64, i64, vp, i64, i32, vp,
+                                         i64, i64, vp]
+    l.come_gated_matmul.argtypes = [vp, i64, vp, i64, vp, i64, vp, vp, i32, i32, i64, i64, i64, vp, i64, vp]
+    l.come_gated_matmul_grad.argtypes = [vp, i64, vp, i64, vp, i64, vp, vp, i32, i32, i64, i64, i64, vp, i64, vp, vp, i64, vp]
+    l.come_gated_grad_input.argtypes = [vp, vp, i64, vp, i64, vp, i64, i32, i64, i64, i64, vp, i64, vp]
+    l.come_gated_grad_weight.argtypes = [vp, vp, i64, vp, i64, i32, i64, i64, i64, vp, vp, i64, vp]
+    l.come_gated_grad_bias.argtypes = [vp, vp, i64, i32, i64, i64, vp, vp, vp]
     l.come_device_status.argtypes = [C.POINTER(C.c_uint32), i32]
     l.come_selftest_bounded_wait.argtypes = [i64, vp, vp]
     l.come_attn_work_list.argtypes = [vp, i32, i32, i64, i64, i32, vp, i32, vp, i64, vp]

@@ -17,7 +17,7 @@ from .bias_attention import JaggedAttention_w_Bias
 from .plain_attention import JaggedAttention
 from .token_merger import JaggedTokens
 
-__all__ = ["JaggedBlock", "JaggedBlock_w_Bias", "residual_layernorm", "fusable", "forward_fused"]
+__all__ = ["JaggedBlock", "JaggedBlock_w_Bias", "residual_layernorm", "residual_rmsnorm", "fusable", "forward_fused"]
 
 
 class _JaggedBlockBase(torch.nn.Module):
@@ -92,6 +92,52 @@ def residual_layernorm(x: torch.Tensor, branch: Optional[torch.Tensor], scale: O
     with on_device(dev):
         _lib.check(_lib.lib().come_residual_layernorm(ptr(x), ptr(branch), ptr(scale), rows, Cc, dtype_code(dt, "x"), ptr(gamma),
                                                       ptr(beta), eps, ptr(x_out), ptr(normed), stream_ptr(dev)))
+    return (x if branch is None else x_out), normed
+
+
+def residual_rmsnorm(x: torch.Tensor, branch: Optional[torch.Tensor], scale: Optional[torch.Tensor],
+                     norm: torch.nn.RMSNorm, store_stream: bool = True, quantize: bool = False):
+    """``x_out = x + scale * branch`` and ``normed = norm(x_out)`` in one pass over packed rows ``[P, C]`` (``come_residual_rmsnorm``):
+    :func:`residual_layernorm` for a block with root-mean-square norms.  The update is computed in float32 and rounded once; the norm
+    is that of the stream as it is stored.  ``branch`` None: the norm of ``x`` alone; ``scale`` None: no LayerScale.
+    Returns ``(x_out, normed)``; ``x_out`` is ``x`` itself when there is no branch and None when ``store_stream`` is off.  With
+    ``quantize`` the normed rows leave in 8 bits with a scale per row and 128 columns
+    (:class:`come_b200.block_scaled.BlockScaled`), the operand of the block-scaled products.  Inference only."""
+    from . import _lib
+    from ._torch_util import dtype_code, on_device, ptr, require_cuda, stream_ptr
+    require_cuda(x, "x")
+    if x.dim() != 2 or not x.is_contiguous():
+        raise ValueError(f"x must be a contiguous [rows, C] tensor, got {tuple(x.shape)}")
+    if torch.is_grad_enabled() and (x.requires_grad or (branch is not None and branch.requires_grad)):
+        raise RuntimeError("residual_rmsnorm: inference only (no autograd)")
+    rows, Cc = x.shape
+    dt, dev = x.dtype, x.device
+    code = dtype_code(dt, "x")
+    if branch is not None and (branch.shape != x.shape or branch.dtype != dt or branch.device != dev or not branch.is_contiguous()):
+        raise ValueError(f"branch must be contiguous and match x {tuple(x.shape)} {dt}, got {tuple(branch.shape)} {branch.dtype}")
+    if scale is not None:
+        if branch is None:
+            raise ValueError("scale without a branch")
+        scale = scale.detach().to(device=dev, dtype=dt).contiguous()
+        if scale.shape != (Cc,):
+            raise ValueError(f"scale must be [{Cc}], got {tuple(scale.shape)}")
+    if not isinstance(norm, torch.nn.RMSNorm) or tuple(norm.normalized_shape) != (Cc,):
+        raise NotImplementedError("residual_rmsnorm needs an nn.RMSNorm over the channel dimension")
+    weight = norm.weight
+    if weight is not None:
+        weight = weight.detach().to(device=dev, dtype=dt).contiguous()
+    eps = float(norm.eps) if norm.eps is not None else torch.finfo(dt).eps
+    x_out = torch.empty_like(x) if (branch is not None and store_stream) else None
+    if quantize:
+        from .block_scaled import empty_rows
+        normed = empty_rows(rows, Cc, dev)
+        q = (None, normed.data.data_ptr(), normed.data.stride(0), normed.scale.data_ptr(), *normed.scale.stride())
+    else:
+        normed = torch.empty_like(x)
+        q = (normed.data_ptr(), None, 0, None, 0, 0)
+    with on_device(dev):
+        _lib.check(_lib.lib().come_residual_rmsnorm(ptr(x), ptr(branch), ptr(scale), rows, Cc, code, ptr(weight), eps, ptr(x_out), *q,
+                                                    stream_ptr(dev)))
     return (x if branch is None else x_out), normed
 
 

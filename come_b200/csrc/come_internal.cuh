@@ -52,6 +52,8 @@ int sm_count();
 unsigned int *status_word_dev();
 // Its bits that belong to the attention kernel (come_device_status names them as such).
 constexpr unsigned int kStatusAttention = 0x3ffu;
+// ... and to the product kernels of the feed-forward half.
+constexpr unsigned int kStatusMatmul = 0x380000u;
 
 // ---- element conversion -------------------------------------------------------------------------------------
 template <typename T> struct Elem;

@@ -1,0 +1,690 @@
+// Products of the feed-forward half of a block on Blackwell tensor cores (sm_100a): the kernel with one 128 x 128 result tile per
+// CTA (128 rows of both projections in the gated forms), the contraction of a tile split over the CTAs of a cluster.
+//
+//   warps 0-7 : two epilogue warpgroups, columns [0, 64) and [64, 128) of the tile.  Thread r of a warpgroup owns row r (TMEM lane r).
+//               8-bit operands: every K block of 128 is a product of its own (two TMEM buffers), whose sums the thread scales by
+//               a_scale[row, block] * b_scale[column block, block] and adds to float32 registers: the scales are constants of the row
+//               there, so a block costs one FMA per sum.  16-bit operands: the whole contraction is summed in TMEM.
+//               The sums go to shared memory, where the CTAs of the cluster read each other's: row i of the tile is finished by the
+//               CTA of rank i % cluster, which adds the shares in the order of the ranks (no atomics: the same bits in every run),
+//               applies the epilogue with a warp per row and stores whole rows of 128 neighbouring columns.
+//   warp 8    : producer (TMA ring).      warp 9 : MMA issuer.
+//
+// Why a split: a block's products have few tiles where there are few tokens (1 x 2736 -> 1024: eight), and a tile's time is its
+// contraction's; shares of it bring all SMs to read the weights.  The shares meet in shared memory, not in a workspace, so that two
+// graphs captured from the same call share nothing.
+//
+// Shared memory: a CTA takes more than half an SM's, so that no two CTAs that need tensor memory share an SM: CTAs of two clusters
+// that wait for each other's tensor memory while their partners wait at a cluster barrier would never end.
+//
+// Every wait on an mbarrier is bounded (kWaitTicks): a CTA whose wait gave up raises its abort flag and the device status word, goes
+// on to the cluster's barriers, and no CTA of the cluster stores.
+#include "matmul_sm100.cuh"
+
+#include <mutex>
+
+namespace come {
+
+namespace {
+
+constexpr int kTile = 128;
+constexpr int kKBytes = 128;                       // bytes of the contraction per K block
+constexpr int kEpilogueWarps = 8, kProducerWarp = 8, kIssuerWarp = 9, kThreads = 320;
+constexpr int kOperandBytes = kTile * kKBytes;     // 16 KiB: 128 rows of a K block
+constexpr int kRingBytes = 192 * 1024;
+constexpr int kPartRow = kTile + 4;                // floats: rows of the shares in shared memory, no bank conflicts row to row
+constexpr int kPartBytes = kTile * kPartRow * 4;
+constexpr int kMaxCluster = 8;
+
+struct SplitBarriers {
+    uint64_t full[6], empty[6];
+    uint64_t acc_full[2], acc_empty[2];
+    uint64_t drained;
+    uint32_t tmem_base;
+    volatile uint32_t abort_flag;
+};
+constexpr size_t kSmemBytes = kRingBytes + sizeof(SplitBarriers) + 1024;
+static_assert(kSmemBytes <= 227 * 1024 && kSmemBytes > 114 * 1024, "one CTA per SM");
+static_assert(2 * kPartBytes <= kRingBytes, "the shares reuse the ring");
+
+struct SplitParams {
+    CUtensorMap a[2], b[2];
+    const float *a_scale, *b_scale[2];
+    int64_t as_row, as_block, bs_row[2];
+    const void *bias[2], *dh;
+    void *out[2];
+    float *out_scale;
+    int64_t dh_row, out_row[2], os_row, os_block;
+    int M, N, kb_per_sum, k_blocks;  // K blocks of one contraction, of all
+    int tiles_n, tiles_per_problem;
+    int act, dtype, bias_dtype, out_dtype;
+    unsigned int *status;
+};
+
+__device__ __forceinline__ uint32_t cluster_rank() {
+    uint32_t r;
+    asm volatile("mov.u32 %0, %%cluster_ctarank;" : "=r"(r));
+    return r;
+}
+__device__ __forceinline__ uint32_t cluster_size() {
+    uint32_t r;
+    asm volatile("mov.u32 %0, %%cluster_nctarank;" : "=r"(r));
+    return r;
+}
+__device__ __forceinline__ void cluster_sync() {
+    asm volatile("barrier.cluster.arrive.release.aligned;" ::: "memory");
+    asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory");
+}
+__device__ __forceinline__ uint32_t map_rank(uint32_t saddr, uint32_t rank) {
+    uint32_t r;
+    asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(r) : "r"(saddr), "r"(rank));
+    return r;
+}
+__device__ __forceinline__ float4 ld_cluster(uint32_t addr) {
+    float4 v;
+    asm volatile("ld.shared::cluster.v4.f32 {%0, %1, %2, %3}, [%4];" : "=f"(v.x), "=f"(v.y), "=f"(v.z), "=f"(v.w) : "r"(addr) : "memory");
+    return v;
+}
+__device__ __forceinline__ uint32_t ld_cluster_u32(uint32_t addr) {
+    uint32_t v;
+    asm volatile("ld.shared::cluster.u32 %0, [%1];" : "=r"(v) : "r"(addr) : "memory");
+    return v;
+}
+
+// Four neighbouring columns of a row, `valid` of them inside the result.
+__device__ __forceinline__ void store4(void *out, int64_t at, const float (&v)[4], int valid, int dtype) {
+    if (dtype == COME_F32) {
+        float *p = (float *)out + at;
+        if (valid >= 4 && ((uintptr_t)p & 15) == 0) *reinterpret_cast<float4 *>(p) = make_float4(v[0], v[1], v[2], v[3]);
+        else
+#pragma unroll
+            for (int i = 0; i < 4; ++i)
+                if (i < valid) p[i] = v[i];
+        return;
+    }
+    const bool bf16 = dtype == COME_BF16;
+    const uint32_t lo = bf16 ? pack_16<true>(v[0], v[1]) : pack_16<false>(v[0], v[1]), hi = bf16 ? pack_16<true>(v[2], v[3]) : pack_16<false>(v[2], v[3]);
+    uint16_t *p = (uint16_t *)out + at;
+    if (valid >= 4 && ((uintptr_t)p & 7) == 0) *reinterpret_cast<uint2 *>(p) = make_uint2(lo, hi);
+    else {
+        if (valid > 0) p[0] = (uint16_t)lo;
+        if (valid > 1) p[1] = (uint16_t)(lo >> 16);
+        if (valid > 2) p[2] = (uint16_t)hi;
+        if (valid > 3) p[3] = (uint16_t)(hi >> 16);
+    }
+}
+__device__ __forceinline__ void load4(const void *in, int64_t at, float (&v)[4], int valid, int dtype) {
+    const uint16_t *p = (const uint16_t *)in + at;
+    if (dtype != COME_F32 && valid >= 4 && ((uintptr_t)p & 7) == 0) {
+        const uint2 raw = *reinterpret_cast<const uint2 *>(p);
+        if (dtype == COME_BF16) {
+            v[0] = __uint_as_float(raw.x << 16);
+            v[1] = __uint_as_float(raw.x & 0xffff0000u);
+            v[2] = __uint_as_float(raw.y << 16);
+            v[3] = __uint_as_float(raw.y & 0xffff0000u);
+        } else {
+            const float2 lo = __half22float2(*reinterpret_cast<const __half2 *>(&raw.x)), hi = __half22float2(*reinterpret_cast<const __half2 *>(&raw.y));
+            v[0] = lo.x, v[1] = lo.y, v[2] = hi.x, v[3] = hi.y;
+        }
+        return;
+    }
+#pragma unroll
+    for (int i = 0; i < 4; ++i) v[i] = i < valid ? load_any(in, at + i, dtype) : 0.0f;
+}
+
+enum : uint32_t { kErrFull = 1u << 19, kErrEmpty = 1u << 20, kErrSums = 1u << 21 };
+static_assert((kErrFull | kErrEmpty | kErrSums) == kStatusMatmul, "come_device_status names these bits");
+
+template <bool kE4m3, int kMode, bool kAMn, bool kBMn>
+__global__ void __launch_bounds__(kThreads, 1) matmul_split_kernel(const __grid_constant__ SplitParams p) {
+    constexpr int kMats = kMode == kMatmulPlain ? 1 : 2;
+    constexpr int kN = kMats * kTile;
+    constexpr int kStageBytes = kOperandBytes * (1 + kMats), kStages = kRingBytes / kStageBytes;
+    constexpr int kElems = kE4m3 ? 128 : 64;  // contraction elements of a K block
+    constexpr uint32_t kTmemCols = kE4m3 ? 2 * kN : kN;
+    static_assert(kStages <= 6 && kTmemCols <= 512, "");
+    extern __shared__ __align__(1024) uint8_t smem[];
+    SplitBarriers &sh = *reinterpret_cast<SplitBarriers *>(smem + kRingBytes);
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    const uint32_t rank = cluster_rank(), ranks = cluster_size();
+
+    const int tile = (int)(blockIdx.x / ranks), problem = tile / p.tiles_per_problem, t = tile - problem * p.tiles_per_problem;
+    const int m0 = (t / p.tiles_n) * kTile, n0 = (t % p.tiles_n) * kTile;
+    const int kb0 = (int)((int64_t)p.k_blocks * rank / ranks), kb1 = (int)((int64_t)p.k_blocks * (rank + 1) / ranks), n_kb = kb1 - kb0;
+    const int rows = min(kTile, p.M - m0);
+
+    if (warp == kProducerWarp && lane == 0) {
+        sh.abort_flag = (*(volatile unsigned int *)p.status & kStatusMatmul) != 0 ? 1u : 0u;  // an earlier launch gave up
+        for (int i = 0; i < kStages; ++i) {
+            mbar_init(&sh.full[i], 1);
+            mbar_init(&sh.empty[i], 1);
+        }
+        for (int i = 0; i < 2; ++i) {
+            mbar_init(&sh.acc_full[i], 1);
+            mbar_init(&sh.acc_empty[i], kEpilogueWarps);
+        }
+        mbar_init(&sh.drained, 1);
+        asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+    }
+    if (warp == kIssuerWarp) {
+        asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(&sh.tmem_base)), "r"(kTmemCols) : "memory");
+        asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
+    }
+    tc_fence_before();
+    __syncthreads();
+    tc_fence_after();
+    const uint32_t tmem = sh.tmem_base;
+    const uint32_t ring = smem_u32(smem);
+    const auto wait = [&](uint64_t *bar, uint32_t parity, uint32_t code) { return mbar_wait_limit(bar, parity, &sh.abort_flag, p.status, code, kWaitTicks); };
+    const bool dead = sh.abort_flag != 0;
+
+    if (!dead && warp == kProducerWarp) {
+        if (lane == 0) {
+            int i = 0;
+            for (; i < n_kb; ++i) {
+                const int st = i % kStages;
+                if (!wait(&sh.empty[st], ((i / kStages) & 1) ^ 1, kErrEmpty)) break;
+                const int kb = kb0 + i, sum = kb >= p.kb_per_sum ? 1 : 0, k = (kb - sum * p.kb_per_sum) * kElems;
+                const uint32_t dst = ring + st * kStageBytes;
+                mbar_arrive_expect_tx(&sh.full[st], kStageBytes);
+                const CUtensorMap *ma = &p.a[sum + problem], *mb = &p.b[sum];
+                if constexpr (kAMn) {
+                    tma_load_2d(dst, ma, m0, k, &sh.full[st]);
+                    tma_load_2d(dst + kOperandBytes / 2, ma, m0 + 64, k, &sh.full[st]);
+                } else {
+                    tma_load_2d(dst, ma, k, m0, &sh.full[st]);
+                }
+                if constexpr (kBMn) {
+                    tma_load_2d(dst + kOperandBytes, mb, n0, k, &sh.full[st]);
+                    tma_load_2d(dst + kOperandBytes + kOperandBytes / 2, mb, n0 + 64, k, &sh.full[st]);
+                } else {
+                    tma_load_2d(dst + kOperandBytes, mb, k, n0, &sh.full[st]);
+                    if constexpr (kMats == 2) tma_load_2d(dst + 2 * kOperandBytes, &p.b[1], k, n0, &sh.full[st]);
+                }
+            }
+            for (int j = max(i - kStages, 0); j < i; ++j) mbar_drain(&sh.full[j % kStages], (j / kStages) & 1, p.status, kErrFull);
+        }
+        __syncwarp();
+    } else if (!dead && warp == kIssuerWarp) {
+        if (lane == 0) {
+            const uint32_t idesc = matmul_idesc(kE4m3, p.dtype == COME_BF16, kTile, kN, kAMn, kBMn);
+            constexpr uint32_t kAStep = kAMn ? 2048 >> 4 : 32 >> 4, kBStep = kBMn ? 2048 >> 4 : 32 >> 4;
+            for (int i = 0; i < n_kb; ++i) {
+                const int st = i % kStages, buf = kE4m3 ? i & 1 : 0;
+                if (!wait(&sh.full[st], (i / kStages) & 1, kErrFull)) break;
+                if (kE4m3 && !wait(&sh.acc_empty[buf], ((i >> 1) & 1) ^ 1, kErrSums)) break;
+                tc_fence_after();
+                const uint64_t da = operand_desc(ring + st * kStageBytes, kOperandBytes / 2);
+                const uint64_t db = operand_desc(ring + st * kStageBytes + kOperandBytes, kOperandBytes / 2);
+#pragma unroll
+                for (int k = 0; k < 4; ++k) {
+                    const uint32_t more = k > 0 || (!kE4m3 && i > 0) ? 1u : 0u;
+                    if constexpr (kE4m3) tc_mma_f8_ss_1(tmem + buf * kN, da + k * kAStep, db + k * kBStep, idesc, more);
+                    else tc_mma_ss_1(tmem, da + k * kAStep, db + k * kBStep, idesc, more);
+                }
+                tc_commit_1(&sh.empty[st]);
+                if (kE4m3 || i == n_kb - 1) tc_commit_1(&sh.acc_full[buf]);
+            }
+            tc_commit_1(&sh.drained);
+            mbar_drain(&sh.drained, 0, p.status, kErrSums);
+        }
+        __syncwarp();
+    } else if (!dead) {
+        const int part = warp >> 2, r = (warp & 3) * 32 + lane;  // columns [64 part, + 64) of a weight, row of the tile
+        const uint32_t lanes = tmem + ((uint32_t)((warp & 3) * 32) << 16) + part * 64;
+        const bool busy = (warp & 3) * 32 < rows;                // a warp without rows only keeps the barriers going
+        float *share = reinterpret_cast<float *>(smem) + r * kPartRow + part * 64;
+        bool ok = true;
+        if constexpr (kE4m3) {
+            float sum[kMats][64];
+#pragma unroll
+            for (int w = 0; w < kMats; ++w)
+#pragma unroll
+                for (int c = 0; c < 64; ++c) sum[w][c] = 0.0f;
+            const float *as = p.a_scale + (int64_t)(m0 + (r < rows ? r : 0)) * p.as_row;
+            const float *bs[2] = {p.b_scale[0] + (n0 / kTile) * p.bs_row[0], kMats == 2 ? p.b_scale[1] + (n0 / kTile) * p.bs_row[1] : nullptr};
+            float sa = as[kb0 * p.as_block], sb[2] = {bs[0][kb0], kMats == 2 ? bs[1][kb0] : 0.0f};
+            for (int i = 0; i < n_kb; ++i) {
+                const int buf = i & 1;
+                const float s[2] = {sa * sb[0], sa * sb[1]};
+                if (i + 1 < n_kb) {
+                    sa = as[(kb0 + i + 1) * p.as_block];
+                    sb[0] = bs[0][kb0 + i + 1];
+                    if constexpr (kMats == 2) sb[1] = bs[1][kb0 + i + 1];
+                }
+                ok = wait(&sh.acc_full[buf], (i >> 1) & 1, kErrSums);
+                ok = __all_sync(0xffffffffu, ok);
+                if (!ok) break;
+                if (busy) {
+                    tc_fence_after();
+#pragma unroll
+                    for (int w = 0; w < kMats; ++w)
+#pragma unroll
+                        for (int c = 0; c < 64; c += 32) {
+                            uint32_t d[32];
+                            tmem_ld32(lanes + buf * kN + w * kTile + c, d);
+                            tc_wait_ld();
+#pragma unroll
+                            for (int j = 0; j < 32; ++j) sum[w][c + j] = fmaf(__uint_as_float(d[j]), s[w], sum[w][c + j]);
+                        }
+                    tc_fence_before();
+                }
+                __syncwarp();
+                if (lane == 0) mbar_arrive(&sh.acc_empty[buf]);
+            }
+            // the last product has completed and with it every read of the ring: the shares may take its place
+            if (ok && busy) {
+#pragma unroll
+                for (int w = 0; w < kMats; ++w)
+#pragma unroll
+                    for (int c = 0; c < 64; c += 4)
+                        *reinterpret_cast<float4 *>(share + w * (kPartBytes / 4) + c) = make_float4(sum[w][c], sum[w][c + 1], sum[w][c + 2], sum[w][c + 3]);
+            }
+        } else {
+            ok = wait(&sh.acc_full[0], 0, kErrSums);
+            ok = __all_sync(0xffffffffu, ok);
+            if (ok && busy) {
+                tc_fence_after();
+#pragma unroll
+                for (int w = 0; w < kMats; ++w)
+#pragma unroll
+                    for (int c = 0; c < 64; c += 32) {
+                        uint32_t d[32];
+                        tmem_ld32(lanes + w * kTile + c, d);
+                        tc_wait_ld();
+#pragma unroll
+                        for (int j = 0; j < 32; j += 4)
+                            *reinterpret_cast<uint4 *>(share + w * (kPartBytes / 4) + c + j) = make_uint4(d[j], d[j + 1], d[j + 2], d[j + 3]);
+                    }
+            }
+        }
+    }
+
+    tc_fence_before();
+    cluster_sync();
+    bool store = true;
+    for (uint32_t s = 0; s < ranks; ++s) store &= ld_cluster_u32(map_rank(smem_u32((const void *)&sh.abort_flag), s)) == 0;
+    if (store && warp < kEpilogueWarps) {
+        const int n = n0 + 4 * lane, valid = p.N - n;
+        float bias[2][4] = {};
+#pragma unroll
+        for (int w = 0; w < kMats; ++w)
+            if (p.bias[w])
+#pragma unroll
+                for (int i = 0; i < 4; ++i)
+                    if (i < valid) bias[w][i] = load_any(p.bias[w], n + i, p.bias_dtype);
+        for (int r = (int)(rank + ranks * warp); r < rows; r += (int)ranks * kEpilogueWarps) {
+            float v[2][4] = {};
+            for (uint32_t s = 0; s < ranks; ++s) {
+                const uint32_t at = map_rank(ring + (r * kPartRow + 4 * lane) * 4, s);
+#pragma unroll
+                for (int w = 0; w < kMats; ++w) {
+                    const float4 x = ld_cluster(at + w * kPartBytes);
+                    v[w][0] += x.x, v[w][1] += x.y, v[w][2] += x.z, v[w][3] += x.w;
+                }
+            }
+#pragma unroll
+            for (int w = 0; w < kMats; ++w)
+#pragma unroll
+                for (int i = 0; i < 4; ++i) v[w][i] += bias[w][i];
+            const int64_t row = m0 + r, at = row * p.out_row[problem] + n;
+            if constexpr (kMode == kMatmulPlain) {
+                store4(p.out[problem], at, v[0], valid, p.out_dtype);
+            } else if constexpr (kMode == kMatmulGated) {
+                float h[4], top = 0.0f;
+#pragma unroll
+                for (int i = 0; i < 4; ++i) {
+                    h[i] = i < valid ? activation(v[0][i], p.act) * v[1][i] : 0.0f;
+                    top = fmaxf(top, fabsf(h[i]));
+                }
+                if (p.out_dtype != COME_E4M3) {
+                    store4(p.out[0], at, h, valid, p.out_dtype);
+                } else {
+#pragma unroll
+                    for (int s = 16; s >= 1; s >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, s));
+                    top = fmaxf(top, kSmallestMax);
+                    const float inv = kE4m3Max / top;
+                    const uint32_t q = pack_e4m3(h[0] * inv, h[1] * inv, h[2] * inv, h[3] * inv);
+                    uint8_t *out = (uint8_t *)p.out[0] + at;  // rows start at multiples of 16 bytes
+                    if (valid >= 4) *reinterpret_cast<uint32_t *>(out) = q;
+                    else
+#pragma unroll
+                        for (int i = 0; i < 4; ++i)
+                            if (i < valid) out[i] = (uint8_t)(q >> (8 * i));
+                    if (lane == 0) p.out_scale[row * p.os_row + (n0 / kTile) * p.os_block] = top / kE4m3Max;
+                }
+            } else {
+                float dh[4], dg[4], du[4];
+                load4(p.dh, row * p.dh_row + n, dh, valid, p.dtype);
+#pragma unroll
+                for (int i = 0; i < 4; ++i) {
+                    float a, slope;
+                    activation_grad(v[0][i], p.act, a, slope);
+                    dg[i] = dh[i] * v[1][i] * slope;
+                    du[i] = dh[i] * a;
+                }
+                store4(p.out[0], at, dg, valid, p.out_dtype);
+                store4(p.out[1], row * p.out_row[1] + n, du, valid, p.out_dtype);
+            }
+        }
+    }
+    cluster_sync();  // no CTA leaves while another reads its share
+    if (warp == kIssuerWarp) {
+        tc_fence_after();
+        asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(kTmemCols));
+    }
+}
+
+// The shared-memory opt-in of a kernel, once per device and instantiation and before its first launch (launches stay cheap and
+// legal inside a stream capture).
+template <auto kernel> int allow_smem(size_t bytes) {
+    static std::mutex mu;
+    static bool done[64];
+    int dev = 0;
+    COME_CUDA(cudaGetDevice(&dev));
+    COME_REQUIRE(dev >= 0 && dev < 64, "device ordinal %d is out of the supported range", dev);
+    std::lock_guard<std::mutex> lock(mu);
+    if (done[dev]) return COME_OK;
+    COME_CUDA(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)bytes));
+    done[dev] = true;
+    return COME_OK;
+}
+
+template <bool kE4m3, int kMode, bool kAMn, bool kBMn> int launch_split(const SplitParams &p, int64_t tiles, int cluster, cudaStream_t st) {
+    constexpr auto kernel = matmul_split_kernel<kE4m3, kMode, kAMn, kBMn>;
+    if (int rc = allow_smem<kernel>(kSmemBytes); rc != COME_OK) return rc;
+    cudaLaunchAttribute attr = {};
+    attr.id = cudaLaunchAttributeClusterDimension;
+    attr.val.clusterDim.x = (unsigned)cluster;
+    attr.val.clusterDim.y = attr.val.clusterDim.z = 1;
+    cudaLaunchConfig_t cfg = {};
+    cfg.gridDim = dim3((unsigned)(tiles * cluster));
+    cfg.blockDim = dim3(kThreads);
+    cfg.dynamicSmemBytes = kSmemBytes;
+    cfg.stream = st;
+    cfg.attrs = &attr;
+    cfg.numAttrs = 1;
+    const cudaError_t e = cudaLaunchKernelEx(&cfg, kernel, p);
+    if (e != cudaSuccess) {
+        cudaGetLastError();
+        set_error("product kernel: launch failed: %s", cudaGetErrorString(e));
+        return COME_ERR_CUDA;
+    }
+    return COME_OK;
+}
+
+// CTAs that share a tile's contraction: as many as fill the SMs once, at least one K block each.
+int pick_cluster(int64_t tiles, int64_t k_blocks) {
+    int c = 1;
+    while (c < kMaxCluster && tiles * c * 2 <= sm_count() && c * 2 <= k_blocks) c *= 2;
+    return c;
+}
+
+int run_matmul(const MatmulArgs &a, cudaStream_t st) {
+    const int mats = a.mode == kMatmulPlain ? 1 : 2;
+    SplitParams p = {};
+    p.status = status_word_dev();
+    if (!p.status) return COME_ERR_CUDA;
+    int rc;
+    for (int i = 0; i < (a.sums > a.problems ? a.sums : a.problems); ++i) {
+        rc = a.a_mn ? make_rows_map(&p.a[i], a.a[i], a.e4m3, a.dtype, a.K, a.M, a.a_row[i], 64) : make_rows_map(&p.a[i], a.a[i], a.e4m3, a.dtype, a.M, a.K, a.a_row[i], kTile);
+        if (rc != COME_OK) return rc;
+    }
+    for (int i = 0; i < (a.sums > mats ? a.sums : mats); ++i) {
+        rc = a.b_mn ? make_rows_map(&p.b[i], a.b[i], a.e4m3, a.dtype, a.K, a.N, a.b_row[i], 64) : make_rows_map(&p.b[i], a.b[i], a.e4m3, a.dtype, a.N, a.K, a.b_row[i], kTile);
+        if (rc != COME_OK) return rc;
+    }
+    p.a_scale = a.a_scale;
+    p.as_row = a.as_row;
+    p.as_block = a.as_block;
+    for (int i = 0; i < 2; ++i) {
+        p.b_scale[i] = a.b_scale[i];
+        p.bs_row[i] = a.bs_row[i];
+        p.bias[i] = a.bias[i];
+        p.out[i] = a.out[i];
+        p.out_row[i] = a.out_row[i];
+    }
+    p.dh = a.dh;
+    p.dh_row = a.dh_row;
+    p.out_scale = a.out_scale;
+    p.os_row = a.os_row;
+    p.os_block = a.os_block;
+    p.M = (int)a.M;
+    p.N = (int)a.N;
+    const int elems = a.e4m3 ? 128 : 64;
+    p.kb_per_sum = (int)((a.K + elems - 1) / elems);
+    p.k_blocks = p.kb_per_sum * a.sums;
+    p.tiles_n = (int)((a.N + kTile - 1) / kTile);
+    const int64_t per_problem = (a.M + kTile - 1) / kTile * p.tiles_n, tiles = per_problem * a.problems;
+    COME_REQUIRE(tiles < (1ll << 27), "the result has %lld tiles of 128 x 128: too many for one launch", (long long)tiles);
+    p.tiles_per_problem = (int)per_problem;
+    p.act = a.act;
+    p.dtype = a.dtype;
+    p.bias_dtype = a.e4m3 ? COME_F32 : a.dtype;
+    p.out_dtype = a.out_dtype;
+    const int cluster = pick_cluster(tiles, p.k_blocks);
+    if (a.e4m3) return a.mode == kMatmulPlain ? launch_split<true, kMatmulPlain, false, false>(p, tiles, cluster, st) : launch_split<true, kMatmulGated, false, false>(p, tiles, cluster, st);
+    if (a.mode == kMatmulGated) return launch_split<false, kMatmulGated, false, false>(p, tiles, cluster, st);
+    if (a.mode == kMatmulGatedGrad) return launch_split<false, kMatmulGatedGrad, false, false>(p, tiles, cluster, st);
+    return a.a_mn ? launch_split<false, kMatmulPlain, true, true>(p, tiles, cluster, st) : launch_split<false, kMatmulPlain, false, true>(p, tiles, cluster, st);
+}
+
+// ---- column sums (gradients of the biases) --------------------------------------------------------------------------------
+// One CTA per 32 columns of one matrix: 4 lanes x 16 bytes cover a row's columns, 64 rows per pass; a thread adds its rows in
+// float32, then the 64 threads of a column are added in their order: one launch, no workspace, the same bits in every run.
+template <typename T>
+__global__ void __launch_bounds__(256) column_sums_kernel(const T *__restrict__ x0, const T *__restrict__ x1, int64_t row_stride, int64_t rows, int cols,
+                                                          T *__restrict__ out0, T *__restrict__ out1) {
+    __shared__ float part[64][33];
+    const T *x = blockIdx.y ? x1 : x0;
+    T *out = blockIdx.y ? out1 : out0;
+    if (!out) return;
+    const int c = blockIdx.x * 32 + (threadIdx.x & 3) * 8, r0 = threadIdx.x >> 2;
+    float sum[8] = {};
+    if (c < cols)  // rows are stored with a stride of whole 16 bytes: a vector that begins inside a row ends inside its stride
+        for (int64_t r = r0; r < rows; r += 64) {
+            const uint4 raw = *reinterpret_cast<const uint4 *>(x + r * row_stride + c);
+            const T *e = reinterpret_cast<const T *>(&raw);
+#pragma unroll
+            for (int i = 0; i < 8; ++i) sum[i] += Elem<T>::to_f32(e[i]);
+        }
+#pragma unroll
+    for (int i = 0; i < 8; ++i) part[r0][(threadIdx.x & 3) * 8 + i] = sum[i];
+    __syncthreads();
+    const int col = blockIdx.x * 32 + threadIdx.x;
+    if (threadIdx.x < 32 && col < cols) {
+        float s = 0.0f;
+        for (int r = 0; r < 64; ++r) s += part[r][threadIdx.x];
+        out[col] = Elem<T>::from_f32(s);
+    }
+}
+
+bool rows_ok(const void *p, int64_t row_stride, int size) { return p && (uintptr_t)p % 16 == 0 && row_stride >= 0 && row_stride * size % 16 == 0 && row_stride * size < (1ll << 40); }
+bool is_16_bit(int dtype) { return dtype == COME_F16 || dtype == COME_BF16; }
+constexpr int64_t kMaxExtent = (1ll << 31) - 256;
+
+}  // namespace
+
+}  // namespace come
+
+#define COME_REQUIRE_SIZES(what, m, n, k)                                                                                              \
+    COME_REQUIRE((m) >= 0 && (n) >= 0 && (k) > 0 && (m) < come::kMaxExtent && (n) < come::kMaxExtent && (k) < come::kMaxExtent,           \
+                 what ": sizes must be positive and fit int32 (got %lld, %lld, %lld)", (long long)(m), (long long)(n), (long long)(k))
+#define COME_REQUIRE_ROWS(what, ptr, stride, size, least)                                                                             \
+    COME_REQUIRE(come::rows_ok(ptr, stride, size) && (stride) >= (least), what " must be given, 16-byte aligned, with a row stride of whole 16 bytes that holds its rows")
+
+extern "C" int come_matmul_e4m3(const void *x_dev, int64_t x_row_stride, const float *x_scale_dev, int64_t x_scale_row_stride, int64_t x_scale_block_stride,
+                                const void *w_dev, int64_t w_row_stride, const float *w_scale_dev, int64_t w_scale_row_stride, const float *bias_dev, int64_t tokens,
+                                int64_t features, int64_t channels, void *out_dev, int64_t out_row_stride, int out_dtype, void *stream) {
+    COME_REQUIRE_SIZES("come_matmul_e4m3", tokens, features, channels);
+    COME_REQUIRE(out_dtype == COME_F32 || come::is_16_bit(out_dtype), "unknown dtype %d", out_dtype);
+    if (tokens == 0 || features == 0) return COME_OK;
+    COME_REQUIRE_ROWS("x", x_dev, x_row_stride, 1, channels);
+    COME_REQUIRE_ROWS("w", w_dev, w_row_stride, 1, channels);
+    COME_REQUIRE(x_scale_dev && w_scale_dev && out_dev && out_row_stride >= features, "scales and result must be given");
+    come::MatmulArgs a = {};
+    a.mode = come::kMatmulPlain;
+    a.e4m3 = true;
+    a.M = tokens, a.N = features, a.K = channels;
+    a.a[0] = x_dev, a.a_row[0] = x_row_stride;
+    a.b[0] = w_dev, a.b_row[0] = w_row_stride;
+    a.sums = a.problems = 1;
+    a.a_scale = x_scale_dev, a.as_row = x_scale_row_stride, a.as_block = x_scale_block_stride;
+    a.b_scale[0] = w_scale_dev, a.bs_row[0] = w_scale_row_stride;
+    a.bias[0] = bias_dev;
+    a.out[0] = out_dev, a.out_row[0] = out_row_stride;
+    a.out_dtype = out_dtype;
+    return come::run_matmul(a, (cudaStream_t)stream);
+}
+
+extern "C" int come_gated_matmul_e4m3(const void *x_dev, int64_t x_row_stride, const float *x_scale_dev, int64_t x_scale_row_stride,
+                                      int64_t x_scale_block_stride, const void *gate_dev, int64_t gate_row_stride, const float *gate_scale_dev,
+                                      int64_t gate_scale_row_stride, const void *up_dev, int64_t up_row_stride, const float *up_scale_dev,
+                                      int64_t up_scale_row_stride, const float *gate_bias_dev, const float *up_bias_dev, int activation, int64_t tokens,
+                                      int64_t features, int64_t channels, void *out_dev, int64_t out_row_stride, int out_dtype, float *out_scale_dev,
+                                      int64_t out_scale_row_stride, int64_t out_scale_block_stride, void *stream) {
+    COME_REQUIRE_SIZES("come_gated_matmul_e4m3", tokens, features, channels);
+    COME_REQUIRE(out_dtype == COME_E4M3 || come::is_16_bit(out_dtype), "the result is float16, bfloat16 or 8 bits with scales (got dtype %d)", out_dtype);
+    COME_REQUIRE(activation == COME_ACT_SILU || activation == COME_ACT_GELU, "unknown activation %d", activation);
+    if (tokens == 0 || features == 0) return COME_OK;
+    COME_REQUIRE_ROWS("x", x_dev, x_row_stride, 1, channels);
+    COME_REQUIRE_ROWS("gate", gate_dev, gate_row_stride, 1, channels);
+    COME_REQUIRE_ROWS("up", up_dev, up_row_stride, 1, channels);
+    COME_REQUIRE(x_scale_dev && gate_scale_dev && up_scale_dev && out_dev && out_row_stride >= features, "scales and result must be given");
+    COME_REQUIRE(out_dtype != COME_E4M3 || (out_scale_dev && come::rows_ok(out_dev, out_row_stride, 1)),
+                 "an 8-bit result needs its scales, 16-byte aligned rows and a row stride of whole 16 bytes");
+    come::MatmulArgs a = {};
+    a.mode = come::kMatmulGated;
+    a.e4m3 = true;
+    a.M = tokens, a.N = features, a.K = channels;
+    a.a[0] = x_dev, a.a_row[0] = x_row_stride;
+    a.b[0] = gate_dev, a.b_row[0] = gate_row_stride;
+    a.b[1] = up_dev, a.b_row[1] = up_row_stride;
+    a.sums = a.problems = 1;
+    a.a_scale = x_scale_dev, a.as_row = x_scale_row_stride, a.as_block = x_scale_block_stride;
+    a.b_scale[0] = gate_scale_dev, a.bs_row[0] = gate_scale_row_stride;
+    a.b_scale[1] = up_scale_dev, a.bs_row[1] = up_scale_row_stride;
+    a.bias[0] = gate_bias_dev, a.bias[1] = up_bias_dev;
+    a.act = activation;
+    a.out[0] = out_dev, a.out_row[0] = out_row_stride;
+    a.out_dtype = out_dtype;
+    a.out_scale = out_scale_dev, a.os_row = out_scale_row_stride, a.os_block = out_scale_block_stride;
+    return come::run_matmul(a, (cudaStream_t)stream);
+}
+
+static int gated_common(come::MatmulArgs &a, const void *x, int64_t x_row, const void *gate, int64_t gate_row, const void *up, int64_t up_row, const void *gate_bias,
+                        const void *up_bias, int dtype, int activation, int64_t tokens, int64_t features, int64_t channels) {
+    COME_REQUIRE_SIZES("come_gated_matmul", tokens, features, channels);
+    COME_REQUIRE(come::is_16_bit(dtype), "the gated projections need float16 or bfloat16 (got dtype %d)", dtype);
+    COME_REQUIRE(activation == COME_ACT_SILU || activation == COME_ACT_GELU, "unknown activation %d", activation);
+    if (tokens == 0 || features == 0) return COME_OK;
+    COME_REQUIRE_ROWS("x", x, x_row, 2, channels);
+    COME_REQUIRE_ROWS("gate", gate, gate_row, 2, channels);
+    COME_REQUIRE_ROWS("up", up, up_row, 2, channels);
+    a.dtype = dtype;
+    a.M = tokens, a.N = features, a.K = channels;
+    a.a[0] = x, a.a_row[0] = x_row;
+    a.b[0] = gate, a.b_row[0] = gate_row;
+    a.b[1] = up, a.b_row[1] = up_row;
+    a.bias[0] = gate_bias, a.bias[1] = up_bias;
+    a.sums = a.problems = 1;
+    a.act = activation;
+    a.out_dtype = dtype;
+    return COME_OK;
+}
+
+extern "C" int come_gated_matmul(const void *x_dev, int64_t x_row_stride, const void *gate_dev, int64_t gate_row_stride, const void *up_dev, int64_t up_row_stride,
+                                 const void *gate_bias_dev, const void *up_bias_dev, int dtype, int activation, int64_t tokens, int64_t features,
+                                 int64_t channels, void *out_dev, int64_t out_row_stride, void *stream) {
+    come::MatmulArgs a = {};
+    const int rc = gated_common(a, x_dev, x_row_stride, gate_dev, gate_row_stride, up_dev, up_row_stride, gate_bias_dev, up_bias_dev, dtype, activation, tokens, features, channels);
+    if (rc != COME_OK || tokens == 0 || features == 0) return rc;
+    COME_REQUIRE(out_dev && out_row_stride >= features, "out must be given, with a row stride that holds its rows");
+    a.mode = come::kMatmulGated;
+    a.out[0] = out_dev, a.out_row[0] = out_row_stride;
+    return come::run_matmul(a, (cudaStream_t)stream);
+}
+
+extern "C" int come_gated_matmul_grad(const void *x_dev, int64_t x_row_stride, const void *gate_dev, int64_t gate_row_stride, const void *up_dev, int64_t up_row_stride,
+                                      const void *gate_bias_dev, const void *up_bias_dev, int dtype, int activation, int64_t tokens, int64_t features,
+                                      int64_t channels, const void *dh_dev, int64_t dh_row_stride, void *dgate_dev, void *dup_dev, int64_t d_row_stride, void *stream) {
+    come::MatmulArgs a = {};
+    const int rc = gated_common(a, x_dev, x_row_stride, gate_dev, gate_row_stride, up_dev, up_row_stride, gate_bias_dev, up_bias_dev, dtype, activation, tokens, features, channels);
+    if (rc != COME_OK || tokens == 0 || features == 0) return rc;
+    COME_REQUIRE(dh_dev && dh_row_stride >= 0 && dgate_dev && dup_dev && d_row_stride >= features, "dh and the two results must be given");
+    a.mode = come::kMatmulGatedGrad;
+    a.dh = dh_dev, a.dh_row = dh_row_stride;
+    a.out[0] = dgate_dev, a.out[1] = dup_dev;
+    a.out_row[0] = a.out_row[1] = d_row_stride;
+    return come::run_matmul(a, (cudaStream_t)stream);
+}
+
+extern "C" int come_gated_grad_input(const void *dgate_dev, const void *dup_dev, int64_t d_row_stride, const void *gate_dev, int64_t gate_row_stride, const void *up_dev,
+                                     int64_t up_row_stride, int dtype, int64_t tokens, int64_t features, int64_t channels, void *dx_dev, int64_t dx_row_stride,
+                                     void *stream) {
+    COME_REQUIRE_SIZES("come_gated_grad_input", tokens, channels, features);
+    COME_REQUIRE(come::is_16_bit(dtype), "the gated projections need float16 or bfloat16 (got dtype %d)", dtype);
+    if (tokens == 0 || channels == 0) return COME_OK;
+    COME_REQUIRE_ROWS("dgate", dgate_dev, d_row_stride, 2, features);
+    COME_REQUIRE_ROWS("dup", dup_dev, d_row_stride, 2, features);
+    COME_REQUIRE_ROWS("gate", gate_dev, gate_row_stride, 2, channels);
+    COME_REQUIRE_ROWS("up", up_dev, up_row_stride, 2, channels);
+    COME_REQUIRE(dx_dev && dx_row_stride >= channels, "dx must be given, with a row stride that holds its rows");
+    come::MatmulArgs a = {};
+    a.mode = come::kMatmulPlain;
+    a.dtype = a.out_dtype = dtype;
+    a.b_mn = true;
+    a.M = tokens, a.N = channels, a.K = features;
+    a.a[0] = dgate_dev, a.a[1] = dup_dev, a.a_row[0] = a.a_row[1] = d_row_stride;
+    a.b[0] = gate_dev, a.b_row[0] = gate_row_stride;
+    a.b[1] = up_dev, a.b_row[1] = up_row_stride;
+    a.sums = 2, a.problems = 1;
+    a.out[0] = dx_dev, a.out_row[0] = dx_row_stride;
+    return come::run_matmul(a, (cudaStream_t)stream);
+}
+
+extern "C" int come_gated_grad_weight(const void *dgate_dev, const void *dup_dev, int64_t d_row_stride, const void *x_dev, int64_t x_row_stride, int dtype, int64_t tokens,
+                                      int64_t features, int64_t channels, void *dgate_weight_dev, void *dup_weight_dev, int64_t dw_row_stride, void *stream) {
+    COME_REQUIRE_SIZES("come_gated_grad_weight", features, channels, tokens);
+    COME_REQUIRE(come::is_16_bit(dtype), "the gated projections need float16 or bfloat16 (got dtype %d)", dtype);
+    COME_REQUIRE(dgate_weight_dev || dup_weight_dev, "nothing to write");
+    if (features == 0 || channels == 0) return COME_OK;
+    COME_REQUIRE_ROWS("x", x_dev, x_row_stride, 2, channels);
+    COME_REQUIRE(dw_row_stride >= channels, "the row stride of the results must hold their rows");
+    come::MatmulArgs a = {};
+    a.mode = come::kMatmulPlain;
+    a.dtype = a.out_dtype = dtype;
+    a.a_mn = a.b_mn = true;
+    a.M = features, a.N = channels, a.K = tokens;
+    a.b[0] = x_dev, a.b_row[0] = x_row_stride;
+    a.sums = 1;
+    if (dgate_weight_dev) {
+        COME_REQUIRE_ROWS("dgate", dgate_dev, d_row_stride, 2, features);
+        a.a[a.problems] = dgate_dev, a.a_row[a.problems] = d_row_stride;
+        a.out[a.problems] = dgate_weight_dev, a.out_row[a.problems++] = dw_row_stride;
+    }
+    if (dup_weight_dev) {
+        COME_REQUIRE_ROWS("dup", dup_dev, d_row_stride, 2, features);
+        a.a[a.problems] = dup_dev, a.a_row[a.problems] = d_row_stride;
+        a.out[a.problems] = dup_weight_dev, a.out_row[a.problems++] = dw_row_stride;
+    }
+    return come::run_matmul(a, (cudaStream_t)stream);
+}
+
+extern "C" int come_gated_grad_bias(const void *dgate_dev, const void *dup_dev, int64_t d_row_stride, int dtype, int64_t tokens, int64_t features, void *dgate_bias_dev,
+                                    void *dup_bias_dev, void *stream) {
+    COME_REQUIRE(tokens >= 0 && features >= 0 && features < come::kMaxExtent, "bad sizes");
+    COME_REQUIRE(come::is_16_bit(dtype), "the gated projections need float16 or bfloat16 (got dtype %d)", dtype);
+    COME_REQUIRE(dgate_bias_dev || dup_bias_dev, "nothing to write");
+    if (features == 0) return COME_OK;
+    COME_REQUIRE(tokens == 0 || !dgate_bias_dev || (come::rows_ok(dgate_dev, d_row_stride, 2) && d_row_stride >= features), "dgate must be 16-byte aligned, with a row stride of whole 16 bytes");
+    COME_REQUIRE(tokens == 0 || !dup_bias_dev || (come::rows_ok(dup_dev, d_row_stride, 2) && d_row_stride >= features), "dup must be 16-byte aligned, with a row stride of whole 16 bytes");
+    const dim3 grid((unsigned)((features + 31) / 32), 2);
+    cudaStream_t st = (cudaStream_t)stream;
+    if (dtype == COME_F16)
+        come::column_sums_kernel<__half><<<grid, 256, 0, st>>>((const __half *)dgate_dev, (const __half *)dup_dev, d_row_stride, tokens, (int)features, (__half *)dgate_bias_dev, (__half *)dup_bias_dev);
+    else
+        come::column_sums_kernel<__nv_bfloat16><<<grid, 256, 0, st>>>((const __nv_bfloat16 *)dgate_dev, (const __nv_bfloat16 *)dup_dev, d_row_stride, tokens, (int)features,
+                                                                      (__nv_bfloat16 *)dgate_bias_dev, (__nv_bfloat16 *)dup_bias_dev);
+    return come::check_launch("come_gated_grad_bias");
+}

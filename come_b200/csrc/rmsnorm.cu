@@ -1,0 +1,310 @@
+// Residual add fused with the root-mean-square norm behind it, and the 8-bit quantisers of the block-scaled products.
+//
+//   x_out  = x + scale * branch                        (float32, rounded once to the stream's type)
+//   y      = x_out * rsqrt(mean(x_out^2) + eps) * weight   (float32, of the stream as it is stored)
+//   normed = y rounded to the stream's type, or
+//   q      = e4m3(y / s),  s = max(max|y|, 448 * 2^-126) / 448 over each 128 columns of a row
+//
+// Memory bound: both inputs are read once, both results written once.  A row is owned by one warp (many rows) or by a thread
+// group of several warps (few rows, where a row's latency counts, and wide rows, whose float32 copy would not fit one warp's
+// registers): thread i of the group holds the vectors i, i + group size, ... of the row, so the 128 columns of a scale always lie
+// in 16 (16-bit types) or 32 (float32) neighbouring lanes and their maximum needs shuffles only.
+#include "block_scale.cuh"
+
+namespace come {
+
+namespace {
+
+struct RmsNormArgs {
+    const void *x, *branch, *scale, *weight;
+    int64_t rows, x_row;  // row stride of x in elements; branch, x_out and normed are contiguous
+    int C;
+    float eps;
+    bool norm;            // off: quantise x as it is
+    void *x_out, *normed;
+    uint8_t *q;
+    int64_t q_row;
+    float *q_scale;
+    int64_t s_row, s_block;
+};
+
+// VEC elements of a row from column c on; kAligned: one 16-byte access, the row's width is a whole number of them.  kOnce: a
+// row that is read once, against the scale and weight vectors that every row reads.
+template <typename T, int VEC, bool kAligned, bool kOnce> __device__ __forceinline__ void load_row(const T *p, int c, int C, float (&v)[VEC]) {
+    if constexpr (kAligned) {
+        const uint4 raw = kOnce ? __ldcs(reinterpret_cast<const uint4 *>(p + c)) : __ldg(reinterpret_cast<const uint4 *>(p + c));
+        const T *e = reinterpret_cast<const T *>(&raw);
+#pragma unroll
+        for (int i = 0; i < VEC; ++i) v[i] = Elem<T>::to_f32(e[i]);
+    } else {
+#pragma unroll
+        for (int i = 0; i < VEC; ++i) v[i] = c + i < C ? Elem<T>::to_f32(p[c + i]) : 0.0f;
+    }
+}
+template <typename T, int VEC, bool kAligned> __device__ __forceinline__ void store_row(T *p, int c, int C, const float (&v)[VEC]) {
+    if constexpr (kAligned) {
+        uint4 raw;
+        T *e = reinterpret_cast<T *>(&raw);
+#pragma unroll
+        for (int i = 0; i < VEC; ++i) e[i] = Elem<T>::from_f32(v[i]);
+        __stcs(reinterpret_cast<uint4 *>(p + c), raw);
+    } else {
+#pragma unroll
+        for (int i = 0; i < VEC; ++i)
+            if (c + i < C) p[c + i] = Elem<T>::from_f32(v[i]);
+    }
+}
+
+template <int VEC> __device__ __forceinline__ void store_e4m3(uint8_t *p, int c, int C, const float (&v)[VEC], float inv) {
+    uint32_t w[VEC / 4];
+#pragma unroll
+    for (int i = 0; i < VEC / 4; ++i) w[i] = pack_e4m3(v[4 * i] * inv, v[4 * i + 1] * inv, v[4 * i + 2] * inv, v[4 * i + 3] * inv);
+    if (c + VEC <= C) {  // rows are stored with a stride of whole 16 bytes
+        if constexpr (VEC == 8) *reinterpret_cast<uint2 *>(p + c) = make_uint2(w[0], w[1]);
+        else *reinterpret_cast<uint32_t *>(p + c) = w[0];
+    } else {
+#pragma unroll
+        for (int i = 0; i < VEC; ++i)
+            if (c + i < C) p[c + i] = (uint8_t)(w[i / 4] >> (8 * (i & 3)));
+    }
+}
+
+// kWarps warps own a row; a CTA of kThreads threads holds kThreads / (32 * kWarps) of them.
+template <typename T, int kWarps, int NV, int kThreads, bool kAligned>
+__global__ void __launch_bounds__(kThreads) residual_rmsnorm_kernel(const RmsNormArgs a) {
+    constexpr int VEC = 16 / sizeof(T), kGroups = kThreads / (32 * kWarps), kSpan = 32 * kWarps * VEC;
+    __shared__ float part[kGroups][kWarps];
+    const int lane = threadIdx.x & 31, group = threadIdx.x / (32 * kWarps), warp = (threadIdx.x >> 5) % kWarps;
+    const int c0 = (warp * 32 + lane) * VEC, C = a.C;
+    const T *scale = (const T *)a.scale, *weight = (const T *)a.weight;
+    for (int64_t row = (int64_t)blockIdx.x * kGroups + group; row < a.rows; row += (int64_t)gridDim.x * kGroups) {
+        const T *x = (const T *)a.x + row * a.x_row;
+        float v[NV][VEC];
+#pragma unroll
+        for (int j = 0; j < NV; ++j) {
+            if (c0 + j * kSpan < C) load_row<T, VEC, kAligned, true>(x, c0 + j * kSpan, C, v[j]);
+            else
+#pragma unroll
+                for (int i = 0; i < VEC; ++i) v[j][i] = 0.0f;
+        }
+        if (a.branch) {
+            const T *branch = (const T *)a.branch + row * C;
+#pragma unroll
+            for (int j = 0; j < NV; ++j) {
+                const int c = c0 + j * kSpan;
+                if (c < C) {
+                    float b[VEC], g[VEC];
+                    load_row<T, VEC, kAligned, true>(branch, c, C, b);
+                    if (scale) {
+                        load_row<T, VEC, kAligned, false>(scale, c, C, g);
+#pragma unroll
+                        for (int i = 0; i < VEC; ++i) b[i] = fmaf(b[i], g[i], v[j][i]);
+                    } else {
+#pragma unroll
+                        for (int i = 0; i < VEC; ++i) b[i] += v[j][i];
+                    }
+                    // the norm is that of the stream as the next block reads it
+#pragma unroll
+                    for (int i = 0; i < VEC; ++i) v[j][i] = Elem<T>::to_f32(Elem<T>::from_f32(b[i]));
+                    if (a.x_out) store_row<T, VEC, kAligned>((T *)a.x_out + row * C, c, C, v[j]);
+                }
+            }
+        }
+        if (!a.normed && !a.q) continue;
+        if (a.norm) {
+            float sum = 0.0f;
+#pragma unroll
+            for (int j = 0; j < NV; ++j)
+#pragma unroll
+                for (int i = 0; i < VEC; ++i) sum = fmaf(v[j][i], v[j][i], sum);
+#pragma unroll
+            for (int m = 16; m >= 1; m >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, m);
+            if constexpr (kWarps > 1) {  // one group per CTA: a whole-CTA barrier
+                static_assert(kGroups == 1, "the barrier below is the CTA's");
+                if (lane == 0) part[0][warp] = sum;
+                __syncthreads();
+                sum = 0.0f;
+#pragma unroll
+                for (int w = 0; w < kWarps; ++w) sum += part[0][w];
+                __syncthreads();
+            }
+            const float rstd = 1.0f / sqrtf(sum / (float)C + a.eps);
+#pragma unroll
+            for (int j = 0; j < NV; ++j) {
+                const int c = c0 + j * kSpan;
+                if (c < C) {
+                    float w[VEC];
+                    if (weight) load_row<T, VEC, kAligned, false>(weight, c, C, w);
+#pragma unroll
+                    for (int i = 0; i < VEC; ++i) v[j][i] = weight ? v[j][i] * rstd * w[i] : v[j][i] * rstd;
+                }
+            }
+        }
+        if (a.normed) {
+#pragma unroll
+            for (int j = 0; j < NV; ++j)
+                if (c0 + j * kSpan < C) store_row<T, VEC, kAligned>((T *)a.normed + row * C, c0 + j * kSpan, C, v[j]);
+        } else {
+#pragma unroll
+            for (int j = 0; j < NV; ++j) {
+                const int c = c0 + j * kSpan;
+                float top = 0.0f;
+#pragma unroll
+                for (int i = 0; i < VEC; ++i) top = fmaxf(top, fabsf(v[j][i]));
+#pragma unroll
+                for (int m = kScaleBlock / VEC / 2; m >= 1; m >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, m));
+                top = fmaxf(top, kSmallestMax);
+                if (c < C) {
+                    store_e4m3<VEC>(a.q + row * a.q_row, c, C, v[j], kE4m3Max / top);
+                    if (c % kScaleBlock == 0) a.q_scale[row * a.s_row + (c / kScaleBlock) * a.s_block] = top / kE4m3Max;
+                }
+            }
+        }
+    }
+}
+
+template <typename T, bool kAligned> int launch_rmsnorm(const RmsNormArgs &a, cudaStream_t st) {
+    constexpr int VEC = 16 / sizeof(T);
+    const int vectors = (a.C + VEC - 1) / VEC;
+    const int64_t sms = sm_count();
+    const auto grid = [&](int64_t blocks, int64_t per_sm) { return (unsigned)(blocks < sms * per_sm ? blocks : sms * per_sm); };
+#define COME_RMS_LAUNCH(WARPS, NV, THREADS, PER_SM)                                                                       \
+    residual_rmsnorm_kernel<T, WARPS, NV, THREADS, kAligned>                                                              \
+        <<<grid((a.rows * WARPS * 32 + THREADS - 1) / THREADS, PER_SM), THREADS, 0, st>>>(a)
+    if (vectors > 4 * 128 || (a.rows <= 4 * sms && vectors > 32)) {
+        if (vectors <= 128) COME_RMS_LAUNCH(4, 1, 128, 16);
+        else if (vectors <= 256) COME_RMS_LAUNCH(8, 1, 256, 8);
+        else if (vectors <= 512) COME_RMS_LAUNCH(8, 2, 256, 6);
+        else if (vectors <= 1024) COME_RMS_LAUNCH(8, 4, 256, 4);
+        else if (vectors <= 2048) COME_RMS_LAUNCH(8, 8, 256, 2);
+        else {
+            set_error("come_residual_rmsnorm: rows of at most %d elements of this type (got %d)", 2048 * VEC, a.C);
+            return COME_ERR_UNSUPPORTED;
+        }
+    } else if (vectors <= 32) COME_RMS_LAUNCH(1, 1, 128, 16);
+    else if (vectors <= 64) COME_RMS_LAUNCH(1, 2, 128, 12);
+    else if (vectors <= 128) COME_RMS_LAUNCH(1, 4, 128, 8);
+    else if (vectors <= 256) COME_RMS_LAUNCH(1, 8, 128, 5);
+    else COME_RMS_LAUNCH(4, 4, 128, 8);
+#undef COME_RMS_LAUNCH
+    return check_launch("come_residual_rmsnorm");
+}
+
+template <typename T> int dispatch_rmsnorm(const RmsNormArgs &a, cudaStream_t st) {
+    constexpr int VEC = 16 / sizeof(T);
+    const auto al = [](const void *p) { return (uintptr_t)p % 16 == 0; };
+    const bool aligned = a.C % VEC == 0 && a.x_row % VEC == 0 && al(a.x) && al(a.branch) && al(a.scale) && al(a.weight) && al(a.x_out) && al(a.normed);
+    return aligned ? launch_rmsnorm<T, true>(a, st) : launch_rmsnorm<T, false>(a, st);
+}
+
+// One CTA per 128 x 128 block of a weight.
+template <typename T>
+__global__ void __launch_bounds__(256) quantize_weight_kernel(const T *__restrict__ w, int64_t w_row, int rows, int C, uint8_t *__restrict__ q,
+                                                              int64_t q_row, float *__restrict__ q_scale, int64_t s_row) {
+    __shared__ float tops[8];
+    const int r0 = blockIdx.y * kScaleBlock, c0 = blockIdx.x * kScaleBlock;
+    const int r_end = min(rows, r0 + kScaleBlock), c = c0 + (threadIdx.x & 127);
+    float top = 0.0f;
+    if (c < C)
+        for (int r = r0 + (threadIdx.x >> 7); r < r_end; r += 2) top = fmaxf(top, fabsf(Elem<T>::to_f32(w[r * w_row + c])));
+#pragma unroll
+    for (int m = 16; m >= 1; m >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, m));
+    if ((threadIdx.x & 31) == 0) tops[threadIdx.x >> 5] = top;
+    __syncthreads();
+    top = kSmallestMax;
+#pragma unroll
+    for (int i = 0; i < 8; ++i) top = fmaxf(top, tops[i]);
+    if (threadIdx.x == 0) q_scale[blockIdx.y * s_row + blockIdx.x] = top / kE4m3Max;
+    const float inv = kE4m3Max / top;
+    if (c < C)
+        for (int r = r0 + (threadIdx.x >> 7); r < r_end; r += 2)
+            q[r * q_row + c] = __nv_cvt_float_to_fp8(Elem<T>::to_f32(w[r * w_row + c]) * inv, __NV_SATFINITE, __NV_E4M3);
+}
+
+int run_rmsnorm(const RmsNormArgs &a, int dtype, cudaStream_t st) {
+    switch (dtype) {
+        case COME_F32: return dispatch_rmsnorm<float>(a, st);
+        case COME_F16: return dispatch_rmsnorm<__half>(a, st);
+        default: return dispatch_rmsnorm<__nv_bfloat16>(a, st);
+    }
+}
+
+}  // namespace
+
+}  // namespace come
+
+extern "C" int come_residual_rmsnorm(const void *x_dev, const void *branch_dev, const void *scale_dev, int64_t rows, int64_t channels, int dtype,
+                                     const void *weight_dev, float eps, void *x_out_dev, void *normed_dev, void *q_dev, int64_t q_row_stride,
+                                     float *q_scale_dev, int64_t q_scale_row_stride, int64_t q_scale_block_stride, void *stream) {
+    COME_REQUIRE(rows >= 0 && channels >= 0, "rows and channels must be >= 0");
+    COME_REQUIRE(dtype == COME_F32 || dtype == COME_F16 || dtype == COME_BF16, "unknown dtype %d", dtype);
+    COME_REQUIRE(rows < (1ll << 31) && channels < (1ll << 31), "rows and channels must fit int32");
+    if (rows == 0 || channels == 0) return COME_OK;
+    COME_REQUIRE(x_dev != nullptr, "x must not be NULL");
+    COME_REQUIRE(branch_dev || !scale_dev, "scale without a branch");
+    COME_REQUIRE(!x_out_dev || branch_dev, "x_out without a branch");
+    COME_REQUIRE(!normed_dev || !q_dev, "the norm is written once: in the stream's type or in 8 bits");
+    COME_REQUIRE(normed_dev || q_dev || x_out_dev, "nothing to write");
+    COME_REQUIRE(!q_dev || (q_scale_dev && q_row_stride >= channels && q_row_stride % 16 == 0 && (uintptr_t)q_dev % 16 == 0),
+                 "an 8-bit result needs its scales, 16-byte aligned rows and a row stride of whole 16 bytes");
+    come::RmsNormArgs a = {};
+    a.x = x_dev;
+    a.branch = branch_dev;
+    a.scale = scale_dev;
+    a.weight = weight_dev;
+    a.rows = rows;
+    a.x_row = channels;
+    a.C = (int)channels;
+    a.eps = eps;
+    a.norm = normed_dev || q_dev;
+    a.x_out = x_out_dev;
+    a.normed = normed_dev;
+    a.q = (uint8_t *)q_dev;
+    a.q_row = q_row_stride;
+    a.q_scale = q_scale_dev;
+    a.s_row = q_scale_row_stride;
+    a.s_block = q_scale_block_stride;
+    return come::run_rmsnorm(a, dtype, (cudaStream_t)stream);
+}
+
+extern "C" int come_quantize_rows(const void *x_dev, int dtype, int64_t rows, int64_t channels, int64_t x_row_stride, void *q_dev, int64_t q_row_stride,
+                                  float *q_scale_dev, int64_t q_scale_row_stride, int64_t q_scale_block_stride, void *stream) {
+    COME_REQUIRE(rows >= 0 && channels >= 0, "rows and channels must be >= 0");
+    COME_REQUIRE(dtype == COME_F32 || dtype == COME_F16 || dtype == COME_BF16, "unknown dtype %d", dtype);
+    COME_REQUIRE(rows < (1ll << 31) && channels < (1ll << 31), "rows and channels must fit int32");
+    if (rows == 0 || channels == 0) return COME_OK;
+    COME_REQUIRE(x_dev && q_dev && q_scale_dev, "x, q and q_scale must not be NULL");
+    COME_REQUIRE(x_row_stride >= 0, "x_row_stride must not be negative");
+    COME_REQUIRE(q_row_stride >= channels && q_row_stride % 16 == 0 && (uintptr_t)q_dev % 16 == 0, "q needs 16-byte aligned rows and a row stride of whole 16 bytes");
+    come::RmsNormArgs a = {};
+    a.x = x_dev;
+    a.rows = rows;
+    a.x_row = x_row_stride;
+    a.C = (int)channels;
+    a.q = (uint8_t *)q_dev;
+    a.q_row = q_row_stride;
+    a.q_scale = q_scale_dev;
+    a.s_row = q_scale_row_stride;
+    a.s_block = q_scale_block_stride;
+    return come::run_rmsnorm(a, dtype, (cudaStream_t)stream);
+}
+
+extern "C" int come_quantize_weight(const void *w_dev, int dtype, int64_t rows, int64_t channels, int64_t w_row_stride, void *q_dev, int64_t q_row_stride,
+                                    float *q_scale_dev, int64_t q_scale_row_stride, void *stream) {
+    COME_REQUIRE(rows >= 0 && channels >= 0, "rows and channels must be >= 0");
+    COME_REQUIRE(dtype == COME_F32 || dtype == COME_F16 || dtype == COME_BF16, "unknown dtype %d", dtype);
+    COME_REQUIRE(rows < (1ll << 23) && channels < (1ll << 31) - come::kScaleBlock, "at most 2^23 rows, and channels must fit int32");
+    if (rows == 0 || channels == 0) return COME_OK;
+    COME_REQUIRE(w_dev && q_dev && q_scale_dev, "w, q and q_scale must not be NULL");
+    COME_REQUIRE(w_row_stride >= 0 && q_row_stride >= channels && q_scale_row_stride >= 0, "bad strides");
+    const dim3 grid((unsigned)((channels + come::kScaleBlock - 1) / come::kScaleBlock), (unsigned)((rows + come::kScaleBlock - 1) / come::kScaleBlock));
+    cudaStream_t st = (cudaStream_t)stream;
+#define COME_QW_LAUNCH(T)                                                                                                              \
+    come::quantize_weight_kernel<T><<<grid, 256, 0, st>>>((const T *)w_dev, w_row_stride, (int)rows, (int)channels, (uint8_t *)q_dev, \
+                                                          q_row_stride, q_scale_dev, q_scale_row_stride)
+    if (dtype == COME_F32) COME_QW_LAUNCH(float);
+    else if (dtype == COME_F16) COME_QW_LAUNCH(__half);
+    else COME_QW_LAUNCH(__nv_bfloat16);
+#undef COME_QW_LAUNCH
+    return come::check_launch("come_quantize_weight");
+}

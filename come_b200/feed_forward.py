@@ -1,0 +1,129 @@
+"""The gated feed-forward block: ``act(x Wg^T + bg) * (x Wu^T + bu)`` in one kernel, with its backward pass.
+
+:func:`gated_linear` is the operator, :class:`GatedMlp` the module of a block (``block.mlp``), with the parameter layout of the gated
+MLPs of visual transformers: ``w12`` holds both projections, the gate's rows first, ``w3`` the projection back.
+
+A training step keeps only its inputs: the backward pass computes the projections again, in float32, and with them their gradients
+(one kernel, ``come_gated_matmul_grad``), then ``dx = dg Wg + du Wu`` and ``dW = dg^T x`` / ``du^T x``.  ``dg`` and ``du`` are rounded to the
+tokens' type once, as operands of these products; saved 16-bit projections would add their own rounding to every gradient.
+"""
+from __future__ import annotations
+
+from typing import Optional
+
+import torch
+
+from . import _lib
+from ._torch_util import dtype_code, on_device, ptr, require_cuda, stream_ptr
+from .block_scaled import activation_code
+
+__all__ = ["gated_linear", "GatedMlp"]
+
+
+def _operand(t: torch.Tensor) -> torch.Tensor:
+    """``t [rows, C]`` as the tensor cores can read it: rows that are contiguous and start at multiples of 16 bytes (copied if not)."""
+    if t.stride(1) == 1 and t.stride(0) % 8 == 0 and t.stride(0) >= t.shape[1] and t.data_ptr() % 16 == 0:
+        return t
+    return t.clone(memory_format=torch.contiguous_format)
+
+
+def _padded(rows: int, cols: int, like: torch.Tensor) -> torch.Tensor:
+    return torch.empty((rows, -(-cols // 8) * 8), dtype=like.dtype, device=like.device)[:, :cols]
+
+
+class _GatedLinear(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, x, w_gate, w_up, b_gate, b_up, act):
+        tokens, cols = x.shape
+        features, dev = w_gate.shape[0], x.device
+        xo, wg, wu = _operand(x), _operand(w_gate), _operand(w_up)
+        out = torch.empty((tokens, features), dtype=x.dtype, device=dev)
+        with on_device(dev):
+            _lib.check(_lib.lib().come_gated_matmul(xo.data_ptr(), xo.stride(0), wg.data_ptr(), wg.stride(0), wu.data_ptr(), wu.stride(0), ptr(b_gate),
+                                                    ptr(b_up), dtype_code(x.dtype), act, tokens, features, cols, out.data_ptr(), features,
+                                                    stream_ptr(dev)))
+        ctx.act = act
+        ctx.save_for_backward(x, w_gate, w_up, b_gate, b_up)
+        return out
+
+    @staticmethod
+    @torch.autograd.function.once_differentiable
+    def backward(ctx, dh):
+        x, w_gate, w_up, b_gate, b_up = ctx.saved_tensors
+        need_x, need_wg, need_wu, need_bg, need_bu = ctx.needs_input_grad[:5]
+        tokens, cols = x.shape
+        features, dev, lib = w_gate.shape[0], x.device, _lib.lib()
+        dx = torch.empty((tokens, cols), dtype=x.dtype, device=dev) if need_x else None
+        dwg, dwu, dbg, dbu = (torch.empty(shape, dtype=x.dtype, device=dev) if need else None
+                              for need, shape in ((need_wg, (features, cols)), (need_wu, (features, cols)), (need_bg, (features,)), (need_bu, (features,))))
+        if tokens == 0 or features == 0:
+            for t in (dx, dwg, dwu, dbg, dbu):
+                if t is not None:
+                    t.zero_()
+            return dx, dwg, dwu, dbg, dbu, None
+        xo, wg, wu = _operand(x), _operand(w_gate), _operand(w_up)
+        if dh.stride(1) != 1 and features > 1:
+            dh = dh.contiguous()
+        code = dtype_code(x.dtype)
+        dg, du = _padded(tokens, features, x), _padded(tokens, features, x)
+        d_row = dg.stride(0)
+        with on_device(dev):
+            st = stream_ptr(dev)
+            _lib.check(lib.come_gated_matmul_grad(xo.data_ptr(), xo.stride(0), wg.data_ptr(), wg.stride(0), wu.data_ptr(), wu.stride(0), ptr(b_gate), ptr(b_up),
+                                                  code, ctx.act, tokens, features, cols, dh.data_ptr(), dh.stride(0), dg.data_ptr(), du.data_ptr(),
+                                                  d_row, st))
+            if need_x:
+                _lib.check(lib.come_gated_grad_input(dg.data_ptr(), du.data_ptr(), d_row, wg.data_ptr(), wg.stride(0), wu.data_ptr(), wu.stride(0), code,
+                                                     tokens, features, cols, dx.data_ptr(), cols, st))
+            if need_wg or need_wu:
+                _lib.check(lib.come_gated_grad_weight(dg.data_ptr(), du.data_ptr(), d_row, xo.data_ptr(), xo.stride(0), code, tokens, features, cols,
+                                                      ptr(dwg), ptr(dwu), cols, st))
+            if need_bg or need_bu:
+                _lib.check(lib.come_gated_grad_bias(dg.data_ptr(), du.data_ptr(), d_row, code, tokens, features, ptr(dbg), ptr(dbu), st))
+        return dx, dwg, dwu, dbg, dbu, None
+
+
+def gated_linear(x: torch.Tensor, w_gate: torch.Tensor, w_up: torch.Tensor, b_gate: Optional[torch.Tensor] = None,
+                 b_up: Optional[torch.Tensor] = None, activation: str = "silu") -> torch.Tensor:
+    """``act(x @ w_gate.T + b_gate) * (x @ w_up.T + b_up)`` in one kernel, differentiable once in every tensor.
+
+    ``x [..., C]`` float16 or bfloat16, ``w_gate`` / ``w_up [F, C]`` and ``b_gate`` / ``b_up [F]`` in its dtype; ``C`` a multiple of 8.
+    ``activation``: "silu" or "gelu" (the exact one).  Sums in float32, the result rounded once.  Rows that are not contiguous or do
+    not start at multiples of 16 bytes are copied first."""
+    require_cuda(x, "x")
+    act, dev = activation_code(activation), x.device
+    if x.dtype not in (torch.float16, torch.bfloat16):
+        raise RuntimeError(f"x: unsupported dtype {x.dtype}; expected float16 or bfloat16")
+    cols = x.shape[-1] if x.dim() else 0
+    if w_gate.dim() != 2 or w_gate.shape[1] != cols or w_up.shape != w_gate.shape:
+        raise ValueError(f"w_gate and w_up must be [F, {cols}], got {tuple(w_gate.shape)} and {tuple(w_up.shape)}")
+    if cols == 0 or cols % 8 != 0:
+        raise NotImplementedError(f"gated_linear needs a channel count that is a multiple of 8, got {cols}")
+    features = w_gate.shape[0]
+    for name, t, shape in (("w_gate", w_gate, (features, cols)), ("w_up", w_up, (features, cols)), ("b_gate", b_gate, (features,)), ("b_up", b_up, (features,))):
+        if t is None:
+            continue
+        if t.dtype != x.dtype or t.device != dev or tuple(t.shape) != shape:
+            raise ValueError(f"{name} must be {list(shape)} {x.dtype} on {dev}, got {list(t.shape)} {t.dtype} on {t.device}")
+    b_gate, b_up = (b if b is None else b.contiguous() for b in (b_gate, b_up))
+    if x.dim() == 2:
+        return _GatedLinear.apply(x, w_gate, w_up, b_gate, b_up, act)
+    return _GatedLinear.apply(x.reshape(-1, cols), w_gate, w_up, b_gate, b_up, act).view(*x.shape[:-1], features)
+
+
+class GatedMlp(torch.nn.Module):
+    """``w3(act(gate) * up)`` with ``gate, up = w12(x).chunk(2)``: the gated MLP of a block.  The two projections, the activation and the
+    product are one kernel; ``w3`` stays a PyTorch GEMM like the other linear layers of the blocks.  In 8 bits:
+    :class:`come_b200.block_scaled.BlockScaledGatedMlp`."""
+
+    def __init__(self, dim: int, hidden: int, bias: bool = True, activation: str = "silu"):
+        super().__init__()
+        activation_code(activation)
+        self.activation = activation
+        self.w12 = torch.nn.Linear(dim, 2 * hidden, bias=bias)
+        self.w3 = torch.nn.Linear(hidden, dim, bias=bias)
+
+    def forward(self, x: torch.Tensor) -> torch.Tensor:
+        w_gate, w_up = self.w12.weight.chunk(2)
+        b_gate, b_up = (None, None) if self.w12.bias is None else self.w12.bias.chunk(2)
+        return self.w3(gated_linear(x, w_gate, w_up, b_gate, b_up, self.activation))

@@ -26,6 +26,8 @@ extern "C" {
 #define COME_B200_VERSION 100
 
 enum { COME_F32 = 0, COME_F16 = 1, COME_BF16 = 2 };
+enum { COME_E4M3 = 3 };                       /* results only: 8-bit numbers with their scales beside them */
+enum { COME_ACT_SILU = 0, COME_ACT_GELU = 1 }; /* g / (1 + e^-g);  g Phi(g) */
 
 enum {
     COME_OK = 0,
@@ -354,6 +356,68 @@ int come_packed_positions(const uint8_t *mask_dev, const int64_t *rev_id_dev, in
                           const come_layout_t *layout, int64_t *pos_out_dev, void *stream);
 
 /*
+ * The feed-forward half of a block in 8 and 16 bits.  No counterpart in the reference, whose MLPs are PyTorch modules.
+ *
+ * 8-bit tensors are float8 e4m3 numbers with float32 scales, value = number * scale: tokens with one scale per row and 128
+ * columns (x_scale[row * row_stride + block * block_stride]), weights [features, channels] with one per 128 x 128 block
+ * (w_scale[row_block * row_stride + block]).  The last blocks of a row or of a weight may be partial.  A scale is the block's
+ * largest magnitude / 448, that of a block without any (or with less than 448 * 2^-126) the smallest normal number; an infinity
+ * makes its block NaN, a NaN only itself.  Row strides are in elements.  Rows of operands start at multiples of 16 bytes.
+ *
+ * come_residual_rmsnorm   x_out = x + scale * branch (float32, rounded once; branch and scale may be NULL) and the root-mean-square
+ *   norm of that stream as it is stored, x_out * rsqrt(mean(x_out^2) + eps) * weight (weight may be NULL), to normed in dtype or to
+ *   q / q_scale in 8 bits.  x, branch, x_out, normed [rows, channels] contiguous, scale / weight [channels], all in dtype; x_out may be
+ *   x or branch.  Rows of up to 2048 16-byte vectors (16,384 16-bit or 8192 float32 channels).
+ * come_quantize_rows      rows in float32 / float16 / bfloat16 -> tokens in 8 bits.
+ * come_quantize_weight    a weight -> 8 bits.
+ * come_matmul_e4m3        out[t, n] = sum over blocks k of x_scale[t, k] w_scale[n / 128, k] (sum_j x[t, j] w[n, j]) + bias[n]; bias float32 or
+ *   NULL; out in out_dtype (COME_F32 / COME_F16 / COME_BF16).  Sums in float32.
+ * come_gated_matmul_e4m3  out[t, f] = act(x gate^T + gate_bias) * (x up^T + up_bias), in 16 bits or (COME_E4M3) in 8 bits with out_scale,
+ *   the form of the next product's x.
+ * come_gated_matmul       the same with operands, biases and result in float16 or bfloat16.
+ * come_gated_matmul_grad  the projections again, in float32, and the gradients of theirs, dgate = dh up act'(gate), dup = dh act(gate),
+ *   rounded to dtype: what a training step keeps of the forward pass is its inputs.
+ * come_gated_grad_input   dx = dgate gate + dup up.
+ * come_gated_grad_weight  dgate_weight = dgate^T x, dup_weight = dup^T x (either may be NULL).
+ * come_gated_grad_bias    column sums of dgate, dup (either result may be NULL).
+ *
+ * Results are the same bits in every run.  While bits 19-21 of the device status word are raised, the products return at once without
+ * touching their outputs.
+ */
+int come_residual_rmsnorm(const void *x_dev, const void *branch_dev, const void *scale_dev, int64_t rows, int64_t channels, int dtype,
+                          const void *weight_dev, float eps, void *x_out_dev, void *normed_dev, void *q_dev, int64_t q_row_stride,
+                          float *q_scale_dev, int64_t q_scale_row_stride, int64_t q_scale_block_stride, void *stream);
+int come_quantize_rows(const void *x_dev, int dtype, int64_t rows, int64_t channels, int64_t x_row_stride, void *q_dev,
+                       int64_t q_row_stride, float *q_scale_dev, int64_t q_scale_row_stride, int64_t q_scale_block_stride, void *stream);
+int come_quantize_weight(const void *w_dev, int dtype, int64_t rows, int64_t channels, int64_t w_row_stride, void *q_dev,
+                         int64_t q_row_stride, float *q_scale_dev, int64_t q_scale_row_stride, void *stream);
+int come_matmul_e4m3(const void *x_dev, int64_t x_row_stride, const float *x_scale_dev, int64_t x_scale_row_stride,
+                     int64_t x_scale_block_stride, const void *w_dev, int64_t w_row_stride, const float *w_scale_dev,
+                     int64_t w_scale_row_stride, const float *bias_dev, int64_t tokens, int64_t features, int64_t channels,
+                     void *out_dev, int64_t out_row_stride, int out_dtype, void *stream);
+int come_gated_matmul_e4m3(const void *x_dev, int64_t x_row_stride, const float *x_scale_dev, int64_t x_scale_row_stride,
+                           int64_t x_scale_block_stride, const void *gate_dev, int64_t gate_row_stride, const float *gate_scale_dev,
+                           int64_t gate_scale_row_stride, const void *up_dev, int64_t up_row_stride, const float *up_scale_dev,
+                           int64_t up_scale_row_stride, const float *gate_bias_dev, const float *up_bias_dev, int activation,
+                           int64_t tokens, int64_t features, int64_t channels, void *out_dev, int64_t out_row_stride, int out_dtype,
+                           float *out_scale_dev, int64_t out_scale_row_stride, int64_t out_scale_block_stride, void *stream);
+int come_gated_matmul(const void *x_dev, int64_t x_row_stride, const void *gate_dev, int64_t gate_row_stride, const void *up_dev,
+                      int64_t up_row_stride, const void *gate_bias_dev, const void *up_bias_dev, int dtype, int activation,
+                      int64_t tokens, int64_t features, int64_t channels, void *out_dev, int64_t out_row_stride, void *stream);
+int come_gated_matmul_grad(const void *x_dev, int64_t x_row_stride, const void *gate_dev, int64_t gate_row_stride, const void *up_dev,
+                           int64_t up_row_stride, const void *gate_bias_dev, const void *up_bias_dev, int dtype, int activation,
+                           int64_t tokens, int64_t features, int64_t channels, const void *dh_dev, int64_t dh_row_stride,
+                           void *dgate_dev, void *dup_dev, int64_t d_row_stride, void *stream);
+int come_gated_grad_input(const void *dgate_dev, const void *dup_dev, int64_t d_row_stride, const void *gate_dev,
+                          int64_t gate_row_stride, const void *up_dev, int64_t up_row_stride, int dtype, int64_t tokens,
+                          int64_t features, int64_t channels, void *dx_dev, int64_t dx_row_stride, void *stream);
+int come_gated_grad_weight(const void *dgate_dev, const void *dup_dev, int64_t d_row_stride, const void *x_dev, int64_t x_row_stride,
+                           int dtype, int64_t tokens, int64_t features, int64_t channels, void *dgate_weight_dev,
+                           void *dup_weight_dev, int64_t dw_row_stride, void *stream);
+int come_gated_grad_bias(const void *dgate_dev, const void *dup_dev, int64_t d_row_stride, int dtype, int64_t tokens,
+                         int64_t features, void *dgate_bias_dev, void *dup_bias_dev, void *stream);
+
+/*
  * Device status word: kernels that wait on hardware barriers give up after a bounded number of polls and
  * record a non-zero code here instead of hanging.  Reads it back (synchronises the device) and optionally
  * clears it.  Returns COME_OK with *value == 0 when no kernel reported a problem, COME_ERR_DEVICE with the word in
@@ -361,7 +425,7 @@ int come_packed_positions(const uint8_t *mask_dev, const int64_t *rev_id_dev, in
  * 0-8) or its tensor memory was not at column 0 (bit 9); while the word is raised, attention launches return at once without
  * touching their outputs.  Bit 15: the wait self-test below; bit 16: a
  * position outside the rotary table was clamped by come_qkv_prepare; bit 17: a wait of the bulk-copy merge kernel ran out;
- * bit 18: come_peer_wait gave up.
+ * bit 18: come_peer_wait gave up; bits 19-21: a wait of a product kernel of the feed-forward half ran out.
  */
 int come_device_status(uint32_t *value, int clear);
 
