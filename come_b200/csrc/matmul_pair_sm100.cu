@@ -1,0 +1,620 @@
+// Products of the feed-forward half of a block on Blackwell tensor cores (sm_100a): the kernel for results with many tiles.
+//
+// Persistent: one pair of CTAs (two SMs, tcgen05 cta_group::2) per 256 x 256 tile of sums (256 rows x 128 columns of both projections in
+// the gated forms), tiles dealt to the pairs in turn.  CTA c of a pair holds rows [128 c, + 128) of A, half of B (columns [128 c, + 128), or
+// the gate's / the up projection's weight) and the sums of its rows.
+//
+//   warps 0-7 : two epilogue warpgroups of 128 rows each, columns [0, 128) / [128, 256) of the tile, or in the gated forms columns [0, 64) /
+//               [64, 128) of both projections, so that gate and up of an element meet in one thread.  8-bit operands: every K block of
+//               128 is a product of its own in one of two TMEM buffers, scaled and added to float32 registers (two sums per instruction)
+//               while the tensor cores fill the other.  16-bit operands: a tile's sums stay in TMEM; the two buffers let the next tile
+//               begin under this one's epilogue.  Results are staged in 4 KB of shared memory per warp and leave as whole 128-byte rows.
+//   warp 8    : producer (TMA ring, one per CTA; the loads of both CTAs complete on the first CTA's barriers).
+//   warp 9    : MMA issuer (first CTA only).
+//
+// Why pairs: a 128 x 256 tile of one CTA reads 12 KB of shared memory per 128 x 256 x 32-byte step and TMA writes as much again, more than
+// the 128 bytes per clock of an SM let pass in the step's 128 clocks; in a pair each SM holds half of B.
+//
+// Every wait is bounded as in matmul_sm100.cu: after one gave up, the CTA's roles go on without acting, its abort flag keeps it from
+// storing, and the pair meets at the last cluster barrier.
+#include "matmul_sm100.cuh"
+
+#include <type_traits>
+
+namespace come {
+
+namespace {
+
+constexpr int kProducerWarp = 8, kIssuerWarp = 9, kThreads = 384;  // three warpgroups; warps 10 and 11 only keep the third whole
+constexpr int kPairN = 256;                         // columns of sums per tile
+constexpr int kStageBytes = 2 * kOperandBytes;      // 128 rows of A and of B
+constexpr int kStages = 6;
+constexpr int kRingBytes = kStages * kStageBytes;
+constexpr int kStagingBytes = 4096;                 // per epilogue warp: 32 rows of 128 bytes
+constexpr uint32_t kTmemCols = 512;
+
+struct PairBarriers {
+    uint64_t full[kStages], empty[kStages];  // full: of the first CTA, for both
+    uint64_t acc_full[2], acc_empty[2];      // acc_empty: of the first CTA, for both
+    uint64_t drained;
+    uint32_t tmem_base;
+    volatile uint32_t abort_flag;
+    union {
+        float top[2][2][kTile];              // 8 bits: [tile parity][warpgroup][row], largest |h| of a row's columns
+        alignas(16) uint16_t bias[8][128];   // 16 bits: [warp], of its 64 columns of the gate and of the up projection
+    };
+};
+constexpr size_t kSmemBytes = kRingBytes + 8 * kStagingBytes + sizeof(PairBarriers);
+static_assert(kSmemBytes <= 227 * 1024, "");
+
+// ---- PTX of the pair ------------------------------------------------------------------------------------------------------
+__device__ __forceinline__ void tma_load_2d_pair(uint32_t dst, const CUtensorMap *map, int x, int y, uint32_t bar) {
+    asm volatile("cp.async.bulk.tensor.2d.shared::cluster.global.mbarrier::complete_tx::bytes.cta_group::2 [%0], [%1, {%2, %3}], [%4];"
+                 ::"r"(dst), "l"(map), "r"(x), "r"(y), "r"(bar) : "memory");
+}
+template <bool kE4m3> __device__ __forceinline__ void tc_mma_pair(uint32_t d_tmem, uint64_t a_desc, uint64_t b_desc, uint32_t idesc, uint32_t accumulate) {
+    if constexpr (kE4m3)
+        asm volatile("{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %4, 0;\n\ttcgen05.mma.cta_group::2.kind::f8f6f4 [%0], %1, %2, %3, p;\n\t}"
+                     ::"r"(d_tmem), "l"(a_desc), "l"(b_desc), "r"(idesc), "r"(accumulate) : "memory");
+    else
+        asm volatile("{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %4, 0;\n\ttcgen05.mma.cta_group::2.kind::f16 [%0], %1, %2, %3, p;\n\t}"
+                     ::"r"(d_tmem), "l"(a_desc), "l"(b_desc), "r"(idesc), "r"(accumulate) : "memory");
+}
+// Arrives at the barrier of the same offset in both CTAs when all products issued so far have completed.
+__device__ __forceinline__ void tc_commit_pair(uint64_t *bar) {
+    asm volatile("tcgen05.commit.cta_group::2.mbarrier::arrive::one.shared::cluster.multicast::cluster.b64 [%0], %1;" ::"r"(smem_u32(bar)), "h"((uint16_t)3) : "memory");
+}
+__device__ __forceinline__ void mbar_arrive_at(uint32_t cluster_addr) {
+    asm volatile("mbarrier.arrive.shared::cluster.b64 _, [%0];" ::"r"(cluster_addr) : "memory");
+}
+
+// ---- staged rows ------------------------------------------------------------------------------------------------------------
+// A warp's 32 rows of up to 128 bytes; 16-byte chunk c of row r lies at chunk c ^ (r & 7), so that both a thread writing its row and
+// eight lanes reading one row touch all banks.
+__device__ __forceinline__ uint4 *staged(uint8_t *base, int row, int chunk) { return reinterpret_cast<uint4 *>(base + row * 128 + ((chunk ^ (row & 7)) * 16)); }
+
+// Rows [0, rows) x columns [0, cols) of elements of `kSize` bytes, `kRowBytes` staged per row, to out (row stride in bytes).
+template <int kSize, int kRowBytes> __device__ __forceinline__ void store_staged(uint8_t *base, uint8_t *out, int64_t row_bytes, int rows, int cols, int lane) {
+    constexpr int kChunks = kRowBytes / 16, kRowsAtOnce = 32 / kChunks, kPerChunk = 16 / kSize;
+    if (rows <= 0 || cols <= 0) return;
+    if ((((uintptr_t)out | (uintptr_t)row_bytes) & 15) == 0) {
+        const int chunk = lane % kChunks, left = cols - chunk * kPerChunk;
+#pragma unroll
+        for (int r = lane / kChunks; r < 32; r += kRowsAtOnce) {
+            if (r < rows && left > 0) {
+                const uint4 v = *staged(base, r, chunk);
+                uint8_t *p = out + r * row_bytes + chunk * 16;
+                if (left >= kPerChunk) *reinterpret_cast<uint4 *>(p) = v;
+                else {
+                    const uint8_t *e = reinterpret_cast<const uint8_t *>(&v);
+#pragma unroll
+                    for (int i = 0; i < kPerChunk; ++i)
+                        if (i < left) {
+                            if constexpr (kSize == 1) p[i] = e[i];
+                            else if constexpr (kSize == 2) reinterpret_cast<uint16_t *>(p)[i] = reinterpret_cast<const uint16_t *>(e)[i];
+                            else reinterpret_cast<uint32_t *>(p)[i] = reinterpret_cast<const uint32_t *>(e)[i];
+                        }
+                }
+            }
+        }
+    } else {  // rows that do not start at multiples of 16 bytes: element by element, neighbouring lanes neighbouring elements
+        for (int r = 0; r < min(rows, 32); ++r)
+            for (int c = lane; c < min(cols, kRowBytes / kSize); c += 32) {
+                const uint8_t *e = reinterpret_cast<const uint8_t *>(staged(base, r, c / kPerChunk)) + c % kPerChunk * kSize;
+                uint8_t *p = out + r * row_bytes + (int64_t)c * kSize;
+                if constexpr (kSize == 1) *p = *e;
+                else if constexpr (kSize == 2) *reinterpret_cast<uint16_t *>(p) = *reinterpret_cast<const uint16_t *>(e);
+                else *reinterpret_cast<uint32_t *>(p) = *reinterpret_cast<const uint32_t *>(e);
+            }
+    }
+}
+// The way back: 64 16-bit columns of up to 32 rows to shared memory, zeros outside.
+__device__ __forceinline__ void load_staged(uint8_t *base, const uint8_t *in, int64_t row_bytes, int rows, int cols, int lane) {
+    const int chunk = lane & 7, left = cols - chunk * 8;
+    const bool vector = (((uintptr_t)in | (uintptr_t)row_bytes) & 15) == 0 && left >= 8;
+#pragma unroll
+    for (int r = lane >> 3; r < 32; r += 4) {
+        uint4 v = make_uint4(0, 0, 0, 0);
+        if (r < rows) {
+            const uint16_t *p = reinterpret_cast<const uint16_t *>(in + r * row_bytes) + chunk * 8;
+            if (vector) v = *reinterpret_cast<const uint4 *>(p);
+            else {
+                uint16_t *e = reinterpret_cast<uint16_t *>(&v);
+#pragma unroll
+                for (int i = 0; i < 8; ++i)
+                    if (i < left) e[i] = p[i];
+            }
+        }
+        *staged(base, r, chunk) = v;
+    }
+}
+
+template <bool kBF16> __device__ __forceinline__ void unpack_16(uint32_t v, float &lo, float &hi) {
+    if constexpr (kBF16) {
+        lo = __uint_as_float(v << 16);
+        hi = __uint_as_float(v & 0xffff0000u);
+    } else {
+        const float2 f = __half22float2(*reinterpret_cast<const __half2 *>(&v));
+        lo = f.x;
+        hi = f.y;
+    }
+}
+// Calls f with a compile-time truth value: a tile's loops then carry no test of what is the same for the whole launch.
+template <typename F> __device__ __forceinline__ void as_constant(bool value, F f) {
+    if (value) f(std::true_type{});
+    else f(std::false_type{});
+}
+// Waits for a TMEM load; the registers pass through, so that nothing reads them earlier.
+__device__ __forceinline__ void tc_wait_ld_of(uint32_t (&r)[32]) {
+    asm volatile("tcgen05.wait::ld.sync.aligned;"
+                 : "+r"(r[0]), "+r"(r[1]), "+r"(r[2]), "+r"(r[3]), "+r"(r[4]), "+r"(r[5]), "+r"(r[6]), "+r"(r[7]), "+r"(r[8]), "+r"(r[9]), "+r"(r[10]),
+                   "+r"(r[11]), "+r"(r[12]), "+r"(r[13]), "+r"(r[14]), "+r"(r[15]), "+r"(r[16]), "+r"(r[17]), "+r"(r[18]), "+r"(r[19]), "+r"(r[20]),
+                   "+r"(r[21]), "+r"(r[22]), "+r"(r[23]), "+r"(r[24]), "+r"(r[25]), "+r"(r[26]), "+r"(r[27]), "+r"(r[28]), "+r"(r[29]), "+r"(r[30]), "+r"(r[31])
+                 :: "memory");
+}
+
+template <bool kE4m3, int kMode, bool kAMn, bool kBMn>
+__global__ void __launch_bounds__(kThreads, 1) __cluster_dims__(2, 1, 1) matmul_pair_kernel(const __grid_constant__ MatmulParams p) {
+    constexpr bool kGated = kMode != kMatmulPlain;
+    constexpr int kElems = kE4m3 ? 128 : 64;  // contraction elements of a K block
+    constexpr int kCols = kGated ? 64 : 128;  // result columns of a thread
+    extern __shared__ __align__(1024) uint8_t smem[];
+    PairBarriers &sh = *reinterpret_cast<PairBarriers *>(smem + kRingBytes + 8 * kStagingBytes);
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    const uint32_t rank = cluster_rank();
+    const int pair = blockIdx.x >> 1, pairs = gridDim.x >> 1;
+
+    if (warp == kProducerWarp && lane == 0) {
+        sh.abort_flag = (*(volatile unsigned int *)p.status & kStatusMatmul) != 0 ? 1u : 0u;  // an earlier launch gave up
+        for (int i = 0; i < kStages; ++i) {
+            mbar_init(&sh.full[i], 1);
+            mbar_init(&sh.empty[i], 1);
+        }
+        for (int i = 0; i < 2; ++i) {
+            mbar_init(&sh.acc_full[i], 1);
+            mbar_init(&sh.acc_empty[i], 16);
+        }
+        mbar_init(&sh.drained, 1);
+        asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+    }
+    if (warp == kIssuerWarp) {
+        asm volatile("tcgen05.alloc.cta_group::2.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(&sh.tmem_base)), "r"(kTmemCols) : "memory");
+        asm volatile("tcgen05.relinquish_alloc_permit.cta_group::2.sync.aligned;" ::: "memory");
+    }
+    tc_fence_before();
+    cluster_sync();  // both CTAs' barriers exist before either is signalled from the other
+    tc_fence_after();
+    const uint32_t tmem = sh.tmem_base, ring = smem_u32(smem);
+    const auto wait = [&](uint64_t *bar, uint32_t parity, uint32_t code) { return mbar_wait_limit(bar, parity, &sh.abort_flag, p.status, code, kWaitTicks); };
+    const int total = p.tiles_per_problem * p.problems;
+    struct Tile {
+        int problem, m0, n0;
+    };
+    const auto tile_at = [&](int t) {
+        Tile w;
+        w.problem = kAMn && t >= p.tiles_per_problem ? 1 : 0;
+        t -= w.problem * p.tiles_per_problem;
+        w.m0 = (t / p.tiles_n) * 2 * kTile + (int)rank * kTile;
+        w.n0 = (t % p.tiles_n) * (kGated ? kTile : kPairN);
+        return w;
+    };
+    // both CTAs have to agree on whether they run: a flag that only one of them saw raised would leave the other waiting (boundedly)
+    const bool dead = ld_cluster_u32(map_rank(smem_u32((const void *)&sh.abort_flag), 0)) != 0 || ld_cluster_u32(map_rank(smem_u32((const void *)&sh.abort_flag), 1)) != 0;
+
+    // 384 threads x 168 registers at launch = 64,512 = 2 x 128 x 232 + 128 x 40 = 2 x 128 x 216 + 128 x 72: the sums of 8-bit operands
+    // live in registers, those of 16-bit ones in TMEM.  Every warp of a warpgroup executes its setmaxnreg.
+    if (dead) {
+    } else if (warp >= kProducerWarp) {
+    if constexpr (kE4m3) asm volatile("setmaxnreg.dec.sync.aligned.u32 40;");
+    else asm volatile("setmaxnreg.dec.sync.aligned.u32 72;");
+    if (warp == kProducerWarp) {
+        if (lane == 0) {
+            int it = 0;
+            bool ok = true;
+            const uint32_t full0 = map_rank(smem_u32(&sh.full[0]), 0);
+            for (int t = pair; t < total && ok; t += pairs) {
+                const Tile w = tile_at(t);
+                const int b0 = kGated ? w.n0 : w.n0 + (int)rank * kTile;
+                for (int i = 0; i < p.k_blocks; ++i, ++it) {
+                    const int st = it % kStages;
+                    ok = wait(&sh.empty[st], ((it / kStages) & 1) ^ 1, kErrEmpty);
+                    if (!ok) break;
+                    const int sum = i >= p.kb_per_sum ? 1 : 0, k = (i - sum * p.kb_per_sum) * kElems;
+                    const uint32_t dst = ring + st * kStageBytes, bar = full0 + st * 8;
+                    if (rank == 0) mbar_arrive_expect_tx(&sh.full[st], 2 * kStageBytes);
+                    const CUtensorMap *ma = &p.a[sum + w.problem], *mb = &p.b[kGated ? rank : sum];
+                    if constexpr (kAMn) {
+                        tma_load_2d_pair(dst, ma, w.m0, k, bar);
+                        tma_load_2d_pair(dst + kOperandBytes / 2, ma, w.m0 + 64, k, bar);
+                    } else {
+                        tma_load_2d_pair(dst, ma, k, w.m0, bar);
+                    }
+                    if constexpr (kBMn) {
+                        tma_load_2d_pair(dst + kOperandBytes, mb, b0, k, bar);
+                        tma_load_2d_pair(dst + kOperandBytes + kOperandBytes / 2, mb, b0 + 64, k, bar);
+                    } else {
+                        tma_load_2d_pair(dst + kOperandBytes, mb, k, b0, bar);
+                    }
+                }
+            }
+            if (rank == 0)  // what was asked for has landed (both CTAs' loads complete here) before shared memory is released
+                for (int j = max(it - kStages, 0); j < it; ++j) mbar_drain(&sh.full[j % kStages], (j / kStages) & 1, p.status, kErrFull);
+        }
+        __syncwarp();
+    } else if (warp == kIssuerWarp) {
+        if (lane == 0 && rank == 0) {
+            const uint32_t idesc = matmul_idesc(kE4m3, p.dtype == COME_BF16, 2 * kTile, kPairN, kAMn, kBMn);
+            constexpr uint32_t kAStep = kAMn ? 2048 >> 4 : 32 >> 4, kBStep = kBMn ? 2048 >> 4 : 32 >> 4;
+            int it = 0, chunk = 0;  // K blocks, fills of a TMEM buffer so far
+            bool ok = true;
+            for (int t = pair; t < total && ok; t += pairs) {
+                for (int i = 0; i < p.k_blocks; ++i, ++it) {
+                    const int st = it % kStages, buf = chunk & 1;
+                    if (kE4m3 || i == 0) ok = wait(&sh.acc_empty[buf], ((chunk >> 1) & 1) ^ 1, kErrSums);
+                    ok = ok && wait(&sh.full[st], (it / kStages) & 1, kErrFull);
+                    if (!ok) break;
+                    tc_fence_after();
+                    const uint64_t da = operand_desc(ring + st * kStageBytes, kOperandBytes / 2);
+                    const uint64_t db = operand_desc(ring + st * kStageBytes + kOperandBytes, kOperandBytes / 2);
+#pragma unroll
+                    for (int k = 0; k < 4; ++k)
+                        tc_mma_pair<kE4m3>(tmem + buf * kPairN, da + k * kAStep, db + k * kBStep, idesc, k > 0 || (!kE4m3 && i > 0) ? 1u : 0u);
+                    tc_commit_pair(&sh.empty[st]);
+                    if (kE4m3 || i == p.k_blocks - 1) {
+                        tc_commit_pair(&sh.acc_full[buf]);
+                        ++chunk;
+                    }
+                }
+            }
+            tc_commit_pair(&sh.drained);
+            mbar_drain(&sh.drained, 0, p.status, kErrSums);
+        }
+        __syncwarp();
+    }
+    } else {
+    if constexpr (kE4m3) asm volatile("setmaxnreg.inc.sync.aligned.u32 232;");
+    else asm volatile("setmaxnreg.inc.sync.aligned.u32 216;");
+        const int part = warp >> 2, r = (warp & 3) * 32 + lane, warp_row = (warp & 3) * 32;
+        const uint32_t lanes = tmem + ((uint32_t)warp_row << 16) + part * kCols;
+        uint8_t *stage = smem + kRingBytes + warp * kStagingBytes;
+        const uint32_t empty0 = map_rank(smem_u32(&sh.acc_empty[0]), 0);
+        int chunk = 0, tiles = 0;
+        bool ok = true;
+        for (int t = pair; t < total; t += pairs, ++tiles) {
+            const Tile w = tile_at(t);
+            const int rows = min(32, p.M - w.m0 - warp_row);      // of this warp, may be <= 0
+            const int n = w.n0 + part * kCols, cols = p.N - n;    // first result column of the thread, columns from there on
+            const bool busy = rows > 0;
+            const int64_t row0 = w.m0 + warp_row;
+            if constexpr (kE4m3) {
+                const bool with_bias = p.bias[0] != nullptr || (kGated && p.bias[1] != nullptr);
+                float *bias = reinterpret_cast<float *>(stage);   // [128]: of the gate's and the up projection's 64 columns, or of 128
+                if (with_bias) {
+                    __syncwarp();
+#pragma unroll
+                    for (int c = 0; c < 4; ++c) {
+                        const float *b = kGated ? (const float *)p.bias[c >> 1] : (const float *)p.bias[0];
+                        const int col = (kGated ? (c & 1) : c) * 32 + lane;
+                        bias[c * 32 + lane] = b != nullptr && col < cols ? b[n + col] : 0.0f;
+                    }
+                    __syncwarp();
+                }
+                // sums as packed pairs: [0, 32) of the gate or of columns [0, 64), [32, 64) of the up projection or of columns [64, 128)
+                f32x2_t sum[64];
+#pragma unroll
+                for (int c = 0; c < 64; ++c) sum[c] = 0ull;
+                const int nb = min(w.n0 / kTile + (kGated ? 0 : part), (p.N - 1) / kTile);  // column block; past the last one nothing is stored
+                const float *as = p.a_scale + (int64_t)min(w.m0 + r, p.M - 1) * p.as_row;
+                const float *bs0 = p.b_scale[0] + nb * p.bs_row[0], *bs1 = kGated ? p.b_scale[1] + nb * p.bs_row[1] : bs0;
+                // the scales of two K blocks ahead: a load takes longer than a block
+                float sa[2], sb0[2], sb1[2];
+                const auto fetch = [&](int j, int i) {
+                    const int kb = min(i, p.k_blocks - 1);
+                    sa[j] = as[kb * p.as_block];
+                    sb0[j] = bs0[kb];
+                    if constexpr (kGated) sb1[j] = bs1[kb];
+                };
+                fetch(0, 0);
+                fetch(1, 1);
+                for (int i0 = 0; i0 < p.k_blocks; i0 += 2) {
+#pragma unroll
+                    for (int j = 0; j < 2; ++j) {
+                        if (i0 + j < p.k_blocks) {
+                            const int buf = chunk & 1;
+                            const float s0 = sa[j] * sb0[j], s1 = kGated ? sa[j] * sb1[j] : s0;
+                            fetch(j, i0 + j + 2);
+                            ok = ok && wait(&sh.acc_full[buf], (chunk >> 1) & 1, kErrSums);
+                            ok = __all_sync(0xffffffffu, ok);
+                            if (ok && busy) {
+                                tc_fence_after();
+                                const f32x2_t s0p = pack_f32x2(s0, s0), s1p = pack_f32x2(s1, s1);
+                                const auto column = [&](int c) { return lanes + buf * kPairN + (kGated ? (c >> 1) * kTile + (c & 1) * 32 : c * 32); };
+                                uint32_t d[2][32];
+                                tmem_ld32(column(0), d[0]);
+#pragma unroll
+                                for (int c = 0; c < 4; ++c) {
+                                    tc_wait_ld_of(d[c & 1]);
+                                    if (c < 3) tmem_ld32(column(c + 1), d[(c + 1) & 1]);
+#pragma unroll
+                                    for (int e = 0; e < 16; ++e)
+                                        sum[c * 16 + e] = fma_f32x2(pack_f32x2(__uint_as_float(d[c & 1][2 * e]), __uint_as_float(d[c & 1][2 * e + 1])), c >> 1 ? s1p : s0p, sum[c * 16 + e]);
+                                }
+                                tc_fence_before();
+                            }
+                            __syncwarp();
+                            if (ok && lane == 0) mbar_arrive_at(empty0 + buf * 8);
+                            ++chunk;
+                        }
+                    }
+                }
+                if constexpr (!kGated) {
+                    if (ok && busy) {
+                        if (with_bias) {
+#pragma unroll
+                            for (int c = 0; c < 32; ++c) {
+                                const float4 b = *reinterpret_cast<const float4 *>(bias + 4 * c);
+                                sum[2 * c] = add_f32x2(sum[2 * c], pack_f32x2(b.x, b.y));
+                                sum[2 * c + 1] = add_f32x2(sum[2 * c + 1], pack_f32x2(b.z, b.w));
+                            }
+                            __syncwarp();
+                        }
+                        if (p.out_dtype == COME_F32) {
+                            uint8_t *out = (uint8_t *)p.out[0] + (row0 * p.out_row[0] + n) * 4;
+#pragma unroll
+                            for (int h = 0; h < 4; ++h) {
+#pragma unroll
+                                for (int c = 0; c < 8; ++c) {
+                                    float v[4];
+                                    unpack_f32x2(sum[h * 16 + c * 2], v[0], v[1]);
+                                    unpack_f32x2(sum[h * 16 + c * 2 + 1], v[2], v[3]);
+                                    *staged(stage, lane, c) = make_uint4(__float_as_uint(v[0]), __float_as_uint(v[1]), __float_as_uint(v[2]), __float_as_uint(v[3]));
+                                }
+                                __syncwarp();
+                                store_staged<4, 128>(stage, out + h * 128, p.out_row[0] * 4, rows, cols - h * 32, lane);
+                                __syncwarp();
+                            }
+                        } else {
+                            as_constant(p.out_dtype == COME_BF16, [&](auto bf16) {
+                                uint8_t *out = (uint8_t *)p.out[0] + (row0 * p.out_row[0] + n) * 2;
+#pragma unroll
+                                for (int h = 0; h < 2; ++h) {
+#pragma unroll
+                                    for (int c = 0; c < 8; ++c) {
+                                        uint32_t e[4];
+#pragma unroll
+                                        for (int j = 0; j < 4; ++j) {
+                                            float lo, hi;
+                                            unpack_f32x2(sum[h * 32 + c * 4 + j], lo, hi);
+                                            e[j] = pack_16<decltype(bf16)::value>(lo, hi);
+                                        }
+                                        *staged(stage, lane, c) = make_uint4(e[0], e[1], e[2], e[3]);
+                                    }
+                                    __syncwarp();
+                                    store_staged<2, 128>(stage, out + h * 128, p.out_row[0] * 2, rows, cols - h * 64, lane);
+                                    __syncwarp();
+                                }
+                            });
+                        }
+                    }
+                } else {
+                    float h[64], top = 0.0f;
+                    if (ok && busy) {
+                        if (with_bias) {
+#pragma unroll
+                            for (int c = 0; c < 32; ++c) {
+                                const float4 b = *reinterpret_cast<const float4 *>(bias + 4 * c);
+                                sum[2 * c] = add_f32x2(sum[2 * c], pack_f32x2(b.x, b.y));
+                                sum[2 * c + 1] = add_f32x2(sum[2 * c + 1], pack_f32x2(b.z, b.w));
+                            }
+                        }
+                        as_constant(p.act == COME_ACT_SILU, [&](auto silu) {
+                            constexpr int act = decltype(silu)::value ? COME_ACT_SILU : COME_ACT_GELU;
+#pragma unroll
+                            for (int c = 0; c < 32; ++c) {
+                                float g0, g1, u0, u1;
+                                unpack_f32x2(sum[c], g0, g1);
+                                unpack_f32x2(sum[32 + c], u0, u1);
+                                h[2 * c] = activation(g0, act) * u0;
+                                h[2 * c + 1] = activation(g1, act) * u1;
+                            }
+                        });
+                        if (cols < 64)  // columns past the end: the bytes of other rows' products
+#pragma unroll
+                            for (int c = 0; c < 64; ++c) h[c] = c < cols ? h[c] : 0.0f;
+                        __syncwarp();
+                    }
+                    if (p.out_dtype == COME_E4M3) {
+                        if (ok && busy)
+#pragma unroll
+                            for (int c = 0; c < 64; ++c) top = fmaxf(top, fabsf(h[c]));
+                        // the largest magnitude of a row's 128 columns: half of it in the other warpgroup (every warp meets here, also
+                        // one that gave up; a third tile's write to the same place is two barriers away)
+                        sh.top[tiles & 1][part][r] = top;
+                        asm volatile("bar.sync 1, 256;" ::: "memory");
+                        top = fmaxf(fmaxf(top, sh.top[tiles & 1][part ^ 1][r]), kSmallestMax);
+                        if (ok && busy) {
+                            const float inv = kE4m3Max / top;
+#pragma unroll
+                            for (int c = 0; c < 4; ++c) {
+                                uint32_t q[4];
+#pragma unroll
+                                for (int j = 0; j < 4; ++j) {
+                                    const float *e = h + c * 16 + j * 4;
+                                    q[j] = pack_e4m3(e[0] * inv, e[1] * inv, e[2] * inv, e[3] * inv);
+                                }
+                                *staged(stage, lane, c) = make_uint4(q[0], q[1], q[2], q[3]);
+                            }
+                            __syncwarp();
+                            store_staged<1, 64>(stage, (uint8_t *)p.out[0] + row0 * p.out_row[0] + n, p.out_row[0], rows, cols, lane);
+                            if (part == 0 && lane < rows) p.out_scale[(row0 + lane) * p.os_row + (w.n0 / kTile) * p.os_block] = top / kE4m3Max;
+                            __syncwarp();
+                        }
+                    } else if (ok && busy) {
+                        as_constant(p.out_dtype == COME_BF16, [&](auto bf16) {
+#pragma unroll
+                            for (int c = 0; c < 8; ++c) {
+                                const float *e = h + c * 8;
+                                uint32_t q[4];
+#pragma unroll
+                                for (int j = 0; j < 4; ++j) q[j] = pack_16<decltype(bf16)::value>(e[2 * j], e[2 * j + 1]);
+                                *staged(stage, lane, c) = make_uint4(q[0], q[1], q[2], q[3]);
+                            }
+                        });
+                        __syncwarp();
+                        store_staged<2, 128>(stage, (uint8_t *)p.out[0] + (row0 * p.out_row[0] + n) * 2, p.out_row[0] * 2, rows, cols, lane);
+                        __syncwarp();
+                    }
+                }
+            } else {
+                const int buf = chunk & 1;
+                if (kGated && busy) {  // before the wait: the biases of this warp's 64 + 64 columns, and dh
+#pragma unroll
+                    for (int c = 0; c < 4; ++c) {
+                        const uint16_t *b = (const uint16_t *)p.bias[c >> 1];
+                        const int col = (c & 1) * 32 + lane;
+                        sh.bias[warp][c * 32 + lane] = b != nullptr && col < cols ? b[n + col] : (uint16_t)0;
+                    }
+                    if (kMode == kMatmulGatedGrad && ok && cols > 0) load_staged(stage, (const uint8_t *)p.dh + (row0 * p.dh_row + n) * 2, p.dh_row * 2, rows, cols, lane);
+                    __syncwarp();
+                }
+                ok = ok && wait(&sh.acc_full[buf], (chunk >> 1) & 1, kErrSums);
+                ok = __all_sync(0xffffffffu, ok);
+                if (ok && busy) {
+                    tc_fence_after();
+                    const uint32_t from = lanes + buf * kPairN;
+                    as_constant(p.dtype == COME_BF16, [&](auto bf16_c) {
+                        constexpr bool kBF16 = decltype(bf16_c)::value;
+                        if constexpr (!kGated) {
+#pragma unroll
+                            for (int h = 0; h < 2; ++h) {
+                                uint32_t d[2][32];
+                                tmem_ld32(from + h * 64, d[0]);
+                                tmem_ld32(from + h * 64 + 32, d[1]);
+                                tc_wait_ld_of(d[0]);
+                                tc_wait_ld_of(d[1]);
+                                if (h == 1) {  // the sums are in registers: the next tile may begin
+                                    tc_fence_before();
+                                    __syncwarp();
+                                    if (lane == 0) mbar_arrive_at(empty0 + buf * 8);
+                                }
+#pragma unroll
+                                for (int c = 0; c < 8; ++c) {
+                                    uint32_t e[4];
+#pragma unroll
+                                    for (int j = 0; j < 4; ++j) e[j] = pack_16<kBF16>(__uint_as_float(d[c >> 2][(c & 3) * 8 + 2 * j]), __uint_as_float(d[c >> 2][(c & 3) * 8 + 2 * j + 1]));
+                                    *staged(stage, lane, c) = make_uint4(e[0], e[1], e[2], e[3]);
+                                }
+                                __syncwarp();
+                                store_staged<2, 128>(stage, (uint8_t *)p.out[w.problem] + (row0 * p.out_row[w.problem] + n + h * 64) * 2, p.out_row[w.problem] * 2, rows, cols - h * 64, lane);
+                                __syncwarp();
+                            }
+                        } else {
+                            as_constant(p.act == COME_ACT_SILU, [&](auto silu) {
+                                constexpr int act = decltype(silu)::value ? COME_ACT_SILU : COME_ACT_GELU;
+                                [[maybe_unused]] uint32_t second[32];  // du of the row, while dg is staged
+#pragma unroll
+                                for (int q = 0; q < 2; ++q) {
+                                    uint32_t g[32], u[32];
+                                    tmem_ld32(from + q * 32, g);
+                                    tmem_ld32(from + kTile + q * 32, u);
+                                    tc_wait_ld_of(g);
+                                    tc_wait_ld_of(u);
+                                    if (q == 1) {  // the sums are in registers: the next tile may begin
+                                        tc_fence_before();
+                                        __syncwarp();
+                                        if (lane == 0) mbar_arrive_at(empty0 + buf * 8);
+                                    }
+#pragma unroll
+                                    for (int c = 0; c < 4; ++c) {
+                                        const uint4 bg = *reinterpret_cast<const uint4 *>(&sh.bias[warp][q * 32 + c * 8]), bu = *reinterpret_cast<const uint4 *>(&sh.bias[warp][64 + q * 32 + c * 8]);
+                                        const uint32_t bgs[4] = {bg.x, bg.y, bg.z, bg.w}, bus[4] = {bu.x, bu.y, bu.z, bu.w};
+                                        uint32_t e[4];
+                                        [[maybe_unused]] uint32_t dh[4];
+                                        if constexpr (kMode == kMatmulGatedGrad) {
+                                            const uint4 raw = *staged(stage, lane, q * 4 + c);
+                                            dh[0] = raw.x, dh[1] = raw.y, dh[2] = raw.z, dh[3] = raw.w;
+                                        }
+#pragma unroll
+                                        for (int j = 0; j < 4; ++j) {
+                                            float g0, g1, u0, u1;
+                                            unpack_16<kBF16>(bgs[j], g0, g1);
+                                            unpack_16<kBF16>(bus[j], u0, u1);
+                                            g0 += __uint_as_float(g[c * 8 + 2 * j]), g1 += __uint_as_float(g[c * 8 + 2 * j + 1]);
+                                            u0 += __uint_as_float(u[c * 8 + 2 * j]), u1 += __uint_as_float(u[c * 8 + 2 * j + 1]);
+                                            if constexpr (kMode == kMatmulGated) {
+                                                e[j] = pack_16<kBF16>(activation(g0, act) * u0, activation(g1, act) * u1);
+                                            } else {
+                                                float d0, d1, a0, a1, s0, s1;
+                                                unpack_16<kBF16>(dh[j], d0, d1);
+                                                activation_grad(g0, act, a0, s0);
+                                                activation_grad(g1, act, a1, s1);
+                                                e[j] = pack_16<kBF16>(d0 * u0 * s0, d1 * u1 * s1);
+                                                second[(q * 4 + c) * 4 + j] = pack_16<kBF16>(d0 * a0, d1 * a1);
+                                            }
+                                        }
+                                        *staged(stage, lane, q * 4 + c) = make_uint4(e[0], e[1], e[2], e[3]);
+                                    }
+                                }
+                                __syncwarp();
+                                store_staged<2, 128>(stage, (uint8_t *)p.out[0] + (row0 * p.out_row[0] + n) * 2, p.out_row[0] * 2, rows, cols, lane);
+                                __syncwarp();
+                                if constexpr (kMode == kMatmulGatedGrad) {
+#pragma unroll
+                                    for (int c = 0; c < 8; ++c) *staged(stage, lane, c) = make_uint4(second[4 * c], second[4 * c + 1], second[4 * c + 2], second[4 * c + 3]);
+                                    __syncwarp();
+                                    store_staged<2, 128>(stage, (uint8_t *)p.out[1] + (row0 * p.out_row[1] + n) * 2, p.out_row[1] * 2, rows, cols, lane);
+                                    __syncwarp();
+                                }
+                            });
+                        }
+                    });
+                } else if (ok) {
+                    if (lane == 0) mbar_arrive_at(empty0 + buf * 8);
+                }
+                ++chunk;
+            }
+        }
+    }
+    if (sh.abort_flag != 0) {  // the other CTA's copies complete on the first one's barriers: give those in flight time to land
+        const long long t0 = clock64();
+        while (clock64() - t0 < (1ll << 22)) {
+        }
+    }
+    __syncwarp();
+    tc_fence_before();
+    cluster_sync();  // no CTA leaves while the other signals its barriers or reads its operands
+    if (warp == kIssuerWarp) {
+        tc_fence_after();
+        asm volatile("tcgen05.dealloc.cta_group::2.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(kTmemCols));
+    }
+}
+
+template <bool kE4m3, int kMode, bool kAMn, bool kBMn> int launch_pair(const MatmulParams &p, cudaStream_t st) {
+    constexpr auto kernel = matmul_pair_kernel<kE4m3, kMode, kAMn, kBMn>;
+    if (int rc = allow_smem<kernel>(kSmemBytes); rc != COME_OK) return rc;
+    const int tiles = p.tiles_per_problem * p.problems, pairs = sm_count() / 2;
+    kernel<<<2 * (tiles < pairs ? tiles : pairs), kThreads, kSmemBytes, st>>>(p);
+    return check_launch("product kernel");
+}
+
+}  // namespace
+
+bool matmul_pair_takes(const MatmulArgs &a) {
+    const int64_t n = a.mode == kMatmulPlain ? kPairN : kTile;
+    const int64_t tiles = (a.M + 2 * kTile - 1) / (2 * kTile) * ((a.N + n - 1) / n) * a.problems;
+    return tiles * 2 >= sm_count() / 2;
+}
+
+int matmul_pair_launch(const MatmulArgs &a, MatmulParams &p, cudaStream_t st) {
+    const int n = a.mode == kMatmulPlain ? kPairN : kTile;
+    p.tiles_n = (int)((a.N + n - 1) / n);
+    const int64_t per_problem = (a.M + 2 * kTile - 1) / (2 * kTile) * p.tiles_n;
+    COME_REQUIRE(per_problem * a.problems < (1ll << 30), "the result has too many tiles for one launch");
+    p.tiles_per_problem = (int)per_problem;
+    if (a.e4m3) return a.mode == kMatmulPlain ? launch_pair<true, kMatmulPlain, false, false>(p, st) : launch_pair<true, kMatmulGated, false, false>(p, st);
+    if (a.mode == kMatmulGated) return launch_pair<false, kMatmulGated, false, false>(p, st);
+    if (a.mode == kMatmulGatedGrad) return launch_pair<false, kMatmulGatedGrad, false, false>(p, st);
+    return a.a_mn ? launch_pair<false, kMatmulPlain, true, true>(p, st) : launch_pair<false, kMatmulPlain, false, true>(p, st);
+}
+
+}  // namespace come

@@ -27,10 +27,7 @@ namespace come {
 
 namespace {
 
-constexpr int kTile = 128;
-constexpr int kKBytes = 128;                       // bytes of the contraction per K block
 constexpr int kEpilogueWarps = 8, kProducerWarp = 8, kIssuerWarp = 9, kThreads = 320;
-constexpr int kOperandBytes = kTile * kKBytes;     // 16 KiB: 128 rows of a K block
 constexpr int kRingBytes = 192 * 1024;
 constexpr int kPartRow = kTile + 4;                // floats: rows of the shares in shared memory, no bank conflicts row to row
 constexpr int kPartBytes = kTile * kPartRow * 4;
@@ -46,50 +43,6 @@ struct SplitBarriers {
 constexpr size_t kSmemBytes = kRingBytes + sizeof(SplitBarriers) + 1024;
 static_assert(kSmemBytes <= 227 * 1024 && kSmemBytes > 114 * 1024, "one CTA per SM");
 static_assert(2 * kPartBytes <= kRingBytes, "the shares reuse the ring");
-
-struct SplitParams {
-    CUtensorMap a[2], b[2];
-    const float *a_scale, *b_scale[2];
-    int64_t as_row, as_block, bs_row[2];
-    const void *bias[2], *dh;
-    void *out[2];
-    float *out_scale;
-    int64_t dh_row, out_row[2], os_row, os_block;
-    int M, N, kb_per_sum, k_blocks;  // K blocks of one contraction, of all
-    int tiles_n, tiles_per_problem;
-    int act, dtype, bias_dtype, out_dtype;
-    unsigned int *status;
-};
-
-__device__ __forceinline__ uint32_t cluster_rank() {
-    uint32_t r;
-    asm volatile("mov.u32 %0, %%cluster_ctarank;" : "=r"(r));
-    return r;
-}
-__device__ __forceinline__ uint32_t cluster_size() {
-    uint32_t r;
-    asm volatile("mov.u32 %0, %%cluster_nctarank;" : "=r"(r));
-    return r;
-}
-__device__ __forceinline__ void cluster_sync() {
-    asm volatile("barrier.cluster.arrive.release.aligned;" ::: "memory");
-    asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory");
-}
-__device__ __forceinline__ uint32_t map_rank(uint32_t saddr, uint32_t rank) {
-    uint32_t r;
-    asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(r) : "r"(saddr), "r"(rank));
-    return r;
-}
-__device__ __forceinline__ float4 ld_cluster(uint32_t addr) {
-    float4 v;
-    asm volatile("ld.shared::cluster.v4.f32 {%0, %1, %2, %3}, [%4];" : "=f"(v.x), "=f"(v.y), "=f"(v.z), "=f"(v.w) : "r"(addr) : "memory");
-    return v;
-}
-__device__ __forceinline__ uint32_t ld_cluster_u32(uint32_t addr) {
-    uint32_t v;
-    asm volatile("ld.shared::cluster.u32 %0, [%1];" : "=r"(v) : "r"(addr) : "memory");
-    return v;
-}
 
 // Four neighbouring columns of a row, `valid` of them inside the result.
 __device__ __forceinline__ void store4(void *out, int64_t at, const float (&v)[4], int valid, int dtype) {
@@ -132,11 +85,8 @@ __device__ __forceinline__ void load4(const void *in, int64_t at, float (&v)[4],
     for (int i = 0; i < 4; ++i) v[i] = i < valid ? load_any(in, at + i, dtype) : 0.0f;
 }
 
-enum : uint32_t { kErrFull = 1u << 19, kErrEmpty = 1u << 20, kErrSums = 1u << 21 };
-static_assert((kErrFull | kErrEmpty | kErrSums) == kStatusMatmul, "come_device_status names these bits");
-
 template <bool kE4m3, int kMode, bool kAMn, bool kBMn>
-__global__ void __launch_bounds__(kThreads, 1) matmul_split_kernel(const __grid_constant__ SplitParams p) {
+__global__ void __launch_bounds__(kThreads, 1) matmul_split_kernel(const __grid_constant__ MatmulParams p) {
     constexpr int kMats = kMode == kMatmulPlain ? 1 : 2;
     constexpr int kN = kMats * kTile;
     constexpr int kStageBytes = kOperandBytes * (1 + kMats), kStages = kRingBytes / kStageBytes;
@@ -375,22 +325,7 @@ __global__ void __launch_bounds__(kThreads, 1) matmul_split_kernel(const __grid_
     }
 }
 
-// The shared-memory opt-in of a kernel, once per device and instantiation and before its first launch (launches stay cheap and
-// legal inside a stream capture).
-template <auto kernel> int allow_smem(size_t bytes) {
-    static std::mutex mu;
-    static bool done[64];
-    int dev = 0;
-    COME_CUDA(cudaGetDevice(&dev));
-    COME_REQUIRE(dev >= 0 && dev < 64, "device ordinal %d is out of the supported range", dev);
-    std::lock_guard<std::mutex> lock(mu);
-    if (done[dev]) return COME_OK;
-    COME_CUDA(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)bytes));
-    done[dev] = true;
-    return COME_OK;
-}
-
-template <bool kE4m3, int kMode, bool kAMn, bool kBMn> int launch_split(const SplitParams &p, int64_t tiles, int cluster, cudaStream_t st) {
+template <bool kE4m3, int kMode, bool kAMn, bool kBMn> int launch_split(const MatmulParams &p, int64_t tiles, int cluster, cudaStream_t st) {
     constexpr auto kernel = matmul_split_kernel<kE4m3, kMode, kAMn, kBMn>;
     if (int rc = allow_smem<kernel>(kSmemBytes); rc != COME_OK) return rc;
     cudaLaunchAttribute attr = {};
@@ -422,7 +357,7 @@ int pick_cluster(int64_t tiles, int64_t k_blocks) {
 
 int run_matmul(const MatmulArgs &a, cudaStream_t st) {
     const int mats = a.mode == kMatmulPlain ? 1 : 2;
-    SplitParams p = {};
+    MatmulParams p = {};
     p.status = status_word_dev();
     if (!p.status) return COME_ERR_CUDA;
     int rc;
@@ -454,14 +389,16 @@ int run_matmul(const MatmulArgs &a, cudaStream_t st) {
     const int elems = a.e4m3 ? 128 : 64;
     p.kb_per_sum = (int)((a.K + elems - 1) / elems);
     p.k_blocks = p.kb_per_sum * a.sums;
-    p.tiles_n = (int)((a.N + kTile - 1) / kTile);
-    const int64_t per_problem = (a.M + kTile - 1) / kTile * p.tiles_n, tiles = per_problem * a.problems;
-    COME_REQUIRE(tiles < (1ll << 27), "the result has %lld tiles of 128 x 128: too many for one launch", (long long)tiles);
-    p.tiles_per_problem = (int)per_problem;
+    p.problems = a.problems;
     p.act = a.act;
     p.dtype = a.dtype;
     p.bias_dtype = a.e4m3 ? COME_F32 : a.dtype;
     p.out_dtype = a.out_dtype;
+    if (matmul_pair_takes(a)) return matmul_pair_launch(a, p, st);
+    p.tiles_n = (int)((a.N + kTile - 1) / kTile);
+    const int64_t per_problem = (a.M + kTile - 1) / kTile * p.tiles_n, tiles = per_problem * a.problems;
+    COME_REQUIRE(tiles < (1ll << 27), "the result has %lld tiles of 128 x 128: too many for one launch", (long long)tiles);
+    p.tiles_per_problem = (int)per_problem;
     const int cluster = pick_cluster(tiles, p.k_blocks);
     if (a.e4m3) return a.mode == kMatmulPlain ? launch_split<true, kMatmulPlain, false, false>(p, tiles, cluster, st) : launch_split<true, kMatmulGated, false, false>(p, tiles, cluster, st);
     if (a.mode == kMatmulGated) return launch_split<false, kMatmulGated, false, false>(p, tiles, cluster, st);

@@ -42,6 +42,29 @@ struct MatmulArgs {
     int64_t os_row, os_block;
 };
 
+constexpr int kTile = 128;
+constexpr int kKBytes = 128;                       // bytes of the contraction per K block
+constexpr int kOperandBytes = kTile * kKBytes;     // 16 KiB: 128 rows of a K block
+
+// What a launch of either kernel gets.
+struct MatmulParams {
+    CUtensorMap a[2], b[2];
+    const float *a_scale, *b_scale[2];
+    int64_t as_row, as_block, bs_row[2];
+    const void *bias[2], *dh;
+    void *out[2];
+    float *out_scale;
+    int64_t dh_row, out_row[2], os_row, os_block;
+    int M, N, kb_per_sum, k_blocks;  // K blocks of one contraction, of all
+    int tiles_n, tiles_per_problem, problems;
+    int act, dtype, bias_dtype, out_dtype;
+    unsigned int *status;
+};
+
+// The kernel for results with many tiles (matmul_pair_sm100.cu).
+bool matmul_pair_takes(const MatmulArgs &a);
+int matmul_pair_launch(const MatmulArgs &a, MatmulParams &p, cudaStream_t st);
+
 // ---- host ---------------------------------------------------------------------------------------------------------------
 // 2-D tensor map of rows of `inner` elements; box of `box_rows` rows of 128 bytes, 128-byte swizzle, zeros outside.
 inline int make_rows_map(CUtensorMap *map, const void *base, bool e4m3, int dtype, int64_t rows, int64_t inner, int64_t row_stride, int box_rows) {
@@ -74,6 +97,21 @@ inline int make_rows_map(CUtensorMap *map, const void *base, bool e4m3, int dtyp
     return COME_OK;
 }
 
+// The shared-memory opt-in of a kernel, once per device and instantiation and before its first launch (launches stay cheap and
+// legal inside a stream capture).
+template <auto kernel> int allow_smem(size_t bytes) {
+    static std::mutex mu;
+    static bool done[64];
+    int dev = 0;
+    COME_CUDA(cudaGetDevice(&dev));
+    COME_REQUIRE(dev >= 0 && dev < 64, "device ordinal %d is out of the supported range", dev);
+    std::lock_guard<std::mutex> lock(mu);
+    if (done[dev]) return COME_OK;
+    COME_CUDA(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)bytes));
+    done[dev] = true;
+    return COME_OK;
+}
+
 // ---- device -------------------------------------------------------------------------------------------------------------
 __device__ __forceinline__ void tma_load_2d(uint32_t dst, const CUtensorMap *map, int x, int y, uint64_t *bar) {
     asm volatile("cp.async.bulk.tensor.2d.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3}], [%4];"
@@ -99,6 +137,40 @@ __host__ __device__ constexpr uint32_t matmul_idesc(bool e4m3, bool bf16, int M,
     return (1u << 4) | (format << 7) | (format << 10) | ((a_mn ? 1u : 0u) << 15) | ((b_mn ? 1u : 0u) << 16) | ((uint32_t)(N >> 3) << 17) |
            ((uint32_t)(M >> 4) << 24);
 }
+
+__device__ __forceinline__ uint32_t cluster_rank() {
+    uint32_t r;
+    asm volatile("mov.u32 %0, %%cluster_ctarank;" : "=r"(r));
+    return r;
+}
+__device__ __forceinline__ uint32_t cluster_size() {
+    uint32_t r;
+    asm volatile("mov.u32 %0, %%cluster_nctarank;" : "=r"(r));
+    return r;
+}
+__device__ __forceinline__ void cluster_sync() {
+    asm volatile("barrier.cluster.arrive.release.aligned;" ::: "memory");
+    asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory");
+}
+__device__ __forceinline__ uint32_t map_rank(uint32_t saddr, uint32_t rank) {
+    uint32_t r;
+    asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(r) : "r"(saddr), "r"(rank));
+    return r;
+}
+__device__ __forceinline__ float4 ld_cluster(uint32_t addr) {
+    float4 v;
+    asm volatile("ld.shared::cluster.v4.f32 {%0, %1, %2, %3}, [%4];" : "=f"(v.x), "=f"(v.y), "=f"(v.z), "=f"(v.w) : "r"(addr) : "memory");
+    return v;
+}
+__device__ __forceinline__ uint32_t ld_cluster_u32(uint32_t addr) {
+    uint32_t v;
+    asm volatile("ld.shared::cluster.u32 %0, [%1];" : "=r"(v) : "r"(addr) : "memory");
+    return v;
+}
+
+enum : uint32_t { kErrFull = 1u << 19, kErrEmpty = 1u << 20, kErrSums = 1u << 21 };
+static_assert((kErrFull | kErrEmpty | kErrSums) == kStatusMatmul, "come_device_status names these bits");
+
 
 // act(g) and its derivative.  silu: g s with s = 1 / (1 + e^-g), derivative s (1 + g (1 - s)); gelu: g Phi(g), derivative
 // Phi(g) + g phi(g).  A g so low that e^-g overflows gives s = 0 and a product of -0.
