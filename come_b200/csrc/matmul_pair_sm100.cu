@@ -30,7 +30,9 @@ constexpr int kPairN = 256;                         // columns of sums per tile
 constexpr int kStageBytes = 2 * kOperandBytes;      // 128 rows of A and of B
 constexpr int kStages = 6;
 constexpr int kRingBytes = kStages * kStageBytes;
-constexpr int kStagingBytes = 4096;                 // per epilogue warp: 32 rows of 128 bytes
+__host__ __device__ constexpr int staging_row(bool e4m3) { return e4m3 ? 64 : 128; }                // bytes; 8-bit operands: the other half holds scales
+__host__ __device__ constexpr int staging_bytes(bool e4m3) { return 32 * staging_row(e4m3); }       // per epilogue warp
+constexpr int kScaleSlots = 4;                      // K blocks whose scales are in shared memory
 constexpr uint32_t kTmemCols = 512;
 
 struct PairBarriers {
@@ -44,8 +46,11 @@ struct PairBarriers {
         alignas(16) uint16_t bias[8][128];   // 16 bits: [warp], of its 64 columns of the gate and of the up projection
     };
 };
-constexpr size_t kSmemBytes = kRingBytes + 8 * kStagingBytes + sizeof(PairBarriers);
-static_assert(kSmemBytes <= 227 * 1024, "");
+// 8-bit operands, per K block: the product of the row's scale and that of the weight's columns [0, 128) / [128, 256), or of the gate / the
+// up projection.
+typedef float PairScales[kScaleSlots][2][kTile];
+constexpr size_t smem_bytes(bool e4m3) { return kStages * kStageBytes + 8 * staging_bytes(e4m3) + sizeof(PairBarriers) + (e4m3 ? sizeof(PairScales) : 0); }
+static_assert(smem_bytes(true) <= 227 * 1024 && smem_bytes(false) <= 227 * 1024, "");
 
 // ---- PTX of the pair ------------------------------------------------------------------------------------------------------
 __device__ __forceinline__ void tma_load_2d_pair(uint32_t dst, const CUtensorMap *map, int x, int y, uint32_t bar) {
@@ -69,38 +74,41 @@ __device__ __forceinline__ void mbar_arrive_at(uint32_t cluster_addr) {
 }
 
 // ---- staged rows ------------------------------------------------------------------------------------------------------------
-// A warp's 32 rows of up to 128 bytes; 16-byte chunk c of row r lies at chunk c ^ (r & 7), so that both a thread writing its row and
-// eight lanes reading one row touch all banks.
-__device__ __forceinline__ uint4 *staged(uint8_t *base, int row, int chunk) { return reinterpret_cast<uint4 *>(base + row * 128 + ((chunk ^ (row & 7)) * 16)); }
+// A warp's 32 rows of 64 or 128 bytes, in 16-byte chunks whose places are permuted so that neither a thread writing its row nor
+// neighbouring lanes reading one row meet in a bank.
+template <int kRow> __device__ __forceinline__ uint4 *staged(uint8_t *base, int row, int chunk) {
+    return reinterpret_cast<uint4 *>(base + row * kRow + ((chunk ^ (kRow == 128 ? row & 7 : (row >> 1) & 3)) * 16));
+}
 
-// Rows [0, rows) x columns [0, cols) of elements of `kSize` bytes, `kRowBytes` staged per row, to out (row stride in bytes).
-template <int kSize, int kRowBytes> __device__ __forceinline__ void store_staged(uint8_t *base, uint8_t *out, int64_t row_bytes, int rows, int cols, int lane) {
-    constexpr int kChunks = kRowBytes / 16, kRowsAtOnce = 32 / kChunks, kPerChunk = 16 / kSize;
+// Rows [0, rows) x columns [0, cols) of elements of `kSize` bytes, kRow bytes staged per row, to out (row stride in bytes).
+template <int kSize, int kRow> __device__ __forceinline__ void store_staged(uint8_t *base, uint8_t *out, int64_t row_bytes, int rows, int cols, int lane) {
+    constexpr int kChunks = kRow / 16, kRowsAtOnce = 32 / kChunks, kPerChunk = 16 / kSize;
     if (rows <= 0 || cols <= 0) return;
     if ((((uintptr_t)out | (uintptr_t)row_bytes) & 15) == 0) {
         const int chunk = lane % kChunks, left = cols - chunk * kPerChunk;
+        uint8_t *p = out + (lane / kChunks) * row_bytes + chunk * 16;
 #pragma unroll
-        for (int r = lane / kChunks; r < 32; r += kRowsAtOnce) {
+        for (int i = 0; i < 32 / kRowsAtOnce; ++i, p += kRowsAtOnce * row_bytes) {
+            const int r = lane / kChunks + i * kRowsAtOnce;
             if (r < rows && left > 0) {
-                const uint4 v = *staged(base, r, chunk);
-                uint8_t *p = out + r * row_bytes + chunk * 16;
+                const uint4 v = *staged<kRow>(base, r, chunk);
                 if (left >= kPerChunk) *reinterpret_cast<uint4 *>(p) = v;
                 else {
                     const uint8_t *e = reinterpret_cast<const uint8_t *>(&v);
 #pragma unroll
-                    for (int i = 0; i < kPerChunk; ++i)
-                        if (i < left) {
-                            if constexpr (kSize == 1) p[i] = e[i];
-                            else if constexpr (kSize == 2) reinterpret_cast<uint16_t *>(p)[i] = reinterpret_cast<const uint16_t *>(e)[i];
-                            else reinterpret_cast<uint32_t *>(p)[i] = reinterpret_cast<const uint32_t *>(e)[i];
+                    for (int j = 0; j < kPerChunk; ++j)
+                        if (j < left) {
+                            if constexpr (kSize == 1) p[j] = e[j];
+                            else if constexpr (kSize == 2) reinterpret_cast<uint16_t *>(p)[j] = reinterpret_cast<const uint16_t *>(e)[j];
+                            else reinterpret_cast<uint32_t *>(p)[j] = reinterpret_cast<const uint32_t *>(e)[j];
                         }
                 }
             }
         }
     } else {  // rows that do not start at multiples of 16 bytes: element by element, neighbouring lanes neighbouring elements
         for (int r = 0; r < min(rows, 32); ++r)
-            for (int c = lane; c < min(cols, kRowBytes / kSize); c += 32) {
-                const uint8_t *e = reinterpret_cast<const uint8_t *>(staged(base, r, c / kPerChunk)) + c % kPerChunk * kSize;
+            for (int c = lane; c < min(cols, kRow / kSize); c += 32) {
+                const uint8_t *e = reinterpret_cast<const uint8_t *>(staged<kRow>(base, r, c / kPerChunk)) + c % kPerChunk * kSize;
                 uint8_t *p = out + r * row_bytes + (int64_t)c * kSize;
                 if constexpr (kSize == 1) *p = *e;
                 else if constexpr (kSize == 2) *reinterpret_cast<uint16_t *>(p) = *reinterpret_cast<const uint16_t *>(e);
@@ -125,7 +133,7 @@ __device__ __forceinline__ void load_staged(uint8_t *base, const uint8_t *in, in
                     if (i < left) e[i] = p[i];
             }
         }
-        *staged(base, r, chunk) = v;
+        *staged<128>(base, r, chunk) = v;
     }
 }
 
@@ -158,8 +166,9 @@ __global__ void __launch_bounds__(kThreads, 1) __cluster_dims__(2, 1, 1) matmul_
     constexpr bool kGated = kMode != kMatmulPlain;
     constexpr int kElems = kE4m3 ? 128 : 64;  // contraction elements of a K block
     constexpr int kCols = kGated ? 64 : 128;  // result columns of a thread
+    constexpr int kRow = staging_row(kE4m3);
     extern __shared__ __align__(1024) uint8_t smem[];
-    PairBarriers &sh = *reinterpret_cast<PairBarriers *>(smem + kRingBytes + 8 * kStagingBytes);
+    PairBarriers &sh = *reinterpret_cast<PairBarriers *>(smem + kRingBytes + 8 * staging_bytes(kE4m3));
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     const uint32_t rank = cluster_rank();
     const int pair = blockIdx.x >> 1, pairs = gridDim.x >> 1;
@@ -171,7 +180,7 @@ __global__ void __launch_bounds__(kThreads, 1) __cluster_dims__(2, 1, 1) matmul_
             mbar_init(&sh.empty[i], 1);
         }
         for (int i = 0; i < 2; ++i) {
-            mbar_init(&sh.acc_full[i], 1);
+            mbar_init(&sh.acc_full[i], kE4m3 ? 3 : 1);  // the products, and the two warps that bring their scales
             mbar_init(&sh.acc_empty[i], 16);
         }
         mbar_init(&sh.drained, 1);
@@ -184,7 +193,9 @@ __global__ void __launch_bounds__(kThreads, 1) __cluster_dims__(2, 1, 1) matmul_
     tc_fence_before();
     cluster_sync();  // both CTAs' barriers exist before either is signalled from the other
     tc_fence_after();
-    const uint32_t tmem = sh.tmem_base, ring = smem_u32(smem);
+    // All of the SM's tensor memory is allocated, so its base is column 0: the tensor-memory addresses are constants.
+    constexpr uint32_t tmem = 0;
+    const uint32_t ring = smem_u32(smem);
     const auto wait = [&](uint64_t *bar, uint32_t parity, uint32_t code) { return mbar_wait_limit(bar, parity, &sh.abort_flag, p.status, code, kWaitTicks); };
     const int total = p.tiles_per_problem * p.problems;
     struct Tile {
@@ -198,6 +209,11 @@ __global__ void __launch_bounds__(kThreads, 1) __cluster_dims__(2, 1, 1) matmul_
         w.n0 = (t % p.tiles_n) * (kGated ? kTile : kPairN);
         return w;
     };
+    if (sh.tmem_base != tmem && threadIdx.x == 0) {
+        sh.abort_flag = 1;
+        atomicOr(p.status, kErrSums);
+    }
+    cluster_sync();
     // both CTAs have to agree on whether they run: a flag that only one of them saw raised would leave the other waiting (boundedly)
     const bool dead = ld_cluster_u32(map_rank(smem_u32((const void *)&sh.abort_flag), 0)) != 0 || ld_cluster_u32(map_rank(smem_u32((const void *)&sh.abort_flag), 1)) != 0;
 
@@ -242,41 +258,120 @@ __global__ void __launch_bounds__(kThreads, 1) __cluster_dims__(2, 1, 1) matmul_
         }
         __syncwarp();
     } else if (warp == kIssuerWarp) {
-        if (lane == 0 && rank == 0) {
+        if (rank == 0) {
+            // Warp-uniform control flow and constant addresses, so that the operands of the tensor-core instructions are constants or
+            // uniform registers: moved from ordinary ones, a K block's six instructions took 430 to 550 clocks to issue.  `ok` is a
+            // lane's own: after a wait gave up its elected lane issues nothing more; it steers the loop by a vote every 32 blocks only.
             const uint32_t idesc = matmul_idesc(kE4m3, p.dtype == COME_BF16, 2 * kTile, kPairN, kAMn, kBMn);
             constexpr uint32_t kAStep = kAMn ? 2048 >> 4 : 32 >> 4, kBStep = kBMn ? 2048 >> 4 : 32 >> 4;
-            int it = 0, chunk = 0;  // K blocks, fills of a TMEM buffer so far
-            bool ok = true;
-            for (int t = pair; t < total && ok; t += pairs) {
-                for (int i = 0; i < p.k_blocks; ++i, ++it) {
-                    const int st = it % kStages, buf = chunk & 1;
-                    if (kE4m3 || i == 0) ok = wait(&sh.acc_empty[buf], ((chunk >> 1) & 1) ^ 1, kErrSums);
-                    ok = ok && wait(&sh.full[st], (it / kStages) & 1, kErrFull);
-                    if (!ok) break;
+            const uint64_t desc_a = operand_desc(ring, kOperandBytes / 2), desc_b = operand_desc(ring + kOperandBytes, kOperandBytes / 2);
+            uint32_t st = 0, st_phase = 0, buf = 0, buf_phase = 1;
+            bool ok = true, go = true;
+            const auto wait_here = [&](uint64_t *bar, uint32_t parity, uint32_t code) {
+                if (!mbar_try_wait(bar, parity)) ok = ok && wait(bar, parity, code);
+            };
+            for (int t = pair; t < total && go; t += pairs) {
+                for (int i = 0; i < p.k_blocks; ++i) {
+                    if ((i & 31) == 31 || i == 0) {
+                        go = __all_sync(0xffffffffu, ok);
+                        if (!go) break;
+                    }
+                    wait_here(&sh.full[st], st_phase, kErrFull);
+                    if (kE4m3 || i == 0) wait_here(&sh.acc_empty[buf], buf_phase, kErrSums);
+                    __syncwarp();
                     tc_fence_after();
-                    const uint64_t da = operand_desc(ring + st * kStageBytes, kOperandBytes / 2);
-                    const uint64_t db = operand_desc(ring + st * kStageBytes + kOperandBytes, kOperandBytes / 2);
-#pragma unroll
-                    for (int k = 0; k < 4; ++k)
-                        tc_mma_pair<kE4m3>(tmem + buf * kPairN, da + k * kAStep, db + k * kBStep, idesc, k > 0 || (!kE4m3 && i > 0) ? 1u : 0u);
-                    tc_commit_pair(&sh.empty[st]);
-                    if (kE4m3 || i == p.k_blocks - 1) {
-                        tc_commit_pair(&sh.acc_full[buf]);
-                        ++chunk;
+                    const uint64_t da = desc_a + (uint64_t)(st * (kStageBytes >> 4)), db = desc_b + (uint64_t)(st * (kStageBytes >> 4));
+                    const uint32_t d_tmem = buf * kPairN;
+                    const bool last = kE4m3 || i == p.k_blocks - 1;
+                    const uint32_t more = !kE4m3 && i > 0 ? 1u : 0u;
+                    if (elect_one() && ok) {
+                        tc_mma_pair<kE4m3>(d_tmem, da, db, idesc, more);
+                        tc_mma_pair<kE4m3>(d_tmem, da + kAStep, db + kBStep, idesc, 1u);
+                        tc_mma_pair<kE4m3>(d_tmem, da + 2 * kAStep, db + 2 * kBStep, idesc, 1u);
+                        tc_mma_pair<kE4m3>(d_tmem, da + 3 * kAStep, db + 3 * kBStep, idesc, 1u);
+                        tc_commit_pair(&sh.empty[st]);
+                        if (last) tc_commit_pair(&sh.acc_full[buf]);
+                    }
+                    __syncwarp();
+                    if (++st == kStages) {
+                        st = 0;
+                        st_phase ^= 1u;
+                    }
+                    if (last) {
+                        buf ^= 1u;
+                        if (buf == 0) buf_phase ^= 1u;
                     }
                 }
             }
-            tc_commit_pair(&sh.drained);
-            mbar_drain(&sh.drained, 0, p.status, kErrSums);
+            if (elect_one()) {
+                tc_commit_pair(&sh.drained);
+                mbar_drain(&sh.drained, 0, p.status, kErrSums);
+            }
         }
         __syncwarp();
+    } else if constexpr (kE4m3) {
+        // Warps 10, 11: the scales of a K block for 64 rows each, loaded two blocks ahead.  A warp arrives for block i after block i - 2 of
+        // the same TMEM buffer has completed: then every warp has read the scales of block i - 4, whose slot block i takes.
+        PairScales &scales = *reinterpret_cast<PairScales *>(&sh + 1);
+        const int r0 = (warp - kProducerWarp - 2) * 64 + lane;  // rows r0, r0 + 32
+        int chunk = 0;
+        bool ok = true;
+        float row[2][2], block[2][2];  // [parity of the K block]
+        int ahead_t = pair, ahead_k = 0;
+        const float *ahead_row[2] = {}, *ahead_block[2] = {};
+        const auto fetch = [&](int j) {
+            if (ahead_t >= total) return;
+            if (ahead_k == 0) {
+                const Tile w = tile_at(ahead_t);
+                const int nb = w.n0 / kTile, last = (p.N - 1) / kTile;  // past the last column block nothing is stored
+#pragma unroll
+                for (int i = 0; i < 2; ++i) {
+                    ahead_row[i] = p.a_scale + (int64_t)min(w.m0 + r0 + 32 * i, p.M - 1) * p.as_row;
+                    ahead_block[i] = kGated ? p.b_scale[i] + nb * p.bs_row[i] : p.b_scale[0] + min(nb + i, last) * p.bs_row[0];
+                }
+            }
+#pragma unroll
+            for (int i = 0; i < 2; ++i) {
+                row[j][i] = *ahead_row[i];
+                block[j][i] = *ahead_block[i];
+                ahead_row[i] += p.as_block;
+                ahead_block[i] += 1;
+            }
+            if (++ahead_k == p.k_blocks) {
+                ahead_k = 0;
+                ahead_t += pairs;
+            }
+        };
+        const int64_t blocks = (int64_t)((total - pair + pairs - 1) / pairs) * p.k_blocks;
+        fetch(0);
+        fetch(1);
+        for (int64_t i0 = 0; i0 < blocks && ok; i0 += 2) {
+#pragma unroll
+            for (int j = 0; j < 2; ++j) {
+                if (i0 + j < blocks && ok) {
+                    const int slot = chunk % kScaleSlots;
+                    if (chunk >= 2) ok = wait(&sh.acc_full[j], ((chunk >> 1) - 1) & 1, kErrSums);
+                    ok = __all_sync(0xffffffffu, ok);
+#pragma unroll
+                    for (int i = 0; i < 2; ++i) {
+                        scales[slot][0][r0 + 32 * i] = row[j][i] * block[j][0];
+                        scales[slot][1][r0 + 32 * i] = row[j][i] * block[j][1];
+                    }
+                    fetch(j);
+                    __syncwarp();
+                    if (ok && lane == 0) mbar_arrive(&sh.acc_full[j]);
+                    ++chunk;
+                }
+            }
+        }
     }
     } else {
     if constexpr (kE4m3) asm volatile("setmaxnreg.inc.sync.aligned.u32 232;");
     else asm volatile("setmaxnreg.inc.sync.aligned.u32 216;");
         const int part = warp >> 2, r = (warp & 3) * 32 + lane, warp_row = (warp & 3) * 32;
         const uint32_t lanes = tmem + ((uint32_t)warp_row << 16) + part * kCols;
-        uint8_t *stage = smem + kRingBytes + warp * kStagingBytes;
+        uint8_t *stage = smem + kRingBytes + warp * staging_bytes(kE4m3);
+        [[maybe_unused]] const PairScales &scales = *reinterpret_cast<const PairScales *>(&sh + 1);
         const uint32_t empty0 = map_rank(smem_u32(&sh.acc_empty[0]), 0);
         int chunk = 0, tiles = 0;
         bool ok = true;
@@ -303,48 +398,38 @@ __global__ void __launch_bounds__(kThreads, 1) __cluster_dims__(2, 1, 1) matmul_
                 f32x2_t sum[64];
 #pragma unroll
                 for (int c = 0; c < 64; ++c) sum[c] = 0ull;
-                const int nb = min(w.n0 / kTile + (kGated ? 0 : part), (p.N - 1) / kTile);  // column block; past the last one nothing is stored
-                const float *as = p.a_scale + (int64_t)min(w.m0 + r, p.M - 1) * p.as_row;
-                const float *bs0 = p.b_scale[0] + nb * p.bs_row[0], *bs1 = kGated ? p.b_scale[1] + nb * p.bs_row[1] : bs0;
-                // the scales of two K blocks ahead: a load takes longer than a block
-                float sa[2], sb0[2], sb1[2];
-                const auto fetch = [&](int j, int i) {
-                    const int kb = min(i, p.k_blocks - 1);
-                    sa[j] = as[kb * p.as_block];
-                    sb0[j] = bs0[kb];
-                    if constexpr (kGated) sb1[j] = bs1[kb];
-                };
-                fetch(0, 0);
-                fetch(1, 1);
-                for (int i0 = 0; i0 < p.k_blocks; i0 += 2) {
+                for (int i = 0; i < p.k_blocks; ++i, ++chunk) {
+                    const int buf = chunk & 1, slot = chunk % kScaleSlots;
+                    ok = ok && wait(&sh.acc_full[buf], (chunk >> 1) & 1, kErrSums);
+                    ok = __all_sync(0xffffffffu, ok);
+                    if (ok && busy) {
+                        tc_fence_after();
+                        const float s0 = scales[slot][kGated ? 0 : part][r], s1 = kGated ? scales[slot][1][r] : s0;
+                        const f32x2_t s0p = pack_f32x2(s0, s0), s1p = pack_f32x2(s1, s1);
+                        const auto column = [&](int c) { return lanes + buf * kPairN + (kGated ? (c >> 1) * kTile + (c & 1) * 32 : c * 32); };
+                        uint32_t d[2][32];
+                        const auto add = [&](int c) {
 #pragma unroll
-                    for (int j = 0; j < 2; ++j) {
-                        if (i0 + j < p.k_blocks) {
-                            const int buf = chunk & 1;
-                            const float s0 = sa[j] * sb0[j], s1 = kGated ? sa[j] * sb1[j] : s0;
-                            fetch(j, i0 + j + 2);
-                            ok = ok && wait(&sh.acc_full[buf], (chunk >> 1) & 1, kErrSums);
-                            ok = __all_sync(0xffffffffu, ok);
-                            if (ok && busy) {
-                                tc_fence_after();
-                                const f32x2_t s0p = pack_f32x2(s0, s0), s1p = pack_f32x2(s1, s1);
-                                const auto column = [&](int c) { return lanes + buf * kPairN + (kGated ? (c >> 1) * kTile + (c & 1) * 32 : c * 32); };
-                                uint32_t d[2][32];
-                                tmem_ld32(column(0), d[0]);
-#pragma unroll
-                                for (int c = 0; c < 4; ++c) {
-                                    tc_wait_ld_of(d[c & 1]);
-                                    if (c < 3) tmem_ld32(column(c + 1), d[(c + 1) & 1]);
-#pragma unroll
-                                    for (int e = 0; e < 16; ++e)
-                                        sum[c * 16 + e] = fma_f32x2(pack_f32x2(__uint_as_float(d[c & 1][2 * e]), __uint_as_float(d[c & 1][2 * e + 1])), c >> 1 ? s1p : s0p, sum[c * 16 + e]);
-                                }
-                                tc_fence_before();
-                            }
-                            __syncwarp();
-                            if (ok && lane == 0) mbar_arrive_at(empty0 + buf * 8);
-                            ++chunk;
-                        }
+                            for (int e = 0; e < 16; ++e)
+                                sum[c * 16 + e] = fma_f32x2(pack_f32x2(__uint_as_float(d[c & 1][2 * e]), __uint_as_float(d[c & 1][2 * e + 1])), c >> 1 ? s1p : s0p, sum[c * 16 + e]);
+                        };
+                        tmem_ld32(column(0), d[0]);
+                        tmem_ld32(column(1), d[1]);
+                        tc_wait_ld_of(d[0]);
+                        tc_wait_ld_of(d[1]);
+                        add(0);
+                        tmem_ld32(column(2), d[0]);
+                        add(1);
+                        tmem_ld32(column(3), d[1]);
+                        tc_wait_ld_of(d[0]);
+                        tc_wait_ld_of(d[1]);
+                        tc_fence_before();
+                        __syncwarp();
+                        if (lane == 0) mbar_arrive_at(empty0 + buf * 8);  // the buffer is in registers
+                        add(2);
+                        add(3);
+                    } else if (ok && lane == 0) {
+                        mbar_arrive_at(empty0 + buf * 8);
                     }
                 }
                 if constexpr (!kGated) {
@@ -361,36 +446,36 @@ __global__ void __launch_bounds__(kThreads, 1) __cluster_dims__(2, 1, 1) matmul_
                         if (p.out_dtype == COME_F32) {
                             uint8_t *out = (uint8_t *)p.out[0] + (row0 * p.out_row[0] + n) * 4;
 #pragma unroll
-                            for (int h = 0; h < 4; ++h) {
+                            for (int h = 0; h < 8; ++h) {
 #pragma unroll
-                                for (int c = 0; c < 8; ++c) {
+                                for (int c = 0; c < 4; ++c) {
                                     float v[4];
-                                    unpack_f32x2(sum[h * 16 + c * 2], v[0], v[1]);
-                                    unpack_f32x2(sum[h * 16 + c * 2 + 1], v[2], v[3]);
-                                    *staged(stage, lane, c) = make_uint4(__float_as_uint(v[0]), __float_as_uint(v[1]), __float_as_uint(v[2]), __float_as_uint(v[3]));
+                                    unpack_f32x2(sum[h * 8 + c * 2], v[0], v[1]);
+                                    unpack_f32x2(sum[h * 8 + c * 2 + 1], v[2], v[3]);
+                                    *staged<kRow>(stage, lane, c) = make_uint4(__float_as_uint(v[0]), __float_as_uint(v[1]), __float_as_uint(v[2]), __float_as_uint(v[3]));
                                 }
                                 __syncwarp();
-                                store_staged<4, 128>(stage, out + h * 128, p.out_row[0] * 4, rows, cols - h * 32, lane);
+                                store_staged<4, kRow>(stage, out + h * kRow, p.out_row[0] * 4, rows, cols - h * 16, lane);
                                 __syncwarp();
                             }
                         } else {
                             as_constant(p.out_dtype == COME_BF16, [&](auto bf16) {
                                 uint8_t *out = (uint8_t *)p.out[0] + (row0 * p.out_row[0] + n) * 2;
 #pragma unroll
-                                for (int h = 0; h < 2; ++h) {
+                                for (int h = 0; h < 4; ++h) {
 #pragma unroll
-                                    for (int c = 0; c < 8; ++c) {
+                                    for (int c = 0; c < 4; ++c) {
                                         uint32_t e[4];
 #pragma unroll
                                         for (int j = 0; j < 4; ++j) {
                                             float lo, hi;
-                                            unpack_f32x2(sum[h * 32 + c * 4 + j], lo, hi);
+                                            unpack_f32x2(sum[h * 16 + c * 4 + j], lo, hi);
                                             e[j] = pack_16<decltype(bf16)::value>(lo, hi);
                                         }
-                                        *staged(stage, lane, c) = make_uint4(e[0], e[1], e[2], e[3]);
+                                        *staged<kRow>(stage, lane, c) = make_uint4(e[0], e[1], e[2], e[3]);
                                     }
                                     __syncwarp();
-                                    store_staged<2, 128>(stage, out + h * 128, p.out_row[0] * 2, rows, cols - h * 64, lane);
+                                    store_staged<2, kRow>(stage, out + h * kRow, p.out_row[0] * 2, rows, cols - h * 32, lane);
                                     __syncwarp();
                                 }
                             });
@@ -442,27 +527,30 @@ __global__ void __launch_bounds__(kThreads, 1) __cluster_dims__(2, 1, 1) matmul_
                                     const float *e = h + c * 16 + j * 4;
                                     q[j] = pack_e4m3(e[0] * inv, e[1] * inv, e[2] * inv, e[3] * inv);
                                 }
-                                *staged(stage, lane, c) = make_uint4(q[0], q[1], q[2], q[3]);
+                                *staged<kRow>(stage, lane, c) = make_uint4(q[0], q[1], q[2], q[3]);
                             }
                             __syncwarp();
-                            store_staged<1, 64>(stage, (uint8_t *)p.out[0] + row0 * p.out_row[0] + n, p.out_row[0], rows, cols, lane);
+                            store_staged<1, kRow>(stage, (uint8_t *)p.out[0] + row0 * p.out_row[0] + n, p.out_row[0], rows, cols, lane);
                             if (part == 0 && lane < rows) p.out_scale[(row0 + lane) * p.os_row + (w.n0 / kTile) * p.os_block] = top / kE4m3Max;
                             __syncwarp();
                         }
                     } else if (ok && busy) {
                         as_constant(p.out_dtype == COME_BF16, [&](auto bf16) {
 #pragma unroll
-                            for (int c = 0; c < 8; ++c) {
-                                const float *e = h + c * 8;
-                                uint32_t q[4];
+                            for (int half = 0; half < 2; ++half) {
 #pragma unroll
-                                for (int j = 0; j < 4; ++j) q[j] = pack_16<decltype(bf16)::value>(e[2 * j], e[2 * j + 1]);
-                                *staged(stage, lane, c) = make_uint4(q[0], q[1], q[2], q[3]);
+                                for (int c = 0; c < 4; ++c) {
+                                    const float *e = h + half * 32 + c * 8;
+                                    uint32_t q[4];
+#pragma unroll
+                                    for (int j = 0; j < 4; ++j) q[j] = pack_16<decltype(bf16)::value>(e[2 * j], e[2 * j + 1]);
+                                    *staged<kRow>(stage, lane, c) = make_uint4(q[0], q[1], q[2], q[3]);
+                                }
+                                __syncwarp();
+                                store_staged<2, kRow>(stage, (uint8_t *)p.out[0] + (row0 * p.out_row[0] + n + half * 32) * 2, p.out_row[0] * 2, rows, cols - half * 32, lane);
+                                __syncwarp();
                             }
                         });
-                        __syncwarp();
-                        store_staged<2, 128>(stage, (uint8_t *)p.out[0] + (row0 * p.out_row[0] + n) * 2, p.out_row[0] * 2, rows, cols, lane);
-                        __syncwarp();
                     }
                 }
             } else {
@@ -502,10 +590,10 @@ __global__ void __launch_bounds__(kThreads, 1) __cluster_dims__(2, 1, 1) matmul_
                                     uint32_t e[4];
 #pragma unroll
                                     for (int j = 0; j < 4; ++j) e[j] = pack_16<kBF16>(__uint_as_float(d[c >> 2][(c & 3) * 8 + 2 * j]), __uint_as_float(d[c >> 2][(c & 3) * 8 + 2 * j + 1]));
-                                    *staged(stage, lane, c) = make_uint4(e[0], e[1], e[2], e[3]);
+                                    *staged<kRow>(stage, lane, c) = make_uint4(e[0], e[1], e[2], e[3]);
                                 }
                                 __syncwarp();
-                                store_staged<2, 128>(stage, (uint8_t *)p.out[w.problem] + (row0 * p.out_row[w.problem] + n + h * 64) * 2, p.out_row[w.problem] * 2, rows, cols - h * 64, lane);
+                                store_staged<2, kRow>(stage, (uint8_t *)p.out[w.problem] + (row0 * p.out_row[w.problem] + n + h * 64) * 2, p.out_row[w.problem] * 2, rows, cols - h * 64, lane);
                                 __syncwarp();
                             }
                         } else {
@@ -531,7 +619,7 @@ __global__ void __launch_bounds__(kThreads, 1) __cluster_dims__(2, 1, 1) matmul_
                                         uint32_t e[4];
                                         [[maybe_unused]] uint32_t dh[4];
                                         if constexpr (kMode == kMatmulGatedGrad) {
-                                            const uint4 raw = *staged(stage, lane, q * 4 + c);
+                                            const uint4 raw = *staged<kRow>(stage, lane, q * 4 + c);
                                             dh[0] = raw.x, dh[1] = raw.y, dh[2] = raw.z, dh[3] = raw.w;
                                         }
 #pragma unroll
@@ -552,17 +640,17 @@ __global__ void __launch_bounds__(kThreads, 1) __cluster_dims__(2, 1, 1) matmul_
                                                 second[(q * 4 + c) * 4 + j] = pack_16<kBF16>(d0 * a0, d1 * a1);
                                             }
                                         }
-                                        *staged(stage, lane, q * 4 + c) = make_uint4(e[0], e[1], e[2], e[3]);
+                                        *staged<kRow>(stage, lane, q * 4 + c) = make_uint4(e[0], e[1], e[2], e[3]);
                                     }
                                 }
                                 __syncwarp();
-                                store_staged<2, 128>(stage, (uint8_t *)p.out[0] + (row0 * p.out_row[0] + n) * 2, p.out_row[0] * 2, rows, cols, lane);
+                                store_staged<2, kRow>(stage, (uint8_t *)p.out[0] + (row0 * p.out_row[0] + n) * 2, p.out_row[0] * 2, rows, cols, lane);
                                 __syncwarp();
                                 if constexpr (kMode == kMatmulGatedGrad) {
 #pragma unroll
-                                    for (int c = 0; c < 8; ++c) *staged(stage, lane, c) = make_uint4(second[4 * c], second[4 * c + 1], second[4 * c + 2], second[4 * c + 3]);
+                                    for (int c = 0; c < 8; ++c) *staged<kRow>(stage, lane, c) = make_uint4(second[4 * c], second[4 * c + 1], second[4 * c + 2], second[4 * c + 3]);
                                     __syncwarp();
-                                    store_staged<2, 128>(stage, (uint8_t *)p.out[1] + (row0 * p.out_row[1] + n) * 2, p.out_row[1] * 2, rows, cols, lane);
+                                    store_staged<2, kRow>(stage, (uint8_t *)p.out[1] + (row0 * p.out_row[1] + n) * 2, p.out_row[1] * 2, rows, cols, lane);
                                     __syncwarp();
                                 }
                             });
@@ -591,9 +679,9 @@ __global__ void __launch_bounds__(kThreads, 1) __cluster_dims__(2, 1, 1) matmul_
 
 template <bool kE4m3, int kMode, bool kAMn, bool kBMn> int launch_pair(const MatmulParams &p, cudaStream_t st) {
     constexpr auto kernel = matmul_pair_kernel<kE4m3, kMode, kAMn, kBMn>;
-    if (int rc = allow_smem<kernel>(kSmemBytes); rc != COME_OK) return rc;
+    if (int rc = allow_smem<kernel>(smem_bytes(kE4m3)); rc != COME_OK) return rc;
     const int tiles = p.tiles_per_problem * p.problems, pairs = sm_count() / 2;
-    kernel<<<2 * (tiles < pairs ? tiles : pairs), kThreads, kSmemBytes, st>>>(p);
+    kernel<<<2 * (tiles < pairs ? tiles : pairs), kThreads, smem_bytes(kE4m3), st>>>(p);
     return check_launch("product kernel");
 }
 

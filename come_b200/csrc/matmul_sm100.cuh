@@ -173,21 +173,28 @@ static_assert((kErrFull | kErrEmpty | kErrSums) == kStatusMatmul, "come_device_s
 
 
 // act(g) and its derivative.  silu: g s with s = 1 / (1 + e^-g), derivative s (1 + g (1 - s)); gelu: g Phi(g), derivative
-// Phi(g) + g phi(g).  A g so low that e^-g overflows gives s = 0 and a product of -0.
+// Phi(g) + g phi(g).  The logistic function is one exponential and one reciprocal of the special-function unit, each good to about
+// 2^-22 (denormals flushed: where e^-g leaves the range, s is 0 or 1 to float32), so that an element costs six instructions.
+__device__ __forceinline__ float logistic(float g) {
+    float e, s;
+    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(e) : "f"(g * -1.4426950408889634f));
+    asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(s) : "f"(1.0f + e));
+    return s;
+}
 __device__ __forceinline__ float activation(float g, int act) {
-    if (act == COME_ACT_SILU) return __fdividef(g, 1.0f + __expf(-g));
+    if (act == COME_ACT_SILU) return g * logistic(g);
     return 0.5f * g * erfcf(g * -0.70710678118654752f);
 }
 __device__ __forceinline__ void activation_grad(float g, int act, float &value, float &slope) {
     if (act == COME_ACT_SILU) {
-        const float s = __fdividef(1.0f, 1.0f + __expf(-g));
+        const float s = logistic(g);
         value = g * s;
-        slope = s * (1.0f + g * (1.0f - s));
+        slope = fmaf(value, 1.0f - s, s);
     } else {
         const float phi = 0.3989422804014327f * __expf(-0.5f * g * g);
         const float cdf = 0.5f * erfcf(g * -0.70710678118654752f);
         value = g * cdf;
-        slope = cdf + g * phi;
+        slope = fmaf(g, phi, cdf);
     }
 }
 
