@@ -13,7 +13,10 @@ from typing import Optional
 
 import torch
 
+from . import _lib
+from ._torch_util import dtype_code, on_device, ptr, require_cuda, stream_ptr
 from .bias_attention import JaggedAttention_w_Bias
+from .block_scaled import empty_rows
 from .plain_attention import JaggedAttention
 from .token_merger import JaggedTokens
 
@@ -62,8 +65,6 @@ def residual_layernorm(x: torch.Tensor, branch: Optional[torch.Tensor], scale: O
     (``src/accelerate/vggt/module/block.py:66-79``), which the module path runs as three elementwise kernels.
     ``branch`` None: the norm of ``x`` alone; ``scale`` None: no LayerScale; ``norm`` None: the update alone.
     Returns ``(x_out, normed)``; ``x_out`` is ``x`` itself when there is no branch and None when ``store_stream`` is off."""
-    from . import _lib
-    from ._torch_util import dtype_code, on_device, ptr, require_cuda, stream_ptr
     require_cuda(x, "x")
     if x.dim() != 2 or not x.is_contiguous():
         raise ValueError(f"x must be a contiguous [rows, C] tensor, got {tuple(x.shape)}")
@@ -103,42 +104,45 @@ def residual_rmsnorm(x: torch.Tensor, branch: Optional[torch.Tensor], scale: Opt
     Returns ``(x_out, normed)``; ``x_out`` is ``x`` itself when there is no branch and None when ``store_stream`` is off.  With
     ``quantize`` the normed rows leave in 8 bits with a scale per row and 128 columns
     (:class:`come_b200.block_scaled.BlockScaled`), the operand of the block-scaled products.  Inference only."""
-    from . import _lib
-    from ._torch_util import dtype_code, on_device, ptr, require_cuda, stream_ptr
     require_cuda(x, "x")
     if x.dim() != 2 or not x.is_contiguous():
         raise ValueError(f"x must be a contiguous [rows, C] tensor, got {tuple(x.shape)}")
+    rows, Cc = x.shape
+    dt, dev, index = x.dtype, x.device, x.get_device()
+    code = dtype_code(dt, "x")
+    if branch is not None and (branch.shape != x.shape or branch.dtype is not dt or branch.get_device() != index or not branch.is_contiguous()):
+        raise ValueError(f"branch must be contiguous and match x {tuple(x.shape)} {dt}, got {tuple(branch.shape)} {branch.dtype}")
     if torch.is_grad_enabled() and (x.requires_grad or (branch is not None and branch.requires_grad)):
         raise RuntimeError("residual_rmsnorm: inference only (no autograd)")
-    rows, Cc = x.shape
-    dt, dev = x.dtype, x.device
-    code = dtype_code(dt, "x")
-    if branch is not None and (branch.shape != x.shape or branch.dtype != dt or branch.device != dev or not branch.is_contiguous()):
-        raise ValueError(f"branch must be contiguous and match x {tuple(x.shape)} {dt}, got {tuple(branch.shape)} {branch.dtype}")
     if scale is not None:
         if branch is None:
             raise ValueError("scale without a branch")
-        scale = scale.detach().to(device=dev, dtype=dt).contiguous()
+        scale = _channel_vector(scale, dt, dev, index)
         if scale.shape != (Cc,):
             raise ValueError(f"scale must be [{Cc}], got {tuple(scale.shape)}")
     if not isinstance(norm, torch.nn.RMSNorm) or tuple(norm.normalized_shape) != (Cc,):
         raise NotImplementedError("residual_rmsnorm needs an nn.RMSNorm over the channel dimension")
     weight = norm.weight
     if weight is not None:
-        weight = weight.detach().to(device=dev, dtype=dt).contiguous()
+        weight = _channel_vector(weight, dt, dev, index)
     eps = float(norm.eps) if norm.eps is not None else torch.finfo(dt).eps
     x_out = torch.empty_like(x) if (branch is not None and store_stream) else None
     if quantize:
-        from .block_scaled import empty_rows
         normed = empty_rows(rows, Cc, dev)
         q = (None, normed.data.data_ptr(), normed.data.stride(0), normed.scale.data_ptr(), *normed.scale.stride())
     else:
         normed = torch.empty_like(x)
         q = (normed.data_ptr(), None, 0, None, 0, 0)
     with on_device(dev):
-        _lib.check(_lib.lib().come_residual_rmsnorm(ptr(x), ptr(branch), ptr(scale), rows, Cc, code, ptr(weight), eps, ptr(x_out), *q,
+        _lib.check(_lib.lib().come_residual_rmsnorm(x.data_ptr(), ptr(branch), ptr(scale), rows, Cc, code, ptr(weight), eps, ptr(x_out), *q,
                                                     stream_ptr(dev)))
     return (x if branch is None else x_out), normed
+
+
+def _channel_vector(t: torch.Tensor, dtype: torch.dtype, device, index: int) -> torch.Tensor:
+    if t.dtype is dtype and t.get_device() == index and t.is_contiguous():
+        return t
+    return t.detach().to(device=device, dtype=dtype).contiguous()
 
 
 def _layer_scale_gamma(ls: torch.nn.Module):

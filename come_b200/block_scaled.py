@@ -15,7 +15,7 @@ from typing import NamedTuple, Optional
 import torch
 
 from . import _lib
-from ._torch_util import dtype_code, on_device, ptr, require_cuda, stream_ptr
+from ._torch_util import dtype_code, on_device, require_cuda, stream_ptr
 
 __all__ = ["BLOCK", "BlockScaled", "quantize_rows", "quantize_weight", "block_scaled_linear", "block_scaled_gated_linear",
            "BlockScaledLinear", "BlockScaledGatedMlp"]
@@ -48,8 +48,9 @@ class BlockScaled(NamedTuple):
 def empty_rows(rows: int, cols: int, device) -> BlockScaled:
     """Uninitialised tokens in 8 bits: rows padded to whole 16 bytes, scales with the rows next to each other (the order in which a
     product's threads read them)."""
-    data = torch.empty((rows, -(-cols // 16) * 16), dtype=torch.float8_e4m3fn, device=device)[:, :cols]
-    return BlockScaled(data, torch.empty((_blocks(cols), rows), dtype=torch.float32, device=device).t())
+    # (empty_strided: the cheapest of torch's allocating calls, which are half of a small launch's host time)
+    return BlockScaled(torch.empty_strided((rows, cols), ((cols + 15) & ~15, 1), dtype=torch.float8_e4m3fn, device=device),
+                       torch.empty_strided((rows, (cols + 127) >> 7), (1, rows or 1), dtype=torch.float32, device=device))
 
 
 def _matrix(x: torch.Tensor, name: str) -> torch.Tensor:
@@ -86,48 +87,70 @@ def quantize_weight(w: torch.Tensor) -> BlockScaled:
     return BlockScaled(data, scale)
 
 
-def _check_operand(t: BlockScaled, name: str, rows_per_scale: int, cols: Optional[int], device) -> None:
+def _tokens(t: BlockScaled):
+    """(pointer, row stride, scale pointer, its two strides), rows, columns of checked tokens."""
+    data, scale = t
+    if data.dim() == 2 and scale.dim() == 2 and data.is_cuda:
+        rows, cols = data.shape
+        row, col = data.stride()
+        if (data.dtype is torch.float8_e4m3fn and scale.dtype is torch.float32 and cols > 0 and scale.shape == (rows, (cols + 127) >> 7)
+                and data.get_device() == scale.get_device() and ((col == 1 and row % 16 == 0 and row >= cols and data.data_ptr() % 16 == 0) or rows == 0)):
+            return (data.data_ptr(), row, scale.data_ptr(), *scale.stride()), rows, cols
+    raise _operand_error(t, "x", True, None, None)
+
+
+def _weight(t: BlockScaled, name: str, cols: int, index: int):
+    """(pointer, row stride, scale pointer, its row stride), rows of a checked weight."""
+    data, scale = t
+    if data.dim() == 2 and scale.dim() == 2 and data.is_cuda:
+        rows, width = data.shape
+        row, col = data.stride()
+        s_row, s_block = scale.stride()
+        if (data.dtype is torch.float8_e4m3fn and scale.dtype is torch.float32 and width == cols
+                and scale.shape == ((rows + 127) >> 7, (cols + 127) >> 7) and (s_block == 1 or cols <= BLOCK)
+                and data.get_device() == index and scale.get_device() == index
+                and ((col == 1 and row % 16 == 0 and row >= cols and data.data_ptr() % 16 == 0) or rows == 0)):
+            return (data.data_ptr(), row, scale.data_ptr(), s_row), rows
+    raise _operand_error(t, name, False, cols, index)
+
+
+def _operand_error(t: BlockScaled, name: str, tokens: bool, cols: Optional[int], index: Optional[int]) -> Exception:
     data, scale = t
     if data.dtype != torch.float8_e4m3fn or scale.dtype != torch.float32:
-        raise RuntimeError(f"{name}: needs float8_e4m3fn numbers and float32 scales, got {data.dtype} and {scale.dtype}")
-    if not data.is_cuda or data.device != device or scale.device != device:
-        raise RuntimeError(f"{name} must be on CUDA, on the device of x")
+        return RuntimeError(f"{name}: needs float8_e4m3fn numbers and float32 scales, got {data.dtype} and {scale.dtype}")
+    if not data.is_cuda or not scale.is_cuda or data.get_device() != scale.get_device() or (index is not None and data.get_device() != index):
+        return RuntimeError(f"{name} must be on CUDA, its numbers and scales on the device of x")
     if data.dim() != 2 or data.shape[1] == 0 or (cols is not None and data.shape[1] != cols):
-        raise ValueError(f"{name} must be [rows, {'C' if cols is None else cols}], got {tuple(data.shape)}")
+        return ValueError(f"{name} must be [rows, {'C' if cols is None else cols}], got {tuple(data.shape)}")
     rows, width = data.shape
-    want = (rows if rows_per_scale == 1 else -(-rows // BLOCK), -(-width // BLOCK))
-    if tuple(scale.shape) != want:
-        raise ValueError(f"{name}: scales must be {list(want)}, got {list(scale.shape)}")
-    if rows and (data.stride(1) != 1 or data.stride(0) % 16 or data.stride(0) < width or data.data_ptr() % 16):
-        raise ValueError(f"{name}: rows must start at multiples of 16 bytes and be contiguous (strides {data.stride()})")
-    if rows_per_scale != 1 and scale.shape[1] > 1 and scale.stride(1) != 1:
-        raise ValueError(f"{name}: the scales of a weight must have contiguous rows")
+    want = [rows if tokens else -(-rows // BLOCK), -(-width // BLOCK)]
+    if list(scale.shape) != want:
+        return ValueError(f"{name}: scales must be {want}, got {list(scale.shape)}")
+    if data.stride(1) != 1 or data.stride(0) % 16 or data.stride(0) < width or data.data_ptr() % 16:
+        return ValueError(f"{name}: rows must start at multiples of 16 bytes and be contiguous (strides {data.stride()})")
+    return ValueError(f"{name}: the scales of a weight must have contiguous rows (strides {scale.stride()})")
 
 
-def _check_bias(bias: Optional[torch.Tensor], name: str, features: int, device) -> None:
+def _bias_ptr(bias: Optional[torch.Tensor], name: str, features: int, index: int):
     if bias is None:
-        return
-    if bias.dtype != torch.float32 or tuple(bias.shape) != (features,) or bias.device != device or not bias.is_contiguous():
-        raise ValueError(f"{name} must be a contiguous float32 [{features}] on {device}, got {bias.dtype} {tuple(bias.shape)} on {bias.device}")
+        return None
+    if bias.dtype is not torch.float32 or bias.shape != (features,) or bias.get_device() != index or not bias.is_contiguous():
+        raise ValueError(f"{name} must be a contiguous float32 [{features}] on the device of x, got {bias.dtype} {tuple(bias.shape)} on {bias.device}")
+    return bias.data_ptr()
 
 
 def block_scaled_linear(x: BlockScaled, weight: BlockScaled, bias: Optional[torch.Tensor] = None,
                         out_dtype: torch.dtype = torch.bfloat16) -> torch.Tensor:
     """``x @ weight.T + bias`` of 8-bit operands (``come_matmul_e4m3``): ``x [T, C]`` with a scale per row and 128 columns, ``weight
     [N, C]`` with one per 128 x 128 block, ``bias [N]`` float32.  Returns ``[T, N]`` in float32, float16 or bfloat16."""
-    dev = x.data.device
-    _check_operand(x, "x", 1, None, dev)
-    tokens, cols = x.data.shape
-    _check_operand(weight, "weight", BLOCK, cols, dev)
-    features = weight.data.shape[0]
-    _check_bias(bias, "bias", features, dev)
+    x_args, tokens, cols = _tokens(x)
+    index, dev = x.data.get_device(), x.data.device
+    w_args, features = _weight(weight, "weight", cols, index)
+    bias_ptr = _bias_ptr(bias, "bias", features, index)
     code = dtype_code(out_dtype, "out_dtype")
-    out = torch.empty((tokens, features), dtype=out_dtype, device=dev)
-    xs, ws = x.scale, weight.scale
+    out = torch.empty_strided((tokens, features), (features or 1, 1), dtype=out_dtype, device=dev)
     with on_device(dev):
-        _lib.check(_lib.lib().come_matmul_e4m3(x.data.data_ptr(), x.data.stride(0), xs.data_ptr(), xs.stride(0), xs.stride(1),
-                                               weight.data.data_ptr(), weight.data.stride(0), ws.data_ptr(), ws.stride(0), ptr(bias),
-                                               tokens, features, cols, out.data_ptr(), features, code, stream_ptr(dev)))
+        _lib.check(_lib.lib().come_matmul_e4m3(*x_args, *w_args, bias_ptr, tokens, features, cols, out.data_ptr(), features, code, stream_ptr(dev)))
     return out
 
 
@@ -137,31 +160,24 @@ def block_scaled_gated_linear(x: BlockScaled, gate: BlockScaled, up: BlockScaled
     """``act(x @ gate.T + gate_bias) * (x @ up.T + up_bias)`` of 8-bit operands in one kernel (``come_gated_matmul_e4m3``).
     ``activation``: "silu" or "gelu" (the exact one).  Returns ``[T, F]`` in ``out_dtype`` (float16 or bfloat16) or, by default, in
     8 bits (:class:`BlockScaled`): the operand of the down projection, quantised from the float32 values."""
-    dev = x.data.device
-    _check_operand(x, "x", 1, None, dev)
-    tokens, cols = x.data.shape
-    _check_operand(gate, "gate", BLOCK, cols, dev)
-    features = gate.data.shape[0]
-    _check_operand(up, "up", BLOCK, cols, dev)
-    if up.data.shape[0] != features:
-        raise ValueError(f"gate and up must have the same features, got {features} and {up.data.shape[0]}")
-    _check_bias(gate_bias, "gate_bias", features, dev)
-    _check_bias(up_bias, "up_bias", features, dev)
+    x_args, tokens, cols = _tokens(x)
+    index, dev = x.data.get_device(), x.data.device
+    g_args, features = _weight(gate, "gate", cols, index)
+    u_args, up_features = _weight(up, "up", cols, index)
+    if up_features != features:
+        raise ValueError(f"gate and up must have the same features, got {features} and {up_features}")
+    gb, ub = _bias_ptr(gate_bias, "gate_bias", features, index), _bias_ptr(up_bias, "up_bias", features, index)
     act = activation_code(activation)
     if out_dtype is None:
         out = empty_rows(tokens, features, dev)
-        where = (out.data.data_ptr(), out.data.stride(0), _lib.COME_E4M3, out.scale.data_ptr(), out.scale.stride(0), out.scale.stride(1))
+        where = (out.data.data_ptr(), out.data.stride(0), _lib.COME_E4M3, out.scale.data_ptr(), *out.scale.stride())
     else:
         if out_dtype not in (torch.float16, torch.bfloat16):
             raise RuntimeError(f"out_dtype: unsupported dtype {out_dtype}; expected float16, bfloat16 or None (8 bits)")
-        out = torch.empty((tokens, features), dtype=out_dtype, device=dev)
+        out = torch.empty_strided((tokens, features), (features or 1, 1), dtype=out_dtype, device=dev)
         where = (out.data_ptr(), features, dtype_code(out_dtype), None, 0, 0)
-    xs, gs, us = x.scale, gate.scale, up.scale
     with on_device(dev):
-        _lib.check(_lib.lib().come_gated_matmul_e4m3(
-            x.data.data_ptr(), x.data.stride(0), xs.data_ptr(), xs.stride(0), xs.stride(1), gate.data.data_ptr(), gate.data.stride(0),
-            gs.data_ptr(), gs.stride(0), up.data.data_ptr(), up.data.stride(0), us.data_ptr(), us.stride(0), ptr(gate_bias), ptr(up_bias),
-            act, tokens, features, cols, *where, stream_ptr(dev)))
+        _lib.check(_lib.lib().come_gated_matmul_e4m3(*x_args, *g_args, *u_args, gb, ub, act, tokens, features, cols, *where, stream_ptr(dev)))
     return out
 
 

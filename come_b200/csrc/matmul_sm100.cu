@@ -418,13 +418,19 @@ __global__ void __launch_bounds__(256) column_sums_kernel(const T *__restrict__ 
     if (!out) return;
     const int c = blockIdx.x * 32 + (threadIdx.x & 3) * 8, r0 = threadIdx.x >> 2;
     float sum[8] = {};
-    if (c < cols)  // rows are stored with a stride of whole 16 bytes: a vector that begins inside a row ends inside its stride
+    if (c + 8 <= cols) {
         for (int64_t r = r0; r < rows; r += 64) {
             const uint4 raw = *reinterpret_cast<const uint4 *>(x + r * row_stride + c);
             const T *e = reinterpret_cast<const T *>(&raw);
 #pragma unroll
             for (int i = 0; i < 8; ++i) sum[i] += Elem<T>::to_f32(e[i]);
         }
+    } else if (c < cols) {  // the last row may end with its last element
+        for (int64_t r = r0; r < rows; r += 64)
+#pragma unroll
+            for (int i = 0; i < 8; ++i)
+                if (c + i < cols) sum[i] += Elem<T>::to_f32(x[r * row_stride + c + i]);
+    }
 #pragma unroll
     for (int i = 0; i < 8; ++i) part[r0][(threadIdx.x & 3) * 8 + i] = sum[i];
     __syncthreads();

@@ -19,7 +19,7 @@ struct RmsNormArgs {
     const void *x, *branch, *scale, *weight;
     int64_t rows, x_row;  // row stride of x in elements; branch, x_out and normed are contiguous
     int C;
-    float eps;
+    float eps, inv_C;
     bool norm;            // off: quantise x as it is
     void *x_out, *normed;
     uint8_t *q;
@@ -28,30 +28,40 @@ struct RmsNormArgs {
     int64_t s_row, s_block;
 };
 
-// VEC elements of a row from column c on; kAligned: one 16-byte access, the row's width is a whole number of them.  kOnce: a
+// VEC elements of a row from column c on as 16 raw bytes; kAligned: one access, the row's width is a whole number of them.  kOnce: a
 // row that is read once, against the scale and weight vectors that every row reads.
-template <typename T, int VEC, bool kAligned, bool kOnce> __device__ __forceinline__ void load_row(const T *p, int c, int C, float (&v)[VEC]) {
+template <typename T, int VEC, bool kAligned, bool kOnce> __device__ __forceinline__ uint4 load_raw(const T *p, int c, int C) {
     if constexpr (kAligned) {
-        const uint4 raw = kOnce ? __ldcs(reinterpret_cast<const uint4 *>(p + c)) : __ldg(reinterpret_cast<const uint4 *>(p + c));
-        const T *e = reinterpret_cast<const T *>(&raw);
-#pragma unroll
-        for (int i = 0; i < VEC; ++i) v[i] = Elem<T>::to_f32(e[i]);
+        return kOnce ? __ldcs(reinterpret_cast<const uint4 *>(p + c)) : __ldg(reinterpret_cast<const uint4 *>(p + c));
     } else {
-#pragma unroll
-        for (int i = 0; i < VEC; ++i) v[i] = c + i < C ? Elem<T>::to_f32(p[c + i]) : 0.0f;
-    }
-}
-template <typename T, int VEC, bool kAligned> __device__ __forceinline__ void store_row(T *p, int c, int C, const float (&v)[VEC]) {
-    if constexpr (kAligned) {
-        uint4 raw;
+        uint4 raw = make_uint4(0, 0, 0, 0);
         T *e = reinterpret_cast<T *>(&raw);
 #pragma unroll
-        for (int i = 0; i < VEC; ++i) e[i] = Elem<T>::from_f32(v[i]);
+        for (int i = 0; i < VEC; ++i)
+            if (c + i < C) e[i] = p[c + i];
+        return raw;
+    }
+}
+template <typename T, int VEC> __device__ __forceinline__ void unpack_raw(const uint4 &raw, float (&v)[VEC]) {
+    const T *e = reinterpret_cast<const T *>(&raw);
+#pragma unroll
+    for (int i = 0; i < VEC; ++i) v[i] = Elem<T>::to_f32(e[i]);
+}
+template <typename T, int VEC> __device__ __forceinline__ uint4 pack_raw(const float (&v)[VEC]) {
+    uint4 raw;
+    T *e = reinterpret_cast<T *>(&raw);
+#pragma unroll
+    for (int i = 0; i < VEC; ++i) e[i] = Elem<T>::from_f32(v[i]);
+    return raw;
+}
+template <typename T, int VEC, bool kAligned> __device__ __forceinline__ void store_raw(T *p, int c, int C, const uint4 &raw) {
+    if constexpr (kAligned) {
         __stcs(reinterpret_cast<uint4 *>(p + c), raw);
     } else {
+        const T *e = reinterpret_cast<const T *>(&raw);
 #pragma unroll
         for (int i = 0; i < VEC; ++i)
-            if (c + i < C) p[c + i] = Elem<T>::from_f32(v[i]);
+            if (c + i < C) p[c + i] = e[i];
     }
 }
 
@@ -79,44 +89,51 @@ __global__ void __launch_bounds__(kThreads) residual_rmsnorm_kernel(const RmsNor
     const T *scale = (const T *)a.scale, *weight = (const T *)a.weight;
     for (int64_t row = (int64_t)blockIdx.x * kGroups + group; row < a.rows; row += (int64_t)gridDim.x * kGroups) {
         const T *x = (const T *)a.x + row * a.x_row;
-        float v[NV][VEC];
+        uint4 rx[NV], rb[NV];  // everything that a row reads is asked for before anything is used
 #pragma unroll
         for (int j = 0; j < NV; ++j) {
-            if (c0 + j * kSpan < C) load_row<T, VEC, kAligned, true>(x, c0 + j * kSpan, C, v[j]);
-            else
-#pragma unroll
-                for (int i = 0; i < VEC; ++i) v[j][i] = 0.0f;
+            rx[j] = make_uint4(0, 0, 0, 0);
+            if (c0 + j * kSpan < C) rx[j] = load_raw<T, VEC, kAligned, true>(x, c0 + j * kSpan, C);
         }
         if (a.branch) {
             const T *branch = (const T *)a.branch + row * C;
 #pragma unroll
+            for (int j = 0; j < NV; ++j)
+                if (c0 + j * kSpan < C) rb[j] = load_raw<T, VEC, kAligned, true>(branch, c0 + j * kSpan, C);
+#pragma unroll
             for (int j = 0; j < NV; ++j) {
                 const int c = c0 + j * kSpan;
                 if (c < C) {
-                    float b[VEC], g[VEC];
-                    load_row<T, VEC, kAligned, true>(branch, c, C, b);
+                    float s[VEC], b[VEC];
+                    unpack_raw<T, VEC>(rx[j], s);
+                    unpack_raw<T, VEC>(rb[j], b);
                     if (scale) {
-                        load_row<T, VEC, kAligned, false>(scale, c, C, g);
+                        float g[VEC];
+                        unpack_raw<T, VEC>(load_raw<T, VEC, kAligned, false>(scale, c, C), g);
 #pragma unroll
-                        for (int i = 0; i < VEC; ++i) b[i] = fmaf(b[i], g[i], v[j][i]);
+                        for (int i = 0; i < VEC; ++i) s[i] = fmaf(b[i], g[i], s[i]);
                     } else {
 #pragma unroll
-                        for (int i = 0; i < VEC; ++i) b[i] += v[j][i];
+                        for (int i = 0; i < VEC; ++i) s[i] += b[i];
                     }
-                    // the norm is that of the stream as the next block reads it
-#pragma unroll
-                    for (int i = 0; i < VEC; ++i) v[j][i] = Elem<T>::to_f32(Elem<T>::from_f32(b[i]));
-                    if (a.x_out) store_row<T, VEC, kAligned>((T *)a.x_out + row * C, c, C, v[j]);
+                    rx[j] = pack_raw<T, VEC>(s);  // the norm is that of the stream as the next block reads it
+                    if (a.x_out) store_raw<T, VEC, kAligned>((T *)a.x_out + row * C, c, C, rx[j]);
                 }
             }
         }
         if (!a.normed && !a.q) continue;
+        // From here on a row is its raw bytes, unpacked once for the sum and once for the result: registers are what limits the rows in
+        // flight.
+        float rstd = 1.0f;
         if (a.norm) {
             float sum = 0.0f;
 #pragma unroll
-            for (int j = 0; j < NV; ++j)
+            for (int j = 0; j < NV; ++j) {
+                float v[VEC];
+                unpack_raw<T, VEC>(rx[j], v);
 #pragma unroll
-                for (int i = 0; i < VEC; ++i) sum = fmaf(v[j][i], v[j][i], sum);
+                for (int i = 0; i < VEC; ++i) sum = fmaf(v[i], v[i], sum);
+            }
 #pragma unroll
             for (int m = 16; m >= 1; m >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, m);
             if constexpr (kWarps > 1) {  // one group per CTA: a whole-CTA barrier
@@ -128,35 +145,35 @@ __global__ void __launch_bounds__(kThreads) residual_rmsnorm_kernel(const RmsNor
                 for (int w = 0; w < kWarps; ++w) sum += part[0][w];
                 __syncthreads();
             }
-            const float rstd = 1.0f / sqrtf(sum / (float)C + a.eps);
+            rstd = rsqrtf(fmaf(sum, a.inv_C, a.eps));
+        }
 #pragma unroll
-            for (int j = 0; j < NV; ++j) {
-                const int c = c0 + j * kSpan;
-                if (c < C) {
+        for (int j = 0; j < NV; ++j) {
+            const int c = c0 + j * kSpan;
+            float v[VEC];
+            unpack_raw<T, VEC>(rx[j], v);
+            if (a.norm) {
+#pragma unroll
+                for (int i = 0; i < VEC; ++i) v[i] *= rstd;
+                if (weight && c < C) {
                     float w[VEC];
-                    if (weight) load_row<T, VEC, kAligned, false>(weight, c, C, w);
+                    unpack_raw<T, VEC>(load_raw<T, VEC, kAligned, false>(weight, c, C), w);
 #pragma unroll
-                    for (int i = 0; i < VEC; ++i) v[j][i] = weight ? v[j][i] * rstd * w[i] : v[j][i] * rstd;
+                    for (int i = 0; i < VEC; ++i) v[i] *= w[i];
                 }
             }
-        }
-        if (a.normed) {
-#pragma unroll
-            for (int j = 0; j < NV; ++j)
-                if (c0 + j * kSpan < C) store_row<T, VEC, kAligned>((T *)a.normed + row * C, c0 + j * kSpan, C, v[j]);
-        } else {
-#pragma unroll
-            for (int j = 0; j < NV; ++j) {
-                const int c = c0 + j * kSpan;
+            if (a.normed) {
+                if (c < C) store_raw<T, VEC, kAligned>((T *)a.normed + row * C, c, C, pack_raw<T, VEC>(v));
+            } else {
                 float top = 0.0f;
 #pragma unroll
-                for (int i = 0; i < VEC; ++i) top = fmaxf(top, fabsf(v[j][i]));
+                for (int i = 0; i < VEC; ++i) top = fmaxf(top, fabsf(v[i]));
 #pragma unroll
                 for (int m = kScaleBlock / VEC / 2; m >= 1; m >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, m));
                 top = fmaxf(top, kSmallestMax);
                 if (c < C) {
-                    store_e4m3<VEC>(a.q + row * a.q_row, c, C, v[j], kE4m3Max / top);
-                    if (c % kScaleBlock == 0) a.q_scale[row * a.s_row + (c / kScaleBlock) * a.s_block] = top / kE4m3Max;
+                    store_e4m3<VEC>(a.q + row * a.q_row, c, C, v, __fdividef(kE4m3Max, top));
+                    if (c % kScaleBlock == 0) a.q_scale[row * a.s_row + (c / kScaleBlock) * a.s_block] = top * (1.0f / kE4m3Max);
                 }
             }
         }
@@ -184,7 +201,7 @@ template <typename T, bool kAligned> int launch_rmsnorm(const RmsNormArgs &a, cu
     } else if (vectors <= 32) COME_RMS_LAUNCH(1, 1, 128, 16);
     else if (vectors <= 64) COME_RMS_LAUNCH(1, 2, 128, 12);
     else if (vectors <= 128) COME_RMS_LAUNCH(1, 4, 128, 8);
-    else if (vectors <= 256) COME_RMS_LAUNCH(1, 8, 128, 5);
+    else if (vectors <= 256) COME_RMS_LAUNCH(4, 2, 128, 1 << 20);
     else COME_RMS_LAUNCH(4, 4, 128, 8);
 #undef COME_RMS_LAUNCH
     return check_launch("come_residual_rmsnorm");
@@ -256,6 +273,7 @@ extern "C" int come_residual_rmsnorm(const void *x_dev, const void *branch_dev, 
     a.x_row = channels;
     a.C = (int)channels;
     a.eps = eps;
+    a.inv_C = 1.0f / (float)channels;
     a.norm = normed_dev || q_dev;
     a.x_out = x_out_dev;
     a.normed = normed_dev;

@@ -28,20 +28,25 @@ def _operand(t: torch.Tensor) -> torch.Tensor:
 
 
 def _padded(rows: int, cols: int, like: torch.Tensor) -> torch.Tensor:
-    return torch.empty((rows, -(-cols // 8) * 8), dtype=like.dtype, device=like.device)[:, :cols]
+    return torch.empty_strided((rows, cols), ((cols + 7) & ~7, 1), dtype=like.dtype, device=like.device)
+
+
+def _forward(x, w_gate, w_up, b_gate, b_up, act):
+    tokens, cols = x.shape
+    features, dev = w_gate.shape[0], x.device
+    xo, wg, wu = _operand(x), _operand(w_gate), _operand(w_up)
+    out = torch.empty_strided((tokens, features), (features or 1, 1), dtype=x.dtype, device=dev)
+    with on_device(dev):
+        _lib.check(_lib.lib().come_gated_matmul(xo.data_ptr(), xo.stride(0), wg.data_ptr(), wg.stride(0), wu.data_ptr(), wu.stride(0), ptr(b_gate),
+                                                ptr(b_up), dtype_code(x.dtype), act, tokens, features, cols, out.data_ptr(), features,
+                                                stream_ptr(dev)))
+    return out
 
 
 class _GatedLinear(torch.autograd.Function):
     @staticmethod
     def forward(ctx, x, w_gate, w_up, b_gate, b_up, act):
-        tokens, cols = x.shape
-        features, dev = w_gate.shape[0], x.device
-        xo, wg, wu = _operand(x), _operand(w_gate), _operand(w_up)
-        out = torch.empty((tokens, features), dtype=x.dtype, device=dev)
-        with on_device(dev):
-            _lib.check(_lib.lib().come_gated_matmul(xo.data_ptr(), xo.stride(0), wg.data_ptr(), wg.stride(0), wu.data_ptr(), wu.stride(0), ptr(b_gate),
-                                                    ptr(b_up), dtype_code(x.dtype), act, tokens, features, cols, out.data_ptr(), features,
-                                                    stream_ptr(dev)))
+        out = _forward(x, w_gate, w_up, b_gate, b_up, act)
         ctx.act = act
         ctx.save_for_backward(x, w_gate, w_up, b_gate, b_up)
         return out
@@ -91,7 +96,7 @@ def gated_linear(x: torch.Tensor, w_gate: torch.Tensor, w_up: torch.Tensor, b_ga
     ``activation``: "silu" or "gelu" (the exact one).  Sums in float32, the result rounded once.  Rows that are not contiguous or do
     not start at multiples of 16 bytes are copied first."""
     require_cuda(x, "x")
-    act, dev = activation_code(activation), x.device
+    act = activation_code(activation)
     if x.dtype not in (torch.float16, torch.bfloat16):
         raise RuntimeError(f"x: unsupported dtype {x.dtype}; expected float16 or bfloat16")
     cols = x.shape[-1] if x.dim() else 0
@@ -99,16 +104,22 @@ def gated_linear(x: torch.Tensor, w_gate: torch.Tensor, w_up: torch.Tensor, b_ga
         raise ValueError(f"w_gate and w_up must be [F, {cols}], got {tuple(w_gate.shape)} and {tuple(w_up.shape)}")
     if cols == 0 or cols % 8 != 0:
         raise NotImplementedError(f"gated_linear needs a channel count that is a multiple of 8, got {cols}")
-    features = w_gate.shape[0]
-    for name, t, shape in (("w_gate", w_gate, (features, cols)), ("w_up", w_up, (features, cols)), ("b_gate", b_gate, (features,)), ("b_up", b_up, (features,))):
+    features, index = w_gate.shape[0], x.get_device()
+    grad = x.requires_grad
+    for name, t in (("w_gate", w_gate), ("w_up", w_up), ("b_gate", b_gate), ("b_up", b_up)):
         if t is None:
             continue
-        if t.dtype != x.dtype or t.device != dev or tuple(t.shape) != shape:
-            raise ValueError(f"{name} must be {list(shape)} {x.dtype} on {dev}, got {list(t.shape)} {t.dtype} on {t.device}")
-    b_gate, b_up = (b if b is None else b.contiguous() for b in (b_gate, b_up))
+        if t.dtype is not x.dtype or t.get_device() != index or (name[0] == "b" and t.shape != (features,)):
+            raise ValueError(f"{name} must be {[features] if name[0] == 'b' else [features, cols]} {x.dtype} on {x.device}, got {list(t.shape)} {t.dtype} on {t.device}")
+        grad = grad or t.requires_grad
+    if b_gate is not None:
+        b_gate = b_gate.contiguous()
+    if b_up is not None:
+        b_up = b_up.contiguous()
+    apply = _GatedLinear.apply if grad and torch.is_grad_enabled() else _forward
     if x.dim() == 2:
-        return _GatedLinear.apply(x, w_gate, w_up, b_gate, b_up, act)
-    return _GatedLinear.apply(x.reshape(-1, cols), w_gate, w_up, b_gate, b_up, act).view(*x.shape[:-1], features)
+        return apply(x, w_gate, w_up, b_gate, b_up, act)
+    return apply(x.reshape(-1, cols), w_gate, w_up, b_gate, b_up, act).view(*x.shape[:-1], features)
 
 
 class GatedMlp(torch.nn.Module):
