@@ -518,7 +518,7 @@ __global__ void __launch_bounds__(kThreads, 1) __cluster_dims__(2, 1, 1) matmul_
                         asm volatile("bar.sync 1, 256;" ::: "memory");
                         top = fmaxf(fmaxf(top, sh.top[tiles & 1][part ^ 1][r]), kSmallestMax);
                         if (ok && busy) {
-                            const float inv = kE4m3Max / top;
+                            const float inv = __fdividef(kE4m3Max, top);
 #pragma unroll
                             for (int c = 0; c < 4; ++c) {
                                 uint32_t q[4];
@@ -531,7 +531,7 @@ __global__ void __launch_bounds__(kThreads, 1) __cluster_dims__(2, 1, 1) matmul_
                             }
                             __syncwarp();
                             store_staged<1, kRow>(stage, (uint8_t *)p.out[0] + row0 * p.out_row[0] + n, p.out_row[0], rows, cols, lane);
-                            if (part == 0 && lane < rows) p.out_scale[(row0 + lane) * p.os_row + (w.n0 / kTile) * p.os_block] = top / kE4m3Max;
+                            if (part == 0 && lane < rows) p.out_scale[(row0 + lane) * p.os_row + (w.n0 / kTile) * p.os_block] = top * (1.0f / kE4m3Max);
                             __syncwarp();
                         }
                     } else if (ok && busy) {

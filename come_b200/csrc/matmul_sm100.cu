@@ -22,6 +22,7 @@
 #include "matmul_sm100.cuh"
 
 #include <mutex>
+#include <type_traits>
 
 namespace come {
 
@@ -91,8 +92,8 @@ __global__ void __launch_bounds__(kThreads, 1) matmul_split_kernel(const __grid_
     constexpr int kN = kMats * kTile;
     constexpr int kStageBytes = kOperandBytes * (1 + kMats), kStages = kRingBytes / kStageBytes;
     constexpr int kElems = kE4m3 ? 128 : 64;  // contraction elements of a K block
-    constexpr uint32_t kTmemCols = kE4m3 ? 2 * kN : kN;
-    static_assert(kStages <= 6 && kTmemCols <= 512, "");
+    constexpr uint32_t kTmemCols = 512;
+    static_assert(kStages <= 6 && 2 * kN <= kTmemCols, "");
     extern __shared__ __align__(1024) uint8_t smem[];
     SplitBarriers &sh = *reinterpret_cast<SplitBarriers *>(smem + kRingBytes);
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
@@ -123,10 +124,12 @@ __global__ void __launch_bounds__(kThreads, 1) matmul_split_kernel(const __grid_
     tc_fence_before();
     __syncthreads();
     tc_fence_after();
-    const uint32_t tmem = sh.tmem_base;
+    // All of the SM's tensor memory is allocated, so its base is column 0: the tensor-memory addresses are constants.
+    constexpr uint32_t tmem = 0;
     const uint32_t ring = smem_u32(smem);
     const auto wait = [&](uint64_t *bar, uint32_t parity, uint32_t code) { return mbar_wait_limit(bar, parity, &sh.abort_flag, p.status, code, kWaitTicks); };
-    const bool dead = sh.abort_flag != 0;
+    const bool misplaced = sh.tmem_base != tmem, dead = sh.abort_flag != 0 || misplaced;
+    if (misplaced && threadIdx.x == 0) atomicOr(p.status, kErrSums);
 
     if (!dead && warp == kProducerWarp) {
         if (lane == 0) {
@@ -156,25 +159,43 @@ __global__ void __launch_bounds__(kThreads, 1) matmul_split_kernel(const __grid_
         }
         __syncwarp();
     } else if (!dead && warp == kIssuerWarp) {
-        if (lane == 0) {
-            const uint32_t idesc = matmul_idesc(kE4m3, p.dtype == COME_BF16, kTile, kN, kAMn, kBMn);
-            constexpr uint32_t kAStep = kAMn ? 2048 >> 4 : 32 >> 4, kBStep = kBMn ? 2048 >> 4 : 32 >> 4;
-            for (int i = 0; i < n_kb; ++i) {
-                const int st = i % kStages, buf = kE4m3 ? i & 1 : 0;
-                if (!wait(&sh.full[st], (i / kStages) & 1, kErrFull)) break;
-                if (kE4m3 && !wait(&sh.acc_empty[buf], ((i >> 1) & 1) ^ 1, kErrSums)) break;
-                tc_fence_after();
-                const uint64_t da = operand_desc(ring + st * kStageBytes, kOperandBytes / 2);
-                const uint64_t db = operand_desc(ring + st * kStageBytes + kOperandBytes, kOperandBytes / 2);
+        // Warp-uniform control flow and constant tensor-memory addresses: see matmul_pair_sm100.cu.
+        const uint32_t idesc = matmul_idesc(kE4m3, p.dtype == COME_BF16, kTile, kN, kAMn, kBMn);
+        constexpr uint32_t kAStep = kAMn ? 2048 >> 4 : 32 >> 4, kBStep = kBMn ? 2048 >> 4 : 32 >> 4;
+        const uint64_t desc_a = operand_desc(ring, kOperandBytes / 2), desc_b = operand_desc(ring + kOperandBytes, kOperandBytes / 2);
+        uint32_t st = 0, st_phase = 0, buf = 0, buf_phase = 1;
+        bool ok = true;
+        const auto wait_here = [&](uint64_t *bar, uint32_t parity, uint32_t code) {
+            if (!mbar_try_wait(bar, parity)) ok = ok && wait(bar, parity, code);
+        };
+        for (int i = 0; i < n_kb; ++i) {
+            if ((i & 31) == 31 && !__all_sync(0xffffffffu, ok)) break;
+            wait_here(&sh.full[st], st_phase, kErrFull);
+            if (kE4m3) wait_here(&sh.acc_empty[buf], buf_phase, kErrSums);
+            __syncwarp();
+            tc_fence_after();
+            const uint64_t da = desc_a + (uint64_t)(st * (kStageBytes >> 4)), db = desc_b + (uint64_t)(st * (kStageBytes >> 4));
+            if (elect_one() && ok) {
 #pragma unroll
                 for (int k = 0; k < 4; ++k) {
                     const uint32_t more = k > 0 || (!kE4m3 && i > 0) ? 1u : 0u;
-                    if constexpr (kE4m3) tc_mma_f8_ss_1(tmem + buf * kN, da + k * kAStep, db + k * kBStep, idesc, more);
-                    else tc_mma_ss_1(tmem, da + k * kAStep, db + k * kBStep, idesc, more);
+                    if constexpr (kE4m3) tc_mma_f8_ss_1(buf * kN, da + k * kAStep, db + k * kBStep, idesc, more);
+                    else tc_mma_ss_1(0, da + k * kAStep, db + k * kBStep, idesc, more);
                 }
                 tc_commit_1(&sh.empty[st]);
                 if (kE4m3 || i == n_kb - 1) tc_commit_1(&sh.acc_full[buf]);
             }
+            __syncwarp();
+            if (++st == kStages) {
+                st = 0;
+                st_phase ^= 1u;
+            }
+            if (kE4m3) {
+                buf ^= 1u;
+                if (buf == 0) buf_phase ^= 1u;
+            }
+        }
+        if (elect_one()) {
             tc_commit_1(&sh.drained);
             mbar_drain(&sh.drained, 0, p.status, kErrSums);
         }
@@ -250,73 +271,102 @@ __global__ void __launch_bounds__(kThreads, 1) matmul_split_kernel(const __grid_
         }
     }
 
+    const int n = n0 + 4 * lane, valid = p.N - n;  // the lane's four result columns
+    float bias[kMats][4] = {};
+#pragma unroll
+    for (int w = 0; w < kMats; ++w)
+        if (p.bias[w] && warp < kEpilogueWarps)
+#pragma unroll
+            for (int i = 0; i < 4; ++i)
+                if (i < valid) bias[w][i] = load_any(p.bias[w], n + i, p.bias_dtype);
+    if (misplaced && threadIdx.x == 0) sh.abort_flag = 1;  // read by the others behind the barrier
     tc_fence_before();
     cluster_sync();
     bool store = true;
     for (uint32_t s = 0; s < ranks; ++s) store &= ld_cluster_u32(map_rank(smem_u32((const void *)&sh.abort_flag), s)) == 0;
     if (store && warp < kEpilogueWarps) {
-        const int n = n0 + 4 * lane, valid = p.N - n;
-        float bias[2][4] = {};
+        // kRows rows at a time, so that their loads (another SM's shared memory is some 200 clocks away) are in flight together
+        const auto finish = [&](auto rows_at_once) {
+            constexpr int kRows = decltype(rows_at_once)::value;
+            for (int r0 = (int)(rank + ranks * warp); r0 < rows; r0 += (int)ranks * kEpilogueWarps * kRows) {
+                float v[kRows][kMats][4];
 #pragma unroll
-        for (int w = 0; w < kMats; ++w)
-            if (p.bias[w])
+                for (int j = 0; j < kRows; ++j)
 #pragma unroll
-                for (int i = 0; i < 4; ++i)
-                    if (i < valid) bias[w][i] = load_any(p.bias[w], n + i, p.bias_dtype);
-        for (int r = (int)(rank + ranks * warp); r < rows; r += (int)ranks * kEpilogueWarps) {
-            float v[2][4] = {};
-            for (uint32_t s = 0; s < ranks; ++s) {
-                const uint32_t at = map_rank(ring + (r * kPartRow + 4 * lane) * 4, s);
+                    for (int w = 0; w < kMats; ++w)
 #pragma unroll
-                for (int w = 0; w < kMats; ++w) {
-                    const float4 x = ld_cluster(at + w * kPartBytes);
-                    v[w][0] += x.x, v[w][1] += x.y, v[w][2] += x.z, v[w][3] += x.w;
+                        for (int i = 0; i < 4; ++i) v[j][w][i] = bias[w][i];
+                [[maybe_unused]] float dh[kRows][4];
+                if constexpr (kMode == kMatmulGatedGrad) {
+#pragma unroll
+                    for (int j = 0; j < kRows; ++j) {
+                        const int r = r0 + j * (int)ranks * kEpilogueWarps;
+                        if (r < rows) load4(p.dh, (int64_t)(m0 + r) * p.dh_row + n, dh[j], valid, p.dtype);
+                    }
+                }
+                for (uint32_t s = 0; s < ranks; ++s) {
+                    float4 x[kRows][kMats];
+#pragma unroll
+                    for (int j = 0; j < kRows; ++j) {
+                        const int r = min(r0 + j * (int)ranks * kEpilogueWarps, rows - 1);
+                        const uint32_t at = map_rank(ring + (r * kPartRow + 4 * lane) * 4, s);
+#pragma unroll
+                        for (int w = 0; w < kMats; ++w) x[j][w] = ld_cluster(at + w * kPartBytes);
+                    }
+#pragma unroll
+                    for (int j = 0; j < kRows; ++j)
+#pragma unroll
+                        for (int w = 0; w < kMats; ++w) v[j][w][0] += x[j][w].x, v[j][w][1] += x[j][w].y, v[j][w][2] += x[j][w].z, v[j][w][3] += x[j][w].w;
+                }
+#pragma unroll
+                for (int j = 0; j < kRows; ++j) {
+                    const int r = r0 + j * (int)ranks * kEpilogueWarps;
+                    if (r >= rows) break;
+                    const int64_t row = m0 + r, at = row * p.out_row[problem] + n;
+                    if constexpr (kMode == kMatmulPlain) {
+                        store4(p.out[problem], at, v[j][0], valid, p.out_dtype);
+                    } else if constexpr (kMode == kMatmulGated) {
+                        float h[4], top = 0.0f;
+#pragma unroll
+                        for (int i = 0; i < 4; ++i) {
+                            h[i] = i < valid ? activation(v[j][0][i], p.act) * v[j][1][i] : 0.0f;
+                            top = fmaxf(top, fabsf(h[i]));
+                        }
+                        if (p.out_dtype != COME_E4M3) {
+                            store4(p.out[0], at, h, valid, p.out_dtype);
+                        } else {
+#pragma unroll
+                            for (int s = 16; s >= 1; s >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, s));
+                            top = fmaxf(top, kSmallestMax);
+                            const float inv = __fdividef(kE4m3Max, top);
+                            const uint32_t q = pack_e4m3(h[0] * inv, h[1] * inv, h[2] * inv, h[3] * inv);
+                            uint8_t *out = (uint8_t *)p.out[0] + at;  // rows start at multiples of 16 bytes
+                            if (valid >= 4) {
+                                *reinterpret_cast<uint32_t *>(out) = q;
+                            } else {
+#pragma unroll
+                                for (int i = 0; i < 4; ++i)
+                                    if (i < valid) out[i] = (uint8_t)(q >> (8 * i));
+                            }
+                            if (lane == 0) p.out_scale[row * p.os_row + (n0 / kTile) * p.os_block] = top * (1.0f / kE4m3Max);
+                        }
+                    } else {
+                        float dg[4], du[4];
+#pragma unroll
+                        for (int i = 0; i < 4; ++i) {
+                            float a, slope;
+                            activation_grad(v[j][0][i], p.act, a, slope);
+                            dg[i] = dh[j][i] * v[j][1][i] * slope;
+                            du[i] = dh[j][i] * a;
+                        }
+                        store4(p.out[0], at, dg, valid, p.out_dtype);
+                        store4(p.out[1], row * p.out_row[1] + n, du, valid, p.out_dtype);
+                    }
                 }
             }
-#pragma unroll
-            for (int w = 0; w < kMats; ++w)
-#pragma unroll
-                for (int i = 0; i < 4; ++i) v[w][i] += bias[w][i];
-            const int64_t row = m0 + r, at = row * p.out_row[problem] + n;
-            if constexpr (kMode == kMatmulPlain) {
-                store4(p.out[problem], at, v[0], valid, p.out_dtype);
-            } else if constexpr (kMode == kMatmulGated) {
-                float h[4], top = 0.0f;
-#pragma unroll
-                for (int i = 0; i < 4; ++i) {
-                    h[i] = i < valid ? activation(v[0][i], p.act) * v[1][i] : 0.0f;
-                    top = fmaxf(top, fabsf(h[i]));
-                }
-                if (p.out_dtype != COME_E4M3) {
-                    store4(p.out[0], at, h, valid, p.out_dtype);
-                } else {
-#pragma unroll
-                    for (int s = 16; s >= 1; s >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, s));
-                    top = fmaxf(top, kSmallestMax);
-                    const float inv = kE4m3Max / top;
-                    const uint32_t q = pack_e4m3(h[0] * inv, h[1] * inv, h[2] * inv, h[3] * inv);
-                    uint8_t *out = (uint8_t *)p.out[0] + at;  // rows start at multiples of 16 bytes
-                    if (valid >= 4) *reinterpret_cast<uint32_t *>(out) = q;
-                    else
-#pragma unroll
-                        for (int i = 0; i < 4; ++i)
-                            if (i < valid) out[i] = (uint8_t)(q >> (8 * i));
-                    if (lane == 0) p.out_scale[row * p.os_row + (n0 / kTile) * p.os_block] = top / kE4m3Max;
-                }
-            } else {
-                float dh[4], dg[4], du[4];
-                load4(p.dh, row * p.dh_row + n, dh, valid, p.dtype);
-#pragma unroll
-                for (int i = 0; i < 4; ++i) {
-                    float a, slope;
-                    activation_grad(v[0][i], p.act, a, slope);
-                    dg[i] = dh[i] * v[1][i] * slope;
-                    du[i] = dh[i] * a;
-                }
-                store4(p.out[0], at, dg, valid, p.out_dtype);
-                store4(p.out[1], row * p.out_row[1] + n, du, valid, p.out_dtype);
-            }
-        }
+        };
+        if (rows > (int)ranks * kEpilogueWarps) finish(std::integral_constant<int, 4>{});
+        else finish(std::integral_constant<int, 1>{});
     }
     cluster_sync();  // no CTA leaves while another reads its share
     if (warp == kIssuerWarp) {
@@ -407,26 +457,33 @@ int run_matmul(const MatmulArgs &a, cudaStream_t st) {
 }
 
 // ---- column sums (gradients of the biases) --------------------------------------------------------------------------------
-// One CTA per 32 columns of one matrix: 4 lanes x 16 bytes cover a row's columns, 64 rows per pass; a thread adds its rows in
-// float32, then the 64 threads of a column are added in their order: one launch, no workspace, the same bits in every run.
+// One CTA per 32 columns of one matrix: 4 lanes x 16 bytes cover a row's columns, kSumRows rows per pass and four passes in flight; a
+// thread adds its rows in float32, then the threads of a column are added in their order: one launch, no workspace, the same bits in
+// every run.
+constexpr int kSumThreads = 512, kSumRows = kSumThreads / 4;
 template <typename T>
-__global__ void __launch_bounds__(256) column_sums_kernel(const T *__restrict__ x0, const T *__restrict__ x1, int64_t row_stride, int64_t rows, int cols,
-                                                          T *__restrict__ out0, T *__restrict__ out1) {
-    __shared__ float part[64][33];
+__global__ void __launch_bounds__(kSumThreads) column_sums_kernel(const T *__restrict__ x0, const T *__restrict__ x1, int64_t row_stride, int64_t rows, int cols,
+                                                                  T *__restrict__ out0, T *__restrict__ out1) {
+    __shared__ float part[kSumRows][33];
     const T *x = blockIdx.y ? x1 : x0;
     T *out = blockIdx.y ? out1 : out0;
     if (!out) return;
     const int c = blockIdx.x * 32 + (threadIdx.x & 3) * 8, r0 = threadIdx.x >> 2;
     float sum[8] = {};
     if (c + 8 <= cols) {
-        for (int64_t r = r0; r < rows; r += 64) {
-            const uint4 raw = *reinterpret_cast<const uint4 *>(x + r * row_stride + c);
-            const T *e = reinterpret_cast<const T *>(&raw);
+        for (int64_t r = r0; r < rows; r += 4 * kSumRows) {
+            uint4 raw[4];
 #pragma unroll
-            for (int i = 0; i < 8; ++i) sum[i] += Elem<T>::to_f32(e[i]);
+            for (int j = 0; j < 4; ++j) raw[j] = r + j * kSumRows < rows ? *reinterpret_cast<const uint4 *>(x + (r + j * kSumRows) * row_stride + c) : make_uint4(0, 0, 0, 0);
+#pragma unroll
+            for (int j = 0; j < 4; ++j) {
+                const T *e = reinterpret_cast<const T *>(&raw[j]);
+#pragma unroll
+                for (int i = 0; i < 8; ++i) sum[i] += Elem<T>::to_f32(e[i]);
+            }
         }
     } else if (c < cols) {  // the last row may end with its last element
-        for (int64_t r = r0; r < rows; r += 64)
+        for (int64_t r = r0; r < rows; r += kSumRows)
 #pragma unroll
             for (int i = 0; i < 8; ++i)
                 if (c + i < cols) sum[i] += Elem<T>::to_f32(x[r * row_stride + c + i]);
@@ -434,11 +491,19 @@ __global__ void __launch_bounds__(256) column_sums_kernel(const T *__restrict__ 
 #pragma unroll
     for (int i = 0; i < 8; ++i) part[r0][(threadIdx.x & 3) * 8 + i] = sum[i];
     __syncthreads();
-    const int col = blockIdx.x * 32 + threadIdx.x;
-    if (threadIdx.x < 32 && col < cols) {
-        float s = 0.0f;
-        for (int r = 0; r < 64; ++r) s += part[r][threadIdx.x];
-        out[col] = Elem<T>::from_f32(s);
+    // 16 threads per column, then one
+    const int col = threadIdx.x & 31, group = threadIdx.x >> 5;
+    float s = 0.0f;
+#pragma unroll
+    for (int r = 0; r < kSumRows / 16; ++r) s += part[group * (kSumRows / 16) + r][col];
+    __syncthreads();
+    part[group][col] = s;
+    __syncthreads();
+    if (group == 0 && blockIdx.x * 32 + col < cols) {
+        s = 0.0f;
+#pragma unroll
+        for (int r = 0; r < 16; ++r) s += part[r][col];
+        out[blockIdx.x * 32 + col] = Elem<T>::from_f32(s);
     }
 }
 
@@ -548,86 +613,63 @@ extern "C" int come_gated_matmul(const void *x_dev, int64_t x_row_stride, const 
     return come::run_matmul(a, (cudaStream_t)stream);
 }
 
-extern "C" int come_gated_matmul_grad(const void *x_dev, int64_t x_row_stride, const void *gate_dev, int64_t gate_row_stride, const void *up_dev, int64_t up_row_stride,
-                                      const void *gate_bias_dev, const void *up_bias_dev, int dtype, int activation, int64_t tokens, int64_t features,
-                                      int64_t channels, const void *dh_dev, int64_t dh_row_stride, void *dgate_dev, void *dup_dev, int64_t d_row_stride, void *stream) {
-    come::MatmulArgs a = {};
-    const int rc = gated_common(a, x_dev, x_row_stride, gate_dev, gate_row_stride, up_dev, up_row_stride, gate_bias_dev, up_bias_dev, dtype, activation, tokens, features, channels);
-    if (rc != COME_OK || tokens == 0 || features == 0) return rc;
-    COME_REQUIRE(dh_dev && dh_row_stride >= 0 && dgate_dev && dup_dev && d_row_stride >= features, "dh and the two results must be given");
-    a.mode = come::kMatmulGatedGrad;
-    a.dh = dh_dev, a.dh_row = dh_row_stride;
-    a.out[0] = dgate_dev, a.out[1] = dup_dev;
-    a.out_row[0] = a.out_row[1] = d_row_stride;
-    return come::run_matmul(a, (cudaStream_t)stream);
-}
-
-extern "C" int come_gated_grad_input(const void *dgate_dev, const void *dup_dev, int64_t d_row_stride, const void *gate_dev, int64_t gate_row_stride, const void *up_dev,
-                                     int64_t up_row_stride, int dtype, int64_t tokens, int64_t features, int64_t channels, void *dx_dev, int64_t dx_row_stride,
-                                     void *stream) {
-    COME_REQUIRE_SIZES("come_gated_grad_input", tokens, channels, features);
-    COME_REQUIRE(come::is_16_bit(dtype), "the gated projections need float16 or bfloat16 (got dtype %d)", dtype);
-    if (tokens == 0 || channels == 0) return COME_OK;
+extern "C" int come_gated_matmul_backward(const void *x_dev, int64_t x_row_stride, const void *gate_dev, int64_t gate_row_stride, const void *up_dev, int64_t up_row_stride,
+                                          const void *gate_bias_dev, const void *up_bias_dev, int dtype, int activation, int64_t tokens, int64_t features,
+                                          int64_t channels, const void *dout_dev, int64_t dout_row_stride, void *dgate_dev, void *dup_dev, int64_t d_row_stride,
+                                          void *dx_dev, int64_t dx_row_stride, void *dgate_weight_dev, void *dup_weight_dev, int64_t dw_row_stride,
+                                          void *dgate_bias_dev, void *dup_bias_dev, void *stream) {
+    using namespace come;
+    cudaStream_t st = (cudaStream_t)stream;
+    MatmulArgs a = {};
+    int rc = gated_common(a, x_dev, x_row_stride, gate_dev, gate_row_stride, up_dev, up_row_stride, gate_bias_dev, up_bias_dev, dtype, activation, tokens, features, channels);
+    if (rc != COME_OK) return rc;
+    COME_REQUIRE(tokens > 0 && features > 0, "come_gated_matmul_backward: without tokens or features every gradient is zero or empty");
+    COME_REQUIRE(dout_dev && dout_row_stride >= 0, "dout must be given");
     COME_REQUIRE_ROWS("dgate", dgate_dev, d_row_stride, 2, features);
     COME_REQUIRE_ROWS("dup", dup_dev, d_row_stride, 2, features);
-    COME_REQUIRE_ROWS("gate", gate_dev, gate_row_stride, 2, channels);
-    COME_REQUIRE_ROWS("up", up_dev, up_row_stride, 2, channels);
-    COME_REQUIRE(dx_dev && dx_row_stride >= channels, "dx must be given, with a row stride that holds its rows");
-    come::MatmulArgs a = {};
-    a.mode = come::kMatmulPlain;
-    a.dtype = a.out_dtype = dtype;
-    a.b_mn = true;
-    a.M = tokens, a.N = channels, a.K = features;
-    a.a[0] = dgate_dev, a.a[1] = dup_dev, a.a_row[0] = a.a_row[1] = d_row_stride;
-    a.b[0] = gate_dev, a.b_row[0] = gate_row_stride;
-    a.b[1] = up_dev, a.b_row[1] = up_row_stride;
-    a.sums = 2, a.problems = 1;
-    a.out[0] = dx_dev, a.out_row[0] = dx_row_stride;
-    return come::run_matmul(a, (cudaStream_t)stream);
-}
-
-extern "C" int come_gated_grad_weight(const void *dgate_dev, const void *dup_dev, int64_t d_row_stride, const void *x_dev, int64_t x_row_stride, int dtype, int64_t tokens,
-                                      int64_t features, int64_t channels, void *dgate_weight_dev, void *dup_weight_dev, int64_t dw_row_stride, void *stream) {
-    COME_REQUIRE_SIZES("come_gated_grad_weight", features, channels, tokens);
-    COME_REQUIRE(come::is_16_bit(dtype), "the gated projections need float16 or bfloat16 (got dtype %d)", dtype);
-    COME_REQUIRE(dgate_weight_dev || dup_weight_dev, "nothing to write");
-    if (features == 0 || channels == 0) return COME_OK;
-    COME_REQUIRE_ROWS("x", x_dev, x_row_stride, 2, channels);
-    COME_REQUIRE(dw_row_stride >= channels, "the row stride of the results must hold their rows");
-    come::MatmulArgs a = {};
-    a.mode = come::kMatmulPlain;
-    a.dtype = a.out_dtype = dtype;
-    a.a_mn = a.b_mn = true;
-    a.M = features, a.N = channels, a.K = tokens;
-    a.b[0] = x_dev, a.b_row[0] = x_row_stride;
-    a.sums = 1;
-    if (dgate_weight_dev) {
-        COME_REQUIRE_ROWS("dgate", dgate_dev, d_row_stride, 2, features);
-        a.a[a.problems] = dgate_dev, a.a_row[a.problems] = d_row_stride;
-        a.out[a.problems] = dgate_weight_dev, a.out_row[a.problems++] = dw_row_stride;
+    COME_REQUIRE(!dx_dev || dx_row_stride >= channels, "the row stride of dx must hold its rows");
+    COME_REQUIRE((!dgate_weight_dev && !dup_weight_dev) || dw_row_stride >= channels, "the row stride of the weights' gradients must hold their rows");
+    // the gradients of the projections
+    a.mode = kMatmulGatedGrad;
+    a.dh = dout_dev, a.dh_row = dout_row_stride;
+    a.out[0] = dgate_dev, a.out[1] = dup_dev;
+    a.out_row[0] = a.out_row[1] = d_row_stride;
+    if ((rc = run_matmul(a, st)) != COME_OK) return rc;
+    if (dx_dev) {  // dx = dgate gate + dup up
+        MatmulArgs b = {};
+        b.dtype = b.out_dtype = dtype;
+        b.b_mn = true;
+        b.M = tokens, b.N = channels, b.K = features;
+        b.a[0] = dgate_dev, b.a[1] = dup_dev, b.a_row[0] = b.a_row[1] = d_row_stride;
+        b.b[0] = gate_dev, b.b_row[0] = gate_row_stride;
+        b.b[1] = up_dev, b.b_row[1] = up_row_stride;
+        b.sums = 2, b.problems = 1;
+        b.out[0] = dx_dev, b.out_row[0] = dx_row_stride;
+        if ((rc = run_matmul(b, st)) != COME_OK) return rc;
     }
-    if (dup_weight_dev) {
-        COME_REQUIRE_ROWS("dup", dup_dev, d_row_stride, 2, features);
-        a.a[a.problems] = dup_dev, a.a_row[a.problems] = d_row_stride;
-        a.out[a.problems] = dup_weight_dev, a.out_row[a.problems++] = dw_row_stride;
+    if (dgate_weight_dev || dup_weight_dev) {  // dgate^T x, dup^T x
+        MatmulArgs b = {};
+        b.dtype = b.out_dtype = dtype;
+        b.a_mn = b.b_mn = true;
+        b.M = features, b.N = channels, b.K = tokens;
+        b.b[0] = x_dev, b.b_row[0] = x_row_stride;
+        b.sums = 1;
+        for (int i = 0; i < 2; ++i) {
+            void *out = i ? dup_weight_dev : dgate_weight_dev;
+            if (!out) continue;
+            b.a[b.problems] = i ? dup_dev : dgate_dev, b.a_row[b.problems] = d_row_stride;
+            b.out[b.problems] = out, b.out_row[b.problems++] = dw_row_stride;
+        }
+        if ((rc = run_matmul(b, st)) != COME_OK) return rc;
     }
-    return come::run_matmul(a, (cudaStream_t)stream);
-}
-
-extern "C" int come_gated_grad_bias(const void *dgate_dev, const void *dup_dev, int64_t d_row_stride, int dtype, int64_t tokens, int64_t features, void *dgate_bias_dev,
-                                    void *dup_bias_dev, void *stream) {
-    COME_REQUIRE(tokens >= 0 && features >= 0 && features < come::kMaxExtent, "bad sizes");
-    COME_REQUIRE(come::is_16_bit(dtype), "the gated projections need float16 or bfloat16 (got dtype %d)", dtype);
-    COME_REQUIRE(dgate_bias_dev || dup_bias_dev, "nothing to write");
-    if (features == 0) return COME_OK;
-    COME_REQUIRE(tokens == 0 || !dgate_bias_dev || (come::rows_ok(dgate_dev, d_row_stride, 2) && d_row_stride >= features), "dgate must be 16-byte aligned, with a row stride of whole 16 bytes");
-    COME_REQUIRE(tokens == 0 || !dup_bias_dev || (come::rows_ok(dup_dev, d_row_stride, 2) && d_row_stride >= features), "dup must be 16-byte aligned, with a row stride of whole 16 bytes");
-    const dim3 grid((unsigned)((features + 31) / 32), 2);
-    cudaStream_t st = (cudaStream_t)stream;
-    if (dtype == COME_F16)
-        come::column_sums_kernel<__half><<<grid, 256, 0, st>>>((const __half *)dgate_dev, (const __half *)dup_dev, d_row_stride, tokens, (int)features, (__half *)dgate_bias_dev, (__half *)dup_bias_dev);
-    else
-        come::column_sums_kernel<__nv_bfloat16><<<grid, 256, 0, st>>>((const __nv_bfloat16 *)dgate_dev, (const __nv_bfloat16 *)dup_dev, d_row_stride, tokens, (int)features,
-                                                                      (__nv_bfloat16 *)dgate_bias_dev, (__nv_bfloat16 *)dup_bias_dev);
-    return come::check_launch("come_gated_grad_bias");
+    if (dgate_bias_dev || dup_bias_dev) {
+        const dim3 grid((unsigned)((features + 31) / 32), 2);
+        if (dtype == COME_F16)
+            column_sums_kernel<__half><<<grid, kSumThreads, 0, st>>>((const __half *)dgate_dev, (const __half *)dup_dev, d_row_stride, tokens, (int)features, (__half *)dgate_bias_dev, (__half *)dup_bias_dev);
+        else
+            column_sums_kernel<__nv_bfloat16><<<grid, kSumThreads, 0, st>>>((const __nv_bfloat16 *)dgate_dev, (const __nv_bfloat16 *)dup_dev, d_row_stride, tokens, (int)features,
+                                                                            (__nv_bfloat16 *)dgate_bias_dev, (__nv_bfloat16 *)dup_bias_dev);
+        return check_launch("come_gated_matmul_backward");
+    }
+    return COME_OK;
 }

@@ -4,7 +4,7 @@
 MLPs of visual transformers: ``w12`` holds both projections, the gate's rows first, ``w3`` the projection back.
 
 A training step keeps only its inputs: the backward pass computes the projections again, in float32, and with them their gradients
-(one kernel, ``come_gated_matmul_grad``), then ``dx = dg Wg + du Wu`` and ``dW = dg^T x`` / ``du^T x``.  ``dg`` and ``du`` are rounded to the
+(one kernel of ``come_gated_matmul_backward``), then ``dx = dg Wg + du Wu`` and ``dW = dg^T x`` / ``du^T x``.  ``dg`` and ``du`` are rounded to the
 tokens' type once, as operands of these products; saved 16-bit projections would add their own rounding to every gradient.
 """
 from __future__ import annotations
@@ -55,36 +55,30 @@ class _GatedLinear(torch.autograd.Function):
     @torch.autograd.function.once_differentiable
     def backward(ctx, dh):
         x, w_gate, w_up, b_gate, b_up = ctx.saved_tensors
-        need_x, need_wg, need_wu, need_bg, need_bu = ctx.needs_input_grad[:5]
+        need = ctx.needs_input_grad
         tokens, cols = x.shape
-        features, dev, lib = w_gate.shape[0], x.device, _lib.lib()
-        dx = torch.empty((tokens, cols), dtype=x.dtype, device=dev) if need_x else None
-        dwg, dwu, dbg, dbu = (torch.empty(shape, dtype=x.dtype, device=dev) if need else None
-                              for need, shape in ((need_wg, (features, cols)), (need_wu, (features, cols)), (need_bg, (features,)), (need_bu, (features,))))
+        features, dev = w_gate.shape[0], x.device
+
+        def empty(wanted: bool, *shape):
+            if not wanted:
+                return None
+            if tokens == 0 or features == 0:
+                return torch.zeros(shape, dtype=x.dtype, device=dev)
+            return torch.empty_strided(shape, (shape[-1], 1)[-len(shape):], dtype=x.dtype, device=dev)
+
+        dx, dwg, dwu = empty(need[0], tokens, cols), empty(need[1], features, cols), empty(need[2], features, cols)
+        dbg, dbu = empty(need[3], features), empty(need[4], features)
         if tokens == 0 or features == 0:
-            for t in (dx, dwg, dwu, dbg, dbu):
-                if t is not None:
-                    t.zero_()
             return dx, dwg, dwu, dbg, dbu, None
         xo, wg, wu = _operand(x), _operand(w_gate), _operand(w_up)
-        if dh.stride(1) != 1 and features > 1:
+        if dh.stride(1) != 1:
             dh = dh.contiguous()
-        code = dtype_code(x.dtype)
         dg, du = _padded(tokens, features, x), _padded(tokens, features, x)
-        d_row = dg.stride(0)
         with on_device(dev):
-            st = stream_ptr(dev)
-            _lib.check(lib.come_gated_matmul_grad(xo.data_ptr(), xo.stride(0), wg.data_ptr(), wg.stride(0), wu.data_ptr(), wu.stride(0), ptr(b_gate), ptr(b_up),
-                                                  code, ctx.act, tokens, features, cols, dh.data_ptr(), dh.stride(0), dg.data_ptr(), du.data_ptr(),
-                                                  d_row, st))
-            if need_x:
-                _lib.check(lib.come_gated_grad_input(dg.data_ptr(), du.data_ptr(), d_row, wg.data_ptr(), wg.stride(0), wu.data_ptr(), wu.stride(0), code,
-                                                     tokens, features, cols, dx.data_ptr(), cols, st))
-            if need_wg or need_wu:
-                _lib.check(lib.come_gated_grad_weight(dg.data_ptr(), du.data_ptr(), d_row, xo.data_ptr(), xo.stride(0), code, tokens, features, cols,
-                                                      ptr(dwg), ptr(dwu), cols, st))
-            if need_bg or need_bu:
-                _lib.check(lib.come_gated_grad_bias(dg.data_ptr(), du.data_ptr(), d_row, code, tokens, features, ptr(dbg), ptr(dbu), st))
+            _lib.check(_lib.lib().come_gated_matmul_backward(
+                xo.data_ptr(), xo.stride(0), wg.data_ptr(), wg.stride(0), wu.data_ptr(), wu.stride(0), ptr(b_gate), ptr(b_up), dtype_code(x.dtype), ctx.act,
+                tokens, features, cols, dh.data_ptr(), dh.stride(0), dg.data_ptr(), du.data_ptr(), dg.stride(0), ptr(dx), cols, ptr(dwg), ptr(dwu), cols,
+                ptr(dbg), ptr(dbu), stream_ptr(dev)))
         return dx, dwg, dwu, dbg, dbu, None
 
 

@@ -375,11 +375,11 @@ int come_packed_positions(const uint8_t *mask_dev, const int64_t *rev_id_dev, in
  * come_gated_matmul_e4m3  out[t, f] = act(x gate^T + gate_bias) * (x up^T + up_bias), in 16 bits or (COME_E4M3) in 8 bits with out_scale,
  *   the form of the next product's x.
  * come_gated_matmul       the same with operands, biases and result in float16 or bfloat16.
- * come_gated_matmul_grad  the projections again, in float32, and the gradients of theirs, dgate = dh up act'(gate), dup = dh act(gate),
- *   rounded to dtype: what a training step keeps of the forward pass is its inputs.
- * come_gated_grad_input   dx = dgate gate + dup up.
- * come_gated_grad_weight  dgate_weight = dgate^T x, dup_weight = dup^T x (either may be NULL).
- * come_gated_grad_bias    column sums of dgate, dup (either result may be NULL).
+ * come_gated_matmul_backward  gradients of come_gated_matmul's tensors from that of its result.  What a training step keeps of the
+ *   forward pass is its inputs: the projections are computed again, in float32, and with them their gradients dgate = dout up act'(gate),
+ *   dup = dout act(gate), rounded to dtype into the two workspaces dgate_dev / dup_dev [tokens, features] (rows of whole 16 bytes); then
+ *   dx = dgate gate + dup up, dgate_weight = dgate^T x, dup_weight = dup^T x and the column sums of dgate, dup for the biases.  Any of the
+ *   five results may be NULL.  tokens and features must not be zero.
  *
  * Results are the same bits in every run.  While bits 19-21 of the device status word are raised, the products return at once without
  * touching their outputs.
@@ -404,18 +404,12 @@ int come_gated_matmul_e4m3(const void *x_dev, int64_t x_row_stride, const float 
 int come_gated_matmul(const void *x_dev, int64_t x_row_stride, const void *gate_dev, int64_t gate_row_stride, const void *up_dev,
                       int64_t up_row_stride, const void *gate_bias_dev, const void *up_bias_dev, int dtype, int activation,
                       int64_t tokens, int64_t features, int64_t channels, void *out_dev, int64_t out_row_stride, void *stream);
-int come_gated_matmul_grad(const void *x_dev, int64_t x_row_stride, const void *gate_dev, int64_t gate_row_stride, const void *up_dev,
-                           int64_t up_row_stride, const void *gate_bias_dev, const void *up_bias_dev, int dtype, int activation,
-                           int64_t tokens, int64_t features, int64_t channels, const void *dh_dev, int64_t dh_row_stride,
-                           void *dgate_dev, void *dup_dev, int64_t d_row_stride, void *stream);
-int come_gated_grad_input(const void *dgate_dev, const void *dup_dev, int64_t d_row_stride, const void *gate_dev,
-                          int64_t gate_row_stride, const void *up_dev, int64_t up_row_stride, int dtype, int64_t tokens,
-                          int64_t features, int64_t channels, void *dx_dev, int64_t dx_row_stride, void *stream);
-int come_gated_grad_weight(const void *dgate_dev, const void *dup_dev, int64_t d_row_stride, const void *x_dev, int64_t x_row_stride,
-                           int dtype, int64_t tokens, int64_t features, int64_t channels, void *dgate_weight_dev,
-                           void *dup_weight_dev, int64_t dw_row_stride, void *stream);
-int come_gated_grad_bias(const void *dgate_dev, const void *dup_dev, int64_t d_row_stride, int dtype, int64_t tokens,
-                         int64_t features, void *dgate_bias_dev, void *dup_bias_dev, void *stream);
+int come_gated_matmul_backward(const void *x_dev, int64_t x_row_stride, const void *gate_dev, int64_t gate_row_stride, const void *up_dev,
+                               int64_t up_row_stride, const void *gate_bias_dev, const void *up_bias_dev, int dtype, int activation,
+                               int64_t tokens, int64_t features, int64_t channels, const void *dout_dev, int64_t dout_row_stride,
+                               void *dgate_dev, void *dup_dev, int64_t d_row_stride, void *dx_dev, int64_t dx_row_stride,
+                               void *dgate_weight_dev, void *dup_weight_dev, int64_t dw_row_stride, void *dgate_bias_dev,
+                               void *dup_bias_dev, void *stream);
 
 /*
  * Device status word: kernels that wait on hardware barriers give up after a bounded number of polls and
