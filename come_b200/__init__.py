@@ -15,7 +15,11 @@ Host side in Python/PyTorch (device memory, streams), compute in ``libcome_b200.
 * :mod:`come_b200.bias_attention`       -- ``JaggedAttention_w_Bias`` (the reference's attention wrapper module)
 * :mod:`come_b200.plain_attention`      -- ``JaggedAttention`` (the same without the count bias)
 * :mod:`come_b200.block`                -- ``JaggedBlock`` / ``JaggedBlock_w_Bias`` and the block with LayerScale + residual
-  add + LayerNorm fused (``residual_layernorm``, ``forward_fused``)
+  add + LayerNorm or RMSNorm fused (``residual_layernorm``, ``residual_rmsnorm``, ``forward_fused``)
+* :mod:`come_b200.feed_forward`         -- ``gated_linear`` (both projections, activation and product of a gated MLP in one
+  kernel, with its backward pass), ``GatedMlp``
+* :mod:`come_b200.block_scaled`         -- linear layers in 8 bits with a scale per block of 128: ``quantize_rows``,
+  ``quantize_weight``, ``block_scaled_linear``, ``block_scaled_gated_linear``, ``BlockScaledLinear``, ``BlockScaledGatedMlp``
 * :mod:`come_b200.fused`                -- ``FusedAggregator``: the merged forward pass of the alternating-attention
   stack, ``CapturedForward``: its CUDA-graph replay, ``ShardedFusedAggregator``: one scene sharded by frame over GPUs
 * :mod:`come_b200.timer`                -- ``Timer`` (named CUDA-event ranges and their percentile table)

@@ -16,11 +16,11 @@ import torch
 from . import _lib
 from ._torch_util import dtype_code, on_device, ptr, require_cuda, stream_ptr
 from .bias_attention import JaggedAttention_w_Bias
-from .block_scaled import empty_rows
+from .block_scaled import BlockScaledGatedMlp, empty_rows
 from .plain_attention import JaggedAttention
 from .token_merger import JaggedTokens
 
-__all__ = ["JaggedBlock", "JaggedBlock_w_Bias", "residual_layernorm", "residual_rmsnorm", "fusable", "forward_fused"]
+__all__ = ["JaggedBlock", "JaggedBlock_w_Bias", "residual_layernorm", "residual_rmsnorm", "residual_norm", "fusable", "forward_fused"]
 
 
 class _JaggedBlockBase(torch.nn.Module):
@@ -145,6 +145,15 @@ def _channel_vector(t: torch.Tensor, dtype: torch.dtype, device, index: int) -> 
     return t.detach().to(device=device, dtype=dtype).contiguous()
 
 
+def residual_norm(x: torch.Tensor, branch: Optional[torch.Tensor], scale: Optional[torch.Tensor], norm: Optional[torch.nn.Module],
+                  quantize: bool = False):
+    """:func:`residual_rmsnorm` for an ``nn.RMSNorm``, else :func:`residual_layernorm` (``norm`` None: the update alone).  ``quantize``
+    asks for 8-bit rows where the norm can write them: a root-mean-square norm does, a LayerNorm's result stays as it is."""
+    if isinstance(norm, torch.nn.RMSNorm):
+        return residual_rmsnorm(x, branch, scale, norm, quantize=quantize)
+    return residual_layernorm(x, branch, scale, norm)
+
+
 def _layer_scale_gamma(ls: torch.nn.Module):
     """(supported, gamma or None) of a LayerScale-like module: ``x * gamma`` or the identity."""
     if isinstance(ls, torch.nn.Identity):
@@ -155,23 +164,26 @@ def _layer_scale_gamma(ls: torch.nn.Module):
 
 def fusable(wrapper: _JaggedBlockBase, dtype: torch.dtype) -> bool:
     """Whether :func:`forward_fused` can evaluate this block: residual stream already in the attention dtype, plain
-    ``nn.LayerNorm`` norms and LayerScale (or identity) scales."""
+    ``nn.LayerNorm`` or ``nn.RMSNorm`` norms and LayerScale (or identity) scales."""
     b = wrapper.block
-    return (dtype == wrapper.attn.run_dtype and isinstance(b.norm1, torch.nn.LayerNorm) and isinstance(b.norm2, torch.nn.LayerNorm)
+    norms = (torch.nn.LayerNorm, torch.nn.RMSNorm)
+    return (dtype == wrapper.attn.run_dtype and isinstance(b.norm1, norms) and isinstance(b.norm2, norms)
             and _layer_scale_gamma(b.ls1)[0] and _layer_scale_gamma(b.ls2)[0])
 
 
 def forward_fused(wrapper: _JaggedBlockBase, x: JaggedTokens, normed: torch.Tensor, pos: Optional[torch.Tensor],
-                  next_norm: Optional[torch.nn.LayerNorm]):
+                  next_norm: Optional[torch.nn.Module]):
     """The block of :class:`JaggedBlock` / :class:`JaggedBlock_w_Bias` with each ``LayerScale -> residual add ->
     LayerNorm`` run as one kernel.  ``normed`` is ``norm1(x.tokens)`` (computed by the previous block's call, or by
-    :func:`residual_layernorm` for the first block); ``next_norm`` is the ``norm1`` of the block that follows (None after
-    the last).  Returns ``(x_out, next_normed)``.  Same arithmetic as the module path up to the summation order inside
+    :func:`residual_norm` for the first block); ``next_norm`` is the ``norm1`` of the block that follows (None after
+    the last).  An MLP in 8 bits (:class:`come_b200.block_scaled.BlockScaledGatedMlp`) gets its rows in 8 bits from the norm in front of it.
+    Returns ``(x_out, next_normed)``.  Same arithmetic as the module path up to the summation order inside
     the LayerNorm statistics."""
     block = wrapper.block
     P, Cc = x.tokens.shape[1], x.tokens.shape[2]
     attn_x = wrapper.attn(JaggedTokens(normed.unsqueeze(0), x.weight, x.offset, x.max_seqlen, x.max_seqlen_dev, x.exchange, x.cu_seqlens), pos=pos)
-    stream, h = residual_layernorm(x.tokens.reshape(P, Cc), attn_x.tokens.reshape(P, Cc), _layer_scale_gamma(block.ls1)[1], block.norm2)
-    mlp_x = block.mlp(h)
-    stream, next_normed = residual_layernorm(stream, mlp_x, _layer_scale_gamma(block.ls2)[1], next_norm)
+    eight = isinstance(block.mlp, BlockScaledGatedMlp)
+    stream, h = residual_norm(x.tokens.reshape(P, Cc), attn_x.tokens.reshape(P, Cc), _layer_scale_gamma(block.ls1)[1], block.norm2, quantize=eight)
+    mlp_x = block.mlp(h, out_dtype=stream.dtype) if eight else block.mlp(h)
+    stream, next_normed = residual_norm(stream, mlp_x, _layer_scale_gamma(block.ls2)[1], next_norm)
     return JaggedTokens(stream.unsqueeze(0), x.weight, x.offset, x.max_seqlen, x.max_seqlen_dev, x.exchange, x.cu_seqlens), next_normed

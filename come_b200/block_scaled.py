@@ -18,7 +18,7 @@ from . import _lib
 from ._torch_util import dtype_code, on_device, require_cuda, stream_ptr
 
 __all__ = ["BLOCK", "BlockScaled", "quantize_rows", "quantize_weight", "block_scaled_linear", "block_scaled_gated_linear",
-           "BlockScaledLinear", "BlockScaledGatedMlp"]
+           "BlockScaledLinear", "BlockScaledGatedMlp", "to_block_scaled"]
 
 BLOCK = 128
 ACTIVATIONS = {"silu": _lib.COME_ACT_SILU, "gelu": _lib.COME_ACT_GELU}
@@ -189,7 +189,17 @@ def activation_code(activation: str) -> int:
 
 
 class _QuantizedWeights(torch.nn.Module):
-    """Holds weights in 8 bits as buffers."""
+    """Holds weights in 8 bits as buffers.  They follow the module to another device, not to another dtype: ``module.to(bfloat16)``
+    leaves numbers, scales and biases what they are."""
+
+    def _apply(self, fn, recurse=True):
+        kept = {name: b for name, b in self._buffers.items() if b is not None}
+        super()._apply(fn, recurse)
+        for name, old in kept.items():
+            new = self._buffers[name]
+            if new.dtype != old.dtype:
+                self._buffers[name] = old.to(new.device)
+        return self
 
     def _hold(self, name: str, weight: torch.Tensor, bias: Optional[torch.Tensor]) -> None:
         w = quantize_weight(weight)
@@ -220,8 +230,8 @@ class BlockScaledLinear(_QuantizedWeights):
 
 class BlockScaledGatedMlp(_QuantizedWeights):
     """A :class:`come_b200.feed_forward.GatedMlp` with its weights in 8 bits: two kernels, the gated projections (whose result leaves
-    in 8 bits) and the down projection.  Takes tokens ``[..., C]`` in 16 or 32 bits, or the 8-bit rows that
-    :func:`come_b200.block.residual_rmsnorm` writes (then the result is ``out_dtype``)."""
+    in 8 bits) and the down projection.  Takes tokens ``[..., C]`` in 16 or 32 bits and returns their dtype, or the 8-bit rows that
+    :func:`come_b200.block.residual_rmsnorm` writes and returns ``out_dtype`` (that of the call, else the module's)."""
 
     def __init__(self, mlp: torch.nn.Module, out_dtype: torch.dtype = torch.bfloat16):
         super().__init__()
@@ -233,11 +243,22 @@ class BlockScaledGatedMlp(_QuantizedWeights):
         self._hold("up", mlp.w12.weight[hidden:], None if bias is None else bias[hidden:])
         self._hold("down", mlp.w3.weight, mlp.w3.bias)
 
-    def forward(self, x):
+    def forward(self, x, out_dtype: Optional[torch.dtype] = None):
         if isinstance(x, BlockScaled):
-            return self._forward(x, self.out_dtype)
-        return self._forward(quantize_rows(x.reshape(-1, x.shape[-1])), x.dtype).view(*x.shape[:-1], -1)
+            return self._forward(x, self.out_dtype if out_dtype is None else out_dtype)
+        out = self._forward(quantize_rows(x.reshape(-1, x.shape[-1])), x.dtype if out_dtype is None else out_dtype)
+        return out.view(*x.shape[:-1], out.shape[-1])
 
     def _forward(self, x: BlockScaled, out_dtype: torch.dtype) -> torch.Tensor:
         h = block_scaled_gated_linear(x, self._weight("gate"), self._weight("up"), self.gate_bias, self.up_bias, self.activation)
         return block_scaled_linear(h, self._weight("down"), self.down_bias, out_dtype)
+
+
+def to_block_scaled(module: torch.nn.Module, out_dtype: torch.dtype = torch.bfloat16) -> torch.nn.Module:
+    """Replaces every gated MLP inside ``module`` (on its CUDA device) by its 8-bit form, in place; returns ``module``."""
+    from .feed_forward import GatedMlp
+    for parent in list(module.modules()):
+        for name, child in list(parent.named_children()):
+            if isinstance(child, GatedMlp):
+                setattr(parent, name, BlockScaledGatedMlp(child, out_dtype))
+    return module

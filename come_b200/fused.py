@@ -23,7 +23,7 @@ from typing import Dict, Optional, Tuple
 
 import torch
 
-from .block import JaggedBlock, JaggedBlock_w_Bias, forward_fused, fusable, residual_layernorm
+from .block import JaggedBlock, JaggedBlock_w_Bias, forward_fused, fusable, residual_norm
 from .token_merger import JaggedTokens, MergePlan
 
 __all__ = ["FusedAggregator", "ShardedFusedAggregator", "CapturedForward", "fused_accelerate", "FusedModel", "run_blocks"]
@@ -37,7 +37,7 @@ class FusedAggregator(torch.nn.Module):
                  fuse_elementwise: bool = True):
         """``fuse_elementwise``: run every ``LayerScale -> residual add -> LayerNorm`` of the blocks as one kernel
         (:func:`come_b200.block.forward_fused`) when the model allows it (token stream in the attention dtype, plain
-        LayerNorm / LayerScale modules); otherwise, and when off, the blocks run module by module as in the reference."""
+        LayerNorm or RMSNorm / LayerScale modules); otherwise, and when off, the blocks run module by module as in the reference."""
         super().__init__()
         self.fuse_elementwise = bool(fuse_elementwise)
         block_fn = JaggedBlock_w_Bias if use_attn_bias_correction else JaggedBlock
@@ -73,7 +73,7 @@ class FusedAggregator(torch.nn.Module):
         fused = self.fuse_elementwise and bool(order) and all(fusable(w, x.tokens.dtype) for w in order)
         normed = None
         if fused:
-            _, normed = residual_layernorm(x.tokens.squeeze(0), None, None, order[0].block.norm1)
+            _, normed = residual_norm(x.tokens.squeeze(0), None, None, order[0].block.norm1)
         step = block_idx = 0
         output: Dict[int, torch.Tensor] = {}
         for _ in range(self.aa_block_num):
@@ -239,7 +239,7 @@ def run_blocks(wrappers, x: JaggedTokens, pos: Optional[torch.Tensor], fuse: boo
     if not wrappers:
         return x
     if fuse and all(fusable(w, x.tokens.dtype) for w in wrappers):
-        _, normed = residual_layernorm(x.tokens.squeeze(0), None, None, wrappers[0].block.norm1)
+        _, normed = residual_norm(x.tokens.squeeze(0), None, None, wrappers[0].block.norm1)
         for i, w in enumerate(wrappers):
             nxt = wrappers[i + 1].block.norm1 if i + 1 < len(wrappers) else None
             x, normed = forward_fused(w, x, normed, pos, nxt)

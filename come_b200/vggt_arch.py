@@ -8,6 +8,8 @@ The accelerated modules of this package (:mod:`come_b200.block`, :mod:`come_b200
 aa_block_size / aa_block_num / retain_layers / patch_start_idx`` (``src/thirdparty/vggt/models/aggregator.py:76-131``).
 The classes here provide exactly those, with the VGGT-1B sizes as defaults: width 1024, 16 heads, MLP ratio 4, q/k
 LayerNorm over the head dimension, 2-D rotary embedding with base 100, LayerScale 0.01, 24 frame + 24 global blocks.
+``norm="rms"`` and ``mlp="gated"`` give blocks with root-mean-square norms and the gated MLP
+(:class:`come_b200.feed_forward.GatedMlp`, two thirds of the hidden width, rounded up to a multiple of 8).
 The dense ``forward`` methods of the original model are not provided: the blocks are run by the jagged block
 wrappers, on merged or unmerged tokens alike.
 """
@@ -18,6 +20,7 @@ from typing import FrozenSet, Optional, Sequence
 import torch
 from torch import nn
 
+from .feed_forward import GatedMlp
 from .qkv import RotaryPositionEmbedding2D
 
 __all__ = ["LayerScale", "Mlp", "Attention", "Block", "AggregatorCore", "PatchEncoderCore", "ConfidenceHead"]
@@ -65,13 +68,17 @@ class Attention(nn.Module):
 
 class Block(nn.Module):
     def __init__(self, dim: int, num_heads: int, mlp_ratio: float = 4.0, init_values: Optional[float] = 0.01,
-                 qk_norm: bool = True, rope: Optional[RotaryPositionEmbedding2D] = None):
+                 qk_norm: bool = True, rope: Optional[RotaryPositionEmbedding2D] = None, norm: str = "layer", mlp: str = "gelu"):
         super().__init__()
-        self.norm1 = nn.LayerNorm(dim)
+        if norm not in ("layer", "rms") or mlp not in ("gelu", "gated"):
+            raise ValueError(f"norm must be 'layer' or 'rms' and mlp 'gelu' or 'gated', got {norm!r} and {mlp!r}")
+        norm_layer = nn.LayerNorm if norm == "layer" else lambda d: nn.RMSNorm(d, eps=1e-6)
+        self.norm1 = norm_layer(dim)
         self.attn = Attention(dim, num_heads, qk_norm=qk_norm, rope=rope)
         self.ls1 = LayerScale(dim, init_values) if init_values else nn.Identity()
-        self.norm2 = nn.LayerNorm(dim)
-        self.mlp = Mlp(dim, int(dim * mlp_ratio))
+        self.norm2 = norm_layer(dim)
+        hidden = int(dim * mlp_ratio)
+        self.mlp = Mlp(dim, hidden) if mlp == "gelu" else GatedMlp(dim, (hidden * 2 // 3 + 7) // 8 * 8)
         self.ls2 = LayerScale(dim, init_values) if init_values else nn.Identity()
 
 
@@ -82,12 +89,12 @@ class AggregatorCore(nn.Module):
                  aa_order: Sequence[str] = ("frame", "global"), aa_block_size: int = 1, qk_norm: bool = True,
                  rope_freq: float = 100.0, init_values: Optional[float] = 0.01,
                  retain_layers: Optional[FrozenSet[int]] = frozenset({4, 11, 17, 23}), patch_start_idx: int = 5,
-                 seed: int = 0, weight_std: float = 0.02):
+                 seed: int = 0, weight_std: float = 0.02, norm: str = "layer", mlp: str = "gelu"):
         super().__init__()
         if depth % aa_block_size != 0:
             raise ValueError(f"depth ({depth}) must be divisible by aa_block_size ({aa_block_size})")
         self.rope = RotaryPositionEmbedding2D(frequency=rope_freq) if rope_freq > 0 else None
-        mk = lambda: Block(embed_dim, num_heads, mlp_ratio, init_values, qk_norm, self.rope)  # noqa: E731
+        mk = lambda: Block(embed_dim, num_heads, mlp_ratio, init_values, qk_norm, self.rope, norm, mlp)  # noqa: E731
         self.frame_blocks = nn.ModuleList([mk() for _ in range(depth)])
         self.global_blocks = nn.ModuleList([mk() for _ in range(depth)])
         self.depth, self.aa_order, self.aa_block_size = depth, list(aa_order), aa_block_size
