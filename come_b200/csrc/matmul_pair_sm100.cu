@@ -52,6 +52,15 @@ typedef float PairScales[kScaleSlots][2][kTile];
 constexpr size_t smem_bytes(bool e4m3) { return kStages * kStageBytes + 8 * staging_bytes(e4m3) + sizeof(PairBarriers) + (e4m3 ? sizeof(PairScales) : 0); }
 static_assert(smem_bytes(true) <= 227 * 1024 && smem_bytes(false) <= 227 * 1024, "");
 
+__device__ __forceinline__ void tmem_ld16(uint32_t taddr, uint32_t (&r)[16]) {
+    asm volatile(
+        "tcgen05.ld.sync.aligned.32x32b.x16.b32 "
+        "{%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15}, [%16];"
+        : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]), "=r"(r[8]),
+          "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15])
+        : "r"(taddr)
+        : "memory");
+}
 // ---- PTX of the pair ------------------------------------------------------------------------------------------------------
 __device__ __forceinline__ void tma_load_2d_pair(uint32_t dst, const CUtensorMap *map, int x, int y, uint32_t bar) {
     asm volatile("cp.async.bulk.tensor.2d.shared::cluster.global.mbarrier::complete_tx::bytes.cta_group::2 [%0], [%1, {%2, %3}], [%4];"
@@ -374,25 +383,25 @@ __global__ void __launch_bounds__(kThreads, 1) __cluster_dims__(2, 1, 1) matmul_
         [[maybe_unused]] const PairScales &scales = *reinterpret_cast<const PairScales *>(&sh + 1);
         const uint32_t empty0 = map_rank(smem_u32(&sh.acc_empty[0]), 0);
         int chunk = 0, tiles = 0;
-        bool ok = true;
+        bool ok = true, busy = false;
+        [[maybe_unused]] const bool with_bias = p.bias[0] != nullptr || (kGated && p.bias[1] != nullptr);
+        [[maybe_unused]] float *bias = reinterpret_cast<float *>(stage);  // [128]: of the gate's and the up projection's 64 columns, or of 128
         for (int t = pair; t < total; t += pairs, ++tiles) {
-            const Tile w = tile_at(t);
-            const int rows = min(32, p.M - w.m0 - warp_row);      // of this warp, may be <= 0
-            const int n = w.n0 + part * kCols, cols = p.N - n;    // first result column of the thread, columns from there on
-            const bool busy = rows > 0;
-            const int64_t row0 = w.m0 + warp_row;
             if constexpr (kE4m3) {
-                const bool with_bias = p.bias[0] != nullptr || (kGated && p.bias[1] != nullptr);
-                float *bias = reinterpret_cast<float *>(stage);   // [128]: of the gate's and the up projection's 64 columns, or of 128
-                if (with_bias) {
-                    __syncwarp();
+                {   // the biases of the warp's columns, before the sums
+                    const Tile w = tile_at(t);
+                    const int n = w.n0 + part * kCols, cols = p.N - n;
+                    if (with_bias) {
+                        __syncwarp();
 #pragma unroll
-                    for (int c = 0; c < 4; ++c) {
-                        const float *b = kGated ? (const float *)p.bias[c >> 1] : (const float *)p.bias[0];
-                        const int col = (kGated ? (c & 1) : c) * 32 + lane;
-                        bias[c * 32 + lane] = b != nullptr && col < cols ? b[n + col] : 0.0f;
+                        for (int c = 0; c < 4; ++c) {
+                            const float *b = kGated ? (const float *)p.bias[c >> 1] : (const float *)p.bias[0];
+                            const int col = (kGated ? (c & 1) : c) * 32 + lane;
+                            bias[c * 32 + lane] = b != nullptr && col < cols ? b[n + col] : 0.0f;
+                        }
+                        __syncwarp();
                     }
-                    __syncwarp();
+                    busy = p.M - w.m0 - warp_row > 0;
                 }
                 // sums as packed pairs: [0, 32) of the gate or of columns [0, 64), [32, 64) of the up projection or of columns [64, 128)
                 f32x2_t sum[64];
@@ -407,31 +416,35 @@ __global__ void __launch_bounds__(kThreads, 1) __cluster_dims__(2, 1, 1) matmul_
                         const float s0 = scales[slot][kGated ? 0 : part][r], s1 = kGated ? scales[slot][1][r] : s0;
                         const f32x2_t s0p = pack_f32x2(s0, s0), s1p = pack_f32x2(s1, s1);
                         const auto column = [&](int c) { return lanes + buf * kPairN + (kGated ? (c >> 1) * kTile + (c & 1) * 32 : c * 32); };
-                        uint32_t d[2][32];
-                        const auto add = [&](int c) {
+                        uint32_t d[2][16];
+                        const auto column16 = [&](int c) { return lanes + buf * kPairN + (kGated ? (c >> 2) * kTile + (c & 3) * 16 : c * 16); };
+                        tmem_ld16(column16(0), d[0]);
+                        tmem_ld16(column16(1), d[1]);
 #pragma unroll
-                            for (int e = 0; e < 16; ++e)
-                                sum[c * 16 + e] = fma_f32x2(pack_f32x2(__uint_as_float(d[c & 1][2 * e]), __uint_as_float(d[c & 1][2 * e + 1])), c >> 1 ? s1p : s0p, sum[c * 16 + e]);
-                        };
-                        tmem_ld32(column(0), d[0]);
-                        tmem_ld32(column(1), d[1]);
-                        tc_wait_ld_of(d[0]);
-                        tc_wait_ld_of(d[1]);
-                        add(0);
-                        tmem_ld32(column(2), d[0]);
-                        add(1);
-                        tmem_ld32(column(3), d[1]);
-                        tc_wait_ld_of(d[0]);
-                        tc_wait_ld_of(d[1]);
-                        tc_fence_before();
-                        __syncwarp();
-                        if (lane == 0) mbar_arrive_at(empty0 + buf * 8);  // the buffer is in registers
-                        add(2);
-                        add(3);
+                        for (int c = 0; c < 8; c += 2) {
+                            tc_wait_ld();
+                            if (c == 6) {
+                                tc_fence_before();
+                                __syncwarp();
+                                if (lane == 0) mbar_arrive_at(empty0 + buf * 8);  // the buffer is in registers
+                            }
+#pragma unroll
+                            for (int j = 0; j < 2; ++j) {
+#pragma unroll
+                                for (int e = 0; e < 8; ++e)
+                                    sum[(c + j) * 8 + e] = fma_f32x2(pack_f32x2(__uint_as_float(d[j][2 * e]), __uint_as_float(d[j][2 * e + 1])), (c + j) >> 2 ? s1p : s0p, sum[(c + j) * 8 + e]);
+                                if (c < 6) tmem_ld16(column16(c + 2 + j), d[j]);
+                            }
+                        }
                     } else if (ok && lane == 0) {
                         mbar_arrive_at(empty0 + buf * 8);
                     }
                 }
+                // Where the tile lies is worked out again (the shuffle hides that it is the same number): kept over the loop, it costs
+                // registers that the sums need.
+                const Tile w = tile_at(__shfl_sync(0xffffffffu, t, 0));
+                const int rows = min(32, p.M - w.m0 - warp_row), n = w.n0 + part * kCols, cols = p.N - n;
+                const int64_t row0 = w.m0 + warp_row;
                 if constexpr (!kGated) {
                     if (ok && busy) {
                         if (with_bias) {
@@ -482,7 +495,7 @@ __global__ void __launch_bounds__(kThreads, 1) __cluster_dims__(2, 1, 1) matmul_
                         }
                     }
                 } else {
-                    float h[64], top = 0.0f;
+                    float top = 0.0f;  // the results take the place of the gate's sums
                     if (ok && busy) {
                         if (with_bias) {
 #pragma unroll
@@ -499,19 +512,26 @@ __global__ void __launch_bounds__(kThreads, 1) __cluster_dims__(2, 1, 1) matmul_
                                 float g0, g1, u0, u1;
                                 unpack_f32x2(sum[c], g0, g1);
                                 unpack_f32x2(sum[32 + c], u0, u1);
-                                h[2 * c] = activation(g0, act) * u0;
-                                h[2 * c + 1] = activation(g1, act) * u1;
+                                sum[c] = pack_f32x2(activation(g0, act) * u0, activation(g1, act) * u1);
                             }
                         });
                         if (cols < 64)  // columns past the end: the bytes of other rows' products
 #pragma unroll
-                            for (int c = 0; c < 64; ++c) h[c] = c < cols ? h[c] : 0.0f;
+                            for (int c = 0; c < 32; ++c) {
+                                float h0, h1;
+                                unpack_f32x2(sum[c], h0, h1);
+                                sum[c] = pack_f32x2(2 * c < cols ? h0 : 0.0f, 2 * c + 1 < cols ? h1 : 0.0f);
+                            }
                         __syncwarp();
                     }
                     if (p.out_dtype == COME_E4M3) {
                         if (ok && busy)
 #pragma unroll
-                            for (int c = 0; c < 64; ++c) top = fmaxf(top, fabsf(h[c]));
+                            for (int c = 0; c < 32; ++c) {
+                                float h0, h1;
+                                unpack_f32x2(sum[c], h0, h1);
+                                top = fmaxf(top, fmaxf(fabsf(h0), fabsf(h1)));
+                            }
                         // the largest magnitude of a row's 128 columns: half of it in the other warpgroup (every warp meets here, also
                         // one that gave up; a third tile's write to the same place is two barriers away)
                         sh.top[tiles & 1][part][r] = top;
@@ -524,7 +544,9 @@ __global__ void __launch_bounds__(kThreads, 1) __cluster_dims__(2, 1, 1) matmul_
                                 uint32_t q[4];
 #pragma unroll
                                 for (int j = 0; j < 4; ++j) {
-                                    const float *e = h + c * 16 + j * 4;
+                                    float e[4];
+                                    unpack_f32x2(sum[c * 8 + j * 2], e[0], e[1]);
+                                    unpack_f32x2(sum[c * 8 + j * 2 + 1], e[2], e[3]);
                                     q[j] = pack_e4m3(e[0] * inv, e[1] * inv, e[2] * inv, e[3] * inv);
                                 }
                                 *staged<kRow>(stage, lane, c) = make_uint4(q[0], q[1], q[2], q[3]);
@@ -540,10 +562,13 @@ __global__ void __launch_bounds__(kThreads, 1) __cluster_dims__(2, 1, 1) matmul_
                             for (int half = 0; half < 2; ++half) {
 #pragma unroll
                                 for (int c = 0; c < 4; ++c) {
-                                    const float *e = h + half * 32 + c * 8;
                                     uint32_t q[4];
 #pragma unroll
-                                    for (int j = 0; j < 4; ++j) q[j] = pack_16<decltype(bf16)::value>(e[2 * j], e[2 * j + 1]);
+                                    for (int j = 0; j < 4; ++j) {
+                                        float lo, hi;
+                                        unpack_f32x2(sum[half * 16 + c * 4 + j], lo, hi);
+                                        q[j] = pack_16<decltype(bf16)::value>(lo, hi);
+                                    }
                                     *staged<kRow>(stage, lane, c) = make_uint4(q[0], q[1], q[2], q[3]);
                                 }
                                 __syncwarp();
@@ -554,6 +579,11 @@ __global__ void __launch_bounds__(kThreads, 1) __cluster_dims__(2, 1, 1) matmul_
                     }
                 }
             } else {
+                const Tile w = tile_at(t);
+                const int rows = min(32, p.M - w.m0 - warp_row);      // of this warp, may be <= 0
+                const int n = w.n0 + part * kCols, cols = p.N - n;    // first result column of the thread, columns from there on
+                busy = rows > 0;
+                const int64_t row0 = w.m0 + warp_row;
                 const int buf = chunk & 1;
                 if (kGated && busy) {  // before the wait: the biases of this warp's 64 + 64 columns, and dh
 #pragma unroll
