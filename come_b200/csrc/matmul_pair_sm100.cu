@@ -26,7 +26,7 @@ namespace come {
 namespace {
 
 constexpr int kProducerWarp = 8, kIssuerWarp = 9, kThreads = 384;  // three warpgroups; warps 10 and 11 only keep the third whole
-constexpr int kPairN = 256;                         // columns of sums per tile
+constexpr int kPairN = 256;                         // columns of sums per tile (192 and 128 were slower wherever they gave fuller rounds)
 constexpr int kStageBytes = 2 * kOperandBytes;      // 128 rows of A and of B
 constexpr int kStages = 6;
 constexpr int kRingBytes = kStages * kStageBytes;
@@ -125,25 +125,25 @@ template <int kSize, int kRow> __device__ __forceinline__ void store_staged(uint
             }
     }
 }
-// The way back: 64 16-bit columns of up to 32 rows to shared memory, zeros outside.
+// The way back: 64 16-bit columns of up to 32 rows to shared memory, zeros outside.  All loads are asked for before the first is used.
 __device__ __forceinline__ void load_staged(uint8_t *base, const uint8_t *in, int64_t row_bytes, int rows, int cols, int lane) {
-    const int chunk = lane & 7, left = cols - chunk * 8;
-    const bool vector = (((uintptr_t)in | (uintptr_t)row_bytes) & 15) == 0 && left >= 8;
+    const int chunk = lane & 7, r0 = lane >> 3, left = cols - chunk * 8;
+    uint4 v[8];
+    const uint8_t *p = in + r0 * row_bytes + chunk * 16;
+    if ((((uintptr_t)in | (uintptr_t)row_bytes) & 15) == 0 && cols >= 64) {
 #pragma unroll
-    for (int r = lane >> 3; r < 32; r += 4) {
-        uint4 v = make_uint4(0, 0, 0, 0);
-        if (r < rows) {
-            const uint16_t *p = reinterpret_cast<const uint16_t *>(in + r * row_bytes) + chunk * 8;
-            if (vector) v = *reinterpret_cast<const uint4 *>(p);
-            else {
-                uint16_t *e = reinterpret_cast<uint16_t *>(&v);
+        for (int i = 0; i < 8; ++i) v[i] = r0 + 4 * i < rows ? *reinterpret_cast<const uint4 *>(p + 4 * i * row_bytes) : make_uint4(0, 0, 0, 0);
+    } else {
 #pragma unroll
-                for (int i = 0; i < 8; ++i)
-                    if (i < left) e[i] = p[i];
-            }
+        for (int i = 0; i < 8; ++i) {
+            uint32_t e[8];
+#pragma unroll
+            for (int j = 0; j < 8; ++j) e[j] = r0 + 4 * i < rows && j < left ? reinterpret_cast<const uint16_t *>(p + 4 * i * row_bytes)[j] : 0u;
+            v[i] = make_uint4(e[0] | e[1] << 16, e[2] | e[3] << 16, e[4] | e[5] << 16, e[6] | e[7] << 16);
         }
-        *staged<128>(base, r, chunk) = v;
     }
+#pragma unroll
+    for (int i = 0; i < 8; ++i) *staged<128>(base, r0 + 4 * i, chunk) = v[i];
 }
 
 template <bool kBF16> __device__ __forceinline__ void unpack_16(uint32_t v, float &lo, float &hi) {
@@ -183,6 +183,8 @@ __global__ void __launch_bounds__(kThreads, 1) __cluster_dims__(2, 1, 1) matmul_
     const int pair = blockIdx.x >> 1, pairs = gridDim.x >> 1;
 
     if (warp == kProducerWarp && lane == 0) {
+        prefetch_map(&p.a[0]);
+        prefetch_map(&p.b[kGated ? rank : 0]);
         sh.abort_flag = (*(volatile unsigned int *)p.status & kStatusMatmul) != 0 ? 1u : 0u;  // an earlier launch gave up
         for (int i = 0; i < kStages; ++i) {
             mbar_init(&sh.full[i], 1);
@@ -603,29 +605,27 @@ __global__ void __launch_bounds__(kThreads, 1) __cluster_dims__(2, 1, 1) matmul_
                     as_constant(p.dtype == COME_BF16, [&](auto bf16_c) {
                         constexpr bool kBF16 = decltype(bf16_c)::value;
                         if constexpr (!kGated) {
-#pragma unroll
-                            for (int h = 0; h < 2; ++h) {
-                                uint32_t d[2][32];
-                                tmem_ld32(from + h * 64, d[0]);
-                                tmem_ld32(from + h * 64 + 32, d[1]);
-                                tc_wait_ld_of(d[0]);
-                                tc_wait_ld_of(d[1]);
-                                if (h == 1) {  // the sums are in registers: the next tile may begin
+#pragma unroll 1
+                            for (int h = 0; h < kCols / 32; ++h) {
+                                uint32_t d[32];
+                                tmem_ld32(from + h * 32, d);
+                                tc_wait_ld_of(d);
+                                if (h == kCols / 32 - 1) {  // the sums are in registers: the next tile may begin
                                     tc_fence_before();
                                     __syncwarp();
                                     if (lane == 0) mbar_arrive_at(empty0 + buf * 8);
                                 }
 #pragma unroll
-                                for (int c = 0; c < 8; ++c) {
+                                for (int c = 0; c < 4; ++c) {
                                     uint32_t e[4];
 #pragma unroll
-                                    for (int j = 0; j < 4; ++j) e[j] = pack_16<kBF16>(__uint_as_float(d[c >> 2][(c & 3) * 8 + 2 * j]), __uint_as_float(d[c >> 2][(c & 3) * 8 + 2 * j + 1]));
-                                    *staged<kRow>(stage, lane, c) = make_uint4(e[0], e[1], e[2], e[3]);
+                                    for (int j = 0; j < 4; ++j) e[j] = pack_16<kBF16>(__uint_as_float(d[c * 8 + 2 * j]), __uint_as_float(d[c * 8 + 2 * j + 1]));
+                                    *staged<64>(stage + (h & 1) * 2048, lane, c) = make_uint4(e[0], e[1], e[2], e[3]);
                                 }
                                 __syncwarp();
-                                store_staged<2, kRow>(stage, (uint8_t *)p.out[w.problem] + (row0 * p.out_row[w.problem] + n + h * 64) * 2, p.out_row[w.problem] * 2, rows, cols - h * 64, lane);
-                                __syncwarp();
+                                store_staged<2, 64>(stage + (h & 1) * 2048, (uint8_t *)p.out[w.problem] + (row0 * p.out_row[w.problem] + n + h * 32) * 2, p.out_row[w.problem] * 2, rows, cols - h * 32, lane);
                             }
+                            __syncwarp();
                         } else {
                             as_constant(p.act == COME_ACT_SILU, [&](auto silu) {
                                 constexpr int act = decltype(silu)::value ? COME_ACT_SILU : COME_ACT_GELU;
@@ -717,10 +717,15 @@ template <bool kE4m3, int kMode, bool kAMn, bool kBMn> int launch_pair(const Mat
 
 }  // namespace
 
+// A tile for every second pair of SMs is where this kernel overtakes the split one (us in a graph, split / pair): 8-bit 1374 tokens
+// 1024 -> 1024, 24 tiles: 10.3 / 10.7; 2748 tokens, 44 tiles: 19.3 / 10.9; 300 tokens 4096 -> 4096, 32 tiles: 19.4 / 22.1; 16-bit gated
+// 1024 -> 2736, 100 tokens, 22 tiles: 9.9 / 11.0; 300 tokens, 44 tiles: 11.7 / 11.4.  In the 8-bit gated form every fourth pair is
+// enough, where the rows fill most of a tile: 700 tokens 400 -> 1003, 24 tiles: 11.6 / 10.0; 1024 -> 2736 (22 tiles) with 64 tokens
+// 8.5 / 9.9, with 128 10.5 / 10.0.
 bool matmul_pair_takes(const MatmulArgs &a) {
-    const int64_t n = a.mode == kMatmulPlain ? kPairN : kTile;
+    const int64_t n = a.mode == kMatmulPlain ? kPairN : kTile, pairs = sm_count() / 2;
     const int64_t tiles = (a.M + 2 * kTile - 1) / (2 * kTile) * ((a.N + n - 1) / n) * a.problems;
-    return tiles * 2 >= sm_count() / 2;
+    return tiles * 2 >= pairs || (a.e4m3 && a.mode == kMatmulGated && a.M > 96 && tiles * 4 >= pairs);
 }
 
 int matmul_pair_launch(const MatmulArgs &a, MatmulParams &p, cudaStream_t st) {

@@ -22,7 +22,6 @@
 #include "matmul_sm100.cuh"
 
 #include <mutex>
-#include <type_traits>
 
 namespace come {
 
@@ -105,6 +104,9 @@ __global__ void __launch_bounds__(kThreads, 1) matmul_split_kernel(const __grid_
     const int rows = min(kTile, p.M - m0);
 
     if (warp == kProducerWarp && lane == 0) {
+        prefetch_map(&p.a[problem]);
+        prefetch_map(&p.b[0]);
+        if constexpr (kMats == 2) prefetch_map(&p.b[1]);
         sh.abort_flag = (*(volatile unsigned int *)p.status & kStatusMatmul) != 0 ? 1u : 0u;  // an earlier launch gave up
         for (int i = 0; i < kStages; ++i) {
             mbar_init(&sh.full[i], 1);
@@ -285,88 +287,72 @@ __global__ void __launch_bounds__(kThreads, 1) matmul_split_kernel(const __grid_
     bool store = true;
     for (uint32_t s = 0; s < ranks; ++s) store &= ld_cluster_u32(map_rank(smem_u32((const void *)&sh.abort_flag), s)) == 0;
     if (store && warp < kEpilogueWarps) {
-        // kRows rows at a time, so that their loads (another SM's shared memory is some 200 clocks away) are in flight together
-        const auto finish = [&](auto rows_at_once) {
-            constexpr int kRows = decltype(rows_at_once)::value;
-            for (int r0 = (int)(rank + ranks * warp); r0 < rows; r0 += (int)ranks * kEpilogueWarps * kRows) {
-                float v[kRows][kMats][4];
+        // A warp per row, one copy of the code: a launch of a few microseconds feels every instruction that has to be fetched (four rows
+        // at a time, unrolled, took 12 us where this takes 8).  Two shares are asked for together: another SM's shared memory is some
+        // 200 clocks away.
+#pragma unroll 1
+        for (int r = (int)(rank + ranks * warp); r < rows; r += (int)ranks * kEpilogueWarps) {
+            const int64_t row = m0 + r, at = row * p.out_row[problem] + n;
+            [[maybe_unused]] float dh[4];
+            if constexpr (kMode == kMatmulGatedGrad) load4(p.dh, row * p.dh_row + n, dh, valid, p.dtype);
+            float v[kMats][4];
 #pragma unroll
-                for (int j = 0; j < kRows; ++j)
+            for (int w = 0; w < kMats; ++w)
 #pragma unroll
-                    for (int w = 0; w < kMats; ++w)
+                for (int i = 0; i < 4; ++i) v[w][i] = bias[w][i];
+            const uint32_t from = ring + (r * kPartRow + 4 * lane) * 4;
+#pragma unroll 1
+            for (uint32_t s = 0; s < ranks; s += 2) {
+                float4 x[2][kMats];
 #pragma unroll
-                        for (int i = 0; i < 4; ++i) v[j][w][i] = bias[w][i];
-                [[maybe_unused]] float dh[kRows][4];
-                if constexpr (kMode == kMatmulGatedGrad) {
+                for (uint32_t j = 0; j < 2; ++j)
 #pragma unroll
-                    for (int j = 0; j < kRows; ++j) {
-                        const int r = r0 + j * (int)ranks * kEpilogueWarps;
-                        if (r < rows) load4(p.dh, (int64_t)(m0 + r) * p.dh_row + n, dh[j], valid, p.dtype);
-                    }
-                }
-                for (uint32_t s = 0; s < ranks; ++s) {
-                    float4 x[kRows][kMats];
+                    for (int w = 0; w < kMats; ++w) x[j][w] = s + j < ranks ? ld_cluster(map_rank(from, s + j) + w * kPartBytes) : make_float4(0.0f, 0.0f, 0.0f, 0.0f);
 #pragma unroll
-                    for (int j = 0; j < kRows; ++j) {
-                        const int r = min(r0 + j * (int)ranks * kEpilogueWarps, rows - 1);
-                        const uint32_t at = map_rank(ring + (r * kPartRow + 4 * lane) * 4, s);
+                for (uint32_t j = 0; j < 2; ++j)
 #pragma unroll
-                        for (int w = 0; w < kMats; ++w) x[j][w] = ld_cluster(at + w * kPartBytes);
-                    }
-#pragma unroll
-                    for (int j = 0; j < kRows; ++j)
-#pragma unroll
-                        for (int w = 0; w < kMats; ++w) v[j][w][0] += x[j][w].x, v[j][w][1] += x[j][w].y, v[j][w][2] += x[j][w].z, v[j][w][3] += x[j][w].w;
-                }
-#pragma unroll
-                for (int j = 0; j < kRows; ++j) {
-                    const int r = r0 + j * (int)ranks * kEpilogueWarps;
-                    if (r >= rows) break;
-                    const int64_t row = m0 + r, at = row * p.out_row[problem] + n;
-                    if constexpr (kMode == kMatmulPlain) {
-                        store4(p.out[problem], at, v[j][0], valid, p.out_dtype);
-                    } else if constexpr (kMode == kMatmulGated) {
-                        float h[4], top = 0.0f;
-#pragma unroll
-                        for (int i = 0; i < 4; ++i) {
-                            h[i] = i < valid ? activation(v[j][0][i], p.act) * v[j][1][i] : 0.0f;
-                            top = fmaxf(top, fabsf(h[i]));
-                        }
-                        if (p.out_dtype != COME_E4M3) {
-                            store4(p.out[0], at, h, valid, p.out_dtype);
-                        } else {
-#pragma unroll
-                            for (int s = 16; s >= 1; s >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, s));
-                            top = fmaxf(top, kSmallestMax);
-                            const float inv = __fdividef(kE4m3Max, top);
-                            const uint32_t q = pack_e4m3(h[0] * inv, h[1] * inv, h[2] * inv, h[3] * inv);
-                            uint8_t *out = (uint8_t *)p.out[0] + at;  // rows start at multiples of 16 bytes
-                            if (valid >= 4) {
-                                *reinterpret_cast<uint32_t *>(out) = q;
-                            } else {
-#pragma unroll
-                                for (int i = 0; i < 4; ++i)
-                                    if (i < valid) out[i] = (uint8_t)(q >> (8 * i));
-                            }
-                            if (lane == 0) p.out_scale[row * p.os_row + (n0 / kTile) * p.os_block] = top * (1.0f / kE4m3Max);
-                        }
-                    } else {
-                        float dg[4], du[4];
-#pragma unroll
-                        for (int i = 0; i < 4; ++i) {
-                            float a, slope;
-                            activation_grad(v[j][0][i], p.act, a, slope);
-                            dg[i] = dh[j][i] * v[j][1][i] * slope;
-                            du[i] = dh[j][i] * a;
-                        }
-                        store4(p.out[0], at, dg, valid, p.out_dtype);
-                        store4(p.out[1], row * p.out_row[1] + n, du, valid, p.out_dtype);
-                    }
-                }
+                    for (int w = 0; w < kMats; ++w) v[w][0] += x[j][w].x, v[w][1] += x[j][w].y, v[w][2] += x[j][w].z, v[w][3] += x[j][w].w;
             }
-        };
-        if (rows > (int)ranks * kEpilogueWarps) finish(std::integral_constant<int, 4>{});
-        else finish(std::integral_constant<int, 1>{});
+            if constexpr (kMode == kMatmulPlain) {
+                store4(p.out[problem], at, v[0], valid, p.out_dtype);
+            } else if constexpr (kMode == kMatmulGated) {
+                float h[4], top = 0.0f;
+#pragma unroll
+                for (int i = 0; i < 4; ++i) {
+                    h[i] = i < valid ? activation(v[0][i], p.act) * v[1][i] : 0.0f;
+                    top = fmaxf(top, fabsf(h[i]));
+                }
+                if (p.out_dtype != COME_E4M3) {
+                    store4(p.out[0], at, h, valid, p.out_dtype);
+                } else {
+#pragma unroll
+                    for (int s = 16; s >= 1; s >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, s));
+                    top = fmaxf(top, kSmallestMax);
+                    const float inv = __fdividef(kE4m3Max, top);
+                    const uint32_t q = pack_e4m3(h[0] * inv, h[1] * inv, h[2] * inv, h[3] * inv);
+                    uint8_t *out = (uint8_t *)p.out[0] + at;  // rows start at multiples of 16 bytes
+                    if (valid >= 4) {
+                        *reinterpret_cast<uint32_t *>(out) = q;
+                    } else {
+#pragma unroll
+                        for (int i = 0; i < 4; ++i)
+                            if (i < valid) out[i] = (uint8_t)(q >> (8 * i));
+                    }
+                    if (lane == 0) p.out_scale[row * p.os_row + (n0 / kTile) * p.os_block] = top * (1.0f / kE4m3Max);
+                }
+            } else {
+                float dg[4], du[4];
+#pragma unroll
+                for (int i = 0; i < 4; ++i) {
+                    float a, slope;
+                    activation_grad(v[0][i], p.act, a, slope);
+                    dg[i] = dh[i] * v[1][i] * slope;
+                    du[i] = dh[i] * a;
+                }
+                store4(p.out[0], at, dg, valid, p.out_dtype);
+                store4(p.out[1], row * p.out_row[1] + n, du, valid, p.out_dtype);
+            }
+        }
     }
     cluster_sync();  // no CTA leaves while another reads its share
     if (warp == kIssuerWarp) {
