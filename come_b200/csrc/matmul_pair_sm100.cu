@@ -52,7 +52,7 @@ typedef float PairScales[kScaleSlots][2][kTile];
 constexpr size_t smem_bytes(bool e4m3) { return kStages * kStageBytes + 8 * staging_bytes(e4m3) + sizeof(PairBarriers) + (e4m3 ? sizeof(PairScales) : 0); }
 static_assert(smem_bytes(true) <= 227 * 1024 && smem_bytes(false) <= 227 * 1024, "");
 
-__device__ __forceinline__ void tmem_ld16(uint32_t taddr, uint32_t (&r)[16]) {
+__device__ __forceinline__ void tmem_ld16(uint32_t taddr, uint32_t *r) {
     asm volatile(
         "tcgen05.ld.sync.aligned.32x32b.x16.b32 "
         "{%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15}, [%16];"
@@ -208,18 +208,19 @@ __global__ void __launch_bounds__(kThreads, 1) __cluster_dims__(2, 1, 1) matmul_
     constexpr uint32_t tmem = 0;
     const uint32_t ring = smem_u32(smem);
     const auto wait = [&](uint64_t *bar, uint32_t parity, uint32_t code) { return mbar_wait_limit(bar, parity, &sh.abort_flag, p.status, code, kWaitTicks); };
-    const int total = p.tiles_per_problem * p.problems;
+    const int total = p.tiles_m * p.problems * p.tiles_n;
     struct Tile {
         int problem, m0, n0;
     };
-    const auto tile_at = [&](int t) {
+    const auto tile_of = [&](int row, int col) {  // row and column of the grid of tiles; the second problem's rows follow the first's
         Tile w;
-        w.problem = kAMn && t >= p.tiles_per_problem ? 1 : 0;
-        t -= w.problem * p.tiles_per_problem;
-        w.m0 = (t / p.tiles_n) * 2 * kTile + (int)rank * kTile;
-        w.n0 = (t % p.tiles_n) * (kGated ? kTile : kPairN);
+        w.problem = kAMn && row >= p.tiles_m ? 1 : 0;
+        w.m0 = (row - w.problem * p.tiles_m) * 2 * kTile + (int)rank * kTile;
+        w.n0 = col * (kGated ? kTile : kPairN);
         return w;
     };
+    const auto tile_at = [&](int t) { return tile_of(t / p.tiles_n, t % p.tiles_n); };
+    const int step_row = pairs / p.tiles_n, step_col = pairs - step_row * p.tiles_n;
     if (sh.tmem_base != tmem && threadIdx.x == 0) {
         sh.abort_flag = 1;
         atomicOr(p.status, kErrSums);
@@ -388,10 +389,12 @@ __global__ void __launch_bounds__(kThreads, 1) __cluster_dims__(2, 1, 1) matmul_
         bool ok = true, busy = false;
         [[maybe_unused]] const bool with_bias = p.bias[0] != nullptr || (kGated && p.bias[1] != nullptr);
         [[maybe_unused]] float *bias = reinterpret_cast<float *>(stage);  // [128]: of the gate's and the up projection's 64 columns, or of 128
-        for (int t = pair; t < total; t += pairs, ++tiles) {
+        int tile_row = pair / p.tiles_n, tile_col = pair - tile_row * p.tiles_n;
+        const int count = (total - pair + pairs - 1) / pairs;
+        for (; tiles < count; ++tiles) {
             if constexpr (kE4m3) {
                 {   // the biases of the warp's columns, before the sums
-                    const Tile w = tile_at(t);
+                    const Tile w = tile_of(tile_row, tile_col);
                     const int n = w.n0 + part * kCols, cols = p.N - n;
                     if (with_bias) {
                         __syncwarp();
@@ -417,14 +420,14 @@ __global__ void __launch_bounds__(kThreads, 1) __cluster_dims__(2, 1, 1) matmul_
                         tc_fence_after();
                         const float s0 = scales[slot][kGated ? 0 : part][r], s1 = kGated ? scales[slot][1][r] : s0;
                         const f32x2_t s0p = pack_f32x2(s0, s0), s1p = pack_f32x2(s1, s1);
-                        const auto column = [&](int c) { return lanes + buf * kPairN + (kGated ? (c >> 1) * kTile + (c & 1) * 32 : c * 32); };
-                        uint32_t d[2][16];
-                        const auto column16 = [&](int c) { return lanes + buf * kPairN + (kGated ? (c >> 2) * kTile + (c & 3) * 16 : c * 16); };
-                        tmem_ld16(column16(0), d[0]);
-                        tmem_ld16(column16(1), d[1]);
+                        // 16 columns at a time, two loads in flight: 32 at a time need registers that are not there (spills cost 15 %)
+                        const auto column = [&](int c) { return lanes + buf * kPairN + (kGated ? (c >> 2) * kTile + (c & 3) * 16 : c * 16); };
+                        uint32_t d[32];
+                        tmem_ld16(column(0), d);
+                        tmem_ld16(column(1), d + 16);
 #pragma unroll
                         for (int c = 0; c < 8; c += 2) {
-                            tc_wait_ld();
+                            tc_wait_ld_of(d);
                             if (c == 6) {
                                 tc_fence_before();
                                 __syncwarp();
@@ -434,17 +437,17 @@ __global__ void __launch_bounds__(kThreads, 1) __cluster_dims__(2, 1, 1) matmul_
                             for (int j = 0; j < 2; ++j) {
 #pragma unroll
                                 for (int e = 0; e < 8; ++e)
-                                    sum[(c + j) * 8 + e] = fma_f32x2(pack_f32x2(__uint_as_float(d[j][2 * e]), __uint_as_float(d[j][2 * e + 1])), (c + j) >> 2 ? s1p : s0p, sum[(c + j) * 8 + e]);
-                                if (c < 6) tmem_ld16(column16(c + 2 + j), d[j]);
+                                    sum[(c + j) * 8 + e] = fma_f32x2(pack_f32x2(__uint_as_float(d[j * 16 + 2 * e]), __uint_as_float(d[j * 16 + 2 * e + 1])), (c + j) >> 2 ? s1p : s0p, sum[(c + j) * 8 + e]);
+                                if (c < 6) tmem_ld16(column(c + 2 + j), d + j * 16);
                             }
                         }
                     } else if (ok && lane == 0) {
                         mbar_arrive_at(empty0 + buf * 8);
                     }
                 }
-                // Where the tile lies is worked out again (the shuffle hides that it is the same number): kept over the loop, it costs
+                // Where the tile lies is worked out again (the shuffles hide that they are the same numbers): kept over the loop, it costs
                 // registers that the sums need.
-                const Tile w = tile_at(__shfl_sync(0xffffffffu, t, 0));
+                const Tile w = tile_of(__shfl_sync(0xffffffffu, tile_row, 0), __shfl_sync(0xffffffffu, tile_col, 0));
                 const int rows = min(32, p.M - w.m0 - warp_row), n = w.n0 + part * kCols, cols = p.N - n;
                 const int64_t row0 = w.m0 + warp_row;
                 if constexpr (!kGated) {
@@ -497,7 +500,7 @@ __global__ void __launch_bounds__(kThreads, 1) __cluster_dims__(2, 1, 1) matmul_
                         }
                     }
                 } else {
-                    float top = 0.0f;  // the results take the place of the gate's sums
+                    float tops[4] = {0.0f, 0.0f, 0.0f, 0.0f};  // the results take the place of the gate's sums
                     if (ok && busy) {
                         if (with_bias) {
 #pragma unroll
@@ -514,26 +517,27 @@ __global__ void __launch_bounds__(kThreads, 1) __cluster_dims__(2, 1, 1) matmul_
                                 float g0, g1, u0, u1;
                                 unpack_f32x2(sum[c], g0, g1);
                                 unpack_f32x2(sum[32 + c], u0, u1);
-                                sum[c] = pack_f32x2(activation(g0, act) * u0, activation(g1, act) * u1);
+                                const float h0 = activation(g0, act) * u0, h1 = activation(g1, act) * u1;
+                                tops[c & 3] = fmaxf(tops[c & 3], fmaxf(fabsf(h0), fabsf(h1)));  // under the special-function unit
+                                sum[c] = pack_f32x2(h0, h1);
                             }
                         });
-                        if (cols < 64)  // columns past the end: the bytes of other rows' products
+                        if (cols < 64) {  // columns past the end: the bytes of other rows' products
+                            tops[0] = tops[1] = tops[2] = tops[3] = 0.0f;
 #pragma unroll
                             for (int c = 0; c < 32; ++c) {
                                 float h0, h1;
                                 unpack_f32x2(sum[c], h0, h1);
-                                sum[c] = pack_f32x2(2 * c < cols ? h0 : 0.0f, 2 * c + 1 < cols ? h1 : 0.0f);
+                                h0 = 2 * c < cols ? h0 : 0.0f;
+                                h1 = 2 * c + 1 < cols ? h1 : 0.0f;
+                                tops[0] = fmaxf(tops[0], fmaxf(fabsf(h0), fabsf(h1)));
+                                sum[c] = pack_f32x2(h0, h1);
                             }
+                        }
                         __syncwarp();
                     }
                     if (p.out_dtype == COME_E4M3) {
-                        if (ok && busy)
-#pragma unroll
-                            for (int c = 0; c < 32; ++c) {
-                                float h0, h1;
-                                unpack_f32x2(sum[c], h0, h1);
-                                top = fmaxf(top, fmaxf(fabsf(h0), fabsf(h1)));
-                            }
+                        float top = fmaxf(fmaxf(tops[0], tops[1]), fmaxf(tops[2], tops[3]));
                         // the largest magnitude of a row's 128 columns: half of it in the other warpgroup (every warp meets here, also
                         // one that gave up; a third tile's write to the same place is two barriers away)
                         sh.top[tiles & 1][part][r] = top;
@@ -581,7 +585,7 @@ __global__ void __launch_bounds__(kThreads, 1) __cluster_dims__(2, 1, 1) matmul_
                     }
                 }
             } else {
-                const Tile w = tile_at(t);
+                const Tile w = tile_of(tile_row, tile_col);
                 const int rows = min(32, p.M - w.m0 - warp_row);      // of this warp, may be <= 0
                 const int n = w.n0 + part * kCols, cols = p.N - n;    // first result column of the thread, columns from there on
                 busy = rows > 0;
@@ -691,6 +695,12 @@ __global__ void __launch_bounds__(kThreads, 1) __cluster_dims__(2, 1, 1) matmul_
                 }
                 ++chunk;
             }
+            tile_row += step_row;
+            tile_col += step_col;
+            if (tile_col >= p.tiles_n) {
+                tile_col -= p.tiles_n;
+                ++tile_row;
+            }
         }
     }
     if (sh.abort_flag != 0) {  // the other CTA's copies complete on the first one's barriers: give those in flight time to land
@@ -710,7 +720,7 @@ __global__ void __launch_bounds__(kThreads, 1) __cluster_dims__(2, 1, 1) matmul_
 template <bool kE4m3, int kMode, bool kAMn, bool kBMn> int launch_pair(const MatmulParams &p, cudaStream_t st) {
     constexpr auto kernel = matmul_pair_kernel<kE4m3, kMode, kAMn, kBMn>;
     if (int rc = allow_smem<kernel>(smem_bytes(kE4m3)); rc != COME_OK) return rc;
-    const int tiles = p.tiles_per_problem * p.problems, pairs = sm_count() / 2;
+    const int tiles = p.tiles_m * p.problems * p.tiles_n, pairs = sm_count() / 2;
     kernel<<<2 * (tiles < pairs ? tiles : pairs), kThreads, smem_bytes(kE4m3), st>>>(p);
     return check_launch("product kernel");
 }
@@ -731,9 +741,9 @@ bool matmul_pair_takes(const MatmulArgs &a) {
 int matmul_pair_launch(const MatmulArgs &a, MatmulParams &p, cudaStream_t st) {
     const int n = a.mode == kMatmulPlain ? kPairN : kTile;
     p.tiles_n = (int)((a.N + n - 1) / n);
-    const int64_t per_problem = (a.M + 2 * kTile - 1) / (2 * kTile) * p.tiles_n;
-    COME_REQUIRE(per_problem * a.problems < (1ll << 30), "the result has too many tiles for one launch");
-    p.tiles_per_problem = (int)per_problem;
+    const int64_t rows = (a.M + 2 * kTile - 1) / (2 * kTile);
+    COME_REQUIRE(rows * p.tiles_n * a.problems < (1ll << 30), "the result has too many tiles for one launch");
+    p.tiles_m = (int)rows;
     if (a.e4m3) return a.mode == kMatmulPlain ? launch_pair<true, kMatmulPlain, false, false>(p, st) : launch_pair<true, kMatmulGated, false, false>(p, st);
     if (a.mode == kMatmulGated) return launch_pair<false, kMatmulGated, false, false>(p, st);
     if (a.mode == kMatmulGatedGrad) return launch_pair<false, kMatmulGatedGrad, false, false>(p, st);

@@ -98,7 +98,7 @@ __global__ void __launch_bounds__(kThreads, 1) matmul_split_kernel(const __grid_
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     const uint32_t rank = cluster_rank(), ranks = cluster_size();
 
-    const int tile = (int)(blockIdx.x / ranks), problem = tile / p.tiles_per_problem, t = tile - problem * p.tiles_per_problem;
+    const int tile = (int)(blockIdx.x / ranks), per_problem = p.tiles_m * p.tiles_n, problem = tile / per_problem, t = tile - problem * per_problem;
     const int m0 = (t / p.tiles_n) * kTile, n0 = (t % p.tiles_n) * kTile;
     const int kb0 = (int)((int64_t)p.k_blocks * rank / ranks), kb1 = (int)((int64_t)p.k_blocks * (rank + 1) / ranks), n_kb = kb1 - kb0;
     const int rows = min(kTile, p.M - m0);
@@ -434,7 +434,7 @@ int run_matmul(const MatmulArgs &a, cudaStream_t st) {
     p.tiles_n = (int)((a.N + kTile - 1) / kTile);
     const int64_t per_problem = (a.M + kTile - 1) / kTile * p.tiles_n, tiles = per_problem * a.problems;
     COME_REQUIRE(tiles < (1ll << 27), "the result has %lld tiles of 128 x 128: too many for one launch", (long long)tiles);
-    p.tiles_per_problem = (int)per_problem;
+    p.tiles_m = (int)(per_problem / p.tiles_n);
     const int cluster = pick_cluster(tiles, p.k_blocks);
     if (a.e4m3) return a.mode == kMatmulPlain ? launch_split<true, kMatmulPlain, false, false>(p, tiles, cluster, st) : launch_split<true, kMatmulGated, false, false>(p, tiles, cluster, st);
     if (a.mode == kMatmulGated) return launch_split<false, kMatmulGated, false, false>(p, tiles, cluster, st);

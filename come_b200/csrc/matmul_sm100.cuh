@@ -56,7 +56,7 @@ struct MatmulParams {
     float *out_scale;
     int64_t dh_row, out_row[2], os_row, os_block;
     int M, N, kb_per_sum, k_blocks;  // K blocks of one contraction, of all
-    int tiles_n, tiles_per_problem, problems;
+    int tiles_m, tiles_n, problems;   // grid of tiles of one problem
     int act, dtype, bias_dtype, out_dtype;
     unsigned int *status;
 };
