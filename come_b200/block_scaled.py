@@ -255,8 +255,11 @@ class BlockScaledGatedMlp(_QuantizedWeights):
 
 
 def to_block_scaled(module: torch.nn.Module, out_dtype: torch.dtype = torch.bfloat16) -> torch.nn.Module:
-    """Replaces every gated MLP inside ``module`` (on its CUDA device) by its 8-bit form, in place; returns ``module``."""
+    """Replaces every gated MLP inside ``module`` (on its CUDA device) by its 8-bit form, in place; returns ``module``, or the 8-bit form
+    of ``module`` when it is a gated MLP itself."""
     from .feed_forward import GatedMlp
+    if isinstance(module, GatedMlp):
+        return BlockScaledGatedMlp(module, out_dtype)
     for parent in list(module.modules()):
         for name, child in list(parent.named_children()):
             if isinstance(child, GatedMlp):

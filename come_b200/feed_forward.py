@@ -118,8 +118,8 @@ def gated_linear(x: torch.Tensor, w_gate: torch.Tensor, w_up: torch.Tensor, b_ga
 
 class GatedMlp(torch.nn.Module):
     """``w3(act(gate) * up)`` with ``gate, up = w12(x).chunk(2)``: the gated MLP of a block.  The two projections, the activation and the
-    product are one kernel; ``w3`` stays a PyTorch GEMM like the other linear layers of the blocks.  In 8 bits:
-    :class:`come_b200.block_scaled.BlockScaledGatedMlp`."""
+    product are one kernel; ``w3`` stays a PyTorch GEMM like the other linear layers of the blocks.  float16 and bfloat16, ``dim`` a multiple
+    of 8; float32 streams take the 8-bit form, :class:`come_b200.block_scaled.BlockScaledGatedMlp`."""
 
     def __init__(self, dim: int, hidden: int, bias: bool = True, activation: str = "silu"):
         super().__init__()

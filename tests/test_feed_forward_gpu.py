@@ -555,6 +555,8 @@ def test_gated_mlp_in_16_and_8_bits():
     want, size = h @ w3.t() + b3, h.abs() @ w3.abs().t() + b3.abs()
     within(y, want, (2.0 ** -8 + 16 * chain(328)) * size + 2.0 ** -8 * want.abs(), "bf16 module")
     m8 = BlockScaledGatedMlp(mlp, out_dtype=torch.float32)
+    from come_b200.block_scaled import to_block_scaled
+    assert isinstance(to_block_scaled(mlp), BlockScaledGatedMlp) and isinstance(to_block_scaled(torch.nn.Sequential(m16))[0], BlockScaledGatedMlp)
     assert m8.to(torch.bfloat16).gate_scale.dtype == torch.float32 and m8.gate.dtype == torch.float8_e4m3fn  # a cast leaves 8-bit weights alone
     y8 = m8(x)
     assert y8.dtype == torch.float32 and y8.shape == x.shape
