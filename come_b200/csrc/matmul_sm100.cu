@@ -14,6 +14,9 @@
 // contraction's; shares of it bring all SMs to read the weights.  The shares meet in shared memory, not in a workspace, so that two
 // graphs captured from the same call share nothing.
 //
+// Measured in a graph: 1 token 2736 -> 1024 in 8 bits 6.4 us, 64 tokens 7.7, 128 tokens 9.0 (weights 2.8 MB; launch, cluster barriers and
+// the first loads' latency are most of it), 1374 tokens 1024 -> 1024 10 us.
+//
 // Shared memory: a CTA takes more than half an SM's, so that no two CTAs that need tensor memory share an SM: CTAs of two clusters
 // that wait for each other's tensor memory while their partners wait at a cluster barrier would never end.
 //

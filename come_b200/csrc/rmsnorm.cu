@@ -9,6 +9,9 @@
 // group of several warps (few rows, where a row's latency counts, and wide rows, whose float32 copy would not fit one warp's
 // registers): thread i of the group holds the vectors i, i + group size, ... of the row, so the 128 columns of a scale always lie
 // in 16 (16-bit types) or 32 (float32) neighbouring lanes and their maximum needs shuffles only.
+//
+// Measured: 80,672 x 1024 bf16 with residual and 8-bit result 114 us (5.1 TB/s, 78 % of the copy rate; with a bf16 result 108 us, 6.1
+// TB/s), 10,534 x 1000 float32 28.7 us (5.9 TB/s).
 #include "block_scale.cuh"
 
 namespace come {
@@ -188,6 +191,8 @@ template <typename T, bool kAligned> int launch_rmsnorm(const RmsNormArgs &a, cu
 #define COME_RMS_LAUNCH(WARPS, NV, THREADS, PER_SM)                                                                       \
     residual_rmsnorm_kernel<T, WARPS, NV, THREADS, kAligned>                                                              \
         <<<grid((a.rows * WARPS * 32 + THREADS - 1) / THREADS, PER_SM), THREADS, 0, st>>>(a)
+    // A warp per row up to 128 vectors, four from there on: 80,672 x 1024 bf16 (128 vectors) 114 / 134 us with one / four, 10,534 x 1000
+    // float32 (250 vectors) 35 / 29.  Few rows take four or eight warps each: a row's latency counts there.
     if (vectors > 4 * 128 || (a.rows <= 4 * sms && vectors > 32)) {
         if (vectors <= 128) COME_RMS_LAUNCH(4, 1, 128, 16);
         else if (vectors <= 256) COME_RMS_LAUNCH(8, 1, 256, 8);
