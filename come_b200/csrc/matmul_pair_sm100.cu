@@ -97,6 +97,31 @@ template <int kRow> __device__ __forceinline__ uint4 *staged(uint8_t *base, int 
     return reinterpret_cast<uint4 *>(base + row * kRow + ((chunk ^ (kRow == 128 ? row & 7 : (row >> 1) & 3)) * 16));
 }
 
+// Rows that do not start at multiples of 16 bytes leave in pieces of 8 or 4 bytes, neighbouring lanes neighbouring pieces.
+template <int kBytes> struct Piece;
+template <> struct Piece<8> { typedef uint2 type; };
+template <> struct Piece<4> { typedef uint32_t type; };
+template <> struct Piece<2> { typedef uint16_t type; };
+template <> struct Piece<1> { typedef uint8_t type; };
+template <int kSize, int kRow, int kPiece> __device__ __forceinline__ void store_pieces(uint8_t *base, uint8_t *out, int64_t row_bytes, int rows, int cols, int lane) {
+    typedef typename Piece<kPiece>::type P;
+    typedef typename Piece<kSize>::type E;
+    constexpr int kPerRow = kRow / kPiece;
+#pragma unroll 2
+    for (int i = lane; i < 32 * kPerRow; i += 32) {
+        const int r = i / kPerRow, at = i % kPerRow * kPiece, left = cols * kSize - at;
+        if (r < rows && left > 0) {
+            const uint8_t *from = reinterpret_cast<const uint8_t *>(staged<kRow>(base, r, at / 16)) + at % 16;
+            uint8_t *to = out + r * row_bytes + at;
+            if (left >= kPiece) *reinterpret_cast<P *>(to) = *reinterpret_cast<const P *>(from);
+            else
+#pragma unroll
+                for (int j = 0; j < kPiece / kSize; ++j)
+                    if (j * kSize < left) reinterpret_cast<E *>(to)[j] = reinterpret_cast<const E *>(from)[j];
+        }
+    }
+}
+
 // Rows [0, rows) x columns [0, cols) of elements of `kSize` bytes, kRow bytes staged per row, to out (row stride in bytes).
 template <int kSize, int kRow> __device__ __forceinline__ void store_staged(uint8_t *base, uint8_t *out, int64_t row_bytes, int rows, int cols, int lane) {
     constexpr int kChunks = kRow / 16, kRowsAtOnce = 32 / kChunks, kPerChunk = 16 / kSize;
@@ -122,14 +147,16 @@ template <int kSize, int kRow> __device__ __forceinline__ void store_staged(uint
                 }
             }
         }
-    } else {  // rows that do not start at multiples of 16 bytes: element by element, neighbouring lanes neighbouring elements
+    } else if ((((uintptr_t)out | (uintptr_t)row_bytes) & 7) == 0) {
+        store_pieces<kSize, kRow, 8>(base, out, row_bytes, rows, cols, lane);
+    } else if ((((uintptr_t)out | (uintptr_t)row_bytes) & 3) == 0) {
+        store_pieces<kSize, kRow, 4>(base, out, row_bytes, rows, cols, lane);
+    } else {  // element by element, a row at a time: neighbouring lanes neighbouring elements
         for (int r = 0; r < min(rows, 32); ++r)
             for (int c = lane; c < min(cols, kRow / kSize); c += 32) {
                 const uint8_t *e = reinterpret_cast<const uint8_t *>(staged<kRow>(base, r, c / kPerChunk)) + c % kPerChunk * kSize;
-                uint8_t *p = out + r * row_bytes + (int64_t)c * kSize;
-                if constexpr (kSize == 1) *p = *e;
-                else if constexpr (kSize == 2) *reinterpret_cast<uint16_t *>(p) = *reinterpret_cast<const uint16_t *>(e);
-                else *reinterpret_cast<uint32_t *>(p) = *reinterpret_cast<const uint32_t *>(e);
+                typedef typename Piece<kSize>::type E;
+                *reinterpret_cast<E *>(out + r * row_bytes + (int64_t)c * kSize) = *reinterpret_cast<const E *>(e);
             }
     }
 }
@@ -743,6 +770,7 @@ template <bool kE4m3, int kMode, bool kAMn, bool kBMn> int launch_pair(const Mat
 bool matmul_pair_takes(const MatmulArgs &a) {
     const int64_t n = a.mode == kMatmulPlain ? kPairN : kTile, pairs = sm_count() / 2;
     const int64_t tiles = (a.M + 2 * kTile - 1) / (2 * kTile) * ((a.N + n - 1) / n) * a.problems;
+    if (a.low_rows > 0 || a.sums * a.problems > 2) return false;  // few tokens: the split kernel alone has these forms
     return tiles * 2 >= pairs || (a.e4m3 && a.mode == kMatmulGated && a.M > 96 && tiles * 4 >= pairs);
 }
 

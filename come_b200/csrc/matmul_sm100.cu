@@ -107,7 +107,7 @@ __global__ void __launch_bounds__(kThreads, 1) matmul_split_kernel(const __grid_
     const int rows = min(kTile, p.M - m0);
 
     if (warp == kProducerWarp && lane == 0) {
-        prefetch_map(&p.a[problem]);
+        prefetch_map(&p.a[problem * p.sums]);
         prefetch_map(&p.b[0]);
         if constexpr (kMats == 2) prefetch_map(&p.b[1]);
         sh.abort_flag = (*(volatile unsigned int *)p.status & kStatusMatmul) != 0 ? 1u : 0u;  // an earlier launch gave up
@@ -142,10 +142,10 @@ __global__ void __launch_bounds__(kThreads, 1) matmul_split_kernel(const __grid_
             for (; i < n_kb; ++i) {
                 const int st = i % kStages;
                 if (!wait(&sh.empty[st], ((i / kStages) & 1) ^ 1, kErrEmpty)) break;
-                const int kb = kb0 + i, sum = kb >= p.kb_per_sum ? 1 : 0, k = (kb - sum * p.kb_per_sum) * kElems;
+                const int kb = kb0 + i, sum = kE4m3 || p.sums == 1 ? 0 : kb / p.kb_per_sum, k = (kb - sum * p.kb_per_sum) * kElems;
                 const uint32_t dst = ring + st * kStageBytes;
                 mbar_arrive_expect_tx(&sh.full[st], kStageBytes);
-                const CUtensorMap *ma = &p.a[sum + problem], *mb = &p.b[sum];
+                const CUtensorMap *ma = &p.a[problem * p.sums + sum], *mb = &p.b[kAMn ? 0 : sum & 1];
                 if constexpr (kAMn) {
                     tma_load_2d(dst, ma, m0, k, &sh.full[st]);
                     tma_load_2d(dst + kOperandBytes / 2, ma, m0 + 64, k, &sh.full[st]);
@@ -354,6 +354,15 @@ __global__ void __launch_bounds__(kThreads, 1) matmul_split_kernel(const __grid_
                 }
                 store4(p.out[0], at, dg, valid, p.out_dtype);
                 store4(p.out[1], row * p.out_row[1] + n, du, valid, p.out_dtype);
+                if (p.low_rows > 0) {
+#pragma unroll
+                    for (int i = 0; i < 4; ++i) {
+                        dg[i] -= p.out_dtype == COME_BF16 ? __bfloat162float(__float2bfloat16_rn(dg[i])) : __half2float(__float2half_rn(dg[i]));
+                        du[i] -= p.out_dtype == COME_BF16 ? __bfloat162float(__float2bfloat16_rn(du[i])) : __half2float(__float2half_rn(du[i]));
+                    }
+                    store4(p.out[0], at + p.low_rows * p.out_row[0], dg, valid, p.out_dtype);
+                    store4(p.out[1], (row + p.low_rows) * p.out_row[1] + n, du, valid, p.out_dtype);
+                }
             }
         }
     }
@@ -400,11 +409,11 @@ int run_matmul(const MatmulArgs &a, cudaStream_t st) {
     p.status = status_word_dev();
     if (!p.status) return COME_ERR_CUDA;
     int rc;
-    for (int i = 0; i < (a.sums > a.problems ? a.sums : a.problems); ++i) {
+    for (int i = 0; i < a.sums * a.problems; ++i) {
         rc = a.a_mn ? make_rows_map(&p.a[i], a.a[i], a.e4m3, a.dtype, a.K, a.M, a.a_row[i], 64) : make_rows_map(&p.a[i], a.a[i], a.e4m3, a.dtype, a.M, a.K, a.a_row[i], kTile);
         if (rc != COME_OK) return rc;
     }
-    for (int i = 0; i < (a.sums > mats ? a.sums : mats); ++i) {
+    for (int i = 0; i < (a.a_mn ? 1 : a.sums > 1 ? 2 : mats); ++i) {
         rc = a.b_mn ? make_rows_map(&p.b[i], a.b[i], a.e4m3, a.dtype, a.K, a.N, a.b_row[i], 64) : make_rows_map(&p.b[i], a.b[i], a.e4m3, a.dtype, a.N, a.K, a.b_row[i], kTile);
         if (rc != COME_OK) return rc;
     }
@@ -427,7 +436,9 @@ int run_matmul(const MatmulArgs &a, cudaStream_t st) {
     p.N = (int)a.N;
     const int elems = a.e4m3 ? 128 : 64;
     p.kb_per_sum = (int)((a.K + elems - 1) / elems);
+    p.sums = a.sums;
     p.k_blocks = p.kb_per_sum * a.sums;
+    p.low_rows = a.low_rows;
     p.problems = a.problems;
     p.act = a.act;
     p.dtype = a.dtype;
@@ -602,6 +613,14 @@ extern "C" int come_gated_matmul(const void *x_dev, int64_t x_row_stride, const 
     return come::run_matmul(a, (cudaStream_t)stream);
 }
 
+// Gradients of few tokens, or of few elements, are sums of few rounded numbers: the error is the luck of some hundred roundings rather
+// than their average (up to 1.7 times that of float32 operands after rounding, where large ones have 1.4).  There the operands keep a
+// second 16-bit part, which doubles contractions that are short anyway: a step of 64 tokens 1024 -> 2736 stays with the host.
+extern "C" int64_t come_gated_backward_rows(int64_t tokens, int64_t features) {
+    if (tokens <= 0) return 0;
+    return tokens <= 64 || (features < (1ll << 18) && tokens < (1ll << 18) && tokens * features <= (1ll << 18)) ? 2 * tokens : tokens;
+}
+
 extern "C" int come_gated_matmul_backward(const void *x_dev, int64_t x_row_stride, const void *gate_dev, int64_t gate_row_stride, const void *up_dev, int64_t up_row_stride,
                                           const void *gate_bias_dev, const void *up_bias_dev, int dtype, int activation, int64_t tokens, int64_t features,
                                           int64_t channels, const void *dout_dev, int64_t dout_row_stride, void *dgate_dev, void *dup_dev, int64_t d_row_stride,
@@ -623,16 +642,19 @@ extern "C" int come_gated_matmul_backward(const void *x_dev, int64_t x_row_strid
     a.dh = dout_dev, a.dh_row = dout_row_stride;
     a.out[0] = dgate_dev, a.out[1] = dup_dev;
     a.out_row[0] = a.out_row[1] = d_row_stride;
+    const int parts = (int)(come_gated_backward_rows(tokens, features) / tokens);
+    a.low_rows = parts > 1 ? tokens : 0;
+    const auto part = [&](const void *d, int i) { return (const void *)((const uint16_t *)d + i * tokens * d_row_stride); };
     if ((rc = run_matmul(a, st)) != COME_OK) return rc;
     if (dx_dev) {  // dx = dgate gate + dup up
         MatmulArgs b = {};
         b.dtype = b.out_dtype = dtype;
         b.b_mn = true;
         b.M = tokens, b.N = channels, b.K = features;
-        b.a[0] = dgate_dev, b.a[1] = dup_dev, b.a_row[0] = b.a_row[1] = d_row_stride;
+        for (int i = 0; i < 2 * parts; ++i) b.a[i] = part(i & 1 ? dup_dev : dgate_dev, i >> 1), b.a_row[i] = d_row_stride;
         b.b[0] = gate_dev, b.b_row[0] = gate_row_stride;
         b.b[1] = up_dev, b.b_row[1] = up_row_stride;
-        b.sums = 2, b.problems = 1;
+        b.sums = 2 * parts, b.problems = 1;
         b.out[0] = dx_dev, b.out_row[0] = dx_row_stride;
         if ((rc = run_matmul(b, st)) != COME_OK) return rc;
     }
@@ -642,11 +664,11 @@ extern "C" int come_gated_matmul_backward(const void *x_dev, int64_t x_row_strid
         b.a_mn = b.b_mn = true;
         b.M = features, b.N = channels, b.K = tokens;
         b.b[0] = x_dev, b.b_row[0] = x_row_stride;
-        b.sums = 1;
+        b.sums = parts;
         for (int i = 0; i < 2; ++i) {
             void *out = i ? dup_weight_dev : dgate_weight_dev;
             if (!out) continue;
-            b.a[b.problems] = i ? dup_dev : dgate_dev, b.a_row[b.problems] = d_row_stride;
+            for (int j = 0; j < parts; ++j) b.a[b.problems * parts + j] = part(i ? dup_dev : dgate_dev, j), b.a_row[b.problems * parts + j] = d_row_stride;
             b.out[b.problems] = out, b.out_row[b.problems++] = dw_row_stride;
         }
         if ((rc = run_matmul(b, st)) != COME_OK) return rc;
@@ -654,9 +676,9 @@ extern "C" int come_gated_matmul_backward(const void *x_dev, int64_t x_row_strid
     if (dgate_bias_dev || dup_bias_dev) {
         const dim3 grid((unsigned)((features + 31) / 32), 2);
         if (dtype == COME_F16)
-            column_sums_kernel<__half><<<grid, kSumThreads, 0, st>>>((const __half *)dgate_dev, (const __half *)dup_dev, d_row_stride, tokens, (int)features, (__half *)dgate_bias_dev, (__half *)dup_bias_dev);
+            column_sums_kernel<__half><<<grid, kSumThreads, 0, st>>>((const __half *)dgate_dev, (const __half *)dup_dev, d_row_stride, parts * tokens, (int)features, (__half *)dgate_bias_dev, (__half *)dup_bias_dev);
         else
-            column_sums_kernel<__nv_bfloat16><<<grid, kSumThreads, 0, st>>>((const __nv_bfloat16 *)dgate_dev, (const __nv_bfloat16 *)dup_dev, d_row_stride, tokens, (int)features,
+            column_sums_kernel<__nv_bfloat16><<<grid, kSumThreads, 0, st>>>((const __nv_bfloat16 *)dgate_dev, (const __nv_bfloat16 *)dup_dev, d_row_stride, parts * tokens, (int)features,
                                                                             (__nv_bfloat16 *)dgate_bias_dev, (__nv_bfloat16 *)dup_bias_dev);
         return check_launch("come_gated_matmul_backward");
     }

@@ -23,11 +23,12 @@ struct MatmulArgs {
     int dtype;
     bool a_mn, b_mn;       // operand stored with the contraction as its rows (16 bits)
     int64_t M, N, K;
-    // Operands.  Two contractions that are added (a[0] b[0] + a[1] b[1], plain mode, `sums` 2), two problems that share b[0]
-    // (a[z] b[0] -> outs[z], plain mode, `problems` 2), or two weights b[0], b[1] of one a[0] (gated modes).
-    const void *a[2], *b[2];
-    int64_t a_row[2], b_row[2];  // row strides in elements
+    // Operands.  `sums` contractions that are added and `problems` of them (plain mode): a[problem * sums + sum] times b[sum & 1], or times
+    // b[0] where both are stored with the contraction as their rows; or two weights b[0], b[1] of one a[0] (gated modes).
+    const void *a[4], *b[2];
+    int64_t a_row[4], b_row[2];  // row strides in elements
     int sums, problems;
+    int64_t low_rows;            // gated gradient: what rounding took from row r of a result goes to row r + low_rows; 0: nowhere
     // Scales of 8-bit operands: of a[0] per row and 128 contraction elements, of b[i] per 128 x 128 block.
     const float *a_scale, *b_scale[2];
     int64_t as_row, as_block, bs_row[2];
@@ -48,14 +49,15 @@ constexpr int kOperandBytes = kTile * kKBytes;     // 16 KiB: 128 rows of a K bl
 
 // What a launch of either kernel gets.
 struct MatmulParams {
-    CUtensorMap a[2], b[2];
+    CUtensorMap a[4], b[2];
     const float *a_scale, *b_scale[2];
     int64_t as_row, as_block, bs_row[2];
     const void *bias[2], *dh;
     void *out[2];
     float *out_scale;
     int64_t dh_row, out_row[2], os_row, os_block;
-    int M, N, kb_per_sum, k_blocks;  // K blocks of one contraction, of all
+    int64_t low_rows;
+    int M, N, sums, kb_per_sum, k_blocks;  // K blocks of one contraction, of all
     int tiles_m, tiles_n, problems;   // grid of tiles of one problem
     int act, dtype, bias_dtype, out_dtype;
     unsigned int *status;

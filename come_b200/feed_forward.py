@@ -5,7 +5,8 @@ MLPs of visual transformers: ``w12`` holds both projections, the gate's rows fir
 
 A training step keeps only its inputs: the backward pass computes the projections again, in float32, and with them their gradients
 (one kernel of ``come_gated_matmul_backward``), then ``dx = dg Wg + du Wu`` and ``dW = dg^T x`` / ``du^T x``.  ``dg`` and ``du`` are rounded to the
-tokens' type once, as operands of these products; saved 16-bit projections would add their own rounding to every gradient.
+tokens' type once, as operands of these products (for few tokens, whose sums do not average that out, in two parts); saved 16-bit
+projections would add their own rounding to every gradient.
 """
 from __future__ import annotations
 
@@ -73,9 +74,11 @@ class _GatedLinear(torch.autograd.Function):
         xo, wg, wu = _operand(x), _operand(w_gate), _operand(w_up)
         if dh.stride(1) != 1:
             dh = dh.contiguous()
-        dg, du = _padded(tokens, features, x), _padded(tokens, features, x)
+        lib = _lib.lib()
+        d_rows = lib.come_gated_backward_rows(tokens, features)
+        dg, du = _padded(d_rows, features, x), _padded(d_rows, features, x)
         with on_device(dev):
-            _lib.check(_lib.lib().come_gated_matmul_backward(
+            _lib.check(lib.come_gated_matmul_backward(
                 xo.data_ptr(), xo.stride(0), wg.data_ptr(), wg.stride(0), wu.data_ptr(), wu.stride(0), ptr(b_gate), ptr(b_up), dtype_code(x.dtype), ctx.act,
                 tokens, features, cols, dh.data_ptr(), dh.stride(0), dg.data_ptr(), du.data_ptr(), dg.stride(0), ptr(dx), cols, ptr(dwg), ptr(dwu), cols,
                 ptr(dbg), ptr(dbu), stream_ptr(dev)))

@@ -377,7 +377,8 @@ int come_packed_positions(const uint8_t *mask_dev, const int64_t *rev_id_dev, in
  * come_gated_matmul       the same with operands, biases and result in float16 or bfloat16.
  * come_gated_matmul_backward  gradients of come_gated_matmul's tensors from that of its result.  What a training step keeps of the
  *   forward pass is its inputs: the projections are computed again, in float32, and with them their gradients dgate = dout up act'(gate),
- *   dup = dout act(gate), rounded to dtype into the two workspaces dgate_dev / dup_dev [tokens, features] (rows of whole 16 bytes); then
+ *   dup = dout act(gate), rounded to dtype into the two workspaces dgate_dev / dup_dev [come_gated_backward_rows, features] (rows of whole
+ *   16 bytes): tokens rows, or twice as many where the sums are short and the second half holds what the rounding took away; then
  *   dx = dgate gate + dup up, dgate_weight = dgate^T x, dup_weight = dup^T x and the column sums of dgate, dup for the biases.  Any of the
  *   five results may be NULL.  tokens and features must not be zero.
  *
@@ -410,6 +411,7 @@ int come_gated_matmul_backward(const void *x_dev, int64_t x_row_stride, const vo
                                void *dgate_dev, void *dup_dev, int64_t d_row_stride, void *dx_dev, int64_t dx_row_stride,
                                void *dgate_weight_dev, void *dup_weight_dev, int64_t dw_row_stride, void *dgate_bias_dev,
                                void *dup_bias_dev, void *stream);
+int64_t come_gated_backward_rows(int64_t tokens, int64_t features);
 
 /*
  * Device status word: kernels that wait on hardware barriers give up after a bounded number of polls and

@@ -94,6 +94,12 @@ def test_c_entries_refuse_bad_arguments_before_any_launch():
         _refused(lib.come_gated_matmul_backward(*{**back, **change}.values()), text)
 
 
+def test_rows_of_the_backward_workspaces():
+    lib = _lib.lib()
+    assert [lib.come_gated_backward_rows(t, f) for t, f in ((0, 5), (1, 2736), (64, 1 << 20), (65, 2736), (65, 5000), (1000, 262), (1000, 263), (6456, 2736), (1 << 30, 1 << 30))] == \
+        [0, 2, 128, 130, 65, 2000, 1000, 6456, 1 << 30]
+
+
 def test_status_word_names_the_product_kernels():
     """The header, the library's message and the kernels agree on the bits (19-21)."""
     import os

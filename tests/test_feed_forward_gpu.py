@@ -163,7 +163,8 @@ def values(t):
 
 # from one token to more tiles than the GPU has SMs: both kernels, full and partial tiles, split contractions
 LINEAR_SHAPES = [(1, 1, 1), (1, 16, 8), (1, 2736, 1024), (2, 129, 130), (7, 128, 128), (64, 500, 257), (127, 384, 300), (129, 1000, 40), (300, 64, 1100), (1374, 256, 384),
-                 (2600, 257, 1003), (5000, 130, 1040), (9473, 384, 512)]
+                 (2600, 257, 1003), (5000, 130, 1040), (9473, 384, 512),
+                 (5000, 72, 1010), (5000, 72, 1012)]  # rows of the result at multiples of 4 and of 8 bytes
 
 
 @pytest.mark.parametrize("kind", ["f32", "f16", "bf16"])
@@ -365,6 +366,11 @@ def test_gated_linear_forms_of_its_inputs():
         separate = [t.clone().requires_grad_(True) for t in (x, wg, wg)]
         sx, sg, su = torch.autograd.grad(gated_linear(*separate), separate, ones)
         assert torch.equal(gx, sx) and torch.equal(gw, sg + su)
+        biases = [torch.zeros(F, device="cuda", dtype=torch.bfloat16, requires_grad=True) for _ in range(2)]
+        gated_linear(x, wg, wu, *biases).sum().backward()  # nothing but the biases learns
+        every = [t.clone().requires_grad_(True) for t in (x, wg, wu, *(b.detach() for b in biases))]
+        gated_linear(*every).sum().backward()
+        assert torch.equal(biases[0].grad, every[3].grad) and torch.equal(biases[1].grad, every[4].grad)
         shared = x[:1].clone().requires_grad_(True)
         (gs,) = torch.autograd.grad(gated_linear(shared.expand(T, K), wg, wu), shared, ones)
         assert gs.shape == (1, K) and torch.isfinite(gs).all()
