@@ -21,11 +21,15 @@ from .block_scaled import activation_code
 __all__ = ["gated_linear", "GatedMlp"]
 
 
-def _operand(t: torch.Tensor) -> torch.Tensor:
-    """``t [rows, C]`` as the tensor cores can read it: rows that are contiguous and start at multiples of 16 bytes (copied if not)."""
-    if t.stride(1) == 1 and t.stride(0) % 8 == 0 and t.stride(0) >= t.shape[1] and t.data_ptr() % 16 == 0:
-        return t
-    return t.clone(memory_format=torch.contiguous_format)
+def _operand(t: torch.Tensor):
+    """``t [rows, C]`` as the tensor cores can read it, rows that are contiguous and start at multiples of 16 bytes (copied if not):
+    (tensor, pointer, row stride)."""
+    row, col = t.stride()
+    at = t.data_ptr()
+    if col == 1 and row % 8 == 0 and row >= t.shape[1] and at % 16 == 0:
+        return t, at, row
+    t = t.clone(memory_format=torch.contiguous_format)
+    return t, t.data_ptr(), t.shape[1]
 
 
 def _padded(rows: int, cols: int, like: torch.Tensor) -> torch.Tensor:
@@ -35,12 +39,14 @@ def _padded(rows: int, cols: int, like: torch.Tensor) -> torch.Tensor:
 def _forward(x, w_gate, w_up, b_gate, b_up, act):
     tokens, cols = x.shape
     features, dev = w_gate.shape[0], x.device
-    xo, wg, wu = _operand(x), _operand(w_gate), _operand(w_up)
+    xo, x_at, x_row = _operand(x)  # the tensors are held until the launch is queued
+    wg, g_at, g_row = _operand(w_gate)
+    wu, u_at, u_row = _operand(w_up)
     out = torch.empty_strided((tokens, features), (features or 1, 1), dtype=x.dtype, device=dev)
     with on_device(dev):
-        _lib.check(_lib.lib().come_gated_matmul(xo.data_ptr(), xo.stride(0), wg.data_ptr(), wg.stride(0), wu.data_ptr(), wu.stride(0), ptr(b_gate),
-                                                ptr(b_up), dtype_code(x.dtype), act, tokens, features, cols, out.data_ptr(), features,
-                                                stream_ptr(dev)))
+        _lib.check(_lib.lib().come_gated_matmul(x_at, x_row, g_at, g_row, u_at, u_row, None if b_gate is None else b_gate.data_ptr(),
+                                                None if b_up is None else b_up.data_ptr(), dtype_code(x.dtype), act, tokens, features, cols,
+                                                out.data_ptr(), features, stream_ptr(dev)))
     return out
 
 
@@ -71,7 +77,9 @@ class _GatedLinear(torch.autograd.Function):
         dbg, dbu = empty(need[3], features), empty(need[4], features)
         if tokens == 0 or features == 0:
             return dx, dwg, dwu, dbg, dbu, None
-        xo, wg, wu = _operand(x), _operand(w_gate), _operand(w_up)
+        xo, x_at, x_row = _operand(x)  # the tensors are held until the launches are queued
+        wg, g_at, g_row = _operand(w_gate)
+        wu, u_at, u_row = _operand(w_up)
         if dh.stride(1) != 1:
             dh = dh.contiguous()
         lib = _lib.lib()
@@ -79,7 +87,7 @@ class _GatedLinear(torch.autograd.Function):
         dg, du = _padded(d_rows, features, x), _padded(d_rows, features, x)
         with on_device(dev):
             _lib.check(lib.come_gated_matmul_backward(
-                xo.data_ptr(), xo.stride(0), wg.data_ptr(), wg.stride(0), wu.data_ptr(), wu.stride(0), ptr(b_gate), ptr(b_up), dtype_code(x.dtype), ctx.act,
+                x_at, x_row, g_at, g_row, u_at, u_row, ptr(b_gate), ptr(b_up), dtype_code(x.dtype), ctx.act,
                 tokens, features, cols, dh.data_ptr(), dh.stride(0), dg.data_ptr(), du.data_ptr(), dg.stride(0), ptr(dx), cols, ptr(dwg), ptr(dwu), cols,
                 ptr(dbg), ptr(dbu), stream_ptr(dev)))
         return dx, dwg, dwu, dbg, dbu, None
@@ -101,22 +109,30 @@ def gated_linear(x: torch.Tensor, w_gate: torch.Tensor, w_up: torch.Tensor, b_ga
         raise ValueError(f"w_gate and w_up must be [F, {cols}], got {tuple(w_gate.shape)} and {tuple(w_up.shape)}")
     if cols == 0 or cols % 8 != 0:
         raise NotImplementedError(f"gated_linear needs a channel count that is a multiple of 8, got {cols}")
-    features, index = w_gate.shape[0], x.get_device()
-    grad = x.requires_grad
-    for name, t in (("w_gate", w_gate), ("w_up", w_up), ("b_gate", b_gate), ("b_up", b_up)):
-        if t is None:
-            continue
-        if t.dtype is not x.dtype or t.get_device() != index or (name[0] == "b" and t.shape != (features,)):
-            raise ValueError(f"{name} must be {[features] if name[0] == 'b' else [features, cols]} {x.dtype} on {x.device}, got {list(t.shape)} {t.dtype} on {t.device}")
-        grad = grad or t.requires_grad
+    dtype, index, features = x.dtype, x.get_device(), w_gate.shape[0]
+    grad = x.requires_grad or w_gate.requires_grad or w_up.requires_grad
+    if w_gate.dtype is not dtype or w_gate.get_device() != index:
+        raise _mismatch("w_gate", w_gate, [features, cols], x)
+    if w_up.dtype is not dtype or w_up.get_device() != index:
+        raise _mismatch("w_up", w_up, [features, cols], x)
     if b_gate is not None:
+        if b_gate.dtype is not dtype or b_gate.get_device() != index or b_gate.shape != (features,):
+            raise _mismatch("b_gate", b_gate, [features], x)
+        grad = grad or b_gate.requires_grad
         b_gate = b_gate.contiguous()
     if b_up is not None:
+        if b_up.dtype is not dtype or b_up.get_device() != index or b_up.shape != (features,):
+            raise _mismatch("b_up", b_up, [features], x)
+        grad = grad or b_up.requires_grad
         b_up = b_up.contiguous()
     apply = _GatedLinear.apply if grad and torch.is_grad_enabled() else _forward
     if x.dim() == 2:
         return apply(x, w_gate, w_up, b_gate, b_up, act)
     return apply(x.reshape(-1, cols), w_gate, w_up, b_gate, b_up, act).view(*x.shape[:-1], features)
+
+
+def _mismatch(name: str, t: torch.Tensor, shape, x: torch.Tensor) -> Exception:
+    return ValueError(f"{name} must be {shape} {x.dtype} on {x.device}, got {list(t.shape)} {t.dtype} on {t.device}")
 
 
 class GatedMlp(torch.nn.Module):
