@@ -285,7 +285,7 @@ __global__ void __launch_bounds__(kThreads, 1) __cluster_dims__(2, 1, 1) matmul_
                         const int sum = i >= p.kb_per_sum ? 1 : 0, k = (i - sum * p.kb_per_sum) * kElems;
                         const uint32_t dst = ring + st * kStageBytes, bar = full0 + st * 8;
                         if (rank == 0) mbar_arrive_expect_tx(&sh.full[st], 2 * kStageBytes);
-                        const CUtensorMap *ma = &p.a[sum + w.problem], *mb = &p.b[kGated ? rank : sum];
+                        const CUtensorMap *ma = &p.a[w.problem * p.sums + sum], *mb = &p.b[kGated ? rank : kAMn ? 0 : sum];
                         if constexpr (kAMn) {
                             tma_load_2d_pair(dst, ma, w.m0, k, bar);
                             tma_load_2d_pair(dst + kOperandBytes / 2, ma, w.m0 + 64, k, bar);
@@ -415,328 +415,328 @@ __global__ void __launch_bounds__(kThreads, 1) __cluster_dims__(2, 1, 1) matmul_
     } else {
         if constexpr (kE4m3) asm volatile("setmaxnreg.inc.sync.aligned.u32 232;");
         else asm volatile("setmaxnreg.inc.sync.aligned.u32 216;");
-            const int part = warp >> 2, r = (warp & 3) * 32 + lane, warp_row = (warp & 3) * 32;
-            const uint32_t lanes = tmem + ((uint32_t)warp_row << 16) + part * kCols;
-            uint8_t *stage = smem + kRingBytes + warp * staging_bytes(kE4m3);
-            [[maybe_unused]] const PairScales &scales = *reinterpret_cast<const PairScales *>(&sh + 1);
-            const uint32_t empty0 = map_rank(smem_u32(&sh.acc_empty[0]), 0);
-            int chunk = 0, tiles = 0;
-            bool ok = true, busy = false;
-            [[maybe_unused]] const bool with_bias = p.bias[0] != nullptr || (kGated && p.bias[1] != nullptr);
-            [[maybe_unused]] float *bias = reinterpret_cast<float *>(stage);  // [128]: of the gate's and the up projection's 64 columns, or of 128
-            int tile_row = pair / p.tiles_n, tile_col = pair - tile_row * p.tiles_n;
-            const int count = (total - pair + pairs - 1) / pairs;
-            for (; tiles < count; ++tiles) {
-                if constexpr (kE4m3) {
-                    {   // the biases of the warp's columns, before the sums
-                        const Tile w = tile_of(tile_row, tile_col);
-                        const int n = w.n0 + part * kCols, cols = p.N - n;
-                        if (with_bias) {
-                            __syncwarp();
+        const int part = warp >> 2, r = (warp & 3) * 32 + lane, warp_row = (warp & 3) * 32;
+        const uint32_t lanes = tmem + ((uint32_t)warp_row << 16) + part * kCols;
+        uint8_t *stage = smem + kRingBytes + warp * staging_bytes(kE4m3);
+        [[maybe_unused]] const PairScales &scales = *reinterpret_cast<const PairScales *>(&sh + 1);
+        const uint32_t empty0 = map_rank(smem_u32(&sh.acc_empty[0]), 0);
+        int chunk = 0, tiles = 0;
+        bool ok = true, busy = false;
+        [[maybe_unused]] const bool with_bias = p.bias[0] != nullptr || (kGated && p.bias[1] != nullptr);
+        [[maybe_unused]] float *bias = reinterpret_cast<float *>(stage);  // [128]: of the gate's and the up projection's 64 columns, or of 128
+        int tile_row = pair / p.tiles_n, tile_col = pair - tile_row * p.tiles_n;
+        const int count = (total - pair + pairs - 1) / pairs;
+        for (; tiles < count; ++tiles) {
+            if constexpr (kE4m3) {
+                {   // the biases of the warp's columns, before the sums
+                    const Tile w = tile_of(tile_row, tile_col);
+                    const int n = w.n0 + part * kCols, cols = p.N - n;
+                    if (with_bias) {
+                        __syncwarp();
 #pragma unroll
-                            for (int c = 0; c < 4; ++c) {
-                                const float *b = kGated ? (const float *)p.bias[c >> 1] : (const float *)p.bias[0];
-                                const int col = (kGated ? (c & 1) : c) * 32 + lane;
-                                bias[c * 32 + lane] = b != nullptr && col < cols ? b[n + col] : 0.0f;
-                            }
-                            __syncwarp();
+                        for (int c = 0; c < 4; ++c) {
+                            const float *b = kGated ? (const float *)p.bias[c >> 1] : (const float *)p.bias[0];
+                            const int col = (kGated ? (c & 1) : c) * 32 + lane;
+                            bias[c * 32 + lane] = b != nullptr && col < cols ? b[n + col] : 0.0f;
                         }
-                        busy = p.M - w.m0 - warp_row > 0;
+                        __syncwarp();
                     }
-                    // sums as packed pairs: [0, 32) of the gate or of columns [0, 64), [32, 64) of the up projection or of columns [64, 128)
-                    f32x2_t sum[64];
+                    busy = p.M - w.m0 - warp_row > 0;
+                }
+                // sums as packed pairs: [0, 32) of the gate or of columns [0, 64), [32, 64) of the up projection or of columns [64, 128)
+                f32x2_t sum[64];
 #pragma unroll
-                    for (int c = 0; c < 64; ++c) sum[c] = 0ull;
-                    for (int i = 0; i < p.k_blocks; ++i, ++chunk) {
-                        const int buf = chunk & 1, slot = chunk % kScaleSlots;
-                        ok = ok && wait(&sh.acc_full[buf], (chunk >> 1) & 1, kErrSums);
-                        ok = __all_sync(0xffffffffu, ok);
-                        if (ok && busy) {
-                            tc_fence_after();
-                            const float s0 = scales[slot][kGated ? 0 : part][r], s1 = kGated ? scales[slot][1][r] : s0;
-                            const f32x2_t s0p = pack_f32x2(s0, s0), s1p = pack_f32x2(s1, s1);
-                            // 16 columns at a time, two loads in flight: 32 at a time need registers that are not there (spills cost 15 %)
-                            const auto column = [&](int c) { return lanes + buf * kPairN + (kGated ? (c >> 2) * kTile + (c & 3) * 16 : c * 16); };
-                            uint32_t d[32];
-                            tmem_ld16(column(0), d);
-                            tmem_ld16(column(1), d + 16);
+                for (int c = 0; c < 64; ++c) sum[c] = 0ull;
+                for (int i = 0; i < p.k_blocks; ++i, ++chunk) {
+                    const int buf = chunk & 1, slot = chunk % kScaleSlots;
+                    ok = ok && wait(&sh.acc_full[buf], (chunk >> 1) & 1, kErrSums);
+                    ok = __all_sync(0xffffffffu, ok);
+                    if (ok && busy) {
+                        tc_fence_after();
+                        const float s0 = scales[slot][kGated ? 0 : part][r], s1 = kGated ? scales[slot][1][r] : s0;
+                        const f32x2_t s0p = pack_f32x2(s0, s0), s1p = pack_f32x2(s1, s1);
+                        // 16 columns at a time, two loads in flight: 32 at a time need registers that are not there (spills cost 15 %)
+                        const auto column = [&](int c) { return lanes + buf * kPairN + (kGated ? (c >> 2) * kTile + (c & 3) * 16 : c * 16); };
+                        uint32_t d[32];
+                        tmem_ld16(column(0), d);
+                        tmem_ld16(column(1), d + 16);
 #pragma unroll
-                            for (int c = 0; c < 8; c += 2) {
-                                tc_wait_ld_of(d);
-                                if (c == 6) {
-                                    tc_fence_before();
-                                    __syncwarp();
-                                    if (lane == 0) mbar_arrive_at(empty0 + buf * 8);  // the buffer is in registers
-                                }
-#pragma unroll
-                                for (int j = 0; j < 2; ++j) {
-#pragma unroll
-                                    for (int e = 0; e < 8; ++e)
-                                        sum[(c + j) * 8 + e] = fma_f32x2(pack_f32x2(__uint_as_float(d[j * 16 + 2 * e]), __uint_as_float(d[j * 16 + 2 * e + 1])), (c + j) >> 2 ? s1p : s0p, sum[(c + j) * 8 + e]);
-                                    if (c < 6) tmem_ld16(column(c + 2 + j), d + j * 16);
-                                }
-                            }
-                        } else if (ok && lane == 0) {
-                            mbar_arrive_at(empty0 + buf * 8);
-                        }
-                    }
-                    // Where the tile lies is worked out again (the shuffles hide that they are the same numbers): kept over the loop, it costs
-                    // registers that the sums need.
-                    const Tile w = tile_of(__shfl_sync(0xffffffffu, tile_row, 0), __shfl_sync(0xffffffffu, tile_col, 0));
-                    const int rows = min(32, p.M - w.m0 - warp_row), n = w.n0 + part * kCols, cols = p.N - n;
-                    const int64_t row0 = w.m0 + warp_row;
-                    if constexpr (!kGated) {
-                        if (ok && busy) {
-                            if (with_bias) {
-#pragma unroll
-                                for (int c = 0; c < 32; ++c) {
-                                    const float4 b = *reinterpret_cast<const float4 *>(bias + 4 * c);
-                                    sum[2 * c] = add_f32x2(sum[2 * c], pack_f32x2(b.x, b.y));
-                                    sum[2 * c + 1] = add_f32x2(sum[2 * c + 1], pack_f32x2(b.z, b.w));
-                                }
+                        for (int c = 0; c < 8; c += 2) {
+                            tc_wait_ld_of(d);
+                            if (c == 6) {
+                                tc_fence_before();
                                 __syncwarp();
+                                if (lane == 0) mbar_arrive_at(empty0 + buf * 8);  // the buffer is in registers
                             }
-                            if (p.out_dtype == COME_F32) {
-                                uint8_t *out = (uint8_t *)p.out[0] + (row0 * p.out_row[0] + n) * 4;
 #pragma unroll
-                                for (int h = 0; h < 8; ++h) {
+                            for (int j = 0; j < 2; ++j) {
 #pragma unroll
-                                    for (int c = 0; c < 4; ++c) {
-                                        float v[4];
-                                        unpack_f32x2(sum[h * 8 + c * 2], v[0], v[1]);
-                                        unpack_f32x2(sum[h * 8 + c * 2 + 1], v[2], v[3]);
-                                        *staged<kRow>(stage, lane, c) = make_uint4(__float_as_uint(v[0]), __float_as_uint(v[1]), __float_as_uint(v[2]), __float_as_uint(v[3]));
-                                    }
-                                    __syncwarp();
-                                    store_staged<4, kRow>(stage, out + h * kRow, p.out_row[0] * 4, rows, cols - h * 16, lane);
-                                    __syncwarp();
-                                }
-                            } else {
-                                as_constant(p.out_dtype == COME_BF16, [&](auto bf16) {
-                                    uint8_t *out = (uint8_t *)p.out[0] + (row0 * p.out_row[0] + n) * 2;
-#pragma unroll
-                                    for (int h = 0; h < 4; ++h) {
-#pragma unroll
-                                        for (int c = 0; c < 4; ++c) {
-                                            uint32_t e[4];
-#pragma unroll
-                                            for (int j = 0; j < 4; ++j) {
-                                                float lo, hi;
-                                                unpack_f32x2(sum[h * 16 + c * 4 + j], lo, hi);
-                                                e[j] = pack_16<decltype(bf16)::value>(lo, hi);
-                                            }
-                                            *staged<kRow>(stage, lane, c) = make_uint4(e[0], e[1], e[2], e[3]);
-                                        }
-                                        __syncwarp();
-                                        store_staged<2, kRow>(stage, out + h * kRow, p.out_row[0] * 2, rows, cols - h * 32, lane);
-                                        __syncwarp();
-                                    }
-                                });
+                                for (int e = 0; e < 8; ++e)
+                                    sum[(c + j) * 8 + e] = fma_f32x2(pack_f32x2(__uint_as_float(d[j * 16 + 2 * e]), __uint_as_float(d[j * 16 + 2 * e + 1])), (c + j) >> 2 ? s1p : s0p, sum[(c + j) * 8 + e]);
+                                if (c < 6) tmem_ld16(column(c + 2 + j), d + j * 16);
                             }
                         }
-                    } else {
-                        float tops[4] = {0.0f, 0.0f, 0.0f, 0.0f};  // the results take the place of the gate's sums
-                        if (ok && busy) {
-                            if (with_bias) {
+                    } else if (ok && lane == 0) {
+                        mbar_arrive_at(empty0 + buf * 8);
+                    }
+                }
+                // Where the tile lies is worked out again (the shuffles hide that they are the same numbers): kept over the loop, it costs
+                // registers that the sums need.
+                const Tile w = tile_of(__shfl_sync(0xffffffffu, tile_row, 0), __shfl_sync(0xffffffffu, tile_col, 0));
+                const int rows = min(32, p.M - w.m0 - warp_row), n = w.n0 + part * kCols, cols = p.N - n;
+                const int64_t row0 = w.m0 + warp_row;
+                if constexpr (!kGated) {
+                    if (ok && busy) {
+                        if (with_bias) {
 #pragma unroll
-                                for (int c = 0; c < 32; ++c) {
-                                    const float4 b = *reinterpret_cast<const float4 *>(bias + 4 * c);
-                                    sum[2 * c] = add_f32x2(sum[2 * c], pack_f32x2(b.x, b.y));
-                                    sum[2 * c + 1] = add_f32x2(sum[2 * c + 1], pack_f32x2(b.z, b.w));
-                                }
-                            }
-                            as_constant(p.act == COME_ACT_SILU, [&](auto silu) {
-                                constexpr int act = decltype(silu)::value ? COME_ACT_SILU : COME_ACT_GELU;
-#pragma unroll
-                                for (int c = 0; c < 32; ++c) {
-                                    float g0, g1, u0, u1;
-                                    unpack_f32x2(sum[c], g0, g1);
-                                    unpack_f32x2(sum[32 + c], u0, u1);
-                                    const float h0 = activation(g0, act) * u0, h1 = activation(g1, act) * u1;
-                                    tops[c & 3] = fmaxf(tops[c & 3], fmaxf(fabsf(h0), fabsf(h1)));  // under the special-function unit
-                                    sum[c] = pack_f32x2(h0, h1);
-                                }
-                            });
-                            if (cols < 64) {  // columns past the end: the bytes of other rows' products
-                                tops[0] = tops[1] = tops[2] = tops[3] = 0.0f;
-#pragma unroll
-                                for (int c = 0; c < 32; ++c) {
-                                    float h0, h1;
-                                    unpack_f32x2(sum[c], h0, h1);
-                                    h0 = 2 * c < cols ? h0 : 0.0f;
-                                    h1 = 2 * c + 1 < cols ? h1 : 0.0f;
-                                    tops[0] = fmaxf(tops[0], fmaxf(fabsf(h0), fabsf(h1)));
-                                    sum[c] = pack_f32x2(h0, h1);
-                                }
+                            for (int c = 0; c < 32; ++c) {
+                                const float4 b = *reinterpret_cast<const float4 *>(bias + 4 * c);
+                                sum[2 * c] = add_f32x2(sum[2 * c], pack_f32x2(b.x, b.y));
+                                sum[2 * c + 1] = add_f32x2(sum[2 * c + 1], pack_f32x2(b.z, b.w));
                             }
                             __syncwarp();
                         }
-                        if (p.out_dtype == COME_E4M3) {
-                            float top = fmaxf(fmaxf(tops[0], tops[1]), fmaxf(tops[2], tops[3]));
-                            // the largest magnitude of a row's 128 columns: half of it in the other warpgroup (every warp meets here, also
-                            // one that gave up; a third tile's write to the same place is two barriers away)
-                            sh.top[tiles & 1][part][r] = top;
-                            asm volatile("bar.sync 1, 256;" ::: "memory");
-                            top = fmaxf(fmaxf(top, sh.top[tiles & 1][part ^ 1][r]), kSmallestMax);
-                            if (ok && busy) {
-                                const float inv = __fdividef(kE4m3Max, top);
+                        if (p.out_dtype == COME_F32) {
+                            uint8_t *out = (uint8_t *)p.out[0] + (row0 * p.out_row[0] + n) * 4;
+#pragma unroll
+                            for (int h = 0; h < 8; ++h) {
 #pragma unroll
                                 for (int c = 0; c < 4; ++c) {
-                                    uint32_t q[4];
-#pragma unroll
-                                    for (int j = 0; j < 4; ++j) {
-                                        float e[4];
-                                        unpack_f32x2(sum[c * 8 + j * 2], e[0], e[1]);
-                                        unpack_f32x2(sum[c * 8 + j * 2 + 1], e[2], e[3]);
-                                        q[j] = pack_e4m3(e[0] * inv, e[1] * inv, e[2] * inv, e[3] * inv);
-                                    }
-                                    *staged<kRow>(stage, lane, c) = make_uint4(q[0], q[1], q[2], q[3]);
+                                    float v[4];
+                                    unpack_f32x2(sum[h * 8 + c * 2], v[0], v[1]);
+                                    unpack_f32x2(sum[h * 8 + c * 2 + 1], v[2], v[3]);
+                                    *staged<kRow>(stage, lane, c) = make_uint4(__float_as_uint(v[0]), __float_as_uint(v[1]), __float_as_uint(v[2]), __float_as_uint(v[3]));
                                 }
                                 __syncwarp();
-                                store_staged<1, kRow>(stage, (uint8_t *)p.out[0] + row0 * p.out_row[0] + n, p.out_row[0], rows, cols, lane);
-                                if (part == 0 && lane < rows) p.out_scale[(row0 + lane) * p.os_row + (w.n0 / kTile) * p.os_block] = top * (1.0f / kE4m3Max);
+                                store_staged<4, kRow>(stage, out + h * kRow, p.out_row[0] * 4, rows, cols - h * 16, lane);
                                 __syncwarp();
                             }
-                        } else if (ok && busy) {
+                        } else {
                             as_constant(p.out_dtype == COME_BF16, [&](auto bf16) {
+                                uint8_t *out = (uint8_t *)p.out[0] + (row0 * p.out_row[0] + n) * 2;
 #pragma unroll
-                                for (int half = 0; half < 2; ++half) {
+                                for (int h = 0; h < 4; ++h) {
 #pragma unroll
                                     for (int c = 0; c < 4; ++c) {
-                                        uint32_t q[4];
+                                        uint32_t e[4];
 #pragma unroll
                                         for (int j = 0; j < 4; ++j) {
                                             float lo, hi;
-                                            unpack_f32x2(sum[half * 16 + c * 4 + j], lo, hi);
-                                            q[j] = pack_16<decltype(bf16)::value>(lo, hi);
+                                            unpack_f32x2(sum[h * 16 + c * 4 + j], lo, hi);
+                                            e[j] = pack_16<decltype(bf16)::value>(lo, hi);
                                         }
-                                        *staged<kRow>(stage, lane, c) = make_uint4(q[0], q[1], q[2], q[3]);
+                                        *staged<kRow>(stage, lane, c) = make_uint4(e[0], e[1], e[2], e[3]);
                                     }
                                     __syncwarp();
-                                    store_staged<2, kRow>(stage, (uint8_t *)p.out[0] + (row0 * p.out_row[0] + n + half * 32) * 2, p.out_row[0] * 2, rows, cols - half * 32, lane);
+                                    store_staged<2, kRow>(stage, out + h * kRow, p.out_row[0] * 2, rows, cols - h * 32, lane);
                                     __syncwarp();
                                 }
                             });
                         }
                     }
                 } else {
-                    const Tile w = tile_of(tile_row, tile_col);
-                    const int rows = min(32, p.M - w.m0 - warp_row);      // of this warp, may be <= 0
-                    const int n = w.n0 + part * kCols, cols = p.N - n;    // first result column of the thread, columns from there on
-                    busy = rows > 0;
-                    const int64_t row0 = w.m0 + warp_row;
-                    const int buf = chunk & 1;
-                    if (kGated && busy) {  // before the wait: the biases of this warp's 64 + 64 columns, and dh
+                    float tops[4] = {0.0f, 0.0f, 0.0f, 0.0f};  // the results take the place of the gate's sums
+                    if (ok && busy) {
+                        if (with_bias) {
 #pragma unroll
-                        for (int c = 0; c < 4; ++c) {
-                            const uint16_t *b = (const uint16_t *)p.bias[c >> 1];
-                            const int col = (c & 1) * 32 + lane;
-                            sh.bias[warp][c * 32 + lane] = b != nullptr && col < cols ? b[n + col] : (uint16_t)0;
+                            for (int c = 0; c < 32; ++c) {
+                                const float4 b = *reinterpret_cast<const float4 *>(bias + 4 * c);
+                                sum[2 * c] = add_f32x2(sum[2 * c], pack_f32x2(b.x, b.y));
+                                sum[2 * c + 1] = add_f32x2(sum[2 * c + 1], pack_f32x2(b.z, b.w));
+                            }
                         }
-                        if (kMode == kMatmulGatedGrad && ok && cols > 0) load_staged(stage, (const uint8_t *)p.dh + (row0 * p.dh_row + n) * 2, p.dh_row * 2, rows, cols, lane);
+                        as_constant(p.act == COME_ACT_SILU, [&](auto silu) {
+                            constexpr int act = decltype(silu)::value ? COME_ACT_SILU : COME_ACT_GELU;
+#pragma unroll
+                            for (int c = 0; c < 32; ++c) {
+                                float g0, g1, u0, u1;
+                                unpack_f32x2(sum[c], g0, g1);
+                                unpack_f32x2(sum[32 + c], u0, u1);
+                                const float h0 = activation(g0, act) * u0, h1 = activation(g1, act) * u1;
+                                tops[c & 3] = fmaxf(tops[c & 3], fmaxf(fabsf(h0), fabsf(h1)));  // under the special-function unit
+                                sum[c] = pack_f32x2(h0, h1);
+                            }
+                        });
+                        if (cols < 64) {  // columns past the end: the bytes of other rows' products
+                            tops[0] = tops[1] = tops[2] = tops[3] = 0.0f;
+#pragma unroll
+                            for (int c = 0; c < 32; ++c) {
+                                float h0, h1;
+                                unpack_f32x2(sum[c], h0, h1);
+                                h0 = 2 * c < cols ? h0 : 0.0f;
+                                h1 = 2 * c + 1 < cols ? h1 : 0.0f;
+                                tops[0] = fmaxf(tops[0], fmaxf(fabsf(h0), fabsf(h1)));
+                                sum[c] = pack_f32x2(h0, h1);
+                            }
+                        }
                         __syncwarp();
                     }
-                    ok = ok && wait(&sh.acc_full[buf], (chunk >> 1) & 1, kErrSums);
-                    ok = __all_sync(0xffffffffu, ok);
-                    if (ok && busy) {
-                        tc_fence_after();
-                        const uint32_t from = lanes + buf * kPairN;
-                        as_constant(p.dtype == COME_BF16, [&](auto bf16_c) {
-                            constexpr bool kBF16 = decltype(bf16_c)::value;
-                            if constexpr (!kGated) {
+                    if (p.out_dtype == COME_E4M3) {
+                        float top = fmaxf(fmaxf(tops[0], tops[1]), fmaxf(tops[2], tops[3]));
+                        // the largest magnitude of a row's 128 columns: half of it in the other warpgroup (every warp meets here, also
+                        // one that gave up; a third tile's write to the same place is two barriers away)
+                        sh.top[tiles & 1][part][r] = top;
+                        asm volatile("bar.sync 1, 256;" ::: "memory");
+                        top = fmaxf(fmaxf(top, sh.top[tiles & 1][part ^ 1][r]), kSmallestMax);
+                        if (ok && busy) {
+                            const float inv = inverse_scale(top);
+#pragma unroll
+                            for (int c = 0; c < 4; ++c) {
+                                uint32_t q[4];
+#pragma unroll
+                                for (int j = 0; j < 4; ++j) {
+                                    float e[4];
+                                    unpack_f32x2(sum[c * 8 + j * 2], e[0], e[1]);
+                                    unpack_f32x2(sum[c * 8 + j * 2 + 1], e[2], e[3]);
+                                    q[j] = pack_e4m3(e[0] * inv, e[1] * inv, e[2] * inv, e[3] * inv);
+                                }
+                                *staged<kRow>(stage, lane, c) = make_uint4(q[0], q[1], q[2], q[3]);
+                            }
+                            __syncwarp();
+                            store_staged<1, kRow>(stage, (uint8_t *)p.out[0] + row0 * p.out_row[0] + n, p.out_row[0], rows, cols, lane);
+                            if (part == 0 && lane < rows) p.out_scale[(row0 + lane) * p.os_row + (w.n0 / kTile) * p.os_block] = top * (1.0f / kE4m3Max);
+                            __syncwarp();
+                        }
+                    } else if (ok && busy) {
+                        as_constant(p.out_dtype == COME_BF16, [&](auto bf16) {
+#pragma unroll
+                            for (int half = 0; half < 2; ++half) {
+#pragma unroll
+                                for (int c = 0; c < 4; ++c) {
+                                    uint32_t q[4];
+#pragma unroll
+                                    for (int j = 0; j < 4; ++j) {
+                                        float lo, hi;
+                                        unpack_f32x2(sum[half * 16 + c * 4 + j], lo, hi);
+                                        q[j] = pack_16<decltype(bf16)::value>(lo, hi);
+                                    }
+                                    *staged<kRow>(stage, lane, c) = make_uint4(q[0], q[1], q[2], q[3]);
+                                }
+                                __syncwarp();
+                                store_staged<2, kRow>(stage, (uint8_t *)p.out[0] + (row0 * p.out_row[0] + n + half * 32) * 2, p.out_row[0] * 2, rows, cols - half * 32, lane);
+                                __syncwarp();
+                            }
+                        });
+                    }
+                }
+            } else {
+                const Tile w = tile_of(tile_row, tile_col);
+                const int rows = min(32, p.M - w.m0 - warp_row);      // of this warp, may be <= 0
+                const int n = w.n0 + part * kCols, cols = p.N - n;    // first result column of the thread, columns from there on
+                busy = rows > 0;
+                const int64_t row0 = w.m0 + warp_row;
+                const int buf = chunk & 1;
+                if (kGated && busy) {  // before the wait: the biases of this warp's 64 + 64 columns, and dh
+#pragma unroll
+                    for (int c = 0; c < 4; ++c) {
+                        const uint16_t *b = (const uint16_t *)p.bias[c >> 1];
+                        const int col = (c & 1) * 32 + lane;
+                        sh.bias[warp][c * 32 + lane] = b != nullptr && col < cols ? b[n + col] : (uint16_t)0;
+                    }
+                    if (kMode == kMatmulGatedGrad && ok && cols > 0) load_staged(stage, (const uint8_t *)p.dh + (row0 * p.dh_row + n) * 2, p.dh_row * 2, rows, cols, lane);
+                    __syncwarp();
+                }
+                ok = ok && wait(&sh.acc_full[buf], (chunk >> 1) & 1, kErrSums);
+                ok = __all_sync(0xffffffffu, ok);
+                if (ok && busy) {
+                    tc_fence_after();
+                    const uint32_t from = lanes + buf * kPairN;
+                    as_constant(p.dtype == COME_BF16, [&](auto bf16_c) {
+                        constexpr bool kBF16 = decltype(bf16_c)::value;
+                        if constexpr (!kGated) {
 #pragma unroll 1
-                                for (int h = 0; h < kCols / 32; ++h) {
-                                    uint32_t d[32];
-                                    tmem_ld32(from + h * 32, d);
-                                    tc_wait_ld_of(d);
-                                    if (h == kCols / 32 - 1) {  // the sums are in registers: the next tile may begin
+                            for (int h = 0; h < kCols / 32; ++h) {
+                                uint32_t d[32];
+                                tmem_ld32(from + h * 32, d);
+                                tc_wait_ld_of(d);
+                                if (h == kCols / 32 - 1) {  // the sums are in registers: the next tile may begin
+                                    tc_fence_before();
+                                    __syncwarp();
+                                    if (lane == 0) mbar_arrive_at(empty0 + buf * 8);
+                                }
+#pragma unroll
+                                for (int c = 0; c < 4; ++c) {
+                                    uint32_t e[4];
+#pragma unroll
+                                    for (int j = 0; j < 4; ++j) e[j] = pack_16<kBF16>(__uint_as_float(d[c * 8 + 2 * j]), __uint_as_float(d[c * 8 + 2 * j + 1]));
+                                    *staged<64>(stage + (h & 1) * 2048, lane, c) = make_uint4(e[0], e[1], e[2], e[3]);
+                                }
+                                __syncwarp();
+                                store_staged<2, 64>(stage + (h & 1) * 2048, (uint8_t *)p.out[w.problem] + (row0 * p.out_row[w.problem] + n + h * 32) * 2, p.out_row[w.problem] * 2, rows, cols - h * 32, lane);
+                            }
+                            __syncwarp();
+                        } else {
+                            as_constant(p.act == COME_ACT_SILU, [&](auto silu) {
+                                constexpr int act = decltype(silu)::value ? COME_ACT_SILU : COME_ACT_GELU;
+                                [[maybe_unused]] uint32_t second[32];  // du of the row, while dg is staged
+#pragma unroll
+                                for (int q = 0; q < 2; ++q) {
+                                    uint32_t g[32], u[32];
+                                    tmem_ld32(from + q * 32, g);
+                                    tmem_ld32(from + kTile + q * 32, u);
+                                    tc_wait_ld_of(g);
+                                    tc_wait_ld_of(u);
+                                    if (q == 1) {  // the sums are in registers: the next tile may begin
                                         tc_fence_before();
                                         __syncwarp();
                                         if (lane == 0) mbar_arrive_at(empty0 + buf * 8);
                                     }
 #pragma unroll
                                     for (int c = 0; c < 4; ++c) {
+                                        const uint4 bg = *reinterpret_cast<const uint4 *>(&sh.bias[warp][q * 32 + c * 8]), bu = *reinterpret_cast<const uint4 *>(&sh.bias[warp][64 + q * 32 + c * 8]);
+                                        const uint32_t bgs[4] = {bg.x, bg.y, bg.z, bg.w}, bus[4] = {bu.x, bu.y, bu.z, bu.w};
                                         uint32_t e[4];
+                                        [[maybe_unused]] uint32_t dh[4];
+                                        if constexpr (kMode == kMatmulGatedGrad) {
+                                            const uint4 raw = *staged<kRow>(stage, lane, q * 4 + c);
+                                            dh[0] = raw.x, dh[1] = raw.y, dh[2] = raw.z, dh[3] = raw.w;
+                                        }
 #pragma unroll
-                                        for (int j = 0; j < 4; ++j) e[j] = pack_16<kBF16>(__uint_as_float(d[c * 8 + 2 * j]), __uint_as_float(d[c * 8 + 2 * j + 1]));
-                                        *staged<64>(stage + (h & 1) * 2048, lane, c) = make_uint4(e[0], e[1], e[2], e[3]);
+                                        for (int j = 0; j < 4; ++j) {
+                                            float g0, g1, u0, u1;
+                                            unpack_16<kBF16>(bgs[j], g0, g1);
+                                            unpack_16<kBF16>(bus[j], u0, u1);
+                                            g0 += __uint_as_float(g[c * 8 + 2 * j]), g1 += __uint_as_float(g[c * 8 + 2 * j + 1]);
+                                            u0 += __uint_as_float(u[c * 8 + 2 * j]), u1 += __uint_as_float(u[c * 8 + 2 * j + 1]);
+                                            if constexpr (kMode == kMatmulGated) {
+                                                e[j] = pack_16<kBF16>(activation(g0, act) * u0, activation(g1, act) * u1);
+                                            } else {
+                                                float d0, d1, a0, a1, s0, s1;
+                                                unpack_16<kBF16>(dh[j], d0, d1);
+                                                activation_grad(g0, act, a0, s0);
+                                                activation_grad(g1, act, a1, s1);
+                                                e[j] = pack_16<kBF16>(d0 * u0 * s0, d1 * u1 * s1);
+                                                second[(q * 4 + c) * 4 + j] = pack_16<kBF16>(d0 * a0, d1 * a1);
+                                            }
+                                        }
+                                        *staged<kRow>(stage, lane, q * 4 + c) = make_uint4(e[0], e[1], e[2], e[3]);
                                     }
-                                    __syncwarp();
-                                    store_staged<2, 64>(stage + (h & 1) * 2048, (uint8_t *)p.out[w.problem] + (row0 * p.out_row[w.problem] + n + h * 32) * 2, p.out_row[w.problem] * 2, rows, cols - h * 32, lane);
                                 }
                                 __syncwarp();
-                            } else {
-                                as_constant(p.act == COME_ACT_SILU, [&](auto silu) {
-                                    constexpr int act = decltype(silu)::value ? COME_ACT_SILU : COME_ACT_GELU;
-                                    [[maybe_unused]] uint32_t second[32];  // du of the row, while dg is staged
+                                store_staged<2, kRow>(stage, (uint8_t *)p.out[0] + (row0 * p.out_row[0] + n) * 2, p.out_row[0] * 2, rows, cols, lane);
+                                __syncwarp();
+                                if constexpr (kMode == kMatmulGatedGrad) {
 #pragma unroll
-                                    for (int q = 0; q < 2; ++q) {
-                                        uint32_t g[32], u[32];
-                                        tmem_ld32(from + q * 32, g);
-                                        tmem_ld32(from + kTile + q * 32, u);
-                                        tc_wait_ld_of(g);
-                                        tc_wait_ld_of(u);
-                                        if (q == 1) {  // the sums are in registers: the next tile may begin
-                                            tc_fence_before();
-                                            __syncwarp();
-                                            if (lane == 0) mbar_arrive_at(empty0 + buf * 8);
-                                        }
-#pragma unroll
-                                        for (int c = 0; c < 4; ++c) {
-                                            const uint4 bg = *reinterpret_cast<const uint4 *>(&sh.bias[warp][q * 32 + c * 8]), bu = *reinterpret_cast<const uint4 *>(&sh.bias[warp][64 + q * 32 + c * 8]);
-                                            const uint32_t bgs[4] = {bg.x, bg.y, bg.z, bg.w}, bus[4] = {bu.x, bu.y, bu.z, bu.w};
-                                            uint32_t e[4];
-                                            [[maybe_unused]] uint32_t dh[4];
-                                            if constexpr (kMode == kMatmulGatedGrad) {
-                                                const uint4 raw = *staged<kRow>(stage, lane, q * 4 + c);
-                                                dh[0] = raw.x, dh[1] = raw.y, dh[2] = raw.z, dh[3] = raw.w;
-                                            }
-#pragma unroll
-                                            for (int j = 0; j < 4; ++j) {
-                                                float g0, g1, u0, u1;
-                                                unpack_16<kBF16>(bgs[j], g0, g1);
-                                                unpack_16<kBF16>(bus[j], u0, u1);
-                                                g0 += __uint_as_float(g[c * 8 + 2 * j]), g1 += __uint_as_float(g[c * 8 + 2 * j + 1]);
-                                                u0 += __uint_as_float(u[c * 8 + 2 * j]), u1 += __uint_as_float(u[c * 8 + 2 * j + 1]);
-                                                if constexpr (kMode == kMatmulGated) {
-                                                    e[j] = pack_16<kBF16>(activation(g0, act) * u0, activation(g1, act) * u1);
-                                                } else {
-                                                    float d0, d1, a0, a1, s0, s1;
-                                                    unpack_16<kBF16>(dh[j], d0, d1);
-                                                    activation_grad(g0, act, a0, s0);
-                                                    activation_grad(g1, act, a1, s1);
-                                                    e[j] = pack_16<kBF16>(d0 * u0 * s0, d1 * u1 * s1);
-                                                    second[(q * 4 + c) * 4 + j] = pack_16<kBF16>(d0 * a0, d1 * a1);
-                                                }
-                                            }
-                                            *staged<kRow>(stage, lane, q * 4 + c) = make_uint4(e[0], e[1], e[2], e[3]);
-                                        }
-                                    }
+                                    for (int c = 0; c < 8; ++c) *staged<kRow>(stage, lane, c) = make_uint4(second[4 * c], second[4 * c + 1], second[4 * c + 2], second[4 * c + 3]);
                                     __syncwarp();
-                                    store_staged<2, kRow>(stage, (uint8_t *)p.out[0] + (row0 * p.out_row[0] + n) * 2, p.out_row[0] * 2, rows, cols, lane);
+                                    store_staged<2, kRow>(stage, (uint8_t *)p.out[1] + (row0 * p.out_row[1] + n) * 2, p.out_row[1] * 2, rows, cols, lane);
                                     __syncwarp();
-                                    if constexpr (kMode == kMatmulGatedGrad) {
-#pragma unroll
-                                        for (int c = 0; c < 8; ++c) *staged<kRow>(stage, lane, c) = make_uint4(second[4 * c], second[4 * c + 1], second[4 * c + 2], second[4 * c + 3]);
-                                        __syncwarp();
-                                        store_staged<2, kRow>(stage, (uint8_t *)p.out[1] + (row0 * p.out_row[1] + n) * 2, p.out_row[1] * 2, rows, cols, lane);
-                                        __syncwarp();
-                                    }
-                                });
-                            }
-                        });
-                    } else if (ok) {
-                        if (lane == 0) mbar_arrive_at(empty0 + buf * 8);
-                    }
-                    ++chunk;
+                                }
+                            });
+                        }
+                    });
+                } else if (ok) {
+                    if (lane == 0) mbar_arrive_at(empty0 + buf * 8);
                 }
-                tile_row += step_row;
-                tile_col += step_col;
-                if (tile_col >= p.tiles_n) {
-                    tile_col -= p.tiles_n;
-                    ++tile_row;
-                }
+                ++chunk;
             }
+            tile_row += step_row;
+            tile_col += step_col;
+            if (tile_col >= p.tiles_n) {
+                tile_col -= p.tiles_n;
+                ++tile_row;
+            }
+        }
     }
     if (sh.abort_flag != 0) {  // the other CTA's copies complete on the first one's barriers: give those in flight time to land
         const long long t0 = clock64();

@@ -331,7 +331,7 @@ __global__ void __launch_bounds__(kThreads, 1) matmul_split_kernel(const __grid_
 #pragma unroll
                     for (int s = 16; s >= 1; s >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, s));
                     top = fmaxf(top, kSmallestMax);
-                    const float inv = __fdividef(kE4m3Max, top);
+                    const float inv = inverse_scale(top);
                     const uint32_t q = pack_e4m3(h[0] * inv, h[1] * inv, h[2] * inv, h[3] * inv);
                     uint8_t *out = (uint8_t *)p.out[0] + at;  // rows start at multiples of 16 bytes
                     if (valid >= 4) {

@@ -175,7 +175,7 @@ __global__ void __launch_bounds__(kThreads) residual_rmsnorm_kernel(const RmsNor
                 for (int m = kScaleBlock / VEC / 2; m >= 1; m >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, m));
                 top = fmaxf(top, kSmallestMax);
                 if (c < C) {
-                    store_e4m3<VEC>(a.q + row * a.q_row, c, C, v, __fdividef(kE4m3Max, top));
+                    store_e4m3<VEC>(a.q + row * a.q_row, c, C, v, inverse_scale(top));
                     if (c % kScaleBlock == 0) a.q_scale[row * a.s_row + (c / kScaleBlock) * a.s_block] = top * (1.0f / kE4m3Max);
                 }
             }

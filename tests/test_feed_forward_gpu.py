@@ -124,6 +124,8 @@ def test_residual_rmsnorm_special_rows():
     v = r.dequantize()
     assert v[2, 7].isnan() and torch.isfinite(v[2, :7]).all() and torch.isfinite(v[2, 8:]).all()
     assert torch.isfinite(v[3, :128]).all() and v[3, 128:].isnan().all()
+    large = torch.tensor([[3.4e38, 1e38, -9e37, 1e37] * 32], device="cuda")  # the largest numbers keep their values
+    check_rows8(quantize_rows(large), d(large), torch.zeros((), device="cuda", dtype=torch.float64), "large")
     small = quantize_rows(torch.full((1, 128), 1e-41, device="cuda"))
     assert torch.isfinite(small.scale).all() and (small.scale >= 2.0 ** -126).all() and torch.isfinite(small.dequantize()).all()
 
@@ -331,6 +333,21 @@ def test_the_gradient_formula_against_differences(act):
         slope_there = (f(*up) - f(*down)) / (2 * step)
         # third derivatives of a few hundred: error step^2 * 1e3, and cancellation 1e-16 * |f| / step
         assert abs((grad * v).sum() - slope_there) <= 1e-6 * (1 + abs(slope_there))
+
+
+@pytest.mark.parametrize("T,K,F", [(16, 1024, 2736), (64, 1024, 2736), (65, 1024, 2736)])
+def test_gradient_of_one_weight_of_few_tokens(T, K, F):
+    """One weight of two learns, with and without the second part of the operands, in results that have enough tiles for either kernel."""
+    from come_b200.feed_forward import gated_linear
+    randn = gen(T)
+    x, wg, wu, dh = randn(T, K).bfloat16(), (randn(F, K) / 32).bfloat16(), (randn(F, K) / 32).bfloat16(), randn(T, F).bfloat16()
+    both = [t.clone().requires_grad_(True) for t in (wg, wu)]
+    want = torch.autograd.grad(gated_linear(x, *both), both, dh)
+    for i in range(2):
+        one = [t.clone().requires_grad_(j == i) for j, t in enumerate((wg, wu))]
+        (got,) = torch.autograd.grad(gated_linear(x, *one), one[i], dh)
+        # the two kernels add the same float32 terms in other orders
+        within(got, want[i], 2.0 ** -8 * d(want[i]).abs() + chain(2 * T) * 4 * d(want[i]).abs().amax(), "one weight")
 
 
 def test_gated_linear_forms_of_its_inputs():
