@@ -5,10 +5,10 @@
 //   normed = y rounded to the stream's type, or
 //   q      = e4m3(y / s),  s = max(max|y|, 448 * 2^-126) / 448 over each 128 columns of a row
 //
-// Memory bound: both inputs are read once, both results written once.  A row is owned by one warp (many rows) or by a thread
-// group of several warps (few rows, where a row's latency counts, and wide rows, whose float32 copy would not fit one warp's
-// registers): thread i of the group holds the vectors i, i + group size, ... of the row, so the 128 columns of a scale always lie
-// in 16 (16-bit types) or 32 (float32) neighbouring lanes and their maximum needs shuffles only.
+// Memory bound: both inputs are read once, both results written once.  A row is owned by a group of threads: a quarter of a warp or half
+// of one (narrow rows), a warp, or several (few rows, where a row's latency counts, and wide rows, whose registers would not fit one
+// warp).  Thread i of the group holds the vectors i, i + group size, ... of the row, so the 128 columns of a scale always lie in 16
+// (16-bit types) or 32 (float32) neighbouring lanes, or are the whole row, and their maximum needs shuffles only.
 //
 // Measured: 80,672 x 1024 bf16 with residual and 8-bit result 114 us (5.1 TB/s, 78 % of the copy rate; with a bf16 result 108 us, 6.1
 // TB/s), 10,534 x 1000 float32 28.7 us (5.9 TB/s).
@@ -82,15 +82,19 @@ template <int VEC> __device__ __forceinline__ void store_e4m3(uint8_t *p, int c,
     }
 }
 
-// kWarps warps own a row; a CTA of kThreads threads holds kThreads / (32 * kWarps) of them.
-template <typename T, int kWarps, int NV, int kThreads, bool kAligned>
+// kGroup threads own a row (part of a warp, or whole warps); a CTA of kThreads threads holds kThreads / kGroup of them.
+template <typename T, int kGroup, int NV, int kThreads, bool kAligned>
 __global__ void __launch_bounds__(kThreads) residual_rmsnorm_kernel(const RmsNormArgs a) {
-    constexpr int VEC = 16 / sizeof(T), kGroups = kThreads / (32 * kWarps), kSpan = 32 * kWarps * VEC;
-    __shared__ float part[kGroups][kWarps];
-    const int lane = threadIdx.x & 31, group = threadIdx.x / (32 * kWarps), warp = (threadIdx.x >> 5) % kWarps;
-    const int c0 = (warp * 32 + lane) * VEC, C = a.C;
+    constexpr int VEC = 16 / sizeof(T), kGroups = kThreads / kGroup, kSpan = kGroup * VEC;
+    constexpr int kWarps = kGroup / 32, kPerWarp = kGroup < 32 ? 32 / kGroup : 1;  // warps per row, rows per warp
+    __shared__ float part[kWarps > 1 ? kWarps : 1];
+    const int lane = threadIdx.x & 31, warp = threadIdx.x % kGroup / 32, c0 = threadIdx.x % kGroup * VEC;
     const T *scale = (const T *)a.scale, *weight = (const T *)a.weight;
-    for (int64_t row = (int64_t)blockIdx.x * kGroups + group; row < a.rows; row += (int64_t)gridDim.x * kGroups) {
+    // the loop is the warp's: rows past the last one have no columns
+    int64_t first = (int64_t)blockIdx.x * kGroups + (kGroup < 32 ? threadIdx.x / 32 * kPerWarp : threadIdx.x / kGroup);
+    for (; first < a.rows; first += (int64_t)gridDim.x * kGroups) {
+        const int64_t row = first + (kGroup < 32 ? lane / kGroup : 0);
+        const int C = row < a.rows ? a.C : 0;
         const T *x = (const T *)a.x + row * a.x_row;
         uint4 rx[NV], rb[NV];  // everything that a row reads is asked for before anything is used
 #pragma unroll
@@ -99,7 +103,7 @@ __global__ void __launch_bounds__(kThreads) residual_rmsnorm_kernel(const RmsNor
             if (c0 + j * kSpan < C) rx[j] = load_raw<T, VEC, kAligned, true>(x, c0 + j * kSpan, C);
         }
         if (a.branch) {
-            const T *branch = (const T *)a.branch + row * C;
+            const T *branch = (const T *)a.branch + row * a.C;
 #pragma unroll
             for (int j = 0; j < NV; ++j)
                 if (c0 + j * kSpan < C) rb[j] = load_raw<T, VEC, kAligned, true>(branch, c0 + j * kSpan, C);
@@ -120,7 +124,7 @@ __global__ void __launch_bounds__(kThreads) residual_rmsnorm_kernel(const RmsNor
                         for (int i = 0; i < VEC; ++i) s[i] += b[i];
                     }
                     rx[j] = pack_raw<T, VEC>(s);  // the norm is that of the stream as the next block reads it
-                    if (a.x_out) store_raw<T, VEC, kAligned>((T *)a.x_out + row * C, c, C, rx[j]);
+                    if (a.x_out) store_raw<T, VEC, kAligned>((T *)a.x_out + row * a.C, c, C, rx[j]);
                 }
             }
         }
@@ -138,14 +142,14 @@ __global__ void __launch_bounds__(kThreads) residual_rmsnorm_kernel(const RmsNor
                 for (int i = 0; i < VEC; ++i) sum = fmaf(v[i], v[i], sum);
             }
 #pragma unroll
-            for (int m = 16; m >= 1; m >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, m);
+            for (int m = (kGroup < 32 ? kGroup : 32) / 2; m >= 1; m >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, m);
             if constexpr (kWarps > 1) {  // one group per CTA: a whole-CTA barrier
                 static_assert(kGroups == 1, "the barrier below is the CTA's");
-                if (lane == 0) part[0][warp] = sum;
+                if (lane == 0) part[warp] = sum;
                 __syncthreads();
                 sum = 0.0f;
 #pragma unroll
-                for (int w = 0; w < kWarps; ++w) sum += part[0][w];
+                for (int w = 0; w < kWarps; ++w) sum += part[w];
                 __syncthreads();
             }
             rstd = rsqrtf(fmaf(sum, a.inv_C, a.eps));
@@ -166,13 +170,14 @@ __global__ void __launch_bounds__(kThreads) residual_rmsnorm_kernel(const RmsNor
                 }
             }
             if (a.normed) {
-                if (c < C) store_raw<T, VEC, kAligned>((T *)a.normed + row * C, c, C, pack_raw<T, VEC>(v));
+                if (c < C) store_raw<T, VEC, kAligned>((T *)a.normed + row * a.C, c, C, pack_raw<T, VEC>(v));
             } else {
                 float top = 0.0f;
 #pragma unroll
                 for (int i = 0; i < VEC; ++i) top = fmaxf(top, fabsf(v[i]));
 #pragma unroll
-                for (int m = kScaleBlock / VEC / 2; m >= 1; m >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, m));
+                for (int m = (kGroup < kScaleBlock / VEC ? kGroup : kScaleBlock / VEC) / 2; m >= 1; m >>= 1)
+                    top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, m));
                 top = fmaxf(top, kSmallestMax);
                 if (c < C) {
                     store_e4m3<VEC>(a.q + row * a.q_row, c, C, v, inverse_scale(top));
@@ -188,26 +193,30 @@ template <typename T, bool kAligned> int launch_rmsnorm(const RmsNormArgs &a, cu
     const int vectors = (a.C + VEC - 1) / VEC;
     const int64_t sms = sm_count();
     const auto grid = [&](int64_t blocks, int64_t per_sm) { return (unsigned)(blocks < sms * per_sm ? blocks : sms * per_sm); };
-#define COME_RMS_LAUNCH(WARPS, NV, THREADS, PER_SM)                                                                       \
-    residual_rmsnorm_kernel<T, WARPS, NV, THREADS, kAligned>                                                              \
-        <<<grid((a.rows * WARPS * 32 + THREADS - 1) / THREADS, PER_SM), THREADS, 0, st>>>(a)
+#define COME_RMS_LAUNCH(GROUP, NV, THREADS, PER_SM)                                                                       \
+    residual_rmsnorm_kernel<T, GROUP, NV, THREADS, kAligned>                                                              \
+        <<<grid((a.rows * GROUP + THREADS - 1) / THREADS, PER_SM), THREADS, 0, st>>>(a)
     // A warp per row up to 128 vectors, four from there on: 80,672 x 1024 bf16 (128 vectors) 114 / 134 us with one / four, 10,534 x 1000
-    // float32 (250 vectors) 35 / 29.  Few rows take four or eight warps each: a row's latency counts there.
+    // float32 (250 vectors) 35 / 29.  Up to 16 vectors a warp holds two or four rows, so that its lanes have work: 1,875,000 x 64 bf16
+    // (8 vectors) 471 / 164 us with one / four, 937,500 x 64 float32 (16 vectors) 229 / 161 with one / two.  Few rows take four or eight
+    // warps each: a row's latency counts there.
     if (vectors > 4 * 128 || (a.rows <= 4 * sms && vectors > 32)) {
-        if (vectors <= 128) COME_RMS_LAUNCH(4, 1, 128, 16);
-        else if (vectors <= 256) COME_RMS_LAUNCH(8, 1, 256, 8);
-        else if (vectors <= 512) COME_RMS_LAUNCH(8, 2, 256, 6);
-        else if (vectors <= 1024) COME_RMS_LAUNCH(8, 4, 256, 4);
-        else if (vectors <= 2048) COME_RMS_LAUNCH(8, 8, 256, 2);
+        if (vectors <= 128) COME_RMS_LAUNCH(128, 1, 128, 16);
+        else if (vectors <= 256) COME_RMS_LAUNCH(256, 1, 256, 8);
+        else if (vectors <= 512) COME_RMS_LAUNCH(256, 2, 256, 6);
+        else if (vectors <= 1024) COME_RMS_LAUNCH(256, 4, 256, 4);
+        else if (vectors <= 2048) COME_RMS_LAUNCH(256, 8, 256, 2);
         else {
             set_error("come_residual_rmsnorm: rows of at most %d elements of this type (got %d)", 2048 * VEC, a.C);
             return COME_ERR_UNSUPPORTED;
         }
-    } else if (vectors <= 32) COME_RMS_LAUNCH(1, 1, 128, 16);
-    else if (vectors <= 64) COME_RMS_LAUNCH(1, 2, 128, 12);
-    else if (vectors <= 128) COME_RMS_LAUNCH(1, 4, 128, 8);
-    else if (vectors <= 256) COME_RMS_LAUNCH(4, 2, 128, 1 << 20);
-    else COME_RMS_LAUNCH(4, 4, 128, 8);
+    } else if (vectors <= 8) COME_RMS_LAUNCH(8, 1, 128, 16);
+    else if (vectors <= 16) COME_RMS_LAUNCH(16, 1, 128, 16);
+    else if (vectors <= 32) COME_RMS_LAUNCH(32, 1, 128, 16);
+    else if (vectors <= 64) COME_RMS_LAUNCH(32, 2, 128, 12);
+    else if (vectors <= 128) COME_RMS_LAUNCH(32, 4, 128, 8);
+    else if (vectors <= 256) COME_RMS_LAUNCH(128, 2, 128, 1 << 20);
+    else COME_RMS_LAUNCH(128, 4, 128, 8);
 #undef COME_RMS_LAUNCH
     return check_launch("come_residual_rmsnorm");
 }

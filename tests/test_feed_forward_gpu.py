@@ -66,7 +66,7 @@ def check_rows8(q, want, slack, what):
 
 
 # ---- norm -------------------------------------------------------------------------------------------------------------------
-NORM_SHAPES = [(1, 8), (1, 1024), (2, 40), (3, 127), (5, 128), (7, 129), (64, 1000), (600, 136), (593, 1024), (1200, 250), (9, 2052), (700, 4096), (3, 8192)]
+NORM_SHAPES = [(1, 8), (4001, 24), (3001, 56), (2999, 64), (1003, 100), (1, 1024), (2, 40), (3, 127), (5, 128), (7, 129), (64, 1000), (600, 136), (593, 1024), (1200, 250), (9, 2052), (700, 4096), (3, 8192)]
 
 
 @pytest.mark.parametrize("kind", ["f32", "f16", "bf16"])
