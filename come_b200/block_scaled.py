@@ -190,7 +190,12 @@ def activation_code(activation: str) -> int:
 
 class _QuantizedWeights(torch.nn.Module):
     """Holds weights in 8 bits as buffers.  They follow the module to another device, not to another dtype: ``module.to(bfloat16)``
-    leaves numbers, scales and biases what they are."""
+    leaves numbers, scales and biases what they are.  The numbers' buffer is as wide as its rows are apart (whole 16 bytes, zeros behind
+    the last column): copies to another device and state dicts keep columns, not strides."""
+
+    def __init__(self):
+        super().__init__()
+        self._columns = {}
 
     def _apply(self, fn, recurse=True):
         kept = {name: b for name, b in self._buffers.items() if b is not None}
@@ -203,12 +208,17 @@ class _QuantizedWeights(torch.nn.Module):
 
     def _hold(self, name: str, weight: torch.Tensor, bias: Optional[torch.Tensor]) -> None:
         w = quantize_weight(weight)
-        self.register_buffer(name, w.data)
+        rows, cols = w.shape
+        held = torch.zeros((rows, w.data.stride(0)), dtype=torch.uint8, device=w.data.device)
+        held[:, :cols] = w.data.view(torch.uint8)
+        self._columns[name] = cols
+        self.register_buffer(name, held.view(torch.float8_e4m3fn))
         self.register_buffer(name + "_scale", w.scale)
         self.register_buffer(name + "_bias", None if bias is None else bias.detach().float().contiguous())
 
     def _weight(self, name: str) -> BlockScaled:
-        return BlockScaled(getattr(self, name), getattr(self, name + "_scale"))
+        data, cols = getattr(self, name), self._columns[name]
+        return BlockScaled(data if data.shape[1] == cols else data[:, :cols], getattr(self, name + "_scale"))
 
 
 class BlockScaledLinear(_QuantizedWeights):

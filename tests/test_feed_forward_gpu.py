@@ -596,6 +596,28 @@ def test_gated_mlp_in_16_and_8_bits():
     within(l8(x).view(-1, 70), want, chain(192) * (x8.abs() @ d(l8._weight("weight").dequantize()).abs().t() + 1) * 2 + 2.0 ** -23 * want.abs(), "8-bit linear")
 
 
+@pytest.mark.parametrize("cols", [320, 328, 250])
+def test_8_bit_modules_move_between_devices_and_through_state_dicts(cols):
+    """The buffers keep their numbers and the rows their alignment when a module goes to the host and back, is copied, or is filled from
+    contiguous tensors of its state dict, for widths that are not whole 16 bytes too."""
+    import copy
+    from come_b200.block_scaled import BlockScaledLinear
+    torch.manual_seed(4)
+    lin = torch.nn.Linear(cols, 130).cuda()
+    x = torch.randn(9, cols, device="cuda")
+    module = BlockScaledLinear(lin, out_dtype=torch.float32)
+    want = module(x)
+    state = {k: v.cpu().contiguous() for k, v in module.state_dict().items()}
+    assert torch.equal(copy.deepcopy(module)(x), want)
+    assert torch.equal(module.cpu().cuda()(x), want)
+    assert torch.equal(module.half().cpu().float().cuda()(x), want)
+    other = BlockScaledLinear(torch.nn.Linear(cols, 130).cuda(), out_dtype=torch.float32)
+    other.load_state_dict(state, assign=True)
+    assert torch.equal(other.cuda()(x), want)
+    other.load_state_dict(BlockScaledLinear(lin).state_dict())
+    assert torch.equal(other(x), want)
+
+
 @pytest.mark.parametrize("eight", [False, True])
 def test_aggregator_with_rms_norms_and_gated_mlps(eight):
     """The fused aggregator (norms with their residuals in one kernel, 8-bit rows straight from the norm) against the same modules run one
