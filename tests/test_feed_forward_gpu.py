@@ -558,6 +558,69 @@ def test_training_step_in_a_graph():
         assert all(torch.equal(a, b) for a, b in zip(grads, want))
 
 
+# ---- offsets beyond 32 bits ------------------------------------------------------------------------------------------------------------
+def test_results_of_more_than_2_31_elements():
+    """The last rows of a result with more than 2^31 elements are those of a call on these rows alone.  Two ways to the same real number,
+    each with float32 sums and one rounding: a step of the result's type apart at most, with room for the sums near zero."""
+    from come_b200.block import residual_rmsnorm
+    from come_b200.block_scaled import block_scaled_gated_linear, block_scaled_linear, quantize_rows, quantize_weight
+    from come_b200.feed_forward import gated_linear
+    torch.manual_seed(11)
+    T, K, F, tail = 1_050_000, 64, 2056, 200
+    assert T * F > 2 ** 31
+    x = torch.randn(T, K, device="cuda").bfloat16()
+    wg, wu = (torch.randn(F, K, device="cuda").div_(8).bfloat16() for _ in range(2))
+    last = x[-tail:].clone()
+
+    def near(got, want, what):
+        got, want = got.double(), want.double()
+        assert ((got - want).abs() <= 2.0 ** -7 * want.abs() + 1e-5 * want.abs().max()).all(), what
+
+    x8, last8, g8, u8 = quantize_rows(x), quantize_rows(last), quantize_weight(wg), quantize_weight(wu)
+    near(block_scaled_linear(x8, g8)[-tail:], block_scaled_linear(last8, g8), "8-bit product")
+    near(block_scaled_gated_linear(x8, g8, u8, out_dtype=torch.bfloat16)[-tail:], block_scaled_gated_linear(last8, g8, u8, out_dtype=torch.bfloat16), "8-bit gated")
+    q, want = block_scaled_gated_linear(x8, g8, u8), block_scaled_gated_linear(last8, g8, u8)
+    assert ((q.scale[-tail:] - want.scale).abs() <= 2.0 ** -20 * want.scale).all()
+    got, want = q.data[-tail:].float() * q.scale[-tail:].repeat_interleave(128, 1)[:, :F], want.dequantize()
+    assert ((got - want).abs() <= 2.0 ** -3 * want.abs() + want.abs().max() * 2.0 ** -16).all()
+    del q, got
+
+    def grads(x, dh):
+        x = x.detach().requires_grad_()
+        w = wg.detach().requires_grad_()
+        out = gated_linear(x, w, wu)
+        out.backward(dh)
+        return out.detach()[-tail:].clone(), x.grad[-tail:].clone(), w.grad
+
+    dh = torch.zeros(T, F, device="cuda", dtype=torch.bfloat16)
+    dh[-tail:] = torch.randn(tail, F, device="cuda")
+    out, dx, dw = grads(x, dh)
+    some = 2 ** 18 // F + 1  # as many rows keep the operands of the gradients in one part, like the long call
+    assert tail > some and tail > 64
+    out1, dx1, dw1 = grads(last, dh[-tail:].clone())
+    near(out, out1, "gated")
+    near(dx, dx1, "dx")
+    near(dw, dw1, "dw")
+    del dh, x8, out, dx, dw
+    torch.cuda.empty_cache()
+
+    rows, C = 2_100_000, 1032
+    x = torch.randn(rows, C, device="cuda", dtype=torch.bfloat16)
+    norm = torch.nn.RMSNorm(C, eps=1e-6).cuda().bfloat16()
+    with torch.no_grad():
+        stream, normed = residual_rmsnorm(x, x, None, norm)
+        s1, n1 = residual_rmsnorm(x[-tail:].clone(), x[-tail:].clone(), None, norm)
+        assert torch.equal(stream[-tail:], s1)
+        near(normed[-tail:], n1, "norm")
+        del normed, stream
+        q = residual_rmsnorm(x, None, None, norm, quantize=True)[1]
+        q1 = residual_rmsnorm(x[-tail:].clone(), None, None, norm, quantize=True)[1]
+        got, want = q.data[-tail:].float() * q.scale[-tail:].repeat_interleave(128, 1)[:, :C], q1.dequantize()
+        assert ((got - want).abs() <= 2.0 ** -3 * want.abs() + want.abs().max() * 2.0 ** -16).all()
+    del q, x
+    torch.cuda.empty_cache()
+
+
 # ---- modules and the aggregator ---------------------------------------------------------------------------------------------------------
 def test_gated_mlp_in_16_and_8_bits():
     """The module against its formula, and the 8-bit module against the formula on its own (quantised) weights, activations quantised as
