@@ -24,7 +24,8 @@
 // the 128 bytes per clock of an SM let pass in the step's 128 clocks; in a pair each SM holds half of B.
 //
 // Every wait is bounded as in matmul_sm100.cu: after one gave up, the CTA's roles go on without acting, its abort flag keeps it from
-// storing, and the pair meets at the last cluster barrier.
+// storing, and the pair meets at the last cluster barrier.  A CTA leaves when everything that signals or writes to it has landed: loads
+// and arrivals are waited for, or, after a wait gave up, given a few milliseconds.
 #include "matmul_sm100.cuh"
 
 #include <type_traits>
@@ -302,6 +303,11 @@ __global__ void __launch_bounds__(kThreads, 1) __cluster_dims__(2, 1, 1) matmul_
                 }
                 if (rank == 0)  // what was asked for has landed (both CTAs' loads complete here) before shared memory is released
                     for (int j = max(it - kStages, 0); j < it; ++j) mbar_drain(&sh.full[j % kStages], (j / kStages) & 1, p.status, kErrFull);
+                // The products' arrivals come to the barriers of both CTAs; those that no role waits for are waited for here, or they could
+                // reach the shared memory of whatever runs next on this SM: `empty` of the last stages, and on the second CTA `drained`
+                // (the first one's issuer waits for its own).
+                for (int j = max(it - kStages, 0); j < it && ok; ++j) ok = wait(&sh.empty[j % kStages], (j / kStages) & 1, kErrEmpty);
+                if (rank == 1 && ok) wait(&sh.drained, 0, kErrSums);
             }
             __syncwarp();
         } else if (warp == kIssuerWarp) {
@@ -738,14 +744,16 @@ __global__ void __launch_bounds__(kThreads, 1) __cluster_dims__(2, 1, 1) matmul_
             }
         }
     }
-    if (sh.abort_flag != 0) {  // the other CTA's copies complete on the first one's barriers: give those in flight time to land
+    __syncwarp();
+    if (sh.abort_flag != 0) st_cluster_u32(map_rank(smem_u32((const void *)&sh.abort_flag), rank ^ 1), 1);  // the other CTA learns of it
+    tc_fence_before();
+    cluster_sync();  // both CTAs' roles have ended: nothing more is issued, and every arrival and copy has landed unless a wait gave up
+    if (sh.abort_flag != 0) {  // what was not waited for, of either CTA, gets time to land before either leaves
         const long long t0 = clock64();
         while (clock64() - t0 < (1ll << 22)) {
         }
     }
     __syncwarp();
-    tc_fence_before();
-    cluster_sync();  // no CTA leaves while the other signals its barriers or reads its operands
     if (warp == kIssuerWarp) {
         tc_fence_after();
         asm volatile("tcgen05.dealloc.cta_group::2.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(kTmemCols));

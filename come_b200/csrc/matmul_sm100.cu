@@ -161,6 +161,9 @@ __global__ void __launch_bounds__(kThreads, 1) matmul_split_kernel(const __grid_
                 }
             }
             for (int j = max(i - kStages, 0); j < i; ++j) mbar_drain(&sh.full[j % kStages], (j / kStages) & 1, p.status, kErrFull);
+            if (i == n_kb)  // the last arrivals of the products, which no other role waits for
+                for (int j = max(i - kStages, 0); j < i && wait(&sh.empty[j % kStages], (j / kStages) & 1, kErrEmpty); ++j) {
+                }
         }
         __syncwarp();
     } else if (!dead && warp == kIssuerWarp) {

@@ -170,6 +170,8 @@ __device__ __forceinline__ uint32_t ld_cluster_u32(uint32_t addr) {
     return v;
 }
 
+__device__ __forceinline__ void st_cluster_u32(uint32_t addr, uint32_t v) { asm volatile("st.shared::cluster.u32 [%0], %1;" ::"r"(addr), "r"(v) : "memory"); }
+
 enum : uint32_t { kErrFull = 1u << 19, kErrEmpty = 1u << 20, kErrSums = 1u << 21 };
 static_assert((kErrFull | kErrEmpty | kErrSums) == kStatusMatmul, "come_device_status names these bits");
 
