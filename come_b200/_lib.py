@@ -23,7 +23,7 @@ EXPORTS = (
     "come_attn_varlen_fwd", "come_attn_varlen_fwd_rows", "come_attn_cross_fwd", "come_attn_cross_fwd_parts", "come_attn_combine", "come_attn_combine_parts", "come_attn_set_cta_limit", "come_qkv_prepare", "come_packed_positions",
     "come_residual_rmsnorm", "come_quantize_rows", "come_quantize_weight", "come_matmul_e4m3", "come_gated_matmul_e4m3", "come_gated_matmul",
     "come_gated_matmul_backward", "come_gated_backward_rows",
-    "come_device_status", "come_selftest_bounded_wait", "come_selftest_attn_stall", "come_attn_work_list",
+    "come_device_status", "come_selftest_bounded_wait", "come_selftest_attn_stall", "come_selftest_matmul_stall", "come_attn_work_list",
     "come_peer_alloc", "come_peer_open", "come_peer_close", "come_peer_free", "come_peer_copy", "come_peer_signal", "come_peer_wait",
 )
 COME_PEER_HANDLE_BYTES = 64
@@ -100,6 +100,7 @@ def lib() -> C.CDLL:
     l.come_selftest_bounded_wait.argtypes = [i64, vp, vp]
     l.come_attn_work_list.argtypes = [vp, i32, i32, i64, i64, i32, vp, i32, vp, i64, vp]
     l.come_selftest_attn_stall.argtypes = [vp, i64, i32, vp, f32, i32, vp, vp, vp]
+    l.come_selftest_matmul_stall.argtypes = [vp, vp, vp, vp, vp, i64, i64, i64, i32, i32, i64, vp, vp, vp]
     l.come_peer_alloc.argtypes = [i64, C.POINTER(vp), vp]
     l.come_peer_open.argtypes = [vp, C.POINTER(vp)]
     l.come_peer_close.argtypes = [vp]

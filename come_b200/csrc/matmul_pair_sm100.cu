@@ -206,7 +206,8 @@ __device__ __forceinline__ void tc_wait_ld_of(uint32_t (&r)[32]) {
                  :: "memory");
 }
 
-template <bool kE4m3, int kMode, bool kAMn, bool kBMn>
+// kSelfTest: the producers of some CTAs stop before a K block, so that the waits for it run out, after a limit of the launch's own.
+template <bool kE4m3, int kMode, bool kAMn, bool kBMn, bool kSelfTest>
 __global__ void __launch_bounds__(kThreads, 1) __cluster_dims__(2, 1, 1) matmul_pair_kernel(const __grid_constant__ MatmulParams p) {
     constexpr bool kGated = kMode != kMatmulPlain;
     constexpr int kElems = kE4m3 ? 128 : 64;  // contraction elements of a K block
@@ -243,7 +244,8 @@ __global__ void __launch_bounds__(kThreads, 1) __cluster_dims__(2, 1, 1) matmul_
     // All of the SM's tensor memory is allocated, so its base is column 0: the tensor-memory addresses are constants.
     constexpr uint32_t tmem = 0;
     const uint32_t ring = smem_u32(smem);
-    const auto wait = [&](uint64_t *bar, uint32_t parity, uint32_t code) { return mbar_wait_limit(bar, parity, &sh.abort_flag, p.status, code, kWaitTicks); };
+    const auto limit = [&] { return kSelfTest ? p.wait_limit : kWaitTicks; };
+    const auto wait = [&](uint64_t *bar, uint32_t parity, uint32_t code) { return mbar_wait_limit(bar, parity, &sh.abort_flag, p.status, code, limit()); };
     const int total = p.tiles_m * p.problems * p.tiles_n;
     struct Tile {
         int problem, m0, n0;
@@ -282,6 +284,7 @@ __global__ void __launch_bounds__(kThreads, 1) __cluster_dims__(2, 1, 1) matmul_
                     for (int i = 0; i < p.k_blocks; ++i, ++it) {
                         const int st = it % kStages;
                         ok = wait(&sh.empty[st], ((it / kStages) & 1) ^ 1, kErrEmpty);
+                        if constexpr (kSelfTest) ok = ok && !(it >= p.stall_block && (p.stall_ctas >> rank & 1));
                         if (!ok) break;
                         const int sum = i >= p.kb_per_sum ? 1 : 0, k = (i - sum * p.kb_per_sum) * kElems;
                         const uint32_t dst = ring + st * kStageBytes, bar = full0 + st * 8;
@@ -302,7 +305,7 @@ __global__ void __launch_bounds__(kThreads, 1) __cluster_dims__(2, 1, 1) matmul_
                     }
                 }
                 if (rank == 0)  // what was asked for has landed (both CTAs' loads complete here) before shared memory is released
-                    for (int j = max(it - kStages, 0); j < it; ++j) mbar_drain(&sh.full[j % kStages], (j / kStages) & 1, p.status, kErrFull);
+                    for (int j = max(it - kStages, 0); j < it; ++j) mbar_drain(&sh.full[j % kStages], (j / kStages) & 1, p.status, kErrFull, limit());
                 // The products' arrivals come to the barriers of both CTAs; those that no role waits for are waited for here, or they could
                 // reach the shared memory of whatever runs next on this SM: `empty` of the last stages, and on the second CTA `drained`
                 // (the first one's issuer waits for its own).
@@ -358,7 +361,7 @@ __global__ void __launch_bounds__(kThreads, 1) __cluster_dims__(2, 1, 1) matmul_
                 }
                 if (elect_one()) {
                     tc_commit_pair(&sh.drained);
-                    mbar_drain(&sh.drained, 0, p.status, kErrSums);
+                    mbar_drain(&sh.drained, 0, p.status, kErrSums, limit());
                 }
             }
             __syncwarp();
@@ -760,8 +763,8 @@ __global__ void __launch_bounds__(kThreads, 1) __cluster_dims__(2, 1, 1) matmul_
     }
 }
 
-template <bool kE4m3, int kMode, bool kAMn, bool kBMn> int launch_pair(const MatmulParams &p, cudaStream_t st) {
-    constexpr auto kernel = matmul_pair_kernel<kE4m3, kMode, kAMn, kBMn>;
+template <bool kE4m3, int kMode, bool kAMn, bool kBMn, bool kSelfTest = false> int launch_pair(const MatmulParams &p, cudaStream_t st) {
+    constexpr auto kernel = matmul_pair_kernel<kE4m3, kMode, kAMn, kBMn, kSelfTest>;
     if (int rc = allow_smem<kernel>(smem_bytes(kE4m3)); rc != COME_OK) return rc;
     const int tiles = p.tiles_m * p.problems * p.tiles_n, pairs = sm_count() / 2;
     kernel<<<2 * (tiles < pairs ? tiles : pairs), kThreads, smem_bytes(kE4m3), st>>>(p);
@@ -788,6 +791,7 @@ int matmul_pair_launch(const MatmulArgs &a, MatmulParams &p, cudaStream_t st) {
     const int64_t rows = (a.M + 2 * kTile - 1) / (2 * kTile);
     COME_REQUIRE(rows * p.tiles_n * a.problems < (1ll << 30), "the result has too many tiles for one launch");
     p.tiles_m = (int)rows;
+    if (a.wait_limit > 0) return a.e4m3 ? launch_pair<true, kMatmulGated, false, false, true>(p, st) : launch_pair<false, kMatmulGated, false, false, true>(p, st);
     if (a.e4m3) return a.mode == kMatmulPlain ? launch_pair<true, kMatmulPlain, false, false>(p, st) : launch_pair<true, kMatmulGated, false, false>(p, st);
     if (a.mode == kMatmulGated) return launch_pair<false, kMatmulGated, false, false>(p, st);
     if (a.mode == kMatmulGatedGrad) return launch_pair<false, kMatmulGatedGrad, false, false>(p, st);

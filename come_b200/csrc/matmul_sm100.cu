@@ -88,7 +88,8 @@ __device__ __forceinline__ void load4(const void *in, int64_t at, float (&v)[4],
     for (int i = 0; i < 4; ++i) v[i] = i < valid ? load_any(in, at + i, dtype) : 0.0f;
 }
 
-template <bool kE4m3, int kMode, bool kAMn, bool kBMn>
+// kSelfTest: the producers of some CTAs stop before a K block, so that the waits for it run out, after a limit of the launch's own.
+template <bool kE4m3, int kMode, bool kAMn, bool kBMn, bool kSelfTest>
 __global__ void __launch_bounds__(kThreads, 1) matmul_split_kernel(const __grid_constant__ MatmulParams p) {
     constexpr int kMats = kMode == kMatmulPlain ? 1 : 2;
     constexpr int kN = kMats * kTile;
@@ -132,7 +133,8 @@ __global__ void __launch_bounds__(kThreads, 1) matmul_split_kernel(const __grid_
     // All of the SM's tensor memory is allocated, so its base is column 0: the tensor-memory addresses are constants.
     constexpr uint32_t tmem = 0;
     const uint32_t ring = smem_u32(smem);
-    const auto wait = [&](uint64_t *bar, uint32_t parity, uint32_t code) { return mbar_wait_limit(bar, parity, &sh.abort_flag, p.status, code, kWaitTicks); };
+    const auto limit = [&] { return kSelfTest ? p.wait_limit : kWaitTicks; };
+    const auto wait = [&](uint64_t *bar, uint32_t parity, uint32_t code) { return mbar_wait_limit(bar, parity, &sh.abort_flag, p.status, code, limit()); };
     const bool misplaced = sh.tmem_base != tmem, dead = sh.abort_flag != 0 || misplaced;
     if (misplaced && threadIdx.x == 0) atomicOr(p.status, kErrSums);
 
@@ -142,6 +144,7 @@ __global__ void __launch_bounds__(kThreads, 1) matmul_split_kernel(const __grid_
             for (; i < n_kb; ++i) {
                 const int st = i % kStages;
                 if (!wait(&sh.empty[st], ((i / kStages) & 1) ^ 1, kErrEmpty)) break;
+                if (kSelfTest && i >= p.stall_block && (p.stall_ctas >> rank & 1)) break;
                 const int kb = kb0 + i, sum = kE4m3 || p.sums == 1 ? 0 : kb / p.kb_per_sum, k = (kb - sum * p.kb_per_sum) * kElems;
                 const uint32_t dst = ring + st * kStageBytes;
                 mbar_arrive_expect_tx(&sh.full[st], kStageBytes);
@@ -160,7 +163,7 @@ __global__ void __launch_bounds__(kThreads, 1) matmul_split_kernel(const __grid_
                     if constexpr (kMats == 2) tma_load_2d(dst + 2 * kOperandBytes, &p.b[1], k, n0, &sh.full[st]);
                 }
             }
-            for (int j = max(i - kStages, 0); j < i; ++j) mbar_drain(&sh.full[j % kStages], (j / kStages) & 1, p.status, kErrFull);
+            for (int j = max(i - kStages, 0); j < i; ++j) mbar_drain(&sh.full[j % kStages], (j / kStages) & 1, p.status, kErrFull, limit());
             if (i == n_kb)  // the last arrivals of the products, which no other role waits for
                 for (int j = max(i - kStages, 0); j < i && wait(&sh.empty[j % kStages], (j / kStages) & 1, kErrEmpty); ++j) {
                 }
@@ -205,7 +208,7 @@ __global__ void __launch_bounds__(kThreads, 1) matmul_split_kernel(const __grid_
         }
         if (elect_one()) {
             tc_commit_1(&sh.drained);
-            mbar_drain(&sh.drained, 0, p.status, kErrSums);
+            mbar_drain(&sh.drained, 0, p.status, kErrSums, limit());
         }
         __syncwarp();
     } else if (!dead) {
@@ -376,8 +379,8 @@ __global__ void __launch_bounds__(kThreads, 1) matmul_split_kernel(const __grid_
     }
 }
 
-template <bool kE4m3, int kMode, bool kAMn, bool kBMn> int launch_split(const MatmulParams &p, int64_t tiles, int cluster, cudaStream_t st) {
-    constexpr auto kernel = matmul_split_kernel<kE4m3, kMode, kAMn, kBMn>;
+template <bool kE4m3, int kMode, bool kAMn, bool kBMn, bool kSelfTest = false> int launch_split(const MatmulParams &p, int64_t tiles, int cluster, cudaStream_t st) {
+    constexpr auto kernel = matmul_split_kernel<kE4m3, kMode, kAMn, kBMn, kSelfTest>;
     if (int rc = allow_smem<kernel>(kSmemBytes); rc != COME_OK) return rc;
     cudaLaunchAttribute attr = {};
     attr.id = cudaLaunchAttributeClusterDimension;
@@ -443,6 +446,9 @@ int run_matmul(const MatmulArgs &a, cudaStream_t st) {
     p.k_blocks = p.kb_per_sum * a.sums;
     p.low_rows = a.low_rows;
     p.problems = a.problems;
+    p.wait_limit = a.wait_limit;
+    p.stall_block = a.stall_block;
+    p.stall_ctas = a.stall_ctas;
     p.act = a.act;
     p.dtype = a.dtype;
     p.bias_dtype = a.e4m3 ? COME_F32 : a.dtype;
@@ -453,6 +459,8 @@ int run_matmul(const MatmulArgs &a, cudaStream_t st) {
     COME_REQUIRE(tiles < (1ll << 27), "the result has %lld tiles of 128 x 128: too many for one launch", (long long)tiles);
     p.tiles_m = (int)(per_problem / p.tiles_n);
     const int cluster = pick_cluster(tiles, p.k_blocks);
+    if (a.wait_limit > 0)
+        return a.e4m3 ? launch_split<true, kMatmulGated, false, false, true>(p, tiles, cluster, st) : launch_split<false, kMatmulGated, false, false, true>(p, tiles, cluster, st);
     if (a.e4m3) return a.mode == kMatmulPlain ? launch_split<true, kMatmulPlain, false, false>(p, tiles, cluster, st) : launch_split<true, kMatmulGated, false, false>(p, tiles, cluster, st);
     if (a.mode == kMatmulGated) return launch_split<false, kMatmulGated, false, false>(p, tiles, cluster, st);
     if (a.mode == kMatmulGatedGrad) return launch_split<false, kMatmulGatedGrad, false, false>(p, tiles, cluster, st);
@@ -686,4 +694,39 @@ extern "C" int come_gated_matmul_backward(const void *x_dev, int64_t x_row_strid
         return check_launch("come_gated_matmul_backward");
     }
     return COME_OK;
+}
+
+extern "C" int come_selftest_matmul_stall(const void *x_dev, const float *x_scale_dev, const void *gate_dev, const void *up_dev, const float *w_scale_dev, int64_t tokens,
+                                          int64_t features, int64_t channels, int k_blocks, int ctas, int64_t ticks, void *out_dev, float *out_scale_dev, void *stream) {
+    using namespace come;
+    COME_REQUIRE(x_dev && gate_dev && up_dev && out_dev, "come_selftest_matmul_stall: x, gate, up and out must be given");
+    COME_REQUIRE((x_scale_dev == nullptr) == (w_scale_dev == nullptr) && (x_scale_dev || !out_scale_dev), "come_selftest_matmul_stall: scales of both operands or of none, and no 8-bit result of 16-bit operands");
+    COME_REQUIRE(tokens > 0 && tokens < (1 << 16) && features > 0 && features < (1 << 12) && features % 16 == 0 && channels > 0 && channels < (1 << 12) && channels % 128 == 0,
+                 "come_selftest_matmul_stall: a small launch only (tokens below 2^16, features below 2^12 and a multiple of 16, channels below 2^12 and a multiple of 128)");
+    COME_REQUIRE(k_blocks >= 0 && ctas > 0 && ctas < 256, "come_selftest_matmul_stall: k_blocks must not be negative, ctas a mask of up to 8 ranks");
+    COME_REQUIRE(ticks > 0 && ticks <= (1ll << 26), "come_selftest_matmul_stall: ticks must be in (0, 2^26] (a fraction of a second)");
+    const bool e4m3 = x_scale_dev != nullptr;
+    const int size = e4m3 ? 1 : 2;
+    COME_REQUIRE_ROWS("x", x_dev, channels, size, channels);
+    COME_REQUIRE_ROWS("gate", gate_dev, channels, size, channels);
+    COME_REQUIRE_ROWS("up", up_dev, channels, size, channels);
+    COME_REQUIRE((uintptr_t)out_dev % 16 == 0, "come_selftest_matmul_stall: out must be 16-byte aligned");
+    MatmulArgs a = {};
+    a.mode = kMatmulGated;
+    a.e4m3 = e4m3;
+    a.dtype = COME_BF16;
+    a.M = tokens, a.N = features, a.K = channels;
+    a.a[0] = x_dev, a.b[0] = gate_dev, a.b[1] = up_dev;
+    a.a_row[0] = a.b_row[0] = a.b_row[1] = channels;
+    a.sums = a.problems = 1;
+    a.a_scale = x_scale_dev, a.as_row = channels / kScaleBlock, a.as_block = 1;
+    a.b_scale[0] = a.b_scale[1] = w_scale_dev, a.bs_row[0] = a.bs_row[1] = channels / kScaleBlock;
+    a.act = COME_ACT_SILU;
+    a.out[0] = out_dev, a.out_row[0] = features;
+    a.out_dtype = out_scale_dev ? (int)COME_E4M3 : (int)COME_BF16;
+    a.out_scale = out_scale_dev, a.os_row = (features + kScaleBlock - 1) / kScaleBlock, a.os_block = 1;
+    a.wait_limit = ticks;
+    a.stall_block = k_blocks;
+    a.stall_ctas = (uint32_t)ctas;
+    return run_matmul(a, (cudaStream_t)stream);
 }

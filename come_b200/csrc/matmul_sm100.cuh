@@ -41,6 +41,9 @@ struct MatmulArgs {
     int out_dtype;
     float *out_scale;            // 8-bit result: per row and 128 columns
     int64_t os_row, os_block;
+    long long wait_limit;        // self-test: clock ticks after which a wait gives up; 0: an ordinary launch
+    int stall_block;             // ... K block, counted over a CTA's life, before which the producers of `stall_ctas` stop
+    uint32_t stall_ctas;         // ... ranks of a cluster, as bits
 };
 
 constexpr int kTile = 128;
@@ -61,6 +64,9 @@ struct MatmulParams {
     int tiles_m, tiles_n, problems;   // grid of tiles of one problem
     int act, dtype, bias_dtype, out_dtype;
     unsigned int *status;
+    long long wait_limit;  // self-test only, as in MatmulArgs
+    int stall_block;
+    uint32_t stall_ctas;
 };
 
 // The kernel for results with many tiles (matmul_pair_sm100.cu).

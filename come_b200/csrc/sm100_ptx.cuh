@@ -50,10 +50,10 @@ __device__ __forceinline__ bool mbar_wait_limit(uint64_t *bar, uint32_t parity, 
     }
 }
 // Bounded wait of the exit path, for work of this CTA that completes by itself: it goes on after the abort flag is raised.
-__device__ __forceinline__ void mbar_drain(uint64_t *bar, uint32_t parity, unsigned int *status, uint32_t code) {
+__device__ __forceinline__ void mbar_drain(uint64_t *bar, uint32_t parity, unsigned int *status, uint32_t code, long long limit = kWaitTicks) {
     const long long t0 = clock64();
     while (!mbar_try_wait(bar, parity)) {
-        if (clock64() - t0 > kWaitTicks) {
+        if (clock64() - t0 > limit) {
             atomicOr(status, code);
             return;
         }

@@ -445,6 +445,18 @@ int come_selftest_attn_stall(const void *qkv_dev, int64_t total, int num_heads, 
                              float softmax_scale, int key_tiles, void *out_dev, float *lse_dev, void *stream);
 
 /*
+ * The same for the product kernels: out = silu(x gate^T) * (x up^T) of contiguous operands, bfloat16 (scales NULL), or e4m3 with
+ * x_scale [tokens, channels / 128] and w_scale [ceil(features / 128), channels / 128] (of both weights); out [tokens, features] in
+ * bfloat16, or in 8 bits with out_scale [tokens, ceil(features / 128)].  In every cluster the CTAs whose ranks are set in the mask `ctas` load
+ * their first `k_blocks` blocks of the contraction only (128 e4m3 or 64 bfloat16 numbers).  The waits for the next one give up after
+ * `ticks` clocks (at most 2^26), raise bits 19-21 of the device status word, and the kernel returns normally; every tile of the result is
+ * then right or untouched.  The kernel is the one that come_gated_matmul(_e4m3) picks at these sizes.  Clear the word afterwards.
+ */
+int come_selftest_matmul_stall(const void *x_dev, const float *x_scale_dev, const void *gate_dev, const void *up_dev,
+                               const float *w_scale_dev, int64_t tokens, int64_t features, int64_t channels, int k_blocks, int ctas,
+                               int64_t ticks, void *out_dev, float *out_scale_dev, void *stream);
+
+/*
  * The work list of a self-attention launch of the tensor-core kernel (head_dim 64) on at most max_ctas CTAs (0: one per SM),
  * as the kernel forms it: for tests and for looking at the balance of a launch.  Arguments as in
  * come_attn_varlen_fwd_rows.  out_dev receives items, query tiles per item, first item of a split last round, parts of a

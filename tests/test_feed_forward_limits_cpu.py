@@ -1,0 +1,30 @@
+"""Host-side checks of the feed-forward operators that need no GPU: refusals of the self-test, limits of sizes, and which modules the fused
+path and the 8-bit conversion take."""
+import pytest
+import torch
+
+from come_b200 import _lib
+
+AT = 1 << 20  # an address that passes the checks of alignment; nothing reads it (the calls below end on the host)
+
+
+def test_the_self_test_of_the_products_refuses_what_is_not_small():
+    good = dict(x=AT, xs=AT, gate=AT, up=AT, ws=AT, tokens=64, features=128, channels=256, k_blocks=0, ctas=1, ticks=1000, out=AT, out_scale=AT, stream=None)
+    for change, text in (({"x": None}, "must be given"), ({"out": None}, "must be given"), ({"xs": None}, "both operands or of none"), ({"xs": None, "ws": None}, "no 8-bit result"),
+                         ({"tokens": 1 << 16}, "a small launch only"), ({"features": 24}, "a small launch only"), ({"channels": 192}, "a small launch only"),
+                         ({"k_blocks": -1}, "must not be negative"), ({"ctas": 0}, "a mask"), ({"ctas": 256}, "a mask"), ({"ticks": 0}, "ticks must be"),
+                         ({"ticks": (1 << 26) + 1}, "ticks must be"), ({"gate": AT + 8}, "16-byte aligned"), ({"out": AT + 8}, "16-byte aligned")):
+        rc = _lib.lib().come_selftest_matmul_stall(*{**good, **change}.values())
+        assert rc == _lib.COME_ERR_ARG and text in _lib.last_error(), (change, rc, _lib.last_error())
+
+
+def _wrapper(norm1, norm2):
+    """What `fusable` looks at of a wrapped block."""
+    from types import SimpleNamespace
+    none = torch.nn.Identity()
+    return SimpleNamespace(block=SimpleNamespace(norm1=norm1, norm2=norm2, ls1=none, ls2=none), attn=SimpleNamespace(run_dtype=torch.bfloat16))
+
+
+class _OneMore(torch.nn.RMSNorm):
+    def forward(self, x):
+        return torch.nn.functional.rms_norm(x, self.normalized_shape, 1 + self.weight, self.eps)
