@@ -474,8 +474,9 @@ int run_matmul(const MatmulArgs &a, cudaStream_t st) {
 constexpr int kSumThreads = 512, kSumRows = kSumThreads / 4;
 template <typename T>
 __global__ void __launch_bounds__(kSumThreads) column_sums_kernel(const T *__restrict__ x0, const T *__restrict__ x1, int64_t row_stride, int64_t rows, int cols,
-                                                                  T *__restrict__ out0, T *__restrict__ out1) {
+                                                                  T *__restrict__ out0, T *__restrict__ out1, const unsigned int *status) {
     __shared__ float part[kSumRows][33];
+    if (__syncthreads_or((*(const volatile unsigned int *)status & kStatusMatmul) != 0)) return;  // a product gave up: nothing has filled the rows
     const T *x = blockIdx.y ? x1 : x0;
     T *out = blockIdx.y ? out1 : out0;
     if (!out) return;
@@ -686,11 +687,14 @@ extern "C" int come_gated_matmul_backward(const void *x_dev, int64_t x_row_strid
     }
     if (dgate_bias_dev || dup_bias_dev) {
         const dim3 grid((unsigned)((features + 31) / 32), 2);
+        const unsigned int *status = status_word_dev();
+        if (!status) return COME_ERR_CUDA;
         if (dtype == COME_F16)
-            column_sums_kernel<__half><<<grid, kSumThreads, 0, st>>>((const __half *)dgate_dev, (const __half *)dup_dev, d_row_stride, parts * tokens, (int)features, (__half *)dgate_bias_dev, (__half *)dup_bias_dev);
+            column_sums_kernel<__half><<<grid, kSumThreads, 0, st>>>((const __half *)dgate_dev, (const __half *)dup_dev, d_row_stride, parts * tokens, (int)features, (__half *)dgate_bias_dev, (__half *)dup_bias_dev,
+                                                                     status);
         else
             column_sums_kernel<__nv_bfloat16><<<grid, kSumThreads, 0, st>>>((const __nv_bfloat16 *)dgate_dev, (const __nv_bfloat16 *)dup_dev, d_row_stride, parts * tokens, (int)features,
-                                                                            (__nv_bfloat16 *)dgate_bias_dev, (__nv_bfloat16 *)dup_bias_dev);
+                                                                            (__nv_bfloat16 *)dgate_bias_dev, (__nv_bfloat16 *)dup_bias_dev, status);
         return check_launch("come_gated_matmul_backward");
     }
     return COME_OK;

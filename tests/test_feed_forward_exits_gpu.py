@@ -172,3 +172,30 @@ def test_products_leave_their_outputs_alone_while_the_status_word_is_raised(T, K
         _lib.device_status(clear=True)
     assert all(not bool((t[..., :1] == 7).all()) for t in run())  # cleared: the same launches compute
     assert _lib.device_status(clear=True) == 0
+
+
+@pytest.mark.parametrize("kind", ["f16", "bf16"])
+@pytest.mark.parametrize("T,K,F", [(3, 128, 200), (130, 256, 192), (5003, 128, 1010)])
+def test_no_gradient_is_written_while_the_status_word_is_raised(T, K, F, kind):
+    """All five results of the backward pass, the biases' among them: their sums would be those of workspaces that nothing has filled."""
+    from come_b200 import _lib
+    lib, randn, st = _lib.lib(), gen(6), torch.cuda.current_stream().cuda_stream
+    dtype = torch.float16 if kind == "f16" else torch.bfloat16
+    assert _lib.device_status(clear=True) == 0
+    x, wg, wu, dh, b = (t.to(dtype) for t in (randn(T, K), randn(F, K) / 8, randn(F, K) / 8, randn(T, F), randn(F)))
+    rows, stride = lib.come_gated_backward_rows(T, F), -(-F // 8) * 8
+
+    def run():
+        made = [torch.full(s, 7, dtype=dtype, device="cuda") for s in ((rows, stride), (rows, stride), (T, K), (F, K), (F, K), (F,), (F,))]
+        dg, du, dx, dwg, dwu, dbg, dbu = (t.data_ptr() for t in made)
+        _lib.check(lib.come_gated_matmul_backward(x.data_ptr(), K, wg.data_ptr(), K, wu.data_ptr(), K, b.data_ptr(), b.data_ptr(), _lib.COME_F16 if kind == "f16" else _lib.COME_BF16, 0,
+                                                  T, F, K, dh.data_ptr(), F, dg, du, stride, dx, K, dwg, dwu, K, dbg, dbu, st))
+        return made
+
+    try:
+        raise_status()
+        assert all(bool((t == 7).all()) for t in run())
+    finally:
+        _lib.device_status(clear=True)
+    assert all(not bool((t == 7).all()) for t in run())
+    assert _lib.device_status(clear=True) == 0
