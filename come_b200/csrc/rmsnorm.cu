@@ -29,6 +29,7 @@ struct RmsNormArgs {
     int64_t q_row;
     float *q_scale;
     int64_t s_row, s_block;
+    int64_t chunks;       // quantiser of wide rows: pieces of a row
 };
 
 // VEC elements of a row from column c on as 16 raw bytes; kAligned: one access, the row's width is a whole number of them.  kOnce: a
@@ -82,8 +83,9 @@ template <int VEC> __device__ __forceinline__ void store_e4m3(uint8_t *p, int c,
     }
 }
 
-// kGroup threads own a row (part of a warp, or whole warps); a CTA of kThreads threads holds kThreads / kGroup of them.
-template <typename T, int kGroup, int NV, int kThreads, bool kAligned>
+// kGroup threads own a row (part of a warp, or whole warps); a CTA of kThreads threads holds kThreads / kGroup of them.  kChunked: they own
+// a piece of kGroup * NV vectors of a row instead, which is a whole number of scales: the quantiser alone needs no more of it.
+template <typename T, int kGroup, int NV, int kThreads, bool kAligned, bool kChunked>
 __global__ void __launch_bounds__(kThreads) residual_rmsnorm_kernel(const RmsNormArgs a) {
     constexpr int VEC = 16 / sizeof(T), kGroups = kThreads / kGroup, kSpan = kGroup * VEC;
     constexpr int kWarps = kGroup / 32, kPerWarp = kGroup < 32 ? 32 / kGroup : 1;  // warps per row, rows per warp
@@ -92,10 +94,13 @@ __global__ void __launch_bounds__(kThreads) residual_rmsnorm_kernel(const RmsNor
     const T *scale = (const T *)a.scale, *weight = (const T *)a.weight;
     // the loop is the warp's: rows past the last one have no columns
     int64_t first = (int64_t)blockIdx.x * kGroups + (kGroup < 32 ? threadIdx.x / 32 * kPerWarp : threadIdx.x / kGroup);
-    for (; first < a.rows; first += (int64_t)gridDim.x * kGroups) {
-        const int64_t row = first + (kGroup < 32 ? lane / kGroup : 0);
-        const int C = row < a.rows ? a.C : 0;
-        const T *x = (const T *)a.x + row * a.x_row;
+    const int64_t rows = kChunked ? a.rows * a.chunks : a.rows;
+    for (; first < rows; first += (int64_t)gridDim.x * kGroups) {
+        static_assert(!kChunked || (kGroup >= 32 && kSpan * NV % kScaleBlock == 0), "");
+        const int64_t row = kChunked ? first / a.chunks : first + (kGroup < 32 ? lane / kGroup : 0);
+        const int col0 = kChunked ? (int)(first - row * a.chunks) * (kSpan * NV) : 0;
+        const int C = row >= a.rows ? 0 : kChunked ? min(a.C - col0, kSpan * NV) : a.C;
+        const T *x = (const T *)a.x + row * a.x_row + col0;
         uint4 rx[NV], rb[NV];  // everything that a row reads is asked for before anything is used
 #pragma unroll
         for (int j = 0; j < NV; ++j) {
@@ -180,8 +185,8 @@ __global__ void __launch_bounds__(kThreads) residual_rmsnorm_kernel(const RmsNor
                     top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, m));
                 top = fmaxf(top, kSmallestMax);
                 if (c < C) {
-                    store_e4m3<VEC>(a.q + row * a.q_row, c, C, v, inverse_scale(top));
-                    if (c % kScaleBlock == 0) a.q_scale[row * a.s_row + (c / kScaleBlock) * a.s_block] = top * (1.0f / kE4m3Max);
+                    store_e4m3<VEC>(a.q + row * a.q_row + col0, c, C, v, inverse_scale(top));
+                    if (c % kScaleBlock == 0) a.q_scale[row * a.s_row + ((col0 + c) / kScaleBlock) * a.s_block] = top * (1.0f / kE4m3Max);
                 }
             }
         }
@@ -190,17 +195,21 @@ __global__ void __launch_bounds__(kThreads) residual_rmsnorm_kernel(const RmsNor
 
 template <typename T, bool kAligned> int launch_rmsnorm(const RmsNormArgs &a, cudaStream_t st) {
     constexpr int VEC = 16 / sizeof(T);
-    const int vectors = (a.C + VEC - 1) / VEC;
+    const int64_t vectors = ((int64_t)a.C + VEC - 1) / VEC;
     const int64_t sms = sm_count();
     const auto grid = [&](int64_t blocks, int64_t per_sm) { return (unsigned)(blocks < sms * per_sm ? blocks : sms * per_sm); };
 #define COME_RMS_LAUNCH(GROUP, NV, THREADS, PER_SM)                                                                       \
-    residual_rmsnorm_kernel<T, GROUP, NV, THREADS, kAligned>                                                              \
+    residual_rmsnorm_kernel<T, GROUP, NV, THREADS, kAligned, false>                                                       \
         <<<grid((a.rows * GROUP + THREADS - 1) / THREADS, PER_SM), THREADS, 0, st>>>(a)
     // A warp per row up to 128 vectors, four from there on: 80,672 x 1024 bf16 (128 vectors) 114 / 134 us with one / four, 10,534 x 1000
     // float32 (250 vectors) 35 / 29.  Up to 16 vectors a warp holds two or four rows, so that its lanes have work: 1,875,000 x 64 bf16
     // (8 vectors) 471 / 164 us with one / four, 937,500 x 64 float32 (16 vectors) 229 / 161 with one / two.  Few rows take four or eight
     // warps each: a row's latency counts there.
-    if (vectors > 4 * 128 || (a.rows <= 4 * sms && vectors > 32)) {
+    if (a.q && !a.norm && vectors > 2048) {  // the quantiser, of rows wider than a norm's: a warp per 128 vectors
+        RmsNormArgs b = a;
+        b.chunks = (vectors + 127) / 128;
+        residual_rmsnorm_kernel<T, 32, 4, 128, kAligned, true><<<grid((b.rows * b.chunks + 3) / 4, 8), 128, 0, st>>>(b);
+    } else if (vectors > 4 * 128 || (a.rows <= 4 * sms && vectors > 32)) {
         if (vectors <= 128) COME_RMS_LAUNCH(128, 1, 128, 16);
         else if (vectors <= 256) COME_RMS_LAUNCH(256, 1, 256, 8);
         else if (vectors <= 512) COME_RMS_LAUNCH(256, 2, 256, 6);

@@ -368,7 +368,7 @@ int come_packed_positions(const uint8_t *mask_dev, const int64_t *rev_id_dev, in
  *   norm of that stream as it is stored, x_out * rsqrt(mean(x_out^2) + eps) * weight (weight may be NULL), to normed in dtype or to
  *   q / q_scale in 8 bits.  x, branch, x_out, normed [rows, channels] contiguous, scale / weight [channels], all in dtype; x_out may be
  *   x or branch.  Rows of up to 2048 16-byte vectors (16,384 16-bit or 8192 float32 channels).
- * come_quantize_rows      rows in float32 / float16 / bfloat16 -> tokens in 8 bits.
+ * come_quantize_rows      rows in float32 / float16 / bfloat16, of any width -> tokens in 8 bits.
  * come_quantize_weight    a weight -> 8 bits.
  * come_matmul_e4m3        out[t, n] = sum over blocks k of x_scale[t, k] w_scale[n / 128, k] (sum_j x[t, j] w[n, j]) + bias[n]; bias float32 or
  *   NULL; out in out_dtype (COME_F32 / COME_F16 / COME_BF16).  Sums in float32.

@@ -1,0 +1,33 @@
+"""Feed-forward operators at the edges of what they take: widths, lengths, ranges of gradients, norms and modules as users build them.
+Plain float64 formulas; roundings as in test_feed_forward_gpu.py."""
+import math
+
+import pytest
+import torch
+
+from test_feed_forward_gpu import DT, TINY, act64, chain, check_rows8, d, gated64, gen, rnd, within
+
+pytestmark = pytest.mark.gpu
+
+
+# ---- quantisers -------------------------------------------------------------------------------------------------------------
+@pytest.mark.parametrize("kind,rows,cols", [("f32", 3, 8193), ("f32", 5, 11008), ("bf16", 3, 16392), ("bf16", 4, 28672), ("f16", 2, 20001), ("f32", 700, 9000), ("f32", 1, 100_000)])
+def test_rows_of_any_width_are_quantised(kind, rows, cols):
+    from come_b200.block_scaled import quantize_rows
+    t = (gen(cols)(rows, cols + 7) * torch.exp(gen(5)(rows, 1))).to(DT[kind])
+    none = torch.zeros((), device="cuda", dtype=torch.float64)
+    q = quantize_rows(t[:, :cols])  # rows further apart than they are wide
+    check_rows8(q, d(t[:, :cols]), none, "rows")
+    again = quantize_rows(t[:, :cols].contiguous())
+    assert torch.equal(q.data.view(torch.uint8), again.data.view(torch.uint8)) and torch.equal(q.scale, again.scale)
+
+
+def test_wide_modules_quantise_their_tokens():
+    from come_b200.block_scaled import BlockScaledLinear, quantize_rows
+    torch.manual_seed(7)
+    lin = torch.nn.Linear(11008, 40).cuda()
+    x = torch.randn(5, 11008, device="cuda")
+    module = BlockScaledLinear(lin)
+    xv, wv = d(quantize_rows(x).dequantize()), d(module._weight("weight").dequantize())
+    with torch.no_grad():
+        within(module(x), xv @ wv.t() + d(lin.bias), chain(11008) * (xv.abs() @ wv.abs().t() + 1) + 2.0 ** -23, "out")
