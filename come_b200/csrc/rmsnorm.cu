@@ -237,16 +237,17 @@ template <typename T> int dispatch_rmsnorm(const RmsNormArgs &a, cudaStream_t st
     return aligned ? launch_rmsnorm<T, true>(a, st) : launch_rmsnorm<T, false>(a, st);
 }
 
-// One CTA per 128 x 128 block of a weight.
+// One CTA per 128 x 128 block of a weight, blocks of a row of blocks next to each other.
 template <typename T>
 __global__ void __launch_bounds__(256) quantize_weight_kernel(const T *__restrict__ w, int64_t w_row, int rows, int C, uint8_t *__restrict__ q,
                                                               int64_t q_row, float *__restrict__ q_scale, int64_t s_row) {
     __shared__ float tops[8];
-    const int r0 = blockIdx.y * kScaleBlock, c0 = blockIdx.x * kScaleBlock;
-    const int r_end = min(rows, r0 + kScaleBlock), c = c0 + (threadIdx.x & 127);
+    const int col_blocks = (int)(((unsigned)C + kScaleBlock - 1) / kScaleBlock), row_block = blockIdx.x / col_blocks, col_block = blockIdx.x % col_blocks;
+    const int64_t r0 = (int64_t)row_block * kScaleBlock, r_end = min((int64_t)rows, r0 + kScaleBlock);
+    const int c = col_block * kScaleBlock + (threadIdx.x & 127);
     float top = 0.0f;
     if (c < C)
-        for (int r = r0 + (threadIdx.x >> 7); r < r_end; r += 2) top = fmaxf(top, fabsf(Elem<T>::to_f32(w[r * w_row + c])));
+        for (int64_t r = r0 + (threadIdx.x >> 7); r < r_end; r += 2) top = fmaxf(top, fabsf(Elem<T>::to_f32(w[r * w_row + c])));
 #pragma unroll
     for (int m = 16; m >= 1; m >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, m));
     if ((threadIdx.x & 31) == 0) tops[threadIdx.x >> 5] = top;
@@ -254,10 +255,10 @@ __global__ void __launch_bounds__(256) quantize_weight_kernel(const T *__restric
     top = kSmallestMax;
 #pragma unroll
     for (int i = 0; i < 8; ++i) top = fmaxf(top, tops[i]);
-    if (threadIdx.x == 0) q_scale[blockIdx.y * s_row + blockIdx.x] = top / kE4m3Max;
+    if (threadIdx.x == 0) q_scale[row_block * s_row + col_block] = top / kE4m3Max;
     const float inv = kE4m3Max / top;
     if (c < C)
-        for (int r = r0 + (threadIdx.x >> 7); r < r_end; r += 2)
+        for (int64_t r = r0 + (threadIdx.x >> 7); r < r_end; r += 2)
             q[r * q_row + c] = __nv_cvt_float_to_fp8(Elem<T>::to_f32(w[r * w_row + c]) * inv, __NV_SATFINITE, __NV_E4M3);
 }
 
@@ -334,14 +335,15 @@ extern "C" int come_quantize_weight(const void *w_dev, int dtype, int64_t rows, 
                                     float *q_scale_dev, int64_t q_scale_row_stride, void *stream) {
     COME_REQUIRE(rows >= 0 && channels >= 0, "rows and channels must be >= 0");
     COME_REQUIRE(dtype == COME_F32 || dtype == COME_F16 || dtype == COME_BF16, "unknown dtype %d", dtype);
-    COME_REQUIRE(rows < (1ll << 23) && channels < (1ll << 31) - come::kScaleBlock, "at most 2^23 rows, and channels must fit int32");
+    COME_REQUIRE(rows < (1ll << 31) && channels < (1ll << 31) - come::kScaleBlock, "rows and channels must fit int32");
     if (rows == 0 || channels == 0) return COME_OK;
     COME_REQUIRE(w_dev && q_dev && q_scale_dev, "w, q and q_scale must not be NULL");
     COME_REQUIRE(w_row_stride >= 0 && q_row_stride >= channels && q_scale_row_stride >= 0, "bad strides");
-    const dim3 grid((unsigned)((channels + come::kScaleBlock - 1) / come::kScaleBlock), (unsigned)((rows + come::kScaleBlock - 1) / come::kScaleBlock));
+    const int64_t grid = ((channels + come::kScaleBlock - 1) / come::kScaleBlock) * ((rows + come::kScaleBlock - 1) / come::kScaleBlock);
+    COME_REQUIRE(grid < (1ll << 31), "a weight of %lld blocks of 128 x 128 is too large for one launch", (long long)grid);
     cudaStream_t st = (cudaStream_t)stream;
 #define COME_QW_LAUNCH(T)                                                                                                              \
-    come::quantize_weight_kernel<T><<<grid, 256, 0, st>>>((const T *)w_dev, w_row_stride, (int)rows, (int)channels, (uint8_t *)q_dev, \
+    come::quantize_weight_kernel<T><<<(unsigned)grid, 256, 0, st>>>((const T *)w_dev, w_row_stride, (int)rows, (int)channels, (uint8_t *)q_dev, \
                                                           q_row_stride, q_scale_dev, q_scale_row_stride)
     if (dtype == COME_F32) COME_QW_LAUNCH(float);
     else if (dtype == COME_F16) COME_QW_LAUNCH(__half);

@@ -28,3 +28,10 @@ def _wrapper(norm1, norm2):
 class _OneMore(torch.nn.RMSNorm):
     def forward(self, x):
         return torch.nn.functional.rms_norm(x, self.normalized_shape, 1 + self.weight, self.eps)
+
+
+def test_weights_beyond_the_grid_are_refused_by_name():
+    """Sizes that the check accepts fit the launch: blocks of 128 x 128 are counted in one dimension of 2^31 - 1."""
+    lib = _lib.lib()
+    rc = lib.come_quantize_weight(AT, _lib.COME_BF16, (1 << 31) - 1, 1 << 20, 1 << 20, AT, 1 << 20, AT, 1 << 13, None)
+    assert rc == _lib.COME_ERR_ARG and "blocks" in _lib.last_error(), _lib.last_error()

@@ -31,3 +31,17 @@ def test_wide_modules_quantise_their_tokens():
     xv, wv = d(quantize_rows(x).dequantize()), d(module._weight("weight").dequantize())
     with torch.no_grad():
         within(module(x), xv @ wv.t() + d(lin.bias), chain(11008) * (xv.abs() @ wv.abs().t() + 1) + 2.0 ** -23, "out")
+
+
+@pytest.mark.parametrize("rows,cols", [(8_388_481, 8), (8_388_607, 1), (8_388_736, 8), (3, 8_400_000)])
+def test_weights_of_many_rows_or_columns_are_quantised(rows, cols):
+    from come_b200.block_scaled import quantize_weight
+    w = torch.randn(rows, cols, device="cuda", dtype=torch.bfloat16)
+    q = quantize_weight(w)
+    tops = torch.nn.functional.pad(w.float().abs(), (0, -cols % 128, 0, -rows % 128)).view(-(-rows // 128), 128, -(-cols // 128), 128).amax((1, 3))
+    within(q.scale, tops / 448, tops / 448 * 2.0 ** -21, "scale")
+    for part in (slice(0, 300), slice(rows - 300 if rows > 300 else 0, rows)):
+        start = part.start // 128 * 128
+        at = slice(start, part.stop)
+        wide = d(q.scale[start // 128:]).repeat_interleave(128, 0)[: q.data[at].shape[0]].repeat_interleave(128, 1)[:, :cols]
+        within(d(q.data[at].float()) * wide, w[at], d(w[at]).abs() * (2.0 ** -4 + 2.0 ** -20) + wide * 2.0 ** -10, "values")
