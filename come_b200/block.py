@@ -97,13 +97,15 @@ def residual_layernorm(x: torch.Tensor, branch: Optional[torch.Tensor], scale: O
 
 
 def residual_rmsnorm(x: torch.Tensor, branch: Optional[torch.Tensor], scale: Optional[torch.Tensor],
-                     norm: torch.nn.RMSNorm, store_stream: bool = True, quantize: bool = False):
+                     norm: torch.nn.RMSNorm, store_stream: bool = True, quantize: bool = False, eps: Optional[float] = None):
     """``x_out = x + scale * branch`` and ``normed = norm(x_out)`` in one pass over packed rows ``[P, C]`` (``come_residual_rmsnorm``):
     :func:`residual_layernorm` for a block with root-mean-square norms.  The update is computed in float32 and rounded once; the norm
     is that of the stream as it is stored.  ``branch`` None: the norm of ``x`` alone; ``scale`` None: no LayerScale.
     Returns ``(x_out, normed)``; ``x_out`` is ``x`` itself when there is no branch and None when ``store_stream`` is off.  With
     ``quantize`` the normed rows leave in 8 bits with a scale per row and 128 columns
-    (:class:`come_b200.block_scaled.BlockScaled`), the operand of the block-scaled products.  Inference only."""
+    (:class:`come_b200.block_scaled.BlockScaled`), the operand of the block-scaled products.  Inference only.
+    ``eps``: in place of ``norm.eps``.  Where both are None it is ``torch.finfo(x.dtype).eps``; the module itself then takes float32's for
+    16-bit tokens too, and so does :func:`residual_norm`, which stands for the module."""
     require_cuda(x, "x")
     if x.dim() != 2 or not x.is_contiguous():
         raise ValueError(f"x must be a contiguous [rows, C] tensor, got {tuple(x.shape)}")
@@ -125,7 +127,9 @@ def residual_rmsnorm(x: torch.Tensor, branch: Optional[torch.Tensor], scale: Opt
     weight = norm.weight
     if weight is not None:
         weight = _channel_vector(weight, dt, dev, index)
-    eps = float(norm.eps) if norm.eps is not None else torch.finfo(dt).eps
+    if eps is None:
+        eps = torch.finfo(dt).eps if norm.eps is None else norm.eps
+    eps = float(eps)
     x_out = torch.empty_like(x) if (branch is not None and store_stream) else None
     if quantize:
         normed = empty_rows(rows, Cc, dev)
@@ -149,8 +153,8 @@ def residual_norm(x: torch.Tensor, branch: Optional[torch.Tensor], scale: Option
                   quantize: bool = False):
     """:func:`residual_rmsnorm` for an ``nn.RMSNorm``, else :func:`residual_layernorm` (``norm`` None: the update alone).  ``quantize``
     asks for 8-bit rows where the norm can write them: a root-mean-square norm does, a LayerNorm's result stays as it is."""
-    if isinstance(norm, torch.nn.RMSNorm):
-        return residual_rmsnorm(x, branch, scale, norm, quantize=quantize)
+    if isinstance(norm, torch.nn.RMSNorm):  # without an eps the module computes with that of float32, whatever its input
+        return residual_rmsnorm(x, branch, scale, norm, quantize=quantize, eps=torch.finfo(torch.float32).eps if norm.eps is None else norm.eps)
     return residual_layernorm(x, branch, scale, norm)
 
 

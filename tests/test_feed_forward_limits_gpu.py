@@ -10,6 +10,24 @@ from test_feed_forward_gpu import DT, TINY, act64, chain, check_rows8, d, gated6
 pytestmark = pytest.mark.gpu
 
 
+# ---- norms as modules have them ---------------------------------------------------------------------------------------------
+@pytest.mark.parametrize("kind", ["f32", "f16", "bf16"])
+@pytest.mark.parametrize("quantize", [False, True])
+def test_a_norm_without_an_eps_is_the_module_s(kind, quantize):
+    """Where the framework runs a block's norm in place of the module (residual_norm), an nn.RMSNorm without an eps has float32's, as the
+    module itself; with small streams another one shows in the first digit."""
+    from come_b200.block import residual_norm
+    x = (gen(1)(33, 96) * 2.0 ** -8).to(DT[kind])
+    norm = torch.nn.RMSNorm(96, device="cuda").requires_grad_(False)
+    y = d(x) / torch.sqrt(d(x).pow(2).mean(1, keepdim=True) + torch.finfo(torch.float32).eps)
+    _, normed = residual_norm(x, None, None, norm, quantize=quantize)
+    if quantize:
+        check_rows8(normed, y, y.abs() * 2.0 ** -17, "normed")
+    else:
+        within(normed, y, (rnd(kind) + 2.0 ** -17) * y.abs() + TINY[kind], "normed")
+        within(norm.to(DT[kind])(x), y, (rnd(kind) + 2.0 ** -17) * y.abs() + TINY[kind], "the module")
+
+
 # ---- quantisers -------------------------------------------------------------------------------------------------------------
 @pytest.mark.parametrize("kind,rows,cols", [("f32", 3, 8193), ("f32", 5, 11008), ("bf16", 3, 16392), ("bf16", 4, 28672), ("f16", 2, 20001), ("f32", 700, 9000), ("f32", 1, 100_000)])
 def test_rows_of_any_width_are_quantised(kind, rows, cols):
