@@ -166,12 +166,18 @@ def _layer_scale_gamma(ls: torch.nn.Module):
     return (isinstance(gamma, torch.Tensor) and gamma.dim() == 1), gamma
 
 
+def _norm_fusable(norm: torch.nn.Module, dtype: torch.dtype) -> bool:
+    """Whether the fused kernels compute what ``norm`` does on a stream in ``dtype``."""
+    if isinstance(norm, torch.nn.RMSNorm):
+        return type(norm).forward is torch.nn.RMSNorm.forward  # a subclass may have a formula of its own
+    return isinstance(norm, torch.nn.LayerNorm)
+
+
 def fusable(wrapper: _JaggedBlockBase, dtype: torch.dtype) -> bool:
     """Whether :func:`forward_fused` can evaluate this block: residual stream already in the attention dtype, plain
     ``nn.LayerNorm`` or ``nn.RMSNorm`` norms and LayerScale (or identity) scales."""
     b = wrapper.block
-    norms = (torch.nn.LayerNorm, torch.nn.RMSNorm)
-    return (dtype == wrapper.attn.run_dtype and isinstance(b.norm1, norms) and isinstance(b.norm2, norms)
+    return (dtype == wrapper.attn.run_dtype and _norm_fusable(b.norm1, dtype) and _norm_fusable(b.norm2, dtype)
             and _layer_scale_gamma(b.ls1)[0] and _layer_scale_gamma(b.ls2)[0])
 
 

@@ -30,6 +30,15 @@ class _OneMore(torch.nn.RMSNorm):
         return torch.nn.functional.rms_norm(x, self.normalized_shape, 1 + self.weight, self.eps)
 
 
+def test_norms_with_a_formula_of_their_own_are_not_fused():
+    """A subclass that computes something else (weights stored as differences from one, say) runs as the module that it is."""
+    from come_b200.block import fusable
+    rms = torch.nn.RMSNorm(64)
+    assert fusable(_wrapper(rms, rms), torch.bfloat16)
+    assert not fusable(_wrapper(rms, rms), torch.float32)
+    assert not fusable(_wrapper(_OneMore(64), rms), torch.bfloat16) and not fusable(_wrapper(rms, _OneMore(64)), torch.bfloat16)
+
+
 def test_weights_beyond_the_grid_are_refused_by_name():
     """Sizes that the check accepts fit the launch: blocks of 128 x 128 are counted in one dimension of 2^31 - 1."""
     lib = _lib.lib()
