@@ -96,6 +96,9 @@ def residual_layernorm(x: torch.Tensor, branch: Optional[torch.Tensor], scale: O
     return (x if branch is None else x_out), normed
 
 
+RMSNORM_ROW_BYTES = 2048 * 16  # widest row of come_residual_rmsnorm
+
+
 def residual_rmsnorm(x: torch.Tensor, branch: Optional[torch.Tensor], scale: Optional[torch.Tensor],
                      norm: torch.nn.RMSNorm, store_stream: bool = True, quantize: bool = False, eps: Optional[float] = None):
     """``x_out = x + scale * branch`` and ``normed = norm(x_out)`` in one pass over packed rows ``[P, C]`` (``come_residual_rmsnorm``):
@@ -104,6 +107,7 @@ def residual_rmsnorm(x: torch.Tensor, branch: Optional[torch.Tensor], scale: Opt
     Returns ``(x_out, normed)``; ``x_out`` is ``x`` itself when there is no branch and None when ``store_stream`` is off.  With
     ``quantize`` the normed rows leave in 8 bits with a scale per row and 128 columns
     (:class:`come_b200.block_scaled.BlockScaled`), the operand of the block-scaled products.  Inference only.
+    ``scale`` and the norm's weight are taken in the tokens' dtype, like those of :func:`residual_layernorm`; rows of up to 32 KiB.
     ``eps``: in place of ``norm.eps``.  Where both are None it is ``torch.finfo(x.dtype).eps``; the module itself then takes float32's for
     16-bit tokens too, and so does :func:`residual_norm`, which stands for the module."""
     require_cuda(x, "x")
@@ -169,7 +173,8 @@ def _layer_scale_gamma(ls: torch.nn.Module):
 def _norm_fusable(norm: torch.nn.Module, dtype: torch.dtype) -> bool:
     """Whether the fused kernels compute what ``norm`` does on a stream in ``dtype``."""
     if isinstance(norm, torch.nn.RMSNorm):
-        return type(norm).forward is torch.nn.RMSNorm.forward  # a subclass may have a formula of its own
+        # a subclass may have a formula of its own; a row has to fit the kernel's registers
+        return type(norm).forward is torch.nn.RMSNorm.forward and norm.normalized_shape[-1] * dtype.itemsize <= RMSNORM_ROW_BYTES
     return isinstance(norm, torch.nn.LayerNorm)
 
 

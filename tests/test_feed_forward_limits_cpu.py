@@ -39,6 +39,13 @@ def test_norms_with_a_formula_of_their_own_are_not_fused():
     assert not fusable(_wrapper(_OneMore(64), rms), torch.bfloat16) and not fusable(_wrapper(rms, _OneMore(64)), torch.bfloat16)
 
 
+def test_norms_wider_than_the_kernel_s_rows_are_not_fused():
+    from come_b200.block import fusable
+    narrow, wide = torch.nn.RMSNorm(16384, device="meta"), torch.nn.RMSNorm(16392, device="meta")
+    assert fusable(_wrapper(narrow, narrow), torch.bfloat16)
+    assert not fusable(_wrapper(wide, narrow), torch.bfloat16) and not fusable(_wrapper(narrow, wide), torch.bfloat16)
+
+
 def test_weights_beyond_the_grid_are_refused_by_name():
     """Sizes that the check accepts fit the launch: blocks of 128 x 128 are counted in one dimension of 2^31 - 1."""
     lib = _lib.lib()
