@@ -4,6 +4,7 @@ from __future__ import annotations
 import contextlib
 
 import torch
+from torch.autograd import forward_ad
 
 from . import _lib
 
@@ -20,6 +21,12 @@ def dtype_code(dtype: torch.dtype, what: str = "tensor") -> int:
 def require_cuda(t: torch.Tensor, name: str) -> None:
     if not t.is_cuda:
         raise RuntimeError(f"{name} must be on CUDA")
+
+
+def has_tangent(*tensors) -> bool:
+    """Whether a forward-mode derivative is being carried by one of the tensors: such a tensor has no ``requires_grad``, and a kernel
+    that only reads its numbers would drop the tangent without a word."""
+    return forward_ad._current_level >= 0 and any(t is not None and forward_ad.unpack_dual(t).tangent is not None for t in tensors)
 
 
 def ptr(t):

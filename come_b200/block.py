@@ -14,7 +14,7 @@ from typing import Optional
 import torch
 
 from . import _lib
-from ._torch_util import dtype_code, on_device, ptr, require_cuda, stream_ptr
+from ._torch_util import dtype_code, has_tangent, on_device, ptr, require_cuda, stream_ptr
 from .bias_attention import JaggedAttention_w_Bias
 from .block_scaled import BlockScaledGatedMlp, empty_rows
 from .plain_attention import JaggedAttention
@@ -118,7 +118,7 @@ def residual_rmsnorm(x: torch.Tensor, branch: Optional[torch.Tensor], scale: Opt
     code = dtype_code(dt, "x")
     if branch is not None and (branch.shape != x.shape or branch.dtype is not dt or branch.get_device() != index or not branch.is_contiguous()):
         raise ValueError(f"branch must be contiguous and match x {tuple(x.shape)} {dt}, got {tuple(branch.shape)} {branch.dtype}")
-    if torch.is_grad_enabled() and (x.requires_grad or (branch is not None and branch.requires_grad)):
+    if (torch.is_grad_enabled() and (x.requires_grad or (branch is not None and branch.requires_grad))) or has_tangent(x, branch, scale, getattr(norm, "weight", None)):
         raise RuntimeError("residual_rmsnorm: inference only (no autograd)")
     if scale is not None:
         if branch is None:

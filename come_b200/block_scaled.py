@@ -15,7 +15,7 @@ from typing import NamedTuple, Optional
 import torch
 
 from . import _lib
-from ._torch_util import dtype_code, on_device, require_cuda, stream_ptr
+from ._torch_util import dtype_code, has_tangent, on_device, require_cuda, stream_ptr
 
 __all__ = ["BLOCK", "BlockScaled", "quantize_rows", "quantize_weight", "block_scaled_linear", "block_scaled_gated_linear",
            "BlockScaledLinear", "BlockScaledGatedMlp", "to_block_scaled"]
@@ -57,7 +57,7 @@ def _matrix(x: torch.Tensor, name: str) -> torch.Tensor:
     require_cuda(x, name)
     if x.dim() != 2:
         raise ValueError(f"{name} must be a [rows, C] tensor, got {tuple(x.shape)}")
-    if x.requires_grad and torch.is_grad_enabled():
+    if (x.requires_grad and torch.is_grad_enabled()) or has_tangent(x):
         raise RuntimeError(f"{name}: the 8-bit quantisers are inference only (no autograd)")
     return x if x.stride(1) == 1 or x.shape[1] == 1 else x.contiguous()
 

@@ -15,7 +15,7 @@ from typing import Optional
 import torch
 
 from . import _lib
-from ._torch_util import dtype_code, on_device, ptr, require_cuda, stream_ptr
+from ._torch_util import dtype_code, has_tangent, on_device, ptr, require_cuda, stream_ptr
 from .block_scaled import activation_code
 
 __all__ = ["gated_linear", "GatedMlp"]
@@ -95,7 +95,7 @@ class _GatedLinear(torch.autograd.Function):
 
 def gated_linear(x: torch.Tensor, w_gate: torch.Tensor, w_up: torch.Tensor, b_gate: Optional[torch.Tensor] = None,
                  b_up: Optional[torch.Tensor] = None, activation: str = "silu") -> torch.Tensor:
-    """``act(x @ w_gate.T + b_gate) * (x @ w_up.T + b_up)`` in one kernel, differentiable once in every tensor.
+    """``act(x @ w_gate.T + b_gate) * (x @ w_up.T + b_up)`` in one kernel, differentiable once in every tensor (in reverse mode).
 
     ``x [..., C]`` float16 or bfloat16, ``w_gate`` / ``w_up [F, C]`` and ``b_gate`` / ``b_up [F]`` in its dtype; ``C`` a multiple of 8.
     ``activation``: "silu" or "gelu" (the exact one).  Sums in float32, the result rounded once.  Rows that are not contiguous or do
@@ -125,6 +125,8 @@ def gated_linear(x: torch.Tensor, w_gate: torch.Tensor, w_up: torch.Tensor, b_ga
             raise _mismatch("b_up", b_up, [features], x)
         grad = grad or b_up.requires_grad
         b_up = b_up.contiguous()
+    if has_tangent(x, w_gate, w_up, b_gate, b_up):
+        raise RuntimeError("gated_linear has a backward pass, but no forward-mode derivative")
     apply = _GatedLinear.apply if grad and torch.is_grad_enabled() else _forward
     if x.dim() == 2:
         return apply(x, w_gate, w_up, b_gate, b_up, act)

@@ -63,3 +63,29 @@ def test_weights_of_many_rows_or_columns_are_quantised(rows, cols):
         at = slice(start, part.stop)
         wide = d(q.scale[start // 128:]).repeat_interleave(128, 0)[: q.data[at].shape[0]].repeat_interleave(128, 1)[:, :cols]
         within(d(q.data[at].float()) * wide, w[at], d(w[at]).abs() * (2.0 ** -4 + 2.0 ** -20) + wide * 2.0 ** -10, "values")
+
+
+# ---- forward mode -------------------------------------------------------------------------------------------------------------
+def test_forward_mode_is_refused_not_dropped():
+    """A dual tensor has no requires_grad: without a look at the level its tangent would vanish without a word."""
+    from torch.autograd import forward_ad
+    from come_b200.block import residual_rmsnorm
+    from come_b200.block_scaled import quantize_rows
+    from come_b200.feed_forward import gated_linear
+    randn = gen(3)
+    x, w, b = randn(5, 64).bfloat16(), randn(24, 64).bfloat16(), randn(24).bfloat16()
+    norm = torch.nn.RMSNorm(64, eps=1e-6, device="cuda").requires_grad_(False)
+    with forward_ad.dual_level():
+        dual = lambda t: forward_ad.make_dual(t, torch.ones_like(t))  # noqa: E731
+        for args in ((dual(x), w, w), (x, dual(w), w), (x, w, w, dual(b)), (x, w, w, b, dual(b)), (dual(x)[None], w, w)):
+            with pytest.raises((RuntimeError, NotImplementedError)):
+                gated_linear(*args)
+        with pytest.raises(RuntimeError, match="no autograd"):
+            residual_rmsnorm(dual(x), None, None, norm)
+        with pytest.raises(RuntimeError, match="no autograd"):
+            residual_rmsnorm(x, dual(x), None, norm)
+        with pytest.raises(RuntimeError, match="no autograd"):
+            quantize_rows(dual(x))
+        assert torch.equal(gated_linear(x, w, w), gated_linear(x, w, w))  # tensors without a tangent still go through
+        with torch.no_grad():
+            assert gated_linear(x, w, w).shape == (5, 24)
