@@ -265,13 +265,16 @@ class BlockScaledGatedMlp(_QuantizedWeights):
 
 
 def to_block_scaled(module: torch.nn.Module, out_dtype: torch.dtype = torch.bfloat16) -> torch.nn.Module:
-    """Replaces every gated MLP inside ``module`` (on its CUDA device) by its 8-bit form, in place; returns ``module``, or the 8-bit form
-    of ``module`` when it is a gated MLP itself."""
+    """Replaces every gated MLP inside ``module`` (on its CUDA device) by its 8-bit form, in place and in every place where it stands;
+    returns ``module``, or the 8-bit form of ``module`` when it is a gated MLP itself."""
     from .feed_forward import GatedMlp
     if isinstance(module, GatedMlp):
         return BlockScaledGatedMlp(module, out_dtype)
+    made = {}  # one for every module, however many places it stands in
     for parent in list(module.modules()):
-        for name, child in list(parent.named_children()):
+        for name, child in list(parent._modules.items()):
             if isinstance(child, GatedMlp):
-                setattr(parent, name, BlockScaledGatedMlp(child, out_dtype))
+                if child not in made:
+                    made[child] = BlockScaledGatedMlp(child, out_dtype).train(child.training)
+                setattr(parent, name, made[child])
     return module

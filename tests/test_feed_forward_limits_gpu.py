@@ -89,3 +89,17 @@ def test_forward_mode_is_refused_not_dropped():
         assert torch.equal(gated_linear(x, w, w), gated_linear(x, w, w))  # tensors without a tangent still go through
         with torch.no_grad():
             assert gated_linear(x, w, w).shape == (5, 24)
+
+
+# ---- modules -------------------------------------------------------------------------------------------------------------------
+def test_every_use_of_a_gated_mlp_is_replaced():
+    """A module that stands in several places, under one parent or under two, is replaced in all of them, by one 8-bit module."""
+    from come_b200.block_scaled import BlockScaledGatedMlp, to_block_scaled
+    from come_b200.feed_forward import GatedMlp
+    mlp = GatedMlp(64, 96).cuda().bfloat16().eval()
+    model = torch.nn.ModuleList([torch.nn.Sequential(mlp, mlp), torch.nn.Sequential(mlp), GatedMlp(64, 96).cuda()]).eval()
+    to_block_scaled(model)
+    assert not any(isinstance(m, GatedMlp) for m in model.modules())
+    assert model[0][0] is model[0][1] and model[0][0] is model[1][0] and isinstance(model[2], BlockScaledGatedMlp) and model[2] is not model[0][0]
+    assert not any(m.training for m in model.modules())
+    assert to_block_scaled(model) is model  # a second time there is nothing left to do
