@@ -266,7 +266,8 @@ class BlockScaledGatedMlp(_QuantizedWeights):
 
 def to_block_scaled(module: torch.nn.Module, out_dtype: torch.dtype = torch.bfloat16) -> torch.nn.Module:
     """Replaces every gated MLP inside ``module`` (on its CUDA device) by its 8-bit form, in place and in every place where it stands;
-    returns ``module``, or the 8-bit form of ``module`` when it is a gated MLP itself."""
+    returns ``module``, or the 8-bit form of ``module`` when it is a gated MLP itself.  A module without one is refused: other MLPs keep
+    their 16-bit linear layers."""
     from .feed_forward import GatedMlp
     if isinstance(module, GatedMlp):
         return BlockScaledGatedMlp(module, out_dtype)
@@ -277,4 +278,6 @@ def to_block_scaled(module: torch.nn.Module, out_dtype: torch.dtype = torch.bflo
                 if child not in made:
                     made[child] = BlockScaledGatedMlp(child, out_dtype).train(child.training)
                 setattr(parent, name, made[child])
+    if not made and not any(isinstance(m, BlockScaledGatedMlp) for m in module.modules()):
+        raise ValueError(f"{type(module).__name__} has no gated MLP (come_b200.feed_forward.GatedMlp) to convert")
     return module

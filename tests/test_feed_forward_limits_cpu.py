@@ -46,6 +46,15 @@ def test_norms_wider_than_the_kernel_s_rows_are_not_fused():
     assert not fusable(_wrapper(wide, narrow), torch.bfloat16) and not fusable(_wrapper(narrow, wide), torch.bfloat16)
 
 
+def test_a_conversion_that_finds_nothing_says_so():
+    from come_b200.block_scaled import to_block_scaled
+    from come_b200.vggt_arch import AggregatorCore
+    with pytest.raises(ValueError, match="no gated MLP"):
+        to_block_scaled(AggregatorCore(embed_dim=64, depth=1, num_heads=1))
+    with pytest.raises(ValueError, match="no gated MLP"):
+        to_block_scaled(torch.nn.Linear(4, 4))
+
+
 def test_weights_beyond_the_grid_are_refused_by_name():
     """Sizes that the check accepts fit the launch: blocks of 128 x 128 are counted in one dimension of 2^31 - 1."""
     lib = _lib.lib()
