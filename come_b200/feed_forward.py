@@ -99,9 +99,11 @@ def gated_linear(x: torch.Tensor, w_gate: torch.Tensor, w_up: torch.Tensor, b_ga
 
     ``x [..., C]`` float16 or bfloat16, ``w_gate`` / ``w_up [F, C]`` and ``b_gate`` / ``b_up [F]`` in its dtype; ``C`` a multiple of 8.
     ``activation``: "silu" or "gelu" (the exact one).  Sums in float32, the result rounded once.  Rows that are not contiguous or do
-    not start at multiples of 16 bytes are copied first."""
+    not start at multiples of 16 bytes are copied first.  Under autocast tensors in float32, or of several types, are cast to its type first."""
     require_cuda(x, "x")
     act = activation_code(activation)
+    if torch.is_autocast_enabled("cuda"):
+        x, w_gate, w_up, b_gate, b_up = _autocast(x, w_gate, w_up, b_gate, b_up)
     if x.dtype not in (torch.float16, torch.bfloat16):
         raise RuntimeError(f"x: unsupported dtype {x.dtype}; expected float16 or bfloat16")
     cols = x.shape[-1] if x.dim() else 0
@@ -133,6 +135,15 @@ def gated_linear(x: torch.Tensor, w_gate: torch.Tensor, w_up: torch.Tensor, b_ga
     return apply(x.reshape(-1, cols), w_gate, w_up, b_gate, b_up, act).view(*x.shape[:-1], features)
 
 
+def _autocast(*tensors):
+    """The tensors as a linear layer takes them under autocast, unless they already have one 16-bit type."""
+    have = {t.dtype for t in tensors if t is not None}
+    if len(have) == 1 and have <= {torch.float16, torch.bfloat16}:
+        return tensors
+    dtype = torch.get_autocast_dtype("cuda")
+    return tuple(t.to(dtype) if t is not None and t.dtype in (torch.float32, torch.float16, torch.bfloat16) else t for t in tensors)
+
+
 def _mismatch(name: str, t: torch.Tensor, shape, x: torch.Tensor) -> Exception:
     return ValueError(f"{name} must be {shape} {x.dtype} on {x.device}, got {list(t.shape)} {t.dtype} on {t.device}")
 
@@ -140,7 +151,8 @@ def _mismatch(name: str, t: torch.Tensor, shape, x: torch.Tensor) -> Exception:
 class GatedMlp(torch.nn.Module):
     """``w3(act(gate) * up)`` with ``gate, up = w12(x).chunk(2)``: the gated MLP of a block.  The two projections, the activation and the
     product are one kernel; ``w3`` stays a PyTorch GEMM like the other linear layers of the blocks.  float16 and bfloat16, ``dim`` a multiple
-    of 8; float32 streams take the 8-bit form, :class:`come_b200.block_scaled.BlockScaledGatedMlp`."""
+    of 8, or float32 under autocast; float32 streams without it take the 8-bit form,
+    :class:`come_b200.block_scaled.BlockScaledGatedMlp`."""
 
     def __init__(self, dim: int, hidden: int, bias: bool = True, activation: str = "silu"):
         super().__init__()

@@ -91,6 +91,29 @@ def test_forward_mode_is_refused_not_dropped():
             assert gated_linear(x, w, w).shape == (5, 24)
 
 
+# ---- autocast -----------------------------------------------------------------------------------------------------------------
+@pytest.mark.parametrize("dtype", [torch.float16, torch.bfloat16])
+def test_gated_projections_under_autocast(dtype):
+    """float32 parameters and tokens under autocast are cast as a linear layer casts them, and gradients arrive in float32."""
+    from come_b200.feed_forward import GatedMlp, gated_linear
+    torch.manual_seed(1)
+    mlp = GatedMlp(64, 88).cuda()
+    x = torch.randn(3, 7, 64, device="cuda", requires_grad=True)
+    with torch.autocast("cuda", dtype=dtype):
+        y = mlp(x)
+        half = mlp(x.to(dtype))
+    assert y.dtype == dtype and torch.equal(y, half)
+    y.float().square().sum().backward()
+    w_gate, w_up = (t.detach().to(dtype) for t in mlp.w12.weight.chunk(2))
+    b_gate, b_up = (t.detach().to(dtype) for t in mlp.w12.bias.chunk(2))
+    leaves = [t.requires_grad_(True) for t in (x.detach().to(dtype), w_gate, w_up, b_gate, b_up, mlp.w3.weight.detach().to(dtype), mlp.w3.bias.detach().to(dtype))]
+    want = torch.nn.functional.linear(gated_linear(*leaves[:5]), *leaves[5:])
+    assert torch.equal(want, y)
+    want.float().square().sum().backward()
+    assert x.grad.dtype == torch.float32 and torch.equal(x.grad, leaves[0].grad.float())
+    assert torch.equal(mlp.w12.weight.grad, torch.cat([leaves[1].grad, leaves[2].grad]).float()) and torch.equal(mlp.w12.bias.grad, torch.cat([leaves[3].grad, leaves[4].grad]).float())
+
+
 # ---- modules -------------------------------------------------------------------------------------------------------------------
 def test_every_use_of_a_gated_mlp_is_replaced():
     """A module that stands in several places, under one parent or under two, is replaced in all of them, by one 8-bit module."""
