@@ -22,7 +22,7 @@ EXPORTS = (
     "come_unmerge_strided", "come_unmerge_residual", "come_residual_layernorm", "come_suffix_add", "come_suffix_split",
     "come_attn_varlen_fwd", "come_attn_varlen_fwd_rows", "come_attn_cross_fwd", "come_attn_cross_fwd_parts", "come_attn_combine", "come_attn_combine_parts", "come_attn_set_cta_limit", "come_qkv_prepare", "come_packed_positions",
     "come_residual_rmsnorm", "come_quantize_rows", "come_quantize_weight", "come_matmul_e4m3", "come_gated_matmul_e4m3", "come_gated_matmul",
-    "come_gated_matmul_backward", "come_gated_backward_rows",
+    "come_gated_matmul_backward", "come_gated_matmul_backward_in_range", "come_gated_backward_rows",
     "come_device_status", "come_selftest_bounded_wait", "come_selftest_attn_stall", "come_selftest_matmul_stall", "come_attn_work_list",
     "come_peer_alloc", "come_peer_open", "come_peer_close", "come_peer_free", "come_peer_copy", "come_peer_signal", "come_peer_wait",
 )
@@ -94,6 +94,7 @@ def lib() -> C.CDLL:
     l.come_gated_matmul.argtypes = [vp, i64, vp, i64, vp, i64, vp, vp, i32, i32, i64, i64, i64, vp, i64, vp]
     l.come_gated_matmul_backward.argtypes = [vp, i64, vp, i64, vp, i64, vp, vp, i32, i32, i64, i64, i64, vp, i64, vp, vp, i64, vp, i64, vp, vp,
                                              i64, vp, vp, vp]
+    l.come_gated_matmul_backward_in_range.argtypes = l.come_gated_matmul_backward.argtypes[:-1] + [vp, vp]
     l.come_gated_backward_rows.argtypes = [i64, i64]
     l.come_gated_backward_rows.restype = i64
     l.come_device_status.argtypes = [C.POINTER(C.c_uint32), i32]

@@ -652,6 +652,7 @@ __global__ void __launch_bounds__(kThreads, 1) __cluster_dims__(2, 1, 1) matmul_
                     const uint32_t from = lanes + buf * kPairN;
                     as_constant(p.dtype == COME_BF16, [&](auto bf16_c) {
                         constexpr bool kBF16 = decltype(bf16_c)::value;
+                        [[maybe_unused]] const float factor = kBF16 ? 1.0f : range_factor(p.range, !kGated);
                         if constexpr (!kGated) {
 #pragma unroll 1
                             for (int h = 0; h < kCols / 32; ++h) {
@@ -667,7 +668,10 @@ __global__ void __launch_bounds__(kThreads, 1) __cluster_dims__(2, 1, 1) matmul_
                                 for (int c = 0; c < 4; ++c) {
                                     uint32_t e[4];
 #pragma unroll
-                                    for (int j = 0; j < 4; ++j) e[j] = pack_16<kBF16>(__uint_as_float(d[c * 8 + 2 * j]), __uint_as_float(d[c * 8 + 2 * j + 1]));
+                                    for (int j = 0; j < 4; ++j) {
+                                        const float lo = __uint_as_float(d[c * 8 + 2 * j]), hi = __uint_as_float(d[c * 8 + 2 * j + 1]);
+                                        e[j] = kBF16 ? pack_16<kBF16>(lo, hi) : pack_16<kBF16>(lo * factor, hi * factor);
+                                    }
                                     *staged<64>(stage + (h & 1) * 2048, lane, c) = make_uint4(e[0], e[1], e[2], e[3]);
                                 }
                                 __syncwarp();
@@ -712,6 +716,7 @@ __global__ void __launch_bounds__(kThreads, 1) __cluster_dims__(2, 1, 1) matmul_
                                             } else {
                                                 float d0, d1, a0, a1, s0, s1;
                                                 unpack_16<kBF16>(dh[j], d0, d1);
+                                                if constexpr (!kBF16) d0 *= factor, d1 *= factor;
                                                 activation_grad(g0, act, a0, s0);
                                                 activation_grad(g1, act, a1, s1);
                                                 e[j] = pack_16<kBF16>(d0 * u0 * s0, d1 * u1 * s1);

@@ -290,6 +290,7 @@ __global__ void __launch_bounds__(kThreads, 1) matmul_split_kernel(const __grid_
 #pragma unroll
             for (int i = 0; i < 4; ++i)
                 if (i < valid) bias[w][i] = load_any(p.bias[w], n + i, p.bias_dtype);
+    [[maybe_unused]] const float factor = range_factor(p.range, kMode == kMatmulPlain);
     if (misplaced && threadIdx.x == 0) sh.abort_flag = 1;  // read by the others behind the barrier
     tc_fence_before();
     cluster_sync();
@@ -303,7 +304,11 @@ __global__ void __launch_bounds__(kThreads, 1) matmul_split_kernel(const __grid_
         for (int r = (int)(rank + ranks * warp); r < rows; r += (int)ranks * kEpilogueWarps) {
             const int64_t row = m0 + r, at = row * p.out_row[problem] + n;
             [[maybe_unused]] float dh[4];
-            if constexpr (kMode == kMatmulGatedGrad) load4(p.dh, row * p.dh_row + n, dh, valid, p.dtype);
+            if constexpr (kMode == kMatmulGatedGrad) {
+                load4(p.dh, row * p.dh_row + n, dh, valid, p.dtype);
+#pragma unroll
+                for (int i = 0; i < 4; ++i) dh[i] *= factor;
+            }
             float v[kMats][4];
 #pragma unroll
             for (int w = 0; w < kMats; ++w)
@@ -323,6 +328,10 @@ __global__ void __launch_bounds__(kThreads, 1) matmul_split_kernel(const __grid_
                     for (int w = 0; w < kMats; ++w) v[w][0] += x[j][w].x, v[w][1] += x[j][w].y, v[w][2] += x[j][w].z, v[w][3] += x[j][w].w;
             }
             if constexpr (kMode == kMatmulPlain) {
+                if constexpr (!kE4m3) {
+#pragma unroll
+                    for (int i = 0; i < 4; ++i) v[0][i] *= factor;
+                }
                 store4(p.out[problem], at, v[0], valid, p.out_dtype);
             } else if constexpr (kMode == kMatmulGated) {
                 float h[4], top = 0.0f;
@@ -435,6 +444,7 @@ int run_matmul(const MatmulArgs &a, cudaStream_t st) {
     }
     p.dh = a.dh;
     p.dh_row = a.dh_row;
+    p.range = a.range;
     p.out_scale = a.out_scale;
     p.os_row = a.os_row;
     p.os_block = a.os_block;
@@ -474,7 +484,8 @@ int run_matmul(const MatmulArgs &a, cudaStream_t st) {
 constexpr int kSumThreads = 512, kSumRows = kSumThreads / 4;
 template <typename T>
 __global__ void __launch_bounds__(kSumThreads) column_sums_kernel(const T *__restrict__ x0, const T *__restrict__ x1, int64_t row_stride, int64_t rows, int cols,
-                                                                  T *__restrict__ out0, T *__restrict__ out1, const unsigned int *status) {
+                                                                  T *__restrict__ out0, T *__restrict__ out1, const unsigned int *status,
+                                                                  const uint32_t *range) {
     __shared__ float part[kSumRows][33];
     if (__syncthreads_or((*(const volatile unsigned int *)status & kStatusMatmul) != 0)) return;  // a product gave up: nothing has filled the rows
     const T *x = blockIdx.y ? x1 : x0;
@@ -515,8 +526,49 @@ __global__ void __launch_bounds__(kSumThreads) column_sums_kernel(const T *__res
         s = 0.0f;
 #pragma unroll
         for (int r = 0; r < 16; ++r) s += part[r][col];
-        out[blockIdx.x * 32 + col] = Elem<T>::from_f32(s);
+        out[blockIdx.x * 32 + col] = Elem<T>::from_f32(s * range_factor(range, true));
     }
+}
+
+// ---- largest magnitude (float16 gradients) --------------------------------------------------------------------------------
+// Bits of the largest |x| as float32, an infinity or a NaN above all numbers; `largest` is zero before.  A maximum is the same in any
+// order.  One pass over dh at the copy rate (35 MB: about 7 us).
+constexpr int kLargestThreads = 256;
+__global__ void __launch_bounds__(kLargestThreads) largest_kernel(const uint16_t *__restrict__ x, int64_t rows, int64_t cols, int64_t row_stride, uint32_t *__restrict__ largest) {
+    __shared__ uint32_t tops[kLargestThreads / 32];
+    const bool aligned = (((uintptr_t)x | (uintptr_t)(row_stride * 2)) & 15) == 0;
+    uint32_t top = 0;  // two numbers
+    for (int64_t r = blockIdx.y; r < rows; r += gridDim.y) {
+        const uint16_t *row = x + r * row_stride;
+#pragma unroll 4
+        for (int64_t c = ((int64_t)blockIdx.x * kLargestThreads + threadIdx.x) * 8; c < cols; c += (int64_t)gridDim.x * kLargestThreads * 8) {
+            if (aligned && c + 8 <= cols) {
+                const uint4 v = __ldg(reinterpret_cast<const uint4 *>(row + c));
+                top = __vmaxu2(top, __vmaxu2(__vmaxu2(v.x & 0x7fff7fffu, v.y & 0x7fff7fffu), __vmaxu2(v.z & 0x7fff7fffu, v.w & 0x7fff7fffu)));
+            } else {
+                for (int i = 0; i < 8 && c + i < cols; ++i) top = __vmaxu2(top, row[c + i] & 0x7fffu);
+            }
+        }
+    }
+    top = __reduce_max_sync(0xffffffffu, max(top & 0xffffu, top >> 16));
+    if ((threadIdx.x & 31) == 0) tops[threadIdx.x >> 5] = top;
+    __syncthreads();
+    if (threadIdx.x == 0) {
+        for (int i = 1; i < kLargestThreads / 32; ++i) top = max(top, tops[i]);
+        if (top != 0) atomicMax(largest, __float_as_uint(__half2float(__ushort_as_half((unsigned short)top))) & 0x7fffffffu);
+    }
+}
+int find_largest(const void *x, int64_t rows, int64_t cols, int64_t row_stride, uint32_t *largest, cudaStream_t st) {
+    if (row_stride == cols) {  // one long row
+        cols *= rows;
+        rows = 1;
+        row_stride = 0;
+    }
+    COME_CUDA(cudaMemsetAsync(largest, 0, sizeof(uint32_t), st));
+    const int64_t blocks = (cols + kLargestThreads * 8 - 1) / (kLargestThreads * 8), most = 8 * sm_count();
+    const int64_t gx = blocks < most ? blocks : most, gy = rows < (most + gx - 1) / gx ? rows : (most + gx - 1) / gx;
+    largest_kernel<<<dim3((unsigned)gx, (unsigned)gy), kLargestThreads, 0, st>>>((const uint16_t *)x, rows, cols, row_stride, largest);
+    return check_launch("come_gated_matmul_backward");
 }
 
 bool rows_ok(const void *p, int64_t row_stride, int size) { return p && (uintptr_t)p % 16 == 0 && row_stride >= 0 && row_stride * size % 16 == 0 && row_stride * size < (1ll << 40); }
@@ -633,11 +685,12 @@ extern "C" int64_t come_gated_backward_rows(int64_t tokens, int64_t features) {
     return tokens <= 64 || (features < (1ll << 18) && tokens < (1ll << 18) && tokens * features <= (1ll << 18)) ? 2 * tokens : tokens;
 }
 
-extern "C" int come_gated_matmul_backward(const void *x_dev, int64_t x_row_stride, const void *gate_dev, int64_t gate_row_stride, const void *up_dev, int64_t up_row_stride,
+extern "C" int come_gated_matmul_backward_in_range(const void *x_dev, int64_t x_row_stride, const void *gate_dev, int64_t gate_row_stride, const void *up_dev, int64_t up_row_stride,
                                           const void *gate_bias_dev, const void *up_bias_dev, int dtype, int activation, int64_t tokens, int64_t features,
                                           int64_t channels, const void *dout_dev, int64_t dout_row_stride, void *dgate_dev, void *dup_dev, int64_t d_row_stride,
                                           void *dx_dev, int64_t dx_row_stride, void *dgate_weight_dev, void *dup_weight_dev, int64_t dw_row_stride,
-                                          void *dgate_bias_dev, void *dup_bias_dev, void *stream) {
+                                          void *dgate_bias_dev, void *dup_bias_dev, float *range_dev,
+                                                   void *stream) {
     using namespace come;
     cudaStream_t st = (cudaStream_t)stream;
     MatmulArgs a = {};
@@ -649,8 +702,12 @@ extern "C" int come_gated_matmul_backward(const void *x_dev, int64_t x_row_strid
     COME_REQUIRE_ROWS("dup", dup_dev, d_row_stride, 2, features);
     COME_REQUIRE(!dx_dev || dx_row_stride >= channels, "the row stride of dx must hold its rows");
     COME_REQUIRE((!dgate_weight_dev && !dup_weight_dev) || dw_row_stride >= channels, "the row stride of the weights' gradients must hold their rows");
+    COME_REQUIRE((uintptr_t)range_dev % 4 == 0, "range_dev must be 4-byte aligned");
+    const uint32_t *range = dtype == COME_F16 ? (const uint32_t *)range_dev : nullptr;
+    if (range && (rc = find_largest(dout_dev, tokens, features, dout_row_stride, (uint32_t *)range_dev, st)) != COME_OK) return rc;
     // the gradients of the projections
     a.mode = kMatmulGatedGrad;
+    a.range = range;
     a.dh = dout_dev, a.dh_row = dout_row_stride;
     a.out[0] = dgate_dev, a.out[1] = dup_dev;
     a.out_row[0] = a.out_row[1] = d_row_stride;
@@ -661,6 +718,7 @@ extern "C" int come_gated_matmul_backward(const void *x_dev, int64_t x_row_strid
     if (dx_dev) {  // dx = dgate gate + dup up
         MatmulArgs b = {};
         b.dtype = b.out_dtype = dtype;
+        b.range = range;
         b.b_mn = true;
         b.M = tokens, b.N = channels, b.K = features;
         for (int i = 0; i < 2 * parts; ++i) b.a[i] = part(i & 1 ? dup_dev : dgate_dev, i >> 1), b.a_row[i] = d_row_stride;
@@ -673,6 +731,7 @@ extern "C" int come_gated_matmul_backward(const void *x_dev, int64_t x_row_strid
     if (dgate_weight_dev || dup_weight_dev) {  // dgate^T x, dup^T x
         MatmulArgs b = {};
         b.dtype = b.out_dtype = dtype;
+        b.range = range;
         b.a_mn = b.b_mn = true;
         b.M = features, b.N = channels, b.K = tokens;
         b.b[0] = x_dev, b.b_row[0] = x_row_stride;
@@ -691,13 +750,23 @@ extern "C" int come_gated_matmul_backward(const void *x_dev, int64_t x_row_strid
         if (!status) return COME_ERR_CUDA;
         if (dtype == COME_F16)
             column_sums_kernel<__half><<<grid, kSumThreads, 0, st>>>((const __half *)dgate_dev, (const __half *)dup_dev, d_row_stride, parts * tokens, (int)features, (__half *)dgate_bias_dev, (__half *)dup_bias_dev,
-                                                                     status);
+                                                                     status, range);
         else
             column_sums_kernel<__nv_bfloat16><<<grid, kSumThreads, 0, st>>>((const __nv_bfloat16 *)dgate_dev, (const __nv_bfloat16 *)dup_dev, d_row_stride, parts * tokens, (int)features,
-                                                                            (__nv_bfloat16 *)dgate_bias_dev, (__nv_bfloat16 *)dup_bias_dev, status);
+                                                                            (__nv_bfloat16 *)dgate_bias_dev, (__nv_bfloat16 *)dup_bias_dev, status, range);
         return check_launch("come_gated_matmul_backward");
     }
     return COME_OK;
+}
+
+extern "C" int come_gated_matmul_backward(const void *x_dev, int64_t x_row_stride, const void *gate_dev, int64_t gate_row_stride, const void *up_dev, int64_t up_row_stride,
+                                          const void *gate_bias_dev, const void *up_bias_dev, int dtype, int activation, int64_t tokens, int64_t features,
+                                          int64_t channels, const void *dout_dev, int64_t dout_row_stride, void *dgate_dev, void *dup_dev, int64_t d_row_stride,
+                                          void *dx_dev, int64_t dx_row_stride, void *dgate_weight_dev, void *dup_weight_dev, int64_t dw_row_stride,
+                                          void *dgate_bias_dev, void *dup_bias_dev, void *stream) {
+    return come_gated_matmul_backward_in_range(x_dev, x_row_stride, gate_dev, gate_row_stride, up_dev, up_row_stride, gate_bias_dev, up_bias_dev, dtype, activation, tokens, features,
+                                                channels, dout_dev, dout_row_stride, dgate_dev, dup_dev, d_row_stride, dx_dev, dx_row_stride, dgate_weight_dev, dup_weight_dev, dw_row_stride,
+                                                dgate_bias_dev, dup_bias_dev, nullptr, stream);
 }
 
 extern "C" int come_selftest_matmul_stall(const void *x_dev, const float *x_scale_dev, const void *gate_dev, const void *up_dev, const float *w_scale_dev, int64_t tokens,

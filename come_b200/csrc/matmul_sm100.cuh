@@ -36,6 +36,7 @@ struct MatmulArgs {
     int act;
     const void *dh;              // gated gradient: `dtype`
     int64_t dh_row;
+    const uint32_t *range;       // float16 gradients: bits of the largest |dh| as float32 (see range_factor); NULL: taken as they are
     void *out[2];
     int64_t out_row[2];
     int out_dtype;
@@ -56,6 +57,7 @@ struct MatmulParams {
     const float *a_scale, *b_scale[2];
     int64_t as_row, as_block, bs_row[2];
     const void *bias[2], *dh;
+    const uint32_t *range;
     void *out[2];
     float *out_scale;
     int64_t dh_row, out_row[2], os_row, os_block;
@@ -206,6 +208,14 @@ __device__ __forceinline__ void activation_grad(float g, int act, float &value, 
         value = g * cdf;
         slope = fmaf(g, phi, cdf);
     }
+}
+
+// The power of two that brings the largest |dh| into [1/2, 1), and its inverse.  The gradients of the projections lie around dh; without
+// it those of a mean over many elements fall below float16's smallest number and those of a scaled loss past its largest, while the
+// gradients that they become would not.  Nothing is scaled where the largest is zero, infinite or no number.
+__device__ __forceinline__ float range_factor(const uint32_t *range, bool inverse) {
+    const uint32_t bits = range ? __ldg(range) : 0u, e = bits >> 23;
+    return bits == 0 || e == 255 ? 1.0f : __uint_as_float((inverse ? e + 1 : 253 - e) << 23);
 }
 
 __device__ __forceinline__ float load_any(const void *p, int64_t i, int dtype) {

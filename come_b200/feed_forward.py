@@ -4,9 +4,10 @@
 MLPs of visual transformers: ``w12`` holds both projections, the gate's rows first, ``w3`` the projection back.
 
 A training step keeps only its inputs: the backward pass computes the projections again, in float32, and with them their gradients
-(one kernel of ``come_gated_matmul_backward``), then ``dx = dg Wg + du Wu`` and ``dW = dg^T x`` / ``du^T x``.  ``dg`` and ``du`` are rounded to the
+(one kernel of ``come_gated_matmul_backward_in_range``), then ``dx = dg Wg + du Wu`` and ``dW = dg^T x`` / ``du^T x``.  ``dg`` and ``du`` are rounded to the
 tokens' type once, as operands of these products (for few tokens, whose sums do not average that out, in two parts); saved 16-bit
-projections would add their own rounding to every gradient.
+projections would add their own rounding to every gradient.  In float16 they are held times a power of two that brings the largest
+``|dh|`` to one, so that neither a mean over many elements nor a scaled loss takes them out of the type's range.
 """
 from __future__ import annotations
 
@@ -85,11 +86,12 @@ class _GatedLinear(torch.autograd.Function):
         lib = _lib.lib()
         d_rows = lib.come_gated_backward_rows(tokens, features)
         dg, du = _padded(d_rows, features, x), _padded(d_rows, features, x)
+        largest = torch.empty(1, dtype=torch.float32, device=dev) if x.dtype is torch.float16 else None
         with on_device(dev):
-            _lib.check(lib.come_gated_matmul_backward(
+            _lib.check(lib.come_gated_matmul_backward_in_range(
                 x_at, x_row, g_at, g_row, u_at, u_row, ptr(b_gate), ptr(b_up), dtype_code(x.dtype), ctx.act,
                 tokens, features, cols, dh.data_ptr(), dh.stride(0), dg.data_ptr(), du.data_ptr(), dg.stride(0), ptr(dx), cols, ptr(dwg), ptr(dwu), cols,
-                ptr(dbg), ptr(dbu), stream_ptr(dev)))
+                ptr(dbg), ptr(dbu), ptr(largest), stream_ptr(dev)))
         return dx, dwg, dwu, dbg, dbu, None
 
 

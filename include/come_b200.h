@@ -381,6 +381,9 @@ int come_packed_positions(const uint8_t *mask_dev, const int64_t *rev_id_dev, in
  *   16 bytes): tokens rows, or twice as many where the sums are short and the second half holds what the rounding took away; then
  *   dx = dgate gate + dup up, dgate_weight = dgate^T x, dup_weight = dup^T x and the column sums of dgate, dup for the biases.  Any of the
  *   five results may be NULL.  tokens and features must not be zero.
+ * come_gated_matmul_backward_in_range  the same with one float of workspace, range_dev (NULL: none): float16 gradients are held in the
+ *   workspaces times the power of two that brings the largest |dout| into [1/2, 1), so that they do not leave the type's range on their
+ *   way (without it that of dout times up and act is the caller's affair).  bfloat16 has float32's range and ignores it.
  *
  * Results are the same bits in every run.  While bits 19-21 of the device status word are raised, the products return at once without
  * touching their outputs.
@@ -411,6 +414,13 @@ int come_gated_matmul_backward(const void *x_dev, int64_t x_row_stride, const vo
                                void *dgate_dev, void *dup_dev, int64_t d_row_stride, void *dx_dev, int64_t dx_row_stride,
                                void *dgate_weight_dev, void *dup_weight_dev, int64_t dw_row_stride, void *dgate_bias_dev,
                                void *dup_bias_dev, void *stream);
+int come_gated_matmul_backward_in_range(const void *x_dev, int64_t x_row_stride, const void *gate_dev, int64_t gate_row_stride,
+                                        const void *up_dev, int64_t up_row_stride, const void *gate_bias_dev, const void *up_bias_dev,
+                                        int dtype, int activation, int64_t tokens, int64_t features, int64_t channels,
+                                        const void *dout_dev, int64_t dout_row_stride, void *dgate_dev, void *dup_dev,
+                                        int64_t d_row_stride, void *dx_dev, int64_t dx_row_stride, void *dgate_weight_dev,
+                                        void *dup_weight_dev, int64_t dw_row_stride, void *dgate_bias_dev, void *dup_bias_dev,
+                                        float *range_dev, void *stream);
 int64_t come_gated_backward_rows(int64_t tokens, int64_t features);
 
 /*

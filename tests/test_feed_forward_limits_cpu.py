@@ -60,3 +60,13 @@ def test_weights_beyond_the_grid_are_refused_by_name():
     lib = _lib.lib()
     rc = lib.come_quantize_weight(AT, _lib.COME_BF16, (1 << 31) - 1, 1 << 20, 1 << 20, AT, 1 << 20, AT, 1 << 13, None)
     assert rc == _lib.COME_ERR_ARG and "blocks" in _lib.last_error(), _lib.last_error()
+
+
+def test_the_backward_pass_in_range_refuses_what_the_other_refuses():
+    lib = _lib.lib()
+    good = dict(x=AT, x_row=128, g=AT, g_row=128, u=AT, u_row=128, gb=None, ub=None, dtype=_lib.COME_F16, act=0, tokens=4, features=16, channels=128, dout=AT, dout_row=16,
+                dg=AT, du=AT, d_row=16, dx=AT, dx_row=128, dwg=AT, dwu=AT, dw_row=128, dbg=None, dbu=None, range=AT, stream=None)
+    for change, text in (({"tokens": 0}, "zero or empty"), ({"dout": None}, "dout must be given"), ({"d_row": 20}, "dgate must be given"), ({"dw_row": 64}, "weights' gradients"),
+                         ({"dtype": _lib.COME_F32}, "float16 or bfloat16"), ({"range": AT + 2}, "range_dev must be")):
+        rc = lib.come_gated_matmul_backward_in_range(*{**good, **change}.values())
+        assert rc == _lib.COME_ERR_ARG and text in _lib.last_error(), (change, rc, _lib.last_error())

@@ -65,6 +65,83 @@ def test_weights_of_many_rows_or_columns_are_quantised(rows, cols):
         within(d(q.data[at].float()) * wide, w[at], d(w[at]).abs() * (2.0 ** -4 + 2.0 ** -20) + wide * 2.0 ** -10, "values")
 
 
+# ---- gradients ----------------------------------------------------------------------------------------------------------------
+@pytest.mark.parametrize("T,K,F", [(40, 72, 130), (1001, 200, 1003), (5000, 72, 520)])
+@pytest.mark.parametrize("step", [-24, -18, -10, 0, 6])
+def test_float16_gradients_of_any_size(T, K, F, step):
+    """Gradients of the result from float16's smallest numbers (a mean over many elements without loss scaling) up: those of the projections
+    keep their digits.  Brought to [1/2, 1) by a power of two, the largest |dh| leaves every gradient of a projection at most half a step off,
+    or 2^-25 of that range: 2^-24 of the largest |dh|."""
+    from come_b200.feed_forward import gated_linear
+    randn = gen(T + step)
+    e = rnd("f16")
+    x, wg, wu = randn(T, K).half(), (randn(F, K) * 1.5 / math.sqrt(K)).half(), (randn(F, K) * 1.5 / math.sqrt(K)).half()
+    bg, bu, dh = (0.3 * randn(F)).half(), (0.3 * randn(F)).half(), (randn(T, F) * 2.0 ** step).half()
+    leaves = [t.clone().requires_grad_(True) for t in (x, wg, wu, bg, bu)]
+    grads = torch.autograd.grad(gated_linear(*leaves), leaves, dh)
+    h, slack, g, u, a, slope, eg, eu = gated64(d(x), d(wg), d(wu), d(bg), d(bu), "silu", d(dh))
+    least = d(dh).abs().max() * 2.0 ** -24
+    dg, du = d(dh) * u * slope, d(dh) * a
+    edg = d(dh).abs() * (slope.abs() * eu + (u.abs() + eu) * (0.85 * eg + 2.0 ** -18 * (1 + g.abs())))
+    edu = d(dh).abs() * (1.2 * eg + 2.0 ** -19 * a.abs() + 2.0 ** -140)
+    edg, edu = edg + e * (dg.abs() + edg) + least, edu + e * (du.abs() + edu) + least
+    ag, au = dg.abs() + edg, du.abs() + edu
+    for name, got, want, wobble, size, terms in (
+            ("dx", grads[0], dg @ d(wg) + du @ d(wu), edg @ d(wg).abs() + edu @ d(wu).abs(), ag @ d(wg).abs() + au @ d(wu).abs(), 2 * F),
+            ("dgate", grads[1], dg.t() @ d(x), edg.t() @ d(x).abs(), ag.t() @ d(x).abs(), T),
+            ("dup", grads[2], du.t() @ d(x), edu.t() @ d(x).abs(), au.t() @ d(x).abs(), T),
+            ("dgate_bias", grads[3], dg.sum(0), edg.sum(0), ag.sum(0), T),
+            ("dup_bias", grads[4], du.sum(0), edu.sum(0), au.sum(0), T)):
+        within(got, want, wobble + chain(terms) * size + e * (want.abs() + wobble + chain(terms) * size) + TINY["f16"], name)
+        # the sum of independent roundings of a thousand terms is far below the sum of their bounds
+        rough = 4 * e + TINY["f16"] / want.abs().square().mean().sqrt()
+        assert (d(got) - want).norm() / want.norm() <= rough, (name, ((d(got) - want).norm() / want.norm()).item(), rough.item())
+
+
+def test_float16_gradients_do_not_overflow_on_their_way():
+    """dh up = 180,000 has no float16 number; the gradients that it becomes have, where its product with a weight (0.1) or a token (0.25)
+    lies below 65504.  Products with numbers above 0.36 exceed float16 themselves: those are infinite in any arithmetic."""
+    from come_b200.feed_forward import gated_linear
+    for T in (40, 5000):
+        K, F = 72, 520
+        randn = gen(T)
+        x, wg, wu = (0.25 * randn(T, K)).half(), (0.1 * randn(F, K)).half(), (0.1 * randn(F, K)).half()
+        bg, bu = torch.full((F,), 1.0, device="cuda").half(), torch.full((F,), 3.0, device="cuda").half()
+        dh = torch.zeros(T, F, device="cuda").half()
+        dh[T // 2, 5] = 60000.0
+        leaves = [t.clone().requires_grad_(True) for t in (x, wg, wu)]
+        grads = torch.autograd.grad(gated_linear(*leaves, bg, bu), leaves, dh)
+        h, slack, g, u, a, slope, eg, eu = gated64(d(x), d(wg), d(wu), d(bg), d(bu), "silu", d(dh))
+        dg, du = d(dh) * u * slope, d(dh) * a
+        assert dg.abs().max() > 65504
+        for got, want in zip(grads, (dg @ d(wg) + du @ d(wu), dg.t() @ d(x), du.t() @ d(x))):
+            # one rounding of each projection's gradient, one of the result, float32 sums of a few terms
+            size = (dg.abs() @ d(wg).abs() + du.abs() @ d(wu).abs()) if want.shape == (T, K) else (dg.abs() + du.abs()).t() @ d(x).abs()
+            bound = (3 * rnd("f16") + 2.0 ** -16) * size + TINY["f16"]
+            fits, beyond = want.abs() + bound < 65504, want.abs() - bound > 65520  # from 65520 on float16 rounds to infinity
+            assert want[fits].abs().max() > 2000 and beyond.float().mean() < 0.01
+            within(got[fits], want[fits], bound[fits], "gradient")
+            assert torch.isinf(got[beyond]).all()
+
+
+@pytest.mark.parametrize("special", [float("inf"), float("nan")])
+def test_an_infinite_gradient_spoils_what_it_reaches(special):
+    """A row of dh with an infinity or a NaN (loss scaling gone too far) shows in every gradient that it is part of, and only there."""
+    from come_b200.feed_forward import gated_linear
+    for T in (40, 5000):
+        randn = gen(T)
+        x, wg, wu, dh = randn(T, 72).half(), (0.2 * randn(520, 72)).half(), (0.2 * randn(520, 72)).half(), randn(T, 520).half()
+        leaves = [t.clone().requires_grad_(True) for t in (x, wg, wu)]
+        want = torch.autograd.grad(gated_linear(*leaves), leaves, dh)
+        dh[3, 7] = special
+        got = torch.autograd.grad(gated_linear(*leaves), leaves, dh)
+        assert not torch.isfinite(got[0][3]).any() and not torch.isfinite(got[1][7]).any() and not torch.isfinite(got[2][7]).any()
+        rest = torch.arange(T, device="cuda") != 3
+        within(got[0][rest], want[0][rest], 2.0 ** -9 * d(want[0][rest]).abs() + 2.0 ** -10 * d(want[0]).abs().max(), "dx")
+        keep = torch.arange(520, device="cuda") != 7
+        assert torch.isfinite(got[1][keep]).all() and torch.isfinite(got[2][keep]).all()
+
+
 # ---- forward mode -------------------------------------------------------------------------------------------------------------
 def test_forward_mode_is_refused_not_dropped():
     """A dual tensor has no requires_grad: without a look at the level its tangent would vanish without a word."""
