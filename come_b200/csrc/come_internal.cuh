@@ -8,6 +8,7 @@
 #include <cstdarg>
 #include <cstdint>
 #include <cstdio>
+#include <initializer_list>
 
 #include "../../include/come_b200.h"
 
@@ -32,6 +33,13 @@ void set_error(const char *fmt, ...);
             return COME_ERR_CUDA;                                                            \
         }                                                                                    \
     } while (0)
+
+// Whether every address (NULL: not given) is a multiple of `size`: a kernel's access to an element at any other would fault.
+inline bool multiples_of(size_t size, std::initializer_list<const void *> addresses) {
+    for (const void *p : addresses)
+        if ((uintptr_t)p % size != 0) return false;
+    return true;
+}
 
 inline int check_launch(const char *what) {
     cudaError_t e = cudaGetLastError();

@@ -582,6 +582,7 @@ constexpr int64_t kMaxExtent = (1ll << 31) - 256;
 #define COME_REQUIRE_SIZES(what, m, n, k)                                                                                              \
     COME_REQUIRE((m) >= 0 && (n) >= 0 && (k) > 0 && (m) < come::kMaxExtent && (n) < come::kMaxExtent && (k) < come::kMaxExtent,           \
                  what ": sizes must be positive and fit int32 (got %lld, %lld, %lld)", (long long)(m), (long long)(n), (long long)(k))
+#define COME_REQUIRE_MULTIPLES(size, ...) COME_REQUIRE(come::multiples_of(size, __VA_ARGS__), "addresses must be multiples of their elements' size")
 #define COME_REQUIRE_ROWS(what, ptr, stride, size, least)                                                                             \
     COME_REQUIRE(come::rows_ok(ptr, stride, size) && (stride) >= (least), what " must be given, 16-byte aligned, with a row stride of whole 16 bytes that holds its rows")
 
@@ -594,6 +595,9 @@ extern "C" int come_matmul_e4m3(const void *x_dev, int64_t x_row_stride, const f
     COME_REQUIRE_ROWS("x", x_dev, x_row_stride, 1, channels);
     COME_REQUIRE_ROWS("w", w_dev, w_row_stride, 1, channels);
     COME_REQUIRE(x_scale_dev && w_scale_dev && out_dev && out_row_stride >= features, "scales and result must be given");
+    COME_REQUIRE(x_scale_row_stride >= 0 && x_scale_block_stride >= 0 && w_scale_row_stride >= 0, "strides of scales must not be negative");
+    COME_REQUIRE_MULTIPLES(4, {x_scale_dev, w_scale_dev, bias_dev});
+    COME_REQUIRE_MULTIPLES(come::dtype_size(out_dtype), {out_dev});
     come::MatmulArgs a = {};
     a.mode = come::kMatmulPlain;
     a.e4m3 = true;
@@ -625,6 +629,10 @@ extern "C" int come_gated_matmul_e4m3(const void *x_dev, int64_t x_row_stride, c
     COME_REQUIRE(x_scale_dev && gate_scale_dev && up_scale_dev && out_dev && out_row_stride >= features, "scales and result must be given");
     COME_REQUIRE(out_dtype != COME_E4M3 || (out_scale_dev && come::rows_ok(out_dev, out_row_stride, 1)),
                  "an 8-bit result needs its scales, 16-byte aligned rows and a row stride of whole 16 bytes");
+    COME_REQUIRE(x_scale_row_stride >= 0 && x_scale_block_stride >= 0 && gate_scale_row_stride >= 0 && up_scale_row_stride >= 0 &&
+                     (out_dtype != COME_E4M3 || (out_scale_row_stride >= 0 && out_scale_block_stride >= 0)), "strides of scales must not be negative");
+    COME_REQUIRE_MULTIPLES(4, {x_scale_dev, gate_scale_dev, up_scale_dev, gate_bias_dev, up_bias_dev, out_scale_dev});
+    COME_REQUIRE_MULTIPLES(2, {out_dtype == COME_E4M3 ? nullptr : out_dev});
     come::MatmulArgs a = {};
     a.mode = come::kMatmulGated;
     a.e4m3 = true;
@@ -653,6 +661,7 @@ static int gated_common(come::MatmulArgs &a, const void *x, int64_t x_row, const
     COME_REQUIRE_ROWS("x", x, x_row, 2, channels);
     COME_REQUIRE_ROWS("gate", gate, gate_row, 2, channels);
     COME_REQUIRE_ROWS("up", up, up_row, 2, channels);
+    COME_REQUIRE_MULTIPLES(2, {gate_bias, up_bias});
     a.dtype = dtype;
     a.M = tokens, a.N = features, a.K = channels;
     a.a[0] = x, a.a_row[0] = x_row;
@@ -672,6 +681,7 @@ extern "C" int come_gated_matmul(const void *x_dev, int64_t x_row_stride, const 
     const int rc = gated_common(a, x_dev, x_row_stride, gate_dev, gate_row_stride, up_dev, up_row_stride, gate_bias_dev, up_bias_dev, dtype, activation, tokens, features, channels);
     if (rc != COME_OK || tokens == 0 || features == 0) return rc;
     COME_REQUIRE(out_dev && out_row_stride >= features, "out must be given, with a row stride that holds its rows");
+    COME_REQUIRE_MULTIPLES(2, {out_dev});
     a.mode = come::kMatmulGated;
     a.out[0] = out_dev, a.out_row[0] = out_row_stride;
     return come::run_matmul(a, (cudaStream_t)stream);
@@ -702,7 +712,8 @@ extern "C" int come_gated_matmul_backward_in_range(const void *x_dev, int64_t x_
     COME_REQUIRE_ROWS("dup", dup_dev, d_row_stride, 2, features);
     COME_REQUIRE(!dx_dev || dx_row_stride >= channels, "the row stride of dx must hold its rows");
     COME_REQUIRE((!dgate_weight_dev && !dup_weight_dev) || dw_row_stride >= channels, "the row stride of the weights' gradients must hold their rows");
-    COME_REQUIRE((uintptr_t)range_dev % 4 == 0, "range_dev must be 4-byte aligned");
+    COME_REQUIRE(multiples_of(4, {range_dev}), "range_dev must be 4-byte aligned");
+    COME_REQUIRE_MULTIPLES(2, {dout_dev, dx_dev, dgate_weight_dev, dup_weight_dev, dgate_bias_dev, dup_bias_dev});
     const uint32_t *range = dtype == COME_F16 ? (const uint32_t *)range_dev : nullptr;
     if (range && (rc = find_largest(dout_dev, tokens, features, dout_row_stride, (uint32_t *)range_dev, st)) != COME_OK) return rc;
     // the gradients of the projections

@@ -288,6 +288,9 @@ extern "C" int come_residual_rmsnorm(const void *x_dev, const void *branch_dev, 
     COME_REQUIRE(normed_dev || q_dev || x_out_dev, "nothing to write");
     COME_REQUIRE(!q_dev || (q_scale_dev && q_row_stride >= channels && q_row_stride % 16 == 0 && (uintptr_t)q_dev % 16 == 0),
                  "an 8-bit result needs its scales, 16-byte aligned rows and a row stride of whole 16 bytes");
+    COME_REQUIRE(come::multiples_of(come::dtype_size(dtype), {x_dev, branch_dev, scale_dev, weight_dev, x_out_dev, normed_dev}) && come::multiples_of(4, {q_scale_dev}),
+                 "addresses must be multiples of their elements' size");
+    COME_REQUIRE(q_scale_row_stride >= 0 && q_scale_block_stride >= 0, "strides of scales must not be negative");
     come::RmsNormArgs a = {};
     a.x = x_dev;
     a.branch = branch_dev;
@@ -316,7 +319,8 @@ extern "C" int come_quantize_rows(const void *x_dev, int dtype, int64_t rows, in
     COME_REQUIRE(rows < (1ll << 31) && channels < (1ll << 31), "rows and channels must fit int32");
     if (rows == 0 || channels == 0) return COME_OK;
     COME_REQUIRE(x_dev && q_dev && q_scale_dev, "x, q and q_scale must not be NULL");
-    COME_REQUIRE(x_row_stride >= 0, "x_row_stride must not be negative");
+    COME_REQUIRE(x_row_stride >= 0 && q_scale_row_stride >= 0 && q_scale_block_stride >= 0, "strides must not be negative");
+    COME_REQUIRE(come::multiples_of(come::dtype_size(dtype), {x_dev}) && come::multiples_of(4, {q_scale_dev}), "addresses must be multiples of their elements' size");
     COME_REQUIRE(q_row_stride >= channels && q_row_stride % 16 == 0 && (uintptr_t)q_dev % 16 == 0, "q needs 16-byte aligned rows and a row stride of whole 16 bytes");
     come::RmsNormArgs a = {};
     a.x = x_dev;
@@ -339,6 +343,7 @@ extern "C" int come_quantize_weight(const void *w_dev, int dtype, int64_t rows, 
     if (rows == 0 || channels == 0) return COME_OK;
     COME_REQUIRE(w_dev && q_dev && q_scale_dev, "w, q and q_scale must not be NULL");
     COME_REQUIRE(w_row_stride >= 0 && q_row_stride >= channels && q_scale_row_stride >= 0, "bad strides");
+    COME_REQUIRE(come::multiples_of(come::dtype_size(dtype), {w_dev}) && come::multiples_of(4, {q_scale_dev}), "addresses must be multiples of their elements' size");
     const int64_t grid = ((channels + come::kScaleBlock - 1) / come::kScaleBlock) * ((rows + come::kScaleBlock - 1) / come::kScaleBlock);
     COME_REQUIRE(grid < (1ll << 31), "a weight of %lld blocks of 128 x 128 is too large for one launch", (long long)grid);
     cudaStream_t st = (cudaStream_t)stream;

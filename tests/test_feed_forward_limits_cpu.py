@@ -70,3 +70,29 @@ def test_the_backward_pass_in_range_refuses_what_the_other_refuses():
                          ({"dtype": _lib.COME_F32}, "float16 or bfloat16"), ({"range": AT + 2}, "range_dev must be")):
         rc = lib.come_gated_matmul_backward_in_range(*{**good, **change}.values())
         assert rc == _lib.COME_ERR_ARG and text in _lib.last_error(), (change, rc, _lib.last_error())
+
+
+def test_addresses_that_are_no_multiples_of_their_element_are_refused():
+    """A kernel's access to such an address would fault; the check ends the call on the host."""
+    lib, f32, bf16, e4m3 = _lib.lib(), _lib.COME_F32, _lib.COME_BF16, _lib.COME_E4M3
+    norm = dict(x=AT, branch=AT, scale=AT, rows=4, channels=64, dtype=bf16, weight=AT, eps=1e-6, x_out=AT, normed=None, q=AT, q_row=64, qs=AT, qs_row=1, qs_block=4, stream=None)
+    rows = dict(x=AT, dtype=f32, rows=4, channels=64, x_row=64, q=AT, q_row=64, qs=AT, qs_row=1, qs_block=4, stream=None)
+    weight = dict(w=AT, dtype=f32, rows=4, channels=64, w_row=64, q=AT, q_row=64, qs=AT, qs_row=1, stream=None)
+    linear = dict(x=AT, x_row=128, xs=AT, xs_row=1, xs_block=4, w=AT, w_row=128, ws=AT, ws_row=1, bias=AT, tokens=4, features=16, channels=128, out=AT, out_row=16, dtype=f32, stream=None)
+    gated = dict(x=AT, x_row=128, xs=AT, xs_row=1, xs_block=4, g=AT, g_row=128, gs=AT, gs_row=1, u=AT, u_row=128, us=AT, us_row=1, gb=AT, ub=AT, act=0, tokens=4, features=16,
+                 channels=128, out=AT, out_row=16, dtype=e4m3, os=AT, os_row=1, os_block=4, stream=None)
+    wide = dict(x=AT, x_row=128, g=AT, g_row=128, u=AT, u_row=128, gb=AT, ub=AT, dtype=bf16, act=0, tokens=4, features=16, channels=128, out=AT, out_row=16, stream=None)
+    back = dict(x=AT, x_row=128, g=AT, g_row=128, u=AT, u_row=128, gb=AT, ub=AT, dtype=bf16, act=0, tokens=4, features=16, channels=128, dout=AT, dout_row=16,
+                dg=AT, du=AT, d_row=16, dx=AT, dx_row=128, dwg=AT, dwu=AT, dw_row=128, dbg=AT, dbu=AT, stream=None)
+    for entry, good, pointers in ((lib.come_residual_rmsnorm, norm, ("x", "branch", "scale", "weight", "x_out", "qs")), (lib.come_quantize_rows, rows, ("x", "qs")),
+                                  (lib.come_quantize_weight, weight, ("w", "qs")), (lib.come_matmul_e4m3, linear, ("xs", "ws", "bias", "out")),
+                                  (lib.come_gated_matmul_e4m3, gated, ("xs", "gs", "us", "gb", "ub", "os")), (lib.come_gated_matmul_e4m3, {**gated, "dtype": bf16}, ("out",)),
+                                  (lib.come_gated_matmul, wide, ("gb", "ub", "out")), (lib.come_gated_matmul_backward, back, ("gb", "ub", "dout", "dx", "dwg", "dwu", "dbg", "dbu"))):
+        for name in pointers:
+            rc = entry(*{**good, name: AT + 1}.values())
+            assert rc == _lib.COME_ERR_ARG and "multiple" in _lib.last_error(), (entry, name, rc, _lib.last_error())
+    for entry, good, strides in ((lib.come_residual_rmsnorm, norm, ("qs_row", "qs_block")), (lib.come_quantize_rows, rows, ("qs_row", "qs_block")),
+                                 (lib.come_matmul_e4m3, linear, ("xs_row", "xs_block", "ws_row")), (lib.come_gated_matmul_e4m3, gated, ("xs_row", "xs_block", "gs_row", "us_row", "os_row", "os_block"))):
+        for name in strides:
+            rc = entry(*{**good, name: -1}.values())
+            assert rc == _lib.COME_ERR_ARG and "negative" in _lib.last_error(), (entry, name, rc, _lib.last_error())
