@@ -59,7 +59,8 @@ struct PairBarriers {
 // up projection.
 typedef float PairScales[kScaleSlots][2][kTile];
 constexpr size_t smem_bytes(bool e4m3) { return kStages * kStageBytes + 8 * staging_bytes(e4m3) + sizeof(PairBarriers) + (e4m3 ? sizeof(PairScales) : 0); }
-static_assert(smem_bytes(true) <= 227 * 1024 && smem_bytes(false) <= 227 * 1024, "");
+constexpr size_t kSmemBytes = 227 * 1024;  // all of an SM's, as in matmul_sm100.cu
+static_assert(smem_bytes(true) <= kSmemBytes && smem_bytes(false) <= kSmemBytes, "");
 
 __device__ __forceinline__ void tmem_ld16(uint32_t taddr, uint32_t *r) {
     asm volatile(
@@ -770,9 +771,9 @@ __global__ void __launch_bounds__(kThreads, 1) __cluster_dims__(2, 1, 1) matmul_
 
 template <bool kE4m3, int kMode, bool kAMn, bool kBMn, bool kSelfTest = false> int launch_pair(const MatmulParams &p, cudaStream_t st) {
     constexpr auto kernel = matmul_pair_kernel<kE4m3, kMode, kAMn, kBMn, kSelfTest>;
-    if (int rc = allow_smem<kernel>(smem_bytes(kE4m3)); rc != COME_OK) return rc;
+    if (int rc = allow_smem<kernel>(kSmemBytes); rc != COME_OK) return rc;
     const int tiles = p.tiles_m * p.problems * p.tiles_n, pairs = sm_count() / 2;
-    kernel<<<2 * (tiles < pairs ? tiles : pairs), kThreads, smem_bytes(kE4m3), st>>>(p);
+    kernel<<<2 * (tiles < pairs ? tiles : pairs), kThreads, kSmemBytes, st>>>(p);
     return check_launch("product kernel");
 }
 

@@ -17,8 +17,8 @@
 // Measured in a graph: 1 token 2736 -> 1024 in 8 bits 6.4 us, 64 tokens 7.7, 128 tokens 9.0 (weights 2.8 MB; launch, cluster barriers and
 // the first loads' latency are most of it), 1374 tokens 1024 -> 1024 10 us.
 //
-// Shared memory: a CTA takes more than half an SM's, so that no two CTAs that need tensor memory share an SM: CTAs of two clusters
-// that wait for each other's tensor memory while their partners wait at a cluster barrier would never end.
+// Shared memory: a CTA asks for all of an SM's, so that no other CTA that needs tensor memory, of this library or of another, shares its
+// SM: CTAs of two clusters that wait for each other's tensor memory while their partners wait at a cluster barrier would never end.
 //
 // Every wait on an mbarrier is bounded (kWaitTicks): a CTA whose wait gave up raises its abort flag and the device status word, goes
 // on to the cluster's barriers, and no CTA of the cluster stores.
@@ -43,8 +43,8 @@ struct SplitBarriers {
     uint32_t tmem_base;
     volatile uint32_t abort_flag;
 };
-constexpr size_t kSmemBytes = kRingBytes + sizeof(SplitBarriers) + 1024;
-static_assert(kSmemBytes <= 227 * 1024 && kSmemBytes > 114 * 1024, "one CTA per SM");
+constexpr size_t kSmemBytes = 227 * 1024;
+static_assert(kRingBytes + sizeof(SplitBarriers) <= kSmemBytes, "");
 static_assert(2 * kPartBytes <= kRingBytes, "the shares reuse the ring");
 
 // Four neighbouring columns of a row, `valid` of them inside the result.

@@ -199,3 +199,27 @@ def test_no_gradient_is_written_while_the_status_word_is_raised(T, K, F, kind):
         _lib.device_status(clear=True)
     assert all(not bool((t == 7).all()) for t in run())
     assert _lib.device_status(clear=True) == 0
+
+
+def test_products_beside_library_products_on_another_stream():
+    """Both need tensor memory: the clusters of one and the CTA pairs of the other must not hold parts of each other's SMs."""
+    from come_b200 import _lib
+    from come_b200.block_scaled import block_scaled_linear, quantize_rows, quantize_weight
+    from come_b200.feed_forward import gated_linear
+    randn = gen(8)
+    few, many = randn(60, 1024).bfloat16(), randn(5000, 1024).bfloat16()
+    w, v = (randn(1040, 1024).bfloat16() / 32 for _ in range(2))
+    few8, many8, w8 = quantize_rows(few), quantize_rows(many), quantize_weight(w)
+    calls = (lambda: gated_linear(few, w, v), lambda: block_scaled_linear(few8, w8), lambda: gated_linear(many, w, v), lambda: block_scaled_linear(many8, w8))
+    sizes = [(randn(m, 1024).bfloat16(), randn(n, 1024).bfloat16()) for m, n in ((64, 64), (128, 512), (300, 4096), (5000, 1040))]
+    want, library = [c() for c in calls], [a @ b.t() for a, b in sizes]
+    torch.cuda.synchronize()
+    streams, got, theirs = [torch.cuda.Stream() for _ in range(2)], [], []
+    for _ in range(30):
+        with torch.cuda.stream(streams[0]):
+            got.append([c() for c in calls])
+        with torch.cuda.stream(streams[1]):
+            theirs.append([a @ b.t() for a, b in sizes])
+    torch.cuda.synchronize()
+    assert all(torch.equal(a, b) for r in got for a, b in zip(r, want)) and all(torch.equal(a, b) for r in theirs for a, b in zip(r, library))
+    assert _lib.device_status(clear=True) == 0
