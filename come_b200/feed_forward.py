@@ -85,13 +85,13 @@ class _GatedLinear(torch.autograd.Function):
             dh = dh.contiguous()
         lib = _lib.lib()
         d_rows = lib.come_gated_backward_rows(tokens, features)
-        dg, du = _padded(d_rows, features, x), _padded(d_rows, features, x)
-        largest = torch.empty(1, dtype=torch.float32, device=dev) if x.dtype is torch.float16 else None
+        dg, du = _padded(d_rows + 1, features, x), _padded(d_rows, features, x)
+        largest = dg.data_ptr() + 2 * d_rows * dg.stride(0)  # the float of workspace: in a row behind the last
         with on_device(dev):
             _lib.check(lib.come_gated_matmul_backward_in_range(
                 x_at, x_row, g_at, g_row, u_at, u_row, ptr(b_gate), ptr(b_up), dtype_code(x.dtype), ctx.act,
                 tokens, features, cols, dh.data_ptr(), dh.stride(0), dg.data_ptr(), du.data_ptr(), dg.stride(0), ptr(dx), cols, ptr(dwg), ptr(dwu), cols,
-                ptr(dbg), ptr(dbu), ptr(largest), stream_ptr(dev)))
+                ptr(dbg), ptr(dbu), largest, stream_ptr(dev)))
         return dx, dwg, dwu, dbg, dbu, None
 
 

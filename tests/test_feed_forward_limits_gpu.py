@@ -142,6 +142,42 @@ def test_an_infinite_gradient_spoils_what_it_reaches(special):
         assert torch.isfinite(got[1][keep]).all() and torch.isfinite(got[2][keep]).all()
 
 
+@pytest.mark.parametrize("T", [50, 1001, 4700])
+def test_float16_steps_in_two_graphs_find_their_range_anew(T):
+    """Replays in turn, with result gradients of other magnitudes than at the capture, give the eager bits."""
+    from come_b200.feed_forward import gated_linear
+    randn = gen(T)
+    data = randn(T, 200).half(), (0.1 * randn(520, 200)).half(), (0.1 * randn(520, 200)).half()
+    steps = [(randn(T, 520) * 2.0 ** e).half() for e in (0, -20, 8, -24)]
+
+    def step(dh):
+        leaves = [t.detach().requires_grad_(True) for t in data]
+        return torch.autograd.grad(gated_linear(*leaves), leaves, dh)
+
+    want = [step(dh) for dh in steps]
+    slots, graphs = [], []
+    for _ in range(2):
+        dh, g = steps[0].clone(), torch.cuda.CUDAGraph()
+        with torch.cuda.graph(g):
+            out = step(dh)
+        slots.append((dh, out))
+        graphs.append(g)
+    for first, second in ((0, 1), (2, 3), (1, 2), (3, 0)):
+        for (dh, _), i in zip(slots, (first, second)):
+            dh.copy_(steps[i])
+        for g in graphs + graphs:
+            g.replay()
+        torch.cuda.synchronize()
+        for (_, out), i in zip(slots, (first, second)):
+            assert all(torch.equal(a, b) for a, b in zip(out, want[i]))
+    # rows of the result's gradient that are further apart than they are wide, at an odd address, and one broadcast row
+    wide = torch.full((T, 533), float("nan"), device="cuda").half()
+    wide[:, 7: 527] = steps[1]
+    assert all(torch.equal(a, b) for a, b in zip(step(wide[:, 7: 527]), want[1]))
+    row = steps[1][:1].expand(T, 520)
+    assert all(torch.equal(a, b) for a, b in zip(step(row), step(row.contiguous())))
+
+
 # ---- forward mode -------------------------------------------------------------------------------------------------------------
 def test_forward_mode_is_refused_not_dropped():
     """A dual tensor has no requires_grad: without a look at the level its tangent would vanish without a word."""
