@@ -11,11 +11,12 @@
 //   warp 8    : producer (TMA ring).      warp 9 : MMA issuer.
 //
 // Why a split: a block's products have few tiles where there are few tokens (1 x 2736 -> 1024: eight), and a tile's time is its
-// contraction's; shares of it bring all SMs to read the weights.  The shares meet in shared memory, not in a workspace, so that two
+// contraction's; shares of it bring up to eight SMs per tile to read the weights (64 of 148 there).  The shares meet in shared memory, not in a workspace, so that two
 // graphs captured from the same call share nothing.
 //
 // Measured in a graph: 1 token 2736 -> 1024 in 8 bits 6.4 us, 64 tokens 7.7, 128 tokens 9.0 (weights 2.8 MB; launch, cluster barriers and
-// the first loads' latency are most of it), 1374 tokens 1024 -> 1024 10 us.
+// the first loads' latency are most of it), 1374 tokens 1024 -> 1024 10 us.  The 8-bit gated form spills 72 bytes (128 float32 sums beside
+// the loads in 168 registers).
 //
 // Shared memory: a CTA asks for all of an SM's, so that no other CTA that needs tensor memory, of this library or of another, shares its
 // SM: CTAs of two clusters that wait for each other's tensor memory while their partners wait at a cluster barrier would never end.
@@ -699,7 +700,10 @@ extern "C" int come_gated_matmul(const void *x_dev, int64_t x_row_stride, const 
 
 // Gradients of few tokens, or of few elements, are sums of few rounded numbers: the error is the luck of some hundred roundings rather
 // than their average (up to 1.7 times that of float32 operands after rounding, where large ones have 1.4).  There the operands keep a
-// second 16-bit part, which doubles contractions that are short anyway: a step of 64 tokens 1024 -> 2736 stays with the host.
+// second 16-bit part, which doubles the contractions behind them.  Both sides of the rule, a step in a graph, two parts / one (bf16; error
+// of dx and dW against float64 0.0017 / 0.0023 in every case): by elements, 261 / 262 tokens 392 -> 1003 45 / 40 us, 1000 tokens 64 ->
+// 262 / 263 54 / 48, 95 / 96 tokens 2048 -> 2736 96 / 58; by tokens, 64 / 65 of 4096 -> 11,008 444 / 204.  Launched from Python the small
+// ones take 135-143 us on either side.
 extern "C" int64_t come_gated_backward_rows(int64_t tokens, int64_t features) {
     if (tokens <= 0) return 0;
     return tokens <= 64 || (features < (1ll << 18) && tokens < (1ll << 18) && tokens * features <= (1ll << 18)) ? 2 * tokens : tokens;
