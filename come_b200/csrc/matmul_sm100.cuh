@@ -210,12 +210,15 @@ __device__ __forceinline__ void activation_grad(float g, int act, float &value, 
     }
 }
 
-// The power of two that brings the largest |dh| into [1/2, 1), and its inverse.  The gradients of the projections lie around dh; without
-// it those of a mean over many elements fall below float16's smallest number and those of a scaled loss past its largest, while the
-// gradients that they become would not.  Nothing is scaled where the largest is zero, infinite or no number.
+// The power of two that float16 gradients of the projections, which lie around dh, are held times, and its inverse.  Where the largest
+// |dh| is below 1/2 it is brought to [1/2, 1): those of a mean over many elements would fall below the type's smallest number.  From
+// 2^10 on it is brought to [2^9, 2^10): times the other projection they would pass the type's largest, while the gradients that they
+// become would not.  In between, where neither is near, they stay as they are: making room for one token's would cost the others digits.
+// Nothing is scaled where the largest is zero, infinite or no number.
 __device__ __forceinline__ float range_factor(const uint32_t *range, bool inverse) {
-    const uint32_t bits = range ? __ldg(range) : 0u, e = bits >> 23;
-    return bits == 0 || e == 255 ? 1.0f : __uint_as_float((inverse ? e + 1 : 253 - e) << 23);
+    const uint32_t bits = range ? __ldg(range) : 0u, e = bits >> 23;  // exponent, biased by 127
+    const uint32_t want = bits == 0 || e == 255 ? e : e < 126 ? 126 : e > 136 ? 136 : e;
+    return __uint_as_float((inverse ? 127 + e - want : 127 + want - e) << 23);
 }
 
 __device__ __forceinline__ float load_any(const void *p, int64_t i, int dtype) {

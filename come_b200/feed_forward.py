@@ -6,8 +6,8 @@ MLPs of visual transformers: ``w12`` holds both projections, the gate's rows fir
 A training step keeps only its inputs: the backward pass computes the projections again, in float32, and with them their gradients
 (one kernel of ``come_gated_matmul_backward_in_range``), then ``dx = dg Wg + du Wu`` and ``dW = dg^T x`` / ``du^T x``.  ``dg`` and ``du`` are rounded to the
 tokens' type once, as operands of these products (for few tokens, whose sums do not average that out, in two parts); saved 16-bit
-projections would add their own rounding to every gradient.  In float16 they are held times a power of two that brings the largest
-``|dh|`` to one, so that neither a mean over many elements nor a scaled loss takes them out of the type's range.
+projections would add their own rounding to every gradient.  In float16 they are held times a power of two where the largest ``|dh|``
+is below 1/2 or from 2^10 on, so that neither a mean over many elements nor a scaled loss takes them out of the type's range.
 """
 from __future__ import annotations
 

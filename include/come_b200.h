@@ -382,8 +382,8 @@ int come_packed_positions(const uint8_t *mask_dev, const int64_t *rev_id_dev, in
  *   dx = dgate gate + dup up, dgate_weight = dgate^T x, dup_weight = dup^T x and the column sums of dgate, dup for the biases.  Any of the
  *   five results may be NULL.  tokens and features must not be zero.
  * come_gated_matmul_backward_in_range  the same with one float of workspace, range_dev (NULL: none): float16 gradients are held in the
- *   workspaces times the power of two that brings the largest |dout| into [1/2, 1), so that they do not leave the type's range on their
- *   way (without it that of dout times up and act is the caller's affair).  bfloat16 has float32's range and ignores it.
+ *   workspaces times a power of two where the largest |dout| is below 1/2, which is brought to [1/2, 1), or from 2^10 on, which is brought
+ *   to [2^9, 2^10), so that they do not leave the type's range on their way (without it dout times up and act is the caller's affair).  bfloat16 has float32's range and ignores it.
  *
  * Results are the same bits in every run.  While bits 19-21 of the device status word are raised, the products return at once without
  * touching their outputs.

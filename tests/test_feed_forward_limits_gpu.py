@@ -70,8 +70,8 @@ def test_weights_of_many_rows_or_columns_are_quantised(rows, cols):
 @pytest.mark.parametrize("step", [-24, -18, -10, 0, 6])
 def test_float16_gradients_of_any_size(T, K, F, step):
     """Gradients of the result from float16's smallest numbers (a mean over many elements without loss scaling) up: those of the projections
-    keep their digits.  Brought to [1/2, 1) by a power of two, the largest |dh| leaves every gradient of a projection at most half a step off,
-    or 2^-25 of that range: 2^-24 of the largest |dh|."""
+    keep their digits.  Brought to [1/2, 1) by a power of two where it is smaller, the largest |dh| leaves every gradient of a projection at most
+    half a step off, or half the type's smallest, 2^-25, of that range: 2^-24 of the largest |dh|, and 2^-25 from 1/2 on."""
     from come_b200.feed_forward import gated_linear
     randn = gen(T + step)
     e = rnd("f16")
@@ -80,7 +80,7 @@ def test_float16_gradients_of_any_size(T, K, F, step):
     leaves = [t.clone().requires_grad_(True) for t in (x, wg, wu, bg, bu)]
     grads = torch.autograd.grad(gated_linear(*leaves), leaves, dh)
     h, slack, g, u, a, slope, eg, eu = gated64(d(x), d(wg), d(wu), d(bg), d(bu), "silu", d(dh))
-    least = d(dh).abs().max() * 2.0 ** -24
+    least = d(dh).abs().max().clamp(max=0.5) * 2.0 ** -24
     dg, du = d(dh) * u * slope, d(dh) * a
     edg = d(dh).abs() * (slope.abs() * eu + (u.abs() + eu) * (0.85 * eg + 2.0 ** -18 * (1 + g.abs())))
     edu = d(dh).abs() * (1.2 * eg + 2.0 ** -19 * a.abs() + 2.0 ** -140)
@@ -140,6 +140,33 @@ def test_an_infinite_gradient_spoils_what_it_reaches(special):
         within(got[0][rest], want[0][rest], 2.0 ** -9 * d(want[0][rest]).abs() + 2.0 ** -10 * d(want[0]).abs().max(), "dx")
         keep = torch.arange(520, device="cuda") != 7
         assert torch.isfinite(got[1][keep]).all() and torch.isfinite(got[2][keep]).all()
+
+
+@pytest.mark.parametrize("T", [40, 5000])
+def test_a_large_float16_gradient_of_one_token_leaves_the_others_their_digits(T):
+    """One token's gradients are 2^18 times the others' and still far from the type's largest number: nothing has to make room for them.
+    The other tokens' dx depends on their own gradients only, each at most half a step or half the type's smallest step off."""
+    from come_b200.feed_forward import gated_linear
+    K, F = 72, 520
+    randn = gen(T + 1)
+    e = rnd("f16")
+    x, wg, wu = randn(T, K).half(), (randn(F, K) * 1.5 / math.sqrt(K)).half(), (randn(F, K) * 1.5 / math.sqrt(K)).half()
+    dh = (randn(T, F) * 2.0 ** -10).half()
+    dh[3] = (randn(F) * 2.0 ** 8).clamp(-900, 900).half()
+    leaf = x.clone().requires_grad_(True)
+    (dx,) = torch.autograd.grad(gated_linear(leaf, wg, wu), leaf, dh)
+    zero = torch.zeros(F, device="cuda", dtype=torch.float64)
+    h, slack, g, u, a, slope, eg, eu = gated64(d(x), d(wg), d(wu), zero, zero, "silu", d(dh))
+    dg, du = d(dh) * u * slope, d(dh) * a
+    edg = d(dh).abs() * (slope.abs() * eu + (u.abs() + eu) * (0.85 * eg + 2.0 ** -18 * (1 + g.abs())))
+    edu = d(dh).abs() * (1.2 * eg + 2.0 ** -19 * a.abs() + 2.0 ** -140)
+    edg, edu = edg + e * (dg.abs() + edg) + 2.0 ** -25, edu + e * (du.abs() + edu) + 2.0 ** -25
+    want, wobble = dg @ d(wg) + du @ d(wu), edg @ d(wg).abs() + edu @ d(wu).abs()
+    size = (dg.abs() + edg) @ d(wg).abs() + (du.abs() + edu) @ d(wu).abs()
+    within(dx, want, wobble + chain(2 * F) * size + e * (want.abs() + wobble + chain(2 * F) * size) + TINY["f16"], "dx")
+    others = torch.arange(T, device="cuda") != 3
+    # independent roundings: half a step of a gradient around 2^-10, or of the smallest numbers, and half a step of dx
+    assert (d(dx[others]) - want[others]).norm() / want[others].norm() <= 2.0 ** -10
 
 
 @pytest.mark.parametrize("T", [50, 1001, 4700])
