@@ -270,7 +270,7 @@ def to_block_scaled(module: torch.nn.Module, out_dtype: torch.dtype = torch.bflo
     their 16-bit linear layers."""
     from .feed_forward import GatedMlp
     if isinstance(module, GatedMlp):
-        return BlockScaledGatedMlp(module, out_dtype)
+        return BlockScaledGatedMlp(module, out_dtype).train(module.training)
     made = {}  # one for every module, however many places it stands in
     for parent in list(module.modules()):
         for name, child in list(parent._modules.items()):

@@ -266,3 +266,9 @@ def test_every_use_of_a_gated_mlp_is_replaced():
     assert model[0][0] is model[0][1] and model[0][0] is model[1][0] and isinstance(model[2], BlockScaledGatedMlp) and model[2] is not model[0][0]
     assert not any(m.training for m in model.modules())
     assert to_block_scaled(model) is model  # a second time there is nothing left to do
+
+
+def test_a_converted_mlp_keeps_its_mode():
+    from come_b200.block_scaled import to_block_scaled
+    from come_b200.feed_forward import GatedMlp
+    assert not to_block_scaled(GatedMlp(64, 96).cuda().eval()).training and to_block_scaled(GatedMlp(64, 96).cuda()).training
