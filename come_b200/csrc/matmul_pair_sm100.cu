@@ -14,7 +14,7 @@
 //   warps 10, 11 : 8-bit operands: the scales of a K block, row x column block, two blocks ahead.
 //
 // What it measures and what bounds it.  8-bit operands: the hand-over of a K block, about 950 clocks where its product takes 512 (two TMEM
-// buffers are all there is), then the 1 kW cap: 80,672 tokens 2736 -> 1024 313 us sustained (1450 TFLOP/s), 284 cold; gated 1024 -> 2736
+// buffers are all there is), then the 1 kW cap: 80,672 tokens 2736 -> 1024 313 us sustained (1450 TFLOP/s), 277 cold; gated 1024 -> 2736
 // 624 us (1450), of which a tile's end is 4500 of 11,000 clocks.  What cost most on the way: an arrival with cluster release per K block
 // (8192 x 16,384 x 2048: 703 us, 320 without), operands of the issuer in ordinary registers (430-550 clocks for six instructions, 180
 // in uniform ones), spilled registers in the scaling loop (10-15 %).  16-bit operands: the tensor pipe, at the power cap when sustained

@@ -5,7 +5,7 @@ import math
 import pytest
 import torch
 
-from test_feed_forward_gpu import DT, TINY, act64, chain, check_rows8, d, gated64, gen, rnd, within
+from test_feed_forward_gpu import DT, TINY, chain, check_rows8, d, gated64, gen, rnd, within
 
 pytestmark = pytest.mark.gpu
 
